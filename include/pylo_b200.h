@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define PYLO_B200_ABI_VERSION 19
+#define PYLO_B200_ABI_VERSION 20
 
 /* optimizer families (which feature set / network geometry a launch uses) */
 #define PYLO_FAM_ADAFAC 0 /* AdafacLO_CUDA, ELO_CUDA: 28+11 features, 39-32-32-2 */
@@ -512,6 +512,57 @@ int pylo_b200_step(const pylo_step_plan* plan, const pylo_step_params* prm, int 
 /* Host only: adds 1 to n step counters (HOST pointers to doubles); first: the old value of the first, equal: whether all
  * old values were the same. */
 int pylo_b200_advance_steps(double* const* steps, int n, double* first, int* equal);
+
+/* ---- AdamW over many tensors at once, and the global norm of many gradients ---------------------------------------------
+ * For parameters and gradients of any of three types.  Items and sets are HOST arrays: they are copied into the launches (one per
+ * combination of types and 350 to 1500 tensors), so nothing has to outlive the call and a captured launch keeps what it was given. */
+#define PYLO_FP32 0
+#define PYLO_BF16 1
+#define PYLO_FP16 2
+#define PYLO_ADAMW_BLOCK 256 /* elements that share a scale in the 8-bit states */
+/* One parameter tensor (contiguous).  32-bit states: m, v fp32[n].  8-bit: m and v hold the codes [n] of the first moment and of the ROOT of the
+ * second, OCP e4m3 (torch.float8_e4m3fn), m_scale and v_scale an e8m0 power of two per PYLO_ADAMW_BLOCK elements [ceil(n / 256)]: a value is
+ * code * scale. */
+typedef struct pylo_adamw_item {
+  void* p;
+  const void* g;
+  float* master; /* beside p of 16 bits, or NULL: its fp32 copy, which the step updates; p becomes the rounded copy */
+  void *m, *v;
+  uint8_t *m_scale, *v_scale;
+  const float* step; /* DEVICE counter of the steps before this one, or NULL: sets[set].step */
+  int64_t n;         /* at most 2^34 */
+  int32_t p_type, g_type; /* g_type: p_type or PYLO_FP32, or any beside fp32 parameters */
+  int32_t set;
+  int32_t pad_;
+} pylo_adamw_item;
+typedef struct pylo_adamw_set {
+  double lr, weight_decay, beta1, beta2, eps;
+  double clip_norm;    /* > 0: gradients times clip_norm / max(norm, clip_norm), norm the root of *gnorm_sq */
+  const float* lr_dev; /* DEVICE scalar that stands for lr, or NULL */
+  int64_t step;        /* of this step: 1, 2, ... */
+  uint32_t seed;       /* of the random rounding of 8-bit states, which depends on seed, step and an element's place in its tensor only */
+  int32_t maximize;
+} pylo_adamw_set;
+int pylo_b200_sizeof_adamw_item(void);
+/* p *= 1 - lr wd; m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2; p -= lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps).
+ * bits: 32 or 8.  gnorm_sq: DEVICE scalar, or NULL where no set clips. */
+int pylo_b200_adamw_step(const pylo_adamw_item* items, int n_items, const pylo_adamw_set* sets, int n_sets, int bits, const float* gnorm_sq,
+                         void* stream);
+/* adds 1 to n DEVICE counters (steps is a HOST array) */
+int pylo_b200_adamw_advance(float* const* steps, int n, void* stream);
+
+typedef struct pylo_grad_item {
+  void* g; /* contiguous */
+  int64_t n;
+  int32_t type;
+  int32_t pad_;
+} pylo_grad_item;
+/* floats of scratch that grad_norm needs for these items (host only; -1: bad arguments) */
+int64_t pylo_b200_grad_norm_scratch(const pylo_grad_item* items, int n_items);
+/* out[0] = sum of squares of all elements, out[1] = its root; the same sums in the same order on every call */
+int pylo_b200_grad_norm(const pylo_grad_item* items, int n_items, float* scratch, float* out, void* stream);
+/* all elements times min(1, max_norm / (*norm + 1e-6)), norm a DEVICE scalar; nothing is written where that is 1 */
+int pylo_b200_grad_scale(const pylo_grad_item* items, int n_items, const float* norm, float max_norm, void* stream);
 
 #ifdef __cplusplus
 }

@@ -17,7 +17,7 @@ TILE_ELEMS = 16384
 A_COLS = 1024
 PREP_TABLE = 2048  # table entries (rows x hidden units) per item of pylo_b200_prep_apply
 WFOLD_STRIDE = 4800
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 FAM_ADAFAC, FAM_CELO2, FAM_VELO = 0, 1, 2
 MODE_FAST2D, MODE_GENERIC, MODE_VEC1D, MODE_KERNEL = 0, 1, 2, 3
@@ -49,6 +49,20 @@ ADAM_DTYPE = np.dtype(
      ("lr", np.float32), ("wd", np.float32), ("bc1", np.float32), ("bc2", np.float32),
      ("clip_norm", np.float32), ("pad_", np.float32, (3,))]
 )
+
+FP32, BF16, FP16 = 0, 1, 2   # element types of AdamW's and the gradient norm's items
+ADAMW_BLOCK = 256            # elements that share a scale in the 8-bit states
+ADAMW_DTYPE = np.dtype(
+    [(name, np.uint64) for name in ("p", "g", "master", "m", "v", "m_scale", "v_scale", "step")]
+    + [("n", np.int64)] + [(name, np.int32) for name in ("p_type", "g_type", "set", "pad_")]
+)
+GRAD_DTYPE = np.dtype([("g", np.uint64), ("n", np.int64), ("type", np.int32), ("pad_", np.int32)])
+
+
+class AdamwSet(C.Structure):
+    """pylo_adamw_set: hyper-parameters and step count of some tensors of ``pylo_b200_adamw_step``."""
+    _fields_ = [(name, C.c_double) for name in ("lr", "weight_decay", "beta1", "beta2", "eps", "clip_norm")] + [
+        ("lr_dev", C.c_void_p), ("step", C.c_int64), ("seed", C.c_uint32), ("maximize", C.c_int32)]
 
 
 class StepParams(C.Structure):
@@ -153,15 +167,22 @@ def _load():
         "pylo_b200_velo_rnn": [C.POINTER(VeloRnn), C.POINTER(VeloLoss), vp],
         "pylo_b200_velo_loss_features": [vp, vp, vp, vp, vp, vp, vp],
         "pylo_b200_step": [C.POINTER(StepPlan), C.POINTER(StepParams), i32, vp],
+        "pylo_b200_sizeof_adamw_item": [],
+        "pylo_b200_adamw_step": [vp, i32, C.POINTER(AdamwSet), i32, i32, vp, vp],
+        "pylo_b200_adamw_advance": [vp, i32, vp],
+        "pylo_b200_grad_norm_scratch": [vp, i32],
+        "pylo_b200_grad_norm": [vp, i32, vp, vp, vp],
+        "pylo_b200_grad_scale": [vp, i32, vp, f32, vp],
         "pylo_b200_advance_steps": [vp, i32, C.POINTER(C.c_double), C.POINTER(C.c_int)],
     }
     for name, argtypes in sigs.items():
         fn = getattr(lib, name)  # AttributeError if a declared symbol is missing
         fn.argtypes = argtypes
-        fn.restype = C.c_int64 if name in ("pylo_b200_workspace_bytes", "pylo_b200_newton_schulz_workspace") else C.c_int
+        fn.restype = C.c_int64 if name in ("pylo_b200_workspace_bytes", "pylo_b200_newton_schulz_workspace", "pylo_b200_grad_norm_scratch") else C.c_int
     if lib.pylo_b200_abi_version() != ABI_VERSION:
         raise ImportError("libpylo_b200.so was built from a different ABI version; rebuild it")
-    if lib.pylo_b200_sizeof_desc() != DESC_DTYPE.itemsize or lib.pylo_b200_sizeof_params() != C.sizeof(StepParams):
+    if (lib.pylo_b200_sizeof_desc() != DESC_DTYPE.itemsize or lib.pylo_b200_sizeof_params() != C.sizeof(StepParams)
+            or lib.pylo_b200_sizeof_adamw_item() != ADAMW_DTYPE.itemsize):
         raise ImportError("descriptor layout mismatch between the Python binding and libpylo_b200.so")
     return lib, sorted(sigs)
 

@@ -1,0 +1,472 @@
+"""AdamW over many tensors at once, with states in 32 bits or in 8, and clipping by the global norm.
+
+The step that the learned optimizers are compared with, and that a model can be trained with before or after them: the
+update and the state keys (``step``, ``exp_avg``, ``exp_avg_sq``) of ``torch.optim.AdamW``, whose checkpoints load.
+Parameters are fp32, bf16 or fp16, those of 16 bits with or without an fp32 copy in the state (``master_weights``).
+
+A step is one launch over the tensors of all param groups (one per combination of types, and per few hundred tensors), two
+more before it where gradients are clipped by their global norm.  Nothing of it waits for the device.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+from collections import OrderedDict
+
+import numpy as np
+import torch
+from torch.optim import Optimizer
+
+from .. import _lib as L
+from ..plan import current_stream_ptr, with_gradients
+from ._common import StepCounters, optimizer_step
+
+TYPES = {torch.float32: L.FP32, torch.bfloat16: L.BF16, torch.float16: L.FP16}
+_CODES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def blocks_of(n: int) -> int:
+    return -(-n // L.ADAMW_BLOCK)
+
+
+def to_blocks(x: torch.Tensor):
+    """(codes, scales) of the 8-bit states for the values of a tensor: e4m3 codes of its shape, rounded to nearest, and a power of
+    two for every 256 of its elements that brings the largest magnitude into [128, 256)."""
+    flat = x.detach().to(torch.float32).contiguous().view(-1)
+    n = flat.numel()
+    b = torch.zeros(blocks_of(n) * L.ADAMW_BLOCK, dtype=torch.float32, device=x.device)
+    b[:n] = flat
+    b = b.view(-1, L.ADAMW_BLOCK)
+    finite = torch.where(b.isfinite(), b, 0.0)
+    most = finite.abs().amax(1) if len(b) else b.new_zeros(0)
+    scale = ((most.view(torch.int32) >> 23).clamp(min=8) - 7)
+    codes = (finite / (scale << 23).view(torch.float32)[:, None]).to(_CODES).view(torch.uint8)
+    codes = torch.where(b.isfinite(), codes, 0x7F).view(_CODES)
+    return codes.view(-1)[:n].view(x.shape), scale.to(torch.uint8).view(_SCALES)
+
+
+def from_blocks(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The fp32 values that codes and scales of an 8-bit state stand for."""
+    each = scales.to(torch.float32).repeat_interleave(L.ADAMW_BLOCK)[: codes.numel()]
+    return codes.to(torch.float32) * each.view(codes.shape)
+
+
+def _gradient(g: torch.Tensor, p_dtype) -> torch.Tensor:
+    """``g`` as the kernels take it beside parameters of a type: itself, or a copy."""
+    if not (g.dtype is p_dtype or g.dtype is torch.float32 or (p_dtype is torch.float32 and g.dtype in TYPES)):
+        g = g.detach().to(torch.float32)
+    return g.contiguous()
+
+
+class _Kept:
+    """A state tensor on its way through ``Optimizer.load_state_dict``, which gives every tensor the parameter's type."""
+
+    def __init__(self, value):
+        self.value = value
+
+
+class _Plan:
+    """The host's table of a set of tensors, and what of it the last step has seen."""
+
+    def __init__(self, params, group_of, states, bits):
+        self.device = params[0].device
+        self.p_dtypes = [p.dtype for p in params]
+        self.states, self.group_of = states, group_of
+        self.table = t = np.zeros(len(params), dtype=L.ADAMW_DTYPE)
+        t["p"] = [p.data_ptr() for p in params]
+        t["n"] = [p.numel() for p in params]
+        t["p_type"] = [TYPES[d] for d in self.p_dtypes]
+        ptr = lambda name: [st[name].data_ptr() if name in st else 0 for st in states]
+        t["master"], t["m"] = ptr("master"), ptr("exp_avg")
+        t["v"] = ptr("exp_avg_sq" if bits == 32 else "exp_avg_sq_root")
+        t["m_scale"], t["v_scale"] = ptr("exp_avg_scale"), ptr("exp_avg_sq_root_scale")
+        on_device = [st["step"].is_cuda for st in states]
+        t["step"] = [st["step"].data_ptr() if cuda else 0 for st, cuda in zip(states, on_device)]
+        self.device_steps = [a for a in t["step"].tolist() if a]
+        if self.device_steps:
+            self.device_steps = (C.c_void_p * len(self.device_steps))(*self.device_steps)
+        self.host = [i for i, cuda in enumerate(on_device) if not cuda]
+        self.counters = StepCounters([states[i] for i in self.host])
+        self.moments = [st["exp_avg"] for st in states]
+        t["set"] = group_of
+        self.one_step = True     # the table's sets are the groups'
+        self.g_ptrs, self.g_dtypes = None, None
+        self.address = t.ctypes.data
+        self.grads = np.zeros(len(params), dtype=L.GRAD_DTYPE)
+        self.grads["n"] = t["n"]
+
+    def look_at(self, grads):
+        """Put the gradients' addresses and types into the table; returns the copies that stand in for some of them."""
+        try:
+            ptrs = [g.data_ptr() for g in grads]
+        except RuntimeError:
+            if any(g.is_sparse for g in grads):
+                raise RuntimeError("Sparse gradients not supported") from None
+            raise
+        copies = ()
+        dtypes = [g.dtype for g in grads]
+        if dtypes != self.g_dtypes or not all([g.is_contiguous() for g in grads]):
+            copies = [_gradient(g, d) for g, d in zip(grads, self.p_dtypes)]
+            ptrs = [g.data_ptr() for g in copies]
+            self.table["g_type"] = self.grads["type"] = [TYPES[g.dtype] for g in copies]
+            plain = all([c is g for c, g in zip(copies, grads)])
+            self.g_dtypes = dtypes if plain else None
+        if ptrs != self.g_ptrs:
+            self.table["g"] = self.grads["g"] = ptrs
+            self.g_ptrs = ptrs
+        return copies
+
+
+class _AdamWFamily(Optimizer):
+    _bits = 32
+
+    def _setup(self, params, **defaults):
+        if not torch.cuda.is_available():
+            raise RuntimeError(f"{self._name} requires a CUDA device.")
+        self._check(defaults)
+        super().__init__(params, defaults)
+        self._reset()
+        self.process_group = None   # set (or set _sharded) when the tensors of the model are split over ranks
+        self._sharded = False
+        self.after_group = None     # optional callable(group index), called once the step's kernels are enqueued
+        self.before_group = None    # optional callable(group index), called before them
+
+    def _check(self, group):
+        b1, b2 = group["betas"]
+        for name, value, fine in (("lr", group["lr"], float(group["lr"]) >= 0), ("betas", group["betas"], 0 <= b1 < 1 and 0 <= b2 < 1),
+                                  ("eps", group["eps"], group["eps"] >= 0), ("weight_decay", group["weight_decay"], group["weight_decay"] >= 0),
+                                  ("clip_norm", group["clip_norm"], group["clip_norm"] > 0)):
+            if not fine:
+                raise ValueError(f"{self._name}: invalid {name}: {value}")
+        if group.get("amsgrad"):
+            raise ValueError(f"{self._name}: amsgrad is not supported")
+
+    def _reset(self):
+        self._sig = self._plan = self._sets = self._set_key = self._scratch = None
+
+    # ------------------------------------------------------------------ state
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        self._check(self.param_groups[-1])
+        self._reset()
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for name in ("process_group", "after_group", "before_group"):
+            self.__dict__.setdefault(name, None)
+        self.__dict__.setdefault("_sharded", False)
+        for group in self.param_groups:
+            for name, value in self.defaults.items():   # a checkpoint of torch.optim.AdamW has no entry of some names
+                group.setdefault(name, value)
+            self._check(group)
+        for p, st in self.state.items():
+            for name, value in st.items():
+                if isinstance(value, _Kept):
+                    st[name] = value.value.detach().to(p.device if name != "step" else value.value.device, copy=True)
+        self._reset()
+
+    def load_state_dict(self, state_dict):
+        """As ``Optimizer.load_state_dict``, but every state tensor keeps its type (the base class gives it the parameter's).
+
+        States of 32 bits load into the class of 8, rounded to nearest, and the other way round."""
+        state_dict = state_dict.copy()
+        hooks = self._optimizer_load_state_dict_pre_hooks
+        for hook in hooks.values():
+            changed = hook(self, state_dict)
+            if changed is not None:
+                state_dict = changed
+        keep = lambda v: _Kept(v) if torch.is_tensor(v) else v
+        state_dict["state"] = {k: {n: keep(v) for n, v in st.items()} if isinstance(st, dict) else st for k, st in state_dict["state"].items()}
+        self._optimizer_load_state_dict_pre_hooks = OrderedDict()
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            self._optimizer_load_state_dict_pre_hooks = hooks
+
+    def _init_state(self, p, st, group):
+        """Make what a parameter's state lacks, and bring what it has into the form the kernels take."""
+        dev, n = p.device, p.numel()
+        capturable = group["capturable"]
+        step = st.get("step", 0.0)
+        if not torch.is_tensor(step) or step.is_cuda != bool(capturable) or step.dim() != 0 or not step.dtype.is_floating_point:
+            step = torch.tensor(float(step), dtype=torch.float32 if capturable else torch.float64, device=dev if capturable else "cpu")
+        if capturable:
+            step = step.to(device=dev, dtype=torch.float32)
+        st["step"] = step
+        if self._bits == 32:
+            if "exp_avg_sq_root" in st:
+                st["exp_avg_sq"] = from_blocks(st.pop("exp_avg_sq_root"), st.pop("exp_avg_sq_root_scale")).square_()
+                st["exp_avg"] = from_blocks(st["exp_avg"], st.pop("exp_avg_scale"))
+            wanted = {"exp_avg": (torch.float32, p.shape), "exp_avg_sq": (torch.float32, p.shape)}
+        else:
+            if "exp_avg_sq" in st:
+                st["exp_avg_sq_root"], st["exp_avg_sq_root_scale"] = to_blocks(st.pop("exp_avg_sq").to(torch.float32).sqrt())
+                st["exp_avg"], st["exp_avg_scale"] = to_blocks(st["exp_avg"])
+            each = (blocks_of(n),)
+            wanted = {"exp_avg": (_CODES, p.shape), "exp_avg_scale": (_SCALES, each),
+                      "exp_avg_sq_root": (_CODES, p.shape), "exp_avg_sq_root_scale": (_SCALES, each)}
+        if group["master_weights"] and p.dtype is not torch.float32:
+            wanted["master"] = (torch.float32, p.shape)
+            if "master" not in st:
+                st["master"] = p.detach().to(torch.float32).contiguous()
+        else:
+            st.pop("master", None)
+        for name, (dtype, shape) in wanted.items():
+            x = st.get(name)
+            if x is None:
+                zero = 1 if dtype is _SCALES else 0   # the least scale there is
+                x = torch.full(shape, zero, dtype=torch.uint8, device=dev).view(dtype) if dtype.itemsize == 1 else torch.zeros(shape, dtype=dtype, device=dev)
+            if tuple(x.shape) != tuple(shape):
+                raise ValueError(f"{self._name}: state {name!r} has shape {tuple(x.shape)}, the parameter's needs {tuple(shape)}")
+            if x.dtype is not dtype and (dtype.itemsize == 1 or not x.dtype.is_floating_point):
+                raise ValueError(f"{self._name}: state {name!r} is {x.dtype}, not {dtype}")
+            st[name] = x.to(device=dev, dtype=dtype).contiguous()
+
+    def _build(self, plist, group_of, capturing):
+        dev = plist[0].device
+        for p in plist:
+            if not p.is_cuda:
+                raise RuntimeError(f"{self._name}: parameters must live on a CUDA device (there is no CPU path)")
+            if p.dtype not in TYPES:
+                raise RuntimeError(f"{self._name}: parameters must be fp32, bf16 or fp16, got {p.dtype}")
+            if not p.is_contiguous():
+                raise RuntimeError(f"{self._name}: parameters must be contiguous")
+            if p.device != dev:
+                raise RuntimeError(f"{self._name}: all parameters must live on one device, got {dev} and {p.device}")
+            if getattr(p, "_pylo_peer_ptrs", None):
+                raise RuntimeError(f"{self._name}: writes no other rank's copy of a parameter; use ShardedStep or StagedShardedStep, or push='copies'")
+        at = np.array([p.data_ptr() for p in plist if p.numel()], dtype=np.uint64)
+        end = at + np.array([p.numel() * p.element_size() for p in plist if p.numel()], dtype=np.uint64)
+        order = np.argsort(at)
+        if len(at) and np.any(at[order][1:] < end[order][:-1]):
+            raise ValueError(f"{self._name}: two parameters share memory")
+        states = [self.state[p] for p in plist]
+        if capturing and not all([len(st) for st in states]):
+            raise RuntimeError(f"{self._name}: run a step before the one that is captured: a captured step would make its states anew on every replay")
+        for p, st, gi in zip(plist, states, group_of):
+            self._init_state(p, st, self.param_groups[gi])
+        return _Plan(plist, group_of, states, self._bits)
+
+    # ------------------------------------------------------------------ step
+    @optimizer_step
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        groups = self.param_groups
+        if self.before_group is not None:
+            for gi in range(len(groups)):
+                self.before_group(gi)
+        plist, grads, group_of = [], [], []
+        for gi, group in enumerate(groups):
+            ps, gs = with_gradients(group["params"])
+            plist += ps
+            grads += gs
+            group_of += [gi] * len(ps)
+        clip = any([g["clip_grad"] for g in groups])
+        if plist or clip:
+            device = plist[0].device if plist else torch.device("cuda", torch.cuda.current_device())
+            if device.type == "cuda" and device.index != torch.cuda.current_device():
+                with torch.cuda.device(device):
+                    self._run(plist, grads, group_of, clip, device)
+            else:
+                self._run(plist, grads, group_of, clip, device)
+        if self.after_group is not None:
+            for gi in range(len(groups)):
+                self.after_group(gi)
+        return loss
+
+    def _run(self, plist, grads, group_of, clip, device):
+        capturing = torch.cuda.is_current_stream_capturing()
+        groups = self.param_groups
+        if capturing and not all([g["capturable"] for g in groups]):
+            raise RuntimeError(f"{self._name}: a step can be captured into a graph only with capturable=True")
+        plan = self._plan
+        sig = [(p.data_ptr(), p.numel(), p.dtype) for p in plist]
+        flags = [(g["capturable"], g["master_weights"]) for g in groups]
+        if plan is None or (sig, group_of, flags) != self._sig or not all([st.get("exp_avg") is m for st, m in zip(plan.states, plan.moments)]):
+            plan = self._plan = self._build(plist, group_of, capturing) if plist else None
+            self._sig = (sig, group_of, flags)
+            self._scratch = None
+        stream = current_stream_ptr()
+        copies = plan.look_at(grads) if plan else ()
+        norm = None
+        if clip:
+            norm = self._grad_norm(plan, device, stream, capturing)
+        if plan is None:
+            return
+        sets = self._fill_sets(plan)
+        L.check(L.lib.pylo_b200_adamw_step(plan.address, len(plist), sets, len(sets), self._bits, norm, stream), "adamw_step")
+        if plan.device_steps:
+            L.check(L.lib.pylo_b200_adamw_advance(plan.device_steps, len(plan.device_steps), stream), "adamw_advance")
+        del copies
+
+    def _grad_norm(self, plan, device, stream, capturing):
+        """Address of the sum of squares of all gradients (of all ranks)."""
+        n = len(plan.grads) if plan else 0
+        table = plan.grads.ctypes.data if plan else None
+        out = self._scratch
+        if out is None or capturing or out.device != device:   # a captured step has a buffer of its own, from the graph's memory
+            floats = L.lib.pylo_b200_grad_norm_scratch(table, n)
+            out = torch.empty(2 + max(floats, 0), dtype=torch.float32, device=device)
+            if not capturing:
+                self._scratch = out
+        at = out.data_ptr()
+        L.check(L.lib.pylo_b200_grad_norm(table, n, at + 8, at, stream), "grad_norm")
+        if self.process_group is not None or (torch.distributed.is_initialized() and self._sharded):
+            torch.distributed.all_reduce(out[:1], group=self.process_group)  # each rank holds its own tensors' share
+        return at
+
+    def _fill_sets(self, plan):
+        """The hyper-parameters of the step: a set per group, or per group and count of steps where a group's tensors differ in it."""
+        key = [(g["lr"] if torch.is_tensor(g["lr"]) else float(g["lr"]), g["betas"], g["eps"], g["weight_decay"],
+                g["clip_norm"] if g["clip_grad"] else 0.0, g["maximize"], g.get("seed", 0)) for g in self.param_groups]
+        old = plan.counters.advance() if plan.host else 0.0
+        if isinstance(old, float):
+            if not plan.one_step:
+                plan.table["set"], plan.one_step, self._set_key = plan.group_of, True, None
+            pairs = [(gi, old + 1) for gi in range(len(key))]
+        else:
+            steps = dict(zip(plan.host, old))
+            of = [(gi, steps.get(i, 0.0) + 1) for i, gi in enumerate(plan.group_of)]
+            pairs = sorted(set(of))
+            index = {pair: k for k, pair in enumerate(pairs)}
+            plan.table["set"], plan.one_step, self._set_key = [index[pair] for pair in of], False, None
+        sets = self._sets
+        if self._set_key is None or any([torch.is_tensor(k[0]) for k in key]) or self._set_key != key:
+            sets = self._sets = (L.AdamwSet * len(pairs))()
+            for s, (gi, _) in zip(sets, pairs):
+                lr, (b1, b2), eps, wd, clip_norm, maximize, seed = key[gi]
+                if torch.is_tensor(lr) and lr.is_cuda and self.param_groups[gi]["capturable"]:
+                    if lr.dtype is not torch.float32 or lr.numel() != 1 or lr.device != plan.device:
+                        raise ValueError(f"{self._name}: lr on the device must be one fp32 value on {plan.device}")
+                    s.lr_dev, lr = lr.data_ptr(), 0.0
+                s.lr, s.weight_decay, s.beta1, s.beta2, s.eps, s.clip_norm = float(lr), wd, b1, b2, eps, clip_norm
+                s.maximize, s.seed = bool(maximize), seed & 0xFFFFFFFF
+            self._set_key = key
+        for s, (_, step) in zip(sets, pairs):
+            s.step = int(step)
+        return sets
+
+
+class AdamW_CUDA(_AdamWFamily):
+    """AdamW with fp32 moments.
+
+    ``master_weights``: the state of a bf16 or fp16 parameter holds an fp32 copy (``master``), made from it in its first step,
+    which the steps update; the parameter is its rounded value.  ``clip_grad``, ``clip_norm``: gradients are scaled by
+    ``clip_norm / max(norm, clip_norm)`` within the step, with the norm over the gradients of all groups (they are left as
+    they are in memory).  ``capturable``: the step count lives on the device, as may ``lr``, and a step can be captured into a graph."""
+
+    _name = "AdamW_CUDA"
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, maximize=False, master_weights=False,
+                 clip_grad=False, clip_norm=1.0, capturable=False):
+        self._setup(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize, master_weights=master_weights,
+                    clip_grad=clip_grad, clip_norm=clip_norm, capturable=capturable)
+
+
+class AdamW8bit_CUDA(_AdamWFamily):
+    """AdamW with moments in 8 bits: 2 bytes and a sixty-fourth per parameter.
+
+    The first moment (``exp_avg``) and the root of the second (``exp_avg_sq_root``) are ``float8_e4m3fn`` codes; 256 elements of
+    a tensor share a power of two (``exp_avg_scale``, ``exp_avg_sq_root_scale``, ``float8_e8m0fnu``); a value is code times scale.
+    Codes are rounded up or down at random, so that they are right on the average: the same ``seed``, step and gradients give the same
+    codes, however the tensors are grouped or split over ranks.  Other arguments as :class:`AdamW_CUDA`."""
+
+    _name = "AdamW8bit_CUDA"
+    _bits = 8
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, maximize=False, master_weights=False,
+                 clip_grad=False, clip_norm=1.0, capturable=False, seed=0):
+        self._setup(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize, master_weights=master_weights,
+                    clip_grad=clip_grad, clip_norm=clip_norm, capturable=capturable, seed=int(seed))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# clipping by the global norm
+# ---------------------------------------------------------------------------------------------------------------------
+def _dense(g: torch.Tensor) -> bool:
+    """Whether the elements of a tensor are one run of memory, in whatever order."""
+    step = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(g.stride(), g.shape) if sz != 1):
+        if stride != step:
+            return False
+        step *= size
+    return True
+
+
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Scale the gradients of ``parameters`` in place by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` the 2-norm of all of them
+    together; returns ``norm`` (fp32, on the device), as ``torch.nn.utils.clip_grad_norm_`` does.
+
+    Gradients may be fp32, bf16 and fp16, mixed; the norm is summed up in fp32 and more whatever their type.  One that is given twice
+    counts and is scaled once.  Three launches and no synchronisation (``error_if_nonfinite`` waits for the norm); the gradients are
+    written only where the norm exceeds ``max_norm``, and not read again for ``max_norm = inf``."""
+    if float(norm_type) != 2.0:
+        raise ValueError(f"clip_grad_norm_: only the 2-norm is supported, got norm_type={norm_type}")
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"clip_grad_norm_: invalid max_norm: {max_norm}")
+    grads = [g for g in [p.grad for p in ([parameters] if torch.is_tensor(parameters) else parameters)] if g is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    device = grads[0].device
+    if device.type != "cuda":
+        raise RuntimeError("clip_grad_norm_: gradients must live on a CUDA device (there is no CPU path)")
+    for g in grads:
+        if g.device != device:
+            raise RuntimeError(f"clip_grad_norm_: all gradients must live on one device, got {device} and {g.device}")
+        if g.layout is not torch.strided:
+            raise RuntimeError("Sparse gradients not supported")
+        if g.dtype not in TYPES:
+            raise RuntimeError(f"clip_grad_norm_: gradients must be fp32, bf16 or fp16, got {g.dtype}")
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _clip(grads, max_norm, error_if_nonfinite, device)
+    return _clip(grads, max_norm, error_if_nonfinite, device)
+
+
+def _clip(grads, max_norm, error_if_nonfinite, device):
+    if not all([g.is_contiguous() for g in grads]):
+        with torch.no_grad():
+            parts = [g.detach() if g.is_contiguous() or _dense(g) else g.detach().contiguous() for g in grads]
+    else:
+        parts = grads
+    table = np.zeros(len(parts), dtype=L.GRAD_DTYPE)
+    table["g"] = [g.data_ptr() for g in parts]
+    table["n"] = [g.numel() for g in parts]
+    table["type"] = [TYPES[g.dtype] for g in parts]
+    if len(parts) > 1:
+        table = _distinct(table)
+    stream, at, n = current_stream_ptr(), table.ctypes.data, len(table)
+    floats = L.lib.pylo_b200_grad_norm_scratch(at, n)
+    out = torch.empty(2 + max(floats, 0), dtype=torch.float32, device=device)
+    total = out[1]
+    L.check(L.lib.pylo_b200_grad_norm(at, n, out.data_ptr() + 8, out.data_ptr(), stream), "grad_norm")
+    if error_if_nonfinite and not math.isfinite(float(total)):
+        raise RuntimeError("The total norm of order 2.0 for gradients from `parameters` is non-finite, so it cannot be clipped. To disable this "
+                           "error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
+    if max_norm < math.inf:
+        L.check(L.lib.pylo_b200_grad_scale(at, n, total.data_ptr(), max_norm, stream), "grad_scale")
+        if parts is not grads:
+            with torch.no_grad():
+                for g, part in zip(grads, parts):
+                    if part.data_ptr() != g.data_ptr():
+                        g.copy_(part)
+    return total
+
+
+def _distinct(table):
+    """The table with every gradient once; two that share only a part of their memory are refused."""
+    size = np.array([4, 2, 2], dtype=np.uint64)
+    order = np.argsort(table["g"], kind="stable")
+    g, end = table["g"][order], (table["g"] + table["n"].astype(np.uint64) * size[table["type"]])[order]
+    over = g[1:] < end[:-1]
+    if not over.any():
+        return table
+    twice = (g[1:] == g[:-1]) & (end[1:] == end[:-1])
+    if (over & ~twice).any():
+        raise ValueError("clip_grad_norm_: two gradients share a part of their memory")
+    return np.ascontiguousarray(table[np.sort(order[np.concatenate([[True], ~twice])])])
