@@ -2690,7 +2690,7 @@ template <class P, class G, bool MASTER>
 static int aw_kind(const pylo_adamw_item* items, const int* picked, int n, const pylo_adamw_set* sets, int bits, const float* gnorm_sq, int64_t total,
                    cudaStream_t s) {
   if (bits == 8) {
-    const int tile = aw_tile(total, NWARP * AW_BLOCK, 4 * NWARP * AW_BLOCK, 8);
+    const int tile = aw_tile(total, NWARP * AW_BLOCK, 8 * NWARP * AW_BLOCK, 8);
     if (n <= AW_FEW) return aw_launch<AwItem8, AW_FEW>(k_adamw_8<P, G, MASTER, AW_FEW>, items, picked, n, sets, gnorm_sq, tile, s);
     return aw_launch<AwItem8, AW_MANY_8>(k_adamw_8<P, G, MASTER, AW_MANY_8>, items, picked, n, sets, gnorm_sq, tile, s);
   }
