@@ -515,7 +515,7 @@ int pylo_b200_advance_steps(double* const* steps, int n, double* first, int* equ
 
 /* ---- AdamW over many tensors at once, and the global norm of many gradients ---------------------------------------------
  * For parameters and gradients of any of three types.  Items and sets are HOST arrays: they are copied into the launches (one per
- * combination of types and 350 to 1500 tensors), so nothing has to outlive the call and a captured launch keeps what it was given. */
+ * combination of types and 180 to 800 tensors), so nothing has to outlive the call and a captured launch keeps what it was given. */
 #define PYLO_FP32 0
 #define PYLO_BF16 1
 #define PYLO_FP16 2

@@ -9,8 +9,8 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(os.path.dirname(PKG_DIR), "include")
 LIB_PATH = os.path.join(CSRC, "libpylo_b200.so")
 LOCK_PATH = os.path.join(CSRC, ".build.lock")
-SOURCES = [os.path.join(CSRC, "pylo_kernels.cu")]
-HEADERS = [os.path.join(CSRC, "pylo_common.cuh"), os.path.join(CSRC, "pylo_pipe.cuh"), os.path.join(CSRC, "pylo_small_front.cuh"), os.path.join(CSRC, "pylo_apply_tc.cuh"), os.path.join(CSRC, "pylo_ns_gemm.cuh"), os.path.join(CSRC, "pylo_ns_f16.cuh"), os.path.join(CSRC, "pylo_ns_cluster.cuh"), os.path.join(CSRC, "pylo_adamw.cuh"), os.path.join(INCLUDE, "pylo_b200.h")]
+SOURCES = [os.path.join(CSRC, "pylo_kernels.cu"), os.path.join(CSRC, "pylo_adamw.cu")]
+HEADERS = [os.path.join(CSRC, "pylo_common.cuh"), os.path.join(CSRC, "pylo_pipe.cuh"), os.path.join(CSRC, "pylo_small_front.cuh"), os.path.join(CSRC, "pylo_apply_tc.cuh"), os.path.join(CSRC, "pylo_ns_gemm.cuh"), os.path.join(CSRC, "pylo_ns_f16.cuh"), os.path.join(CSRC, "pylo_ns_cluster.cuh"), os.path.join(CSRC, "pylo_launch.cuh"), os.path.join(INCLUDE, "pylo_b200.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -53,17 +53,25 @@ def build(force=False, verbose=False):
             # clocks of the tensor-core apply kernel)
             extra = os.environ.get("PYLO_B200_NVCC_FLAGS", "").split()
             tmp = f"{LIB_PATH}.tmp.{os.getpid()}"
-            cmd = [nvcc] + NVCC_FLAGS + extra + ["-I", INCLUDE, "-I", CSRC, "-o", tmp] + SOURCES
+            objects = [f"{tmp}.{os.path.basename(src)}.o" for src in SOURCES]
+            command = [nvcc] + NVCC_FLAGS + extra + ["-I", INCLUDE, "-I", CSRC] + (["-Xptxas=-v"] if verbose else [])
+            try:
+                # the sources side by side, then the library
+                runs = [subprocess.Popen(command + ["-c", "-o", obj, src], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+                        for src, obj in zip(SOURCES, objects)]
+                said = [run.communicate()[0] for run in runs]
+                if not any(run.returncode for run in runs):
+                    link = subprocess.run([nvcc] + NVCC_FLAGS + ["-o", tmp] + objects, capture_output=True, text=True)
+                    runs, said = runs + [link], said + [link.stdout + link.stderr]
+                if any(run.returncode for run in runs):
+                    raise RuntimeError("nvcc failed:\n" + "".join(said))
+                os.replace(tmp, LIB_PATH)
+            finally:
+                for path in objects + [tmp]:
+                    if os.path.exists(path):
+                        os.remove(path)
             if verbose:
-                cmd.insert(1, "-Xptxas=-v")
-            res = subprocess.run(cmd, capture_output=True, text=True)
-            if res.returncode != 0:
-                if os.path.exists(tmp):
-                    os.remove(tmp)
-                raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
-            os.replace(tmp, LIB_PATH)
-            if verbose:
-                print(res.stderr)
+                print("".join(said))
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)
     return LIB_PATH

@@ -8,13 +8,13 @@
 // All reductions go through fixed-slot partials and fixed-order final sums, so
 // results are bit-reproducible from run to run (no floating-point atomics).
 
-#include <math.h>
 #include <stddef.h>
 #include <string.h>
 
 #include <mutex>
 
 #include "pylo_common.cuh"
+#include "pylo_launch.cuh"
 #include "pylo_pipe.cuh"
 
 // ================================================================================================
@@ -1623,7 +1623,6 @@ __global__ void __launch_bounds__(NT, CC_CTAS_PER_SM) k_apply_adafac_cols(const 
 #include "pylo_ns_gemm.cuh"
 #include "pylo_ns_f16.cuh"
 #include "pylo_ns_cluster.cuh"
-#include "pylo_adamw.cuh"
 
 // ================================================================================================
 // Phase C for CELO2 / ELO_CELO2 / VeLO on FAST2D tensors: packed kernel.
@@ -2535,70 +2534,6 @@ __global__ void __launch_bounds__(MIX_OUT * MIX_GROUPS) k_velo_mix(const pylo_ve
 // ================================================================================================
 // C ABI
 // ================================================================================================
-// Opt-in limits and caches are kept per device: the library may be used on every GPU of a box from one process.
-#define PYLO_MAX_DEVICES 64
-static int g_sm_count[PYLO_MAX_DEVICES] = {0};
-static int sm_count() {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= PYLO_MAX_DEVICES) return 148;
-  if (g_sm_count[dev] == 0) {
-    int n = 0;
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    g_sm_count[dev] = n > 0 ? n : 148;
-  }
-  return g_sm_count[dev];
-}
-static int grid_for(int n_items, int ctas_per_sm) {
-  const int cap = sm_count() * ctas_per_sm;
-  return n_items < cap ? n_items : cap;
-}
-static int launch_status() { return (int)cudaGetLastError(); }
-
-// Every kernel of this library is launched so that it may become resident while its predecessor in the stream drains
-// (programmatic dependent launch) and waits in pdl_begin() until that one is complete.  A step is a chain of small launches;
-// on a small model the gaps between them are as long as the kernels (AdafacLO over a 118 K MLP: 47.5 -> 38.8 us per step).
-// On large ones there is nothing to gain (GPT-2-medium shapes: 0.7 % slower with it), so a step of more than 134 M elements
-// launches plainly: PlainLaunches says so for the calls of one scope on one host thread.
-static thread_local bool t_plain_launches = false;
-struct PlainLaunches {
-  bool before;
-  explicit PlainLaunches(int n_tiles) : before(t_plain_launches) { t_plain_launches = before || n_tiles > 8192; }
-  ~PlainLaunches() { t_plain_launches = before; }
-};
-// The SMs' memory is split between L1 cache and shared memory anew only when they are idle, which programmatic launches never
-// let them be: the kernels after one with a large share of shared memory would run with what L1 it left (the apply sweep of
-// 6 x 4096 x 4096 VeLO parameters: 921 us after the state sweep's ring, 755 us without).  Such a kernel has itself and the next
-// launch of its thread made plainly.
-static thread_local bool t_plain_next = false;
-template <class... P, class... A>
-static void launch_clusters(void (*kernel)(P...), dim3 grid, dim3 block, int cluster, size_t smem, cudaStream_t stream, A&&... args) {
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (!t_plain_launches && !t_plain_next) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n++].val.programmaticStreamSerializationAllowed = 1;
-  }
-  t_plain_next = false;
-  if (cluster >= 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = cluster;
-    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-}
-template <class... P, class... A>
-static void launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
-  launch_clusters(kernel, grid, block, 0, smem, stream, static_cast<A&&>(args)...);
-}
-
 // Opt a kernel in to more than 48 KB of dynamic shared memory, once per device (the attribute belongs to the
 // device's copy of the function); flags[] is the caller's per-kernel record.
 template <class K>
@@ -2625,127 +2560,6 @@ static int allow_wide_clusters(K kernel, bool (&flags)[PYLO_MAX_DEVICES]) {
   if (dev >= 0 && dev < PYLO_MAX_DEVICES) flags[dev] = true;
   return 0;
 }
-
-// ------------------------------------------------------------------------------------------------
-// AdamW and gradient norms: launches whose arguments hold the tensors
-// ------------------------------------------------------------------------------------------------
-static AwSet aw_set(const pylo_adamw_set& s) {
-  AwSet q;
-  const double t = (double)s.step, bc1 = 1.0 - pow(s.beta1, t), bc2 = 1.0 - pow(s.beta2, t);
-  q.lr_dev = s.lr_dev;
-  q.lr = (float)s.lr; q.wd = (float)s.weight_decay; q.eps = (float)s.eps;
-  q.beta1 = (float)s.beta1; q.omb1 = (float)(1.0 - s.beta1); q.beta2 = (float)s.beta2; q.omb2 = (float)(1.0 - s.beta2);
-  q.ln_beta1 = (float)log(s.beta1); q.ln_beta2 = (float)log(s.beta2);
-  q.clip_norm = (float)s.clip_norm;
-  q.sign = s.maximize ? -1.f : 1.f;
-  q.decay = (float)(1.0 - s.lr * s.weight_decay);
-  q.step_size = (float)(s.lr / bc1);
-  q.inv_sqrt_bc2 = (float)(1.0 / sqrt(bc2));
-  q.seed = (uint32_t)s.seed;
-  q.step = (uint32_t)s.step;
-  return q;
-}
-static AwItem32 aw_of(const pylo_adamw_item& i, AwItem32) { return {i.p, i.g, i.master, (float*)i.m, (float*)i.v, i.step, i.n, 0, 0}; }
-static AwItem8 aw_of(const pylo_adamw_item& i, AwItem8) {
-  return {i.p, i.g, i.master, (uint8_t*)i.m, (uint8_t*)i.v, i.m_scale, i.v_scale, i.step, i.n, 0, 0};
-}
-
-// Elements per tile: the largest power of two from `least` to `most` that gives every SM `per_sm` tiles.
-static int aw_tile(int64_t total, int least, int most, int per_sm) {
-  int e = most;
-  while (e > least && total < (int64_t)e * per_sm * sm_count()) e >>= 1;
-  return e;
-}
-
-// One launch of the items picked[0 .. n): all of one kind.
-template <class Item, int MOST, class Kernel>
-static int aw_launch(Kernel kernel, const pylo_adamw_item* items, const int* picked, int n, const pylo_adamw_set* sets, const float* gnorm_sq, int tile,
-                     cudaStream_t s) {
-  AwArgs<Item, MOST> a;
-  static_assert(sizeof(a) <= 32764, "arguments of a launch");
-  int n_sets = 0, of[AW_SETS];
-  int64_t tiles = 0;
-  a.gnorm_sq = gnorm_sq;
-  a.n_items = n;
-  a.tile = tile;
-  for (int k = 0; k < n; ++k) {
-    const pylo_adamw_item& it = items[picked[k]];
-    int j = 0;
-    while (j < n_sets && of[j] != it.set) ++j;
-    if (j == n_sets) {
-      of[n_sets++] = it.set;
-      a.set[j] = aw_set(sets[it.set]);
-    }
-    a.item[k] = aw_of(it, Item());
-    a.item[k].first = (int)tiles;
-    a.item[k].set = j;
-    tiles += (it.n + tile - 1) / tile;
-  }
-  if (tiles > 0x7fffffff) return -1;
-  launch(kernel, dim3((unsigned)tiles), NT, 0, s, a);
-  return launch_status();
-}
-
-template <class P, class G, bool MASTER>
-static int aw_kind(const pylo_adamw_item* items, const int* picked, int n, const pylo_adamw_set* sets, int bits, const float* gnorm_sq, int64_t total,
-                   cudaStream_t s) {
-  if (bits == 8) {
-    const int tile = aw_tile(total, NWARP * AW_BLOCK, 8 * NWARP * AW_BLOCK, 8);
-    if (n <= AW_FEW) return aw_launch<AwItem8, AW_FEW>(k_adamw_8<P, G, MASTER, AW_FEW>, items, picked, n, sets, gnorm_sq, tile, s);
-    return aw_launch<AwItem8, AW_MANY_8>(k_adamw_8<P, G, MASTER, AW_MANY_8>, items, picked, n, sets, gnorm_sq, tile, s);
-  }
-  const int tile = aw_tile(total, 1024, 8192, 8);
-  if (n <= AW_FEW) return aw_launch<AwItem32, AW_FEW>(k_adamw_32<P, G, MASTER, AW_FEW>, items, picked, n, sets, gnorm_sq, tile, s);
-  return aw_launch<AwItem32, AW_MANY_32>(k_adamw_32<P, G, MASTER, AW_MANY_32>, items, picked, n, sets, gnorm_sq, tile, s);
-}
-
-// The types that go together: p's own gradients, and fp32 ones for all; a copy in fp32 beside parameters of 16 bits.
-template <class... A>
-static int aw_types(int p, int g, bool master, A... args) {
-  using bf16 = __nv_bfloat16;
-  if (p == PYLO_FP32 && !master)
-    return g == PYLO_FP32 ? aw_kind<float, float, false>(args...) : g == PYLO_BF16 ? aw_kind<float, bf16, false>(args...) : g == PYLO_FP16 ? aw_kind<float, __half, false>(args...) : -2;
-  if (p == PYLO_BF16 && g == PYLO_BF16) return master ? aw_kind<bf16, bf16, true>(args...) : aw_kind<bf16, bf16, false>(args...);
-  if (p == PYLO_BF16 && g == PYLO_FP32) return master ? aw_kind<bf16, float, true>(args...) : aw_kind<bf16, float, false>(args...);
-  if (p == PYLO_FP16 && g == PYLO_FP16) return master ? aw_kind<__half, __half, true>(args...) : aw_kind<__half, __half, false>(args...);
-  if (p == PYLO_FP16 && g == PYLO_FP32) return master ? aw_kind<__half, float, true>(args...) : aw_kind<__half, float, false>(args...);
-  return -2;
-}
-
-// Launches over gradients of one type after the other; kernel(first partial, args) starts one.
-#define AW_GRAD_TILE 16384
-static int aw_grad_tile(const pylo_grad_item* items, int n) {
-  int64_t total = 0;
-  for (int i = 0; i < n; ++i) total += items[i].n;
-  return aw_tile(total, 2048, AW_GRAD_TILE, 8);
-}
-template <int MOST, class Kernel>
-static int aw_grads(const pylo_grad_item* items, int n, int type, int tile, int64_t& first, Kernel&& kernel) {
-  AwGradArgs<MOST> a;
-  static_assert(sizeof(a) <= 32764 - 64, "arguments of a launch");
-  for (int i = 0; i < n;) {
-    int64_t tiles = 0;
-    a.n_items = 0;
-    a.tile = tile;
-    for (; i < n && a.n_items < MOST; ++i) {
-      const int64_t more = (items[i].n + tile - 1) / tile;
-      if (items[i].type != type || more == 0) continue;
-      if (tiles + more > 0x7fffffff) break;
-      a.item[a.n_items] = {items[i].g, items[i].n};
-      a.first[a.n_items++] = (int)tiles;
-      tiles += more;
-    }
-    if (!a.n_items) break;
-    kernel(a, (unsigned)tiles, first);
-    first += tiles;
-  }
-  return launch_status();
-}
-
-#define CHECK_ARG(cond) \
-  do {                  \
-    if (!(cond)) return -1; \
-  } while (0)
 
 template <int BM, int BN>
 static long long ns_deal(nf_group& grp) {
@@ -3588,120 +3402,6 @@ int pylo_b200_advance_steps(double* const* steps, int n, double* first, int* equ
     *steps[i] += 1.0;
   }
   return 0;
-}
-
-// ------------------------------------------------------------------------------------------------
-// AdamW over many tensors, the global norm of many gradients
-// ------------------------------------------------------------------------------------------------
-int pylo_b200_sizeof_adamw_item(void) { return (int)sizeof(pylo_adamw_item); }
-
-int pylo_b200_adamw_step(const pylo_adamw_item* items, int n_items, const pylo_adamw_set* sets, int n_sets, int bits, const float* gnorm_sq, void* stream) {
-  CHECK_ARG(n_items >= 0 && n_sets >= 0 && (items || !n_items) && (sets || !n_sets) && (bits == 32 || bits == 8));
-  for (int i = 0; i < n_sets; ++i) {
-    const pylo_adamw_set& s = sets[i];
-    CHECK_ARG(s.beta1 >= 0 && s.beta1 < 1 && s.beta2 >= 0 && s.beta2 < 1 && s.eps >= 0 && s.step >= 1 && s.clip_norm >= 0);
-  }
-  int64_t total = 0;
-  for (int i = 0; i < n_items; ++i) {
-    const pylo_adamw_item& it = items[i];
-    CHECK_ARG(it.n >= 0 && it.n <= ((int64_t)1 << 34) && it.set >= 0 && it.set < n_sets);
-    CHECK_ARG(it.p_type >= 0 && it.p_type <= 2 && it.g_type >= 0 && it.g_type <= 2 && (it.g_type == it.p_type || it.g_type == PYLO_FP32 || it.p_type == PYLO_FP32));
-    CHECK_ARG(!it.n || (it.p && it.g && it.m && it.v && (bits == 32 || (it.m_scale && it.v_scale)) && (it.p_type != PYLO_FP32 || !it.master)));
-    total += it.n;
-  }
-  const PlainLaunches plain((int)(total >> 14 < 1 << 20 ? total >> 14 : 1 << 20));
-  const int most = bits == 8 ? AW_MANY_8 : AW_MANY_32;
-  static_assert(AW_MANY_8 <= AW_MANY_32, "picked");
-  int picked[AW_MANY_32];
-  for (int kind = 0; kind < 18; ++kind) {
-    const int p = kind % 3, g = kind / 3 % 3;
-    const bool master = kind >= 9;
-    for (int i = 0; i < n_items;) {
-      int n = 0, used = 0, of[AW_SETS];
-      for (; i < n_items && n < most; ++i) {
-        const pylo_adamw_item& it = items[i];
-        if (it.p_type != p || it.g_type != g || (it.master != nullptr) != master || !it.n) continue;
-        int j = 0;
-        while (j < used && of[j] != it.set) ++j;
-        if (j == AW_SETS) break;
-        if (j == used) of[used++] = it.set;
-        picked[n++] = i;
-      }
-      if (!n) break;
-      if (int rc = aw_types(p, g, master, items, picked, n, sets, bits, gnorm_sq, total, (cudaStream_t)stream)) return rc;
-    }
-  }
-  return 0;
-}
-
-int pylo_b200_adamw_advance(float* const* steps, int n, void* stream) {
-  CHECK_ARG(n >= 0 && (steps || !n));
-  constexpr int MOST = sizeof(AwCounters) / sizeof(float*);
-  for (int i = 0; i < n; i += MOST) {
-    AwCounters a;
-    const int k = n - i < MOST ? n - i : MOST;
-    memcpy(a.step, steps + i, k * sizeof(float*));
-    launch(k_adamw_advance, 1, NT, 0, (cudaStream_t)stream, a, k);
-  }
-  return launch_status();
-}
-
-int64_t pylo_b200_grad_norm_scratch(const pylo_grad_item* items, int n_items) {
-  if (n_items < 0 || (!items && n_items)) return -1;
-  const int tile = aw_grad_tile(items, n_items);
-  int64_t tiles = 0;
-  for (int i = 0; i < n_items; ++i) {
-    if (items[i].n < 0) return -1;
-    tiles += (items[i].n + tile - 1) / tile;
-  }
-  return tiles <= 0x7fffffff ? tiles : -1;
-}
-
-int pylo_b200_grad_norm(const pylo_grad_item* items, int n_items, float* scratch, float* out, void* stream) {
-  CHECK_ARG(n_items >= 0 && (items || !n_items) && out);
-  for (int i = 0; i < n_items; ++i) CHECK_ARG(items[i].n >= 0 && items[i].type >= 0 && items[i].type <= 2 && (items[i].g || !items[i].n));
-  const int64_t partials = pylo_b200_grad_norm_scratch(items, n_items);
-  CHECK_ARG(partials >= 0 && (scratch || !partials));
-  cudaStream_t s = (cudaStream_t)stream;
-  const int tile = aw_grad_tile(items, n_items);
-  const PlainLaunches plain(tile == AW_GRAD_TILE ? (int)partials : 0);
-  int64_t first = 0;
-  auto all = [&](auto kernel32, auto kernel_bf, auto kernel_h, auto most) {
-    constexpr int MOST = decltype(most)::value;
-    for (int type = 0; type < 3; ++type) {
-      const auto kernel = type == PYLO_FP32 ? kernel32 : type == PYLO_BF16 ? kernel_bf : kernel_h;
-      if (int rc = aw_grads<MOST>(items, n_items, type, tile, first,
-                                  [&](const AwGradArgs<MOST>& a, unsigned tiles, int64_t at) { launch(kernel, dim3(tiles), NT, 0, s, a, scratch + at); }))
-        return rc;
-    }
-    return 0;
-  };
-  int rc = n_items <= AW_FEW ? all(k_grad_norm<float, AW_FEW>, k_grad_norm<__nv_bfloat16, AW_FEW>, k_grad_norm<__half, AW_FEW>, std::integral_constant<int, AW_FEW>{})
-                             : all(k_grad_norm<float, AW_MANY_G>, k_grad_norm<__nv_bfloat16, AW_MANY_G>, k_grad_norm<__half, AW_MANY_G>, std::integral_constant<int, AW_MANY_G>{});
-  if (rc) return rc;
-  launch(k_grad_norm_final, 1, 1024, 0, s, scratch, (int)partials, out);
-  return launch_status();
-}
-
-int pylo_b200_grad_scale(const pylo_grad_item* items, int n_items, const float* norm, float max_norm, void* stream) {
-  CHECK_ARG(n_items >= 0 && (items || !n_items) && norm && max_norm >= 0);
-  for (int i = 0; i < n_items; ++i) CHECK_ARG(items[i].n >= 0 && items[i].type >= 0 && items[i].type <= 2 && (items[i].g || !items[i].n));
-  cudaStream_t s = (cudaStream_t)stream;
-  const int tile = aw_grad_tile(items, n_items);
-  const PlainLaunches plain(tile == AW_GRAD_TILE ? (int)pylo_b200_grad_norm_scratch(items, n_items) : 0);
-  int64_t first = 0;
-  auto all = [&](auto kernel32, auto kernel_bf, auto kernel_h, auto most) {
-    constexpr int MOST = decltype(most)::value;
-    for (int type = 0; type < 3; ++type) {
-      const auto kernel = type == PYLO_FP32 ? kernel32 : type == PYLO_BF16 ? kernel_bf : kernel_h;
-      if (int rc = aw_grads<MOST>(items, n_items, type, tile, first,
-                                  [&](const AwGradArgs<MOST>& a, unsigned tiles, int64_t) { launch(kernel, dim3(tiles), NT, 0, s, a, norm, max_norm); }))
-        return rc;
-    }
-    return 0;
-  };
-  return n_items <= AW_FEW ? all(k_grad_scale<float, AW_FEW>, k_grad_scale<__nv_bfloat16, AW_FEW>, k_grad_scale<__half, AW_FEW>, std::integral_constant<int, AW_FEW>{})
-                           : all(k_grad_scale<float, AW_MANY_G>, k_grad_scale<__nv_bfloat16, AW_MANY_G>, k_grad_scale<__half, AW_MANY_G>, std::integral_constant<int, AW_MANY_G>{});
 }
 
 }  // extern "C"
