@@ -514,8 +514,8 @@ int pylo_b200_step(const pylo_step_plan* plan, const pylo_step_params* prm, int 
 int pylo_b200_advance_steps(double* const* steps, int n, double* first, int* equal);
 
 /* ---- AdamW over many tensors at once, and the global norm of many gradients ---------------------------------------------
- * For parameters and gradients of any of three types.  Items and sets are HOST arrays: they are copied into the launches (one per
- * combination of types and 180 to 800 tensors), so nothing has to outlive the call and a captured launch keeps what it was given. */
+ * For parameters and gradients of any of three types.  Calls, items and sets are HOST memory: they are copied into the launches (one per
+ * combination of types and 180 to 800 tensors), so nothing of them has to outlive the call and a captured launch keeps what it was given. */
 #define PYLO_FP32 0
 #define PYLO_BF16 1
 #define PYLO_FP16 2
@@ -529,7 +529,8 @@ typedef struct pylo_adamw_item {
   float* master; /* beside p of 16 bits, or NULL: its fp32 copy, which the step updates; p becomes the rounded copy */
   void *m, *v;
   uint8_t *m_scale, *v_scale;
-  const float* step; /* DEVICE counter of the steps before this one, or NULL: sets[set].step */
+  float* step_dev;   /* DEVICE count of the tensor's steps so far, or NULL: */
+  double* step;      /* HOST count.  The call adds one to either */
   int64_t n;         /* at most 2^34 */
   int32_t p_type, g_type; /* g_type: p_type or PYLO_FP32, or any beside fp32 parameters */
   int32_t set;
@@ -537,32 +538,35 @@ typedef struct pylo_adamw_item {
 } pylo_adamw_item;
 typedef struct pylo_adamw_set {
   double lr, weight_decay, beta1, beta2, eps;
-  double clip_norm;    /* > 0: gradients times clip_norm / max(norm, clip_norm), norm the root of *gnorm_sq */
+  double clip_norm;    /* > 0: gradients times clip_norm / max(norm, clip_norm), norm the root of call.norm[0] */
   const float* lr_dev; /* DEVICE scalar that stands for lr, or NULL */
-  int64_t step;        /* of this step: 1, 2, ... */
   uint32_t seed;       /* of the random rounding of 8-bit states, which depends on seed, step and an element's place in its tensor only */
   int32_t maximize;
 } pylo_adamw_set;
-int pylo_b200_sizeof_adamw_item(void);
-/* p *= 1 - lr wd; m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2; p -= lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps).
- * bits: 32 or 8.  gnorm_sq: DEVICE scalar, or NULL where no set clips. */
-int pylo_b200_adamw_step(const pylo_adamw_item* items, int n_items, const pylo_adamw_set* sets, int n_sets, int bits, const float* gnorm_sq,
-                         void* stream);
-/* adds 1 to n DEVICE counters (steps is a HOST array) */
-int pylo_b200_adamw_advance(float* const* steps, int n, void* stream);
-
-typedef struct pylo_grad_item {
-  void* g; /* contiguous */
-  int64_t n;
-  int32_t type;
+typedef struct pylo_adamw_call {
+  const pylo_adamw_item* items;
+  const pylo_adamw_set* sets;
+  float* norm;         /* DEVICE, where a set clips: norm[0] sum of squares of all gradients, norm[1] its root, behind them workspace */
+  int64_t norm_floats; /* of norm: 2 + n_items + (elements of all tensors) / 2048 are enough */
+  int32_t n_items, n_sets;
+  int32_t bits;        /* of the states: 32 or 8 */
   int32_t pad_;
-} pylo_grad_item;
-/* floats of scratch that grad_norm needs for these items (host only; -1: bad arguments) */
-int64_t pylo_b200_grad_norm_scratch(const pylo_grad_item* items, int n_items);
-/* out[0] = sum of squares of all elements, out[1] = its root; the same sums in the same order on every call */
-int pylo_b200_grad_norm(const pylo_grad_item* items, int n_items, float* scratch, float* out, void* stream);
-/* all elements times min(1, max_norm / (*norm + 1e-6)), norm a DEVICE scalar; nothing is written where that is 1 */
-int pylo_b200_grad_scale(const pylo_grad_item* items, int n_items, const float* norm, float max_norm, void* stream);
+} pylo_adamw_call;
+int pylo_b200_sizeof_adamw_item(void);
+/* PYLO_ADAMW_NORM: the norm of all items' gradients.  PYLO_ADAMW_STEP: p *= 1 - lr wd; m = beta1 m + (1 - beta1) g;
+ * v = beta2 v + (1 - beta2) g^2; p -= lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps).  Either phase or both in one call (then
+ * norm[0] and norm[1] are not written if there are few partial sums); by themselves where norm[0] has to be summed over ranks in between. */
+#define PYLO_ADAMW_NORM 1
+#define PYLO_ADAMW_STEP 2
+int pylo_b200_adamw_step(const pylo_adamw_call* call, int phases, void* stream);
+
+/* n_items gradients (contiguous; g, n, types: HOST arrays): norm[0] = sum of squares of all elements, norm[1] = its root, the same sums in
+ * the same order on every call; then all elements times min(1, max_norm / (norm[1] + 1e-6)): nothing is written where that is 1, nor read for
+ * max_norm = INFINITY.  norm: DEVICE, norm_floats as above.  distinct: the caller knows that no two share memory; else they have to come in
+ * the order of their addresses, or the call is refused with PYLO_ERR_GRADS_NOT_IN_ORDER. */
+#define PYLO_ERR_GRADS_NOT_IN_ORDER (-5)
+int pylo_b200_clip_grads(void* const* g, const int64_t* n, const int32_t* types, int n_items, float max_norm, float* norm, int64_t norm_floats,
+                         int distinct, void* stream);
 
 #ifdef __cplusplus
 }

@@ -53,16 +53,28 @@ ADAM_DTYPE = np.dtype(
 FP32, BF16, FP16 = 0, 1, 2   # element types of AdamW's and the gradient norm's items
 ADAMW_BLOCK = 256            # elements that share a scale in the 8-bit states
 ADAMW_DTYPE = np.dtype(
-    [(name, np.uint64) for name in ("p", "g", "master", "m", "v", "m_scale", "v_scale", "step")]
+    [(name, np.uint64) for name in ("p", "g", "master", "m", "v", "m_scale", "v_scale", "step_dev", "step")]
     + [("n", np.int64)] + [(name, np.int32) for name in ("p_type", "g_type", "set", "pad_")]
 )
-GRAD_DTYPE = np.dtype([("g", np.uint64), ("n", np.int64), ("type", np.int32), ("pad_", np.int32)])
+ADAMW_NORM, ADAMW_STEP = 1, 2
+ERR_GRADS_NOT_IN_ORDER = -5
 
 
 class AdamwSet(C.Structure):
-    """pylo_adamw_set: hyper-parameters and step count of some tensors of ``pylo_b200_adamw_step``."""
+    """pylo_adamw_set: hyper-parameters of some tensors of ``pylo_b200_adamw_step``."""
     _fields_ = [(name, C.c_double) for name in ("lr", "weight_decay", "beta1", "beta2", "eps", "clip_norm")] + [
-        ("lr_dev", C.c_void_p), ("step", C.c_int64), ("seed", C.c_uint32), ("maximize", C.c_int32)]
+        ("lr_dev", C.c_void_p), ("seed", C.c_uint32), ("maximize", C.c_int32)]
+
+
+class AdamwCall(C.Structure):
+    """pylo_adamw_call: the tensors of a step."""
+    _fields_ = [("items", C.c_void_p), ("sets", C.POINTER(AdamwSet)), ("norm", C.c_void_p), ("norm_floats", C.c_int64)] + [
+        (name, C.c_int32) for name in ("n_items", "n_sets", "bits", "pad_")]
+
+
+def norm_floats(n_items: int, elements: int) -> int:
+    """Floats of ``norm`` that a call over so many tensors and elements needs at most."""
+    return 2 + n_items + elements // 2048
 
 
 class StepParams(C.Structure):
@@ -168,17 +180,14 @@ def _load():
         "pylo_b200_velo_loss_features": [vp, vp, vp, vp, vp, vp, vp],
         "pylo_b200_step": [C.POINTER(StepPlan), C.POINTER(StepParams), i32, vp],
         "pylo_b200_sizeof_adamw_item": [],
-        "pylo_b200_adamw_step": [vp, i32, C.POINTER(AdamwSet), i32, i32, vp, vp],
-        "pylo_b200_adamw_advance": [vp, i32, vp],
-        "pylo_b200_grad_norm_scratch": [vp, i32],
-        "pylo_b200_grad_norm": [vp, i32, vp, vp, vp],
-        "pylo_b200_grad_scale": [vp, i32, vp, f32, vp],
+        "pylo_b200_adamw_step": [C.POINTER(AdamwCall), i32, vp],
+        "pylo_b200_clip_grads": [vp, vp, vp, i32, f32, vp, C.c_int64, i32, vp],
         "pylo_b200_advance_steps": [vp, i32, C.POINTER(C.c_double), C.POINTER(C.c_int)],
     }
     for name, argtypes in sigs.items():
         fn = getattr(lib, name)  # AttributeError if a declared symbol is missing
         fn.argtypes = argtypes
-        fn.restype = C.c_int64 if name in ("pylo_b200_workspace_bytes", "pylo_b200_newton_schulz_workspace", "pylo_b200_grad_norm_scratch") else C.c_int
+        fn.restype = C.c_int64 if name in ("pylo_b200_workspace_bytes", "pylo_b200_newton_schulz_workspace") else C.c_int
     if lib.pylo_b200_abi_version() != ABI_VERSION:
         raise ImportError("libpylo_b200.so was built from a different ABI version; rebuild it")
     if (lib.pylo_b200_sizeof_desc() != DESC_DTYPE.itemsize or lib.pylo_b200_sizeof_params() != C.sizeof(StepParams)

@@ -4,15 +4,17 @@ The step that the learned optimizers are compared with, and that a model can be 
 update and the state keys (``step``, ``exp_avg``, ``exp_avg_sq``) of ``torch.optim.AdamW``, whose checkpoints load.
 Parameters are fp32, bf16 or fp16, those of 16 bits with or without an fp32 copy in the state (``master_weights``).
 
-A step is one launch over the tensors of all param groups (one per combination of types, and per few hundred tensors), two
-more before it where gradients are clipped by their global norm.  Nothing of it waits for the device.
+A step is one native call and one launch over the tensors of all param groups (one per combination of types and two hundred
+tensors), one or two more before it where gradients are clipped by their global norm.  Nothing of it waits for the device.
 """
 
 from __future__ import annotations
 
 import ctypes as C
 import math
+from array import array
 from collections import OrderedDict
+from operator import attrgetter, is_, itemgetter
 
 import numpy as np
 import torch
@@ -20,7 +22,10 @@ from torch.optim import Optimizer
 
 from .. import _lib as L
 from ..plan import current_stream_ptr, with_gradients
-from ._common import StepCounters, optimizer_step
+from ._common import optimizer_step
+
+_numel, _data_ptr, _is_contiguous, _dtype = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.is_contiguous, attrgetter("dtype")   # for map: less per tensor
+_moment_and_step = itemgetter("exp_avg", "step")
 
 TYPES = {torch.float32: L.FP32, torch.bfloat16: L.BF16, torch.float16: L.FP16}
 _CODES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -69,51 +74,56 @@ class _Kept:
 class _Plan:
     """The host's table of a set of tensors, and what of it the last step has seen."""
 
-    def __init__(self, params, group_of, states, bits):
-        self.device = params[0].device
-        self.p_dtypes = [p.dtype for p in params]
-        self.states, self.group_of = states, group_of
+    def __init__(self, params, group_of, flags, state, bits):
+        self.device = params[0].device if params else torch.device("cuda", torch.cuda.current_device())
+        self.p_ptrs, self.numels, self.p_dtypes = [p.data_ptr() for p in params], [p.numel() for p in params], [p.dtype for p in params]
+        self.group_of, self.flags = group_of, flags
+        # the table holds the addresses of these tensors: they stay alive with it, and it is good for them only
+        self.params, self.every_state = params, list(state.values())
+        self.states = states = [state[p] for p in params]
+        self.moments_and_steps = [x for st in states for x in _moment_and_step(st)]
         self.table = t = np.zeros(len(params), dtype=L.ADAMW_DTYPE)
-        t["p"] = [p.data_ptr() for p in params]
-        t["n"] = [p.numel() for p in params]
-        t["p_type"] = [TYPES[d] for d in self.p_dtypes]
+        t["p"], t["n"], t["p_type"] = self.p_ptrs, self.numels, [TYPES[d] for d in self.p_dtypes]
         ptr = lambda name: [st[name].data_ptr() if name in st else 0 for st in states]
         t["master"], t["m"] = ptr("master"), ptr("exp_avg")
         t["v"] = ptr("exp_avg_sq" if bits == 32 else "exp_avg_sq_root")
         t["m_scale"], t["v_scale"] = ptr("exp_avg_scale"), ptr("exp_avg_sq_root_scale")
-        on_device = [st["step"].is_cuda for st in states]
-        t["step"] = [st["step"].data_ptr() if cuda else 0 for st, cuda in zip(states, on_device)]
-        self.device_steps = [a for a in t["step"].tolist() if a]
-        if self.device_steps:
-            self.device_steps = (C.c_void_p * len(self.device_steps))(*self.device_steps)
-        self.host = [i for i, cuda in enumerate(on_device) if not cuda]
-        self.counters = StepCounters([states[i] for i in self.host])
-        self.moments = [st["exp_avg"] for st in states]
+        t["step_dev"] = [st["step"].data_ptr() if st["step"].is_cuda else 0 for st in states]
+        t["step"] = [0 if st["step"].is_cuda else st["step"].data_ptr() for st in states]
         t["set"] = group_of
-        self.one_step = True     # the table's sets are the groups'
         self.g_ptrs, self.g_dtypes = None, None
-        self.address = t.ctypes.data
-        self.grads = np.zeros(len(params), dtype=L.GRAD_DTYPE)
-        self.grads["n"] = t["n"]
+        self.call = L.AdamwCall(items=t.ctypes.data, n_items=len(params), bits=bits, norm_floats=L.norm_floats(len(params), sum(self.numels)))
+        self.call_ref = C.byref(self.call)
+        self.sets, self.set_key, self.norm = None, None, None
+
+    def good_for(self, params, group_of, flags, state):
+        same = lambda new, old: len(new) == len(old) and all(map(is_, new, old))
+        if not (same(params, self.params) and list(map(_data_ptr, params)) == self.p_ptrs and list(map(_numel, params)) == self.numels
+                and list(map(_dtype, params)) == self.p_dtypes and group_of == self.group_of and flags == self.flags
+                and same(state.values(), self.every_state)):
+            return False
+        try:
+            return same([x for st in self.states for x in _moment_and_step(st)], self.moments_and_steps)
+        except KeyError:
+            return False
 
     def look_at(self, grads):
         """Put the gradients' addresses and types into the table; returns the copies that stand in for some of them."""
         try:
-            ptrs = [g.data_ptr() for g in grads]
+            ptrs = list(map(_data_ptr, grads))
         except RuntimeError:
             if any(g.is_sparse for g in grads):
                 raise RuntimeError("Sparse gradients not supported") from None
             raise
         copies = ()
-        dtypes = [g.dtype for g in grads]
-        if dtypes != self.g_dtypes or not all([g.is_contiguous() for g in grads]):
+        dtypes = list(map(_dtype, grads))
+        if dtypes != self.g_dtypes or not all(map(_is_contiguous, grads)):
             copies = [_gradient(g, d) for g, d in zip(grads, self.p_dtypes)]
             ptrs = [g.data_ptr() for g in copies]
-            self.table["g_type"] = self.grads["type"] = [TYPES[g.dtype] for g in copies]
-            plain = all([c is g for c, g in zip(copies, grads)])
-            self.g_dtypes = dtypes if plain else None
+            self.table["g_type"] = [TYPES[g.dtype] for g in copies]
+            self.g_dtypes = dtypes if all([c is g for c, g in zip(copies, grads)]) else None
         if ptrs != self.g_ptrs:
-            self.table["g"] = self.grads["g"] = ptrs
+            self.table["g"] = ptrs
             self.g_ptrs = ptrs
         return copies
 
@@ -143,7 +153,7 @@ class _AdamWFamily(Optimizer):
             raise ValueError(f"{self._name}: amsgrad is not supported")
 
     def _reset(self):
-        self._sig = self._plan = self._sets = self._set_key = self._scratch = None
+        self._plan = None
 
     # ------------------------------------------------------------------ state
     def add_param_group(self, param_group):
@@ -188,11 +198,11 @@ class _AdamWFamily(Optimizer):
         """Make what a parameter's state lacks, and bring what it has into the form the kernels take."""
         dev, n = p.device, p.numel()
         capturable = group["capturable"]
-        step = st.get("step", 0.0)
-        if not torch.is_tensor(step) or step.is_cuda != bool(capturable) or step.dim() != 0 or not step.dtype.is_floating_point:
-            step = torch.tensor(float(step), dtype=torch.float32 if capturable else torch.float64, device=dev if capturable else "cpu")
-        if capturable:
-            step = step.to(device=dev, dtype=torch.float32)
+        step, kind = st.get("step", 0.0), torch.float32 if capturable else torch.float64
+        if not torch.is_tensor(step) or step.is_cuda != bool(capturable) or step.dim() != 0 or step.dtype is not kind:
+            step = torch.tensor(float(step), dtype=kind, device=dev if capturable else "cpu")
+        elif capturable:
+            step = step.to(dev)
         st["step"] = step
         if self._bits == 32:
             if "exp_avg_sq_root" in st:
@@ -223,8 +233,8 @@ class _AdamWFamily(Optimizer):
                 raise ValueError(f"{self._name}: state {name!r} is {x.dtype}, not {dtype}")
             st[name] = x.to(device=dev, dtype=dtype).contiguous()
 
-    def _build(self, plist, group_of, capturing):
-        dev = plist[0].device
+    def _build(self, plist, group_of, flags, capturing):
+        dev = plist[0].device if plist else None
         for p in plist:
             if not p.is_cuda:
                 raise RuntimeError(f"{self._name}: parameters must live on a CUDA device (there is no CPU path)")
@@ -246,7 +256,7 @@ class _AdamWFamily(Optimizer):
             raise RuntimeError(f"{self._name}: run a step before the one that is captured: a captured step would make its states anew on every replay")
         for p, st, gi in zip(plist, states, group_of):
             self._init_state(p, st, self.param_groups[gi])
-        return _Plan(plist, group_of, states, self._bits)
+        return _Plan(plist, group_of, flags, self.state, self._bits)
 
     # ------------------------------------------------------------------ step
     @optimizer_step
@@ -267,88 +277,59 @@ class _AdamWFamily(Optimizer):
             group_of += [gi] * len(ps)
         clip = any([g["clip_grad"] for g in groups])
         if plist or clip:
-            device = plist[0].device if plist else torch.device("cuda", torch.cuda.current_device())
-            if device.type == "cuda" and device.index != torch.cuda.current_device():
-                with torch.cuda.device(device):
-                    self._run(plist, grads, group_of, clip, device)
+            at = plist[0].get_device() if plist else -1
+            if at >= 0 and at != torch._C._cuda_getDevice():
+                with torch.cuda.device(at):
+                    self._run(plist, grads, group_of, clip)
             else:
-                self._run(plist, grads, group_of, clip, device)
+                self._run(plist, grads, group_of, clip)
         if self.after_group is not None:
             for gi in range(len(groups)):
                 self.after_group(gi)
         return loss
 
-    def _run(self, plist, grads, group_of, clip, device):
-        capturing = torch.cuda.is_current_stream_capturing()
-        groups = self.param_groups
-        if capturing and not all([g["capturable"] for g in groups]):
+    def _run(self, plist, grads, group_of, clip):
+        capturing = torch._C._cuda_isCurrentStreamCapturing()
+        flags = [(g["capturable"], g["master_weights"]) for g in self.param_groups]
+        if capturing and not all([capturable for capturable, _ in flags]):
             raise RuntimeError(f"{self._name}: a step can be captured into a graph only with capturable=True")
         plan = self._plan
-        sig = [(p.data_ptr(), p.numel(), p.dtype) for p in plist]
-        flags = [(g["capturable"], g["master_weights"]) for g in groups]
-        if plan is None or (sig, group_of, flags) != self._sig or not all([st.get("exp_avg") is m for st, m in zip(plan.states, plan.moments)]):
-            plan = self._plan = self._build(plist, group_of, capturing) if plist else None
-            self._sig = (sig, group_of, flags)
-            self._scratch = None
+        if plan is None or not plan.good_for(plist, group_of, flags, self.state):
+            plan = self._plan = self._build(plist, group_of, flags, capturing)
         stream = current_stream_ptr()
-        copies = plan.look_at(grads) if plan else ()
-        norm = None
+        copies = plan.look_at(grads)
+        self._fill_sets(plan)
+        phases = L.ADAMW_STEP
         if clip:
-            norm = self._grad_norm(plan, device, stream, capturing)
-        if plan is None:
-            return
-        sets = self._fill_sets(plan)
-        L.check(L.lib.pylo_b200_adamw_step(plan.address, len(plist), sets, len(sets), self._bits, norm, stream), "adamw_step")
-        if plan.device_steps:
-            L.check(L.lib.pylo_b200_adamw_advance(plan.device_steps, len(plan.device_steps), stream), "adamw_advance")
+            phases = L.ADAMW_NORM | L.ADAMW_STEP
+            norm = plan.norm
+            if norm is None or capturing:   # a captured step has a buffer of its own, from the graph's memory
+                norm = torch.empty(plan.call.norm_floats, dtype=torch.float32, device=plan.device)
+                plan.norm = None if capturing else norm
+                plan.call.norm = norm.data_ptr()
+            if self.process_group is not None or (self._sharded and torch.distributed.is_initialized()):
+                L.check(L.lib.pylo_b200_adamw_step(plan.call_ref, L.ADAMW_NORM, stream), "adamw_step")
+                torch.distributed.all_reduce(norm[:1], group=self.process_group)  # each rank holds its own tensors' share
+                phases = L.ADAMW_STEP
+        L.check(L.lib.pylo_b200_adamw_step(plan.call_ref, phases, stream), "adamw_step")
         del copies
 
-    def _grad_norm(self, plan, device, stream, capturing):
-        """Address of the sum of squares of all gradients (of all ranks)."""
-        n = len(plan.grads) if plan else 0
-        table = plan.grads.ctypes.data if plan else None
-        out = self._scratch
-        if out is None or capturing or out.device != device:   # a captured step has a buffer of its own, from the graph's memory
-            floats = L.lib.pylo_b200_grad_norm_scratch(table, n)
-            out = torch.empty(2 + max(floats, 0), dtype=torch.float32, device=device)
-            if not capturing:
-                self._scratch = out
-        at = out.data_ptr()
-        L.check(L.lib.pylo_b200_grad_norm(table, n, at + 8, at, stream), "grad_norm")
-        if self.process_group is not None or (torch.distributed.is_initialized() and self._sharded):
-            torch.distributed.all_reduce(out[:1], group=self.process_group)  # each rank holds its own tensors' share
-        return at
-
     def _fill_sets(self, plan):
-        """The hyper-parameters of the step: a set per group, or per group and count of steps where a group's tensors differ in it."""
-        key = [(g["lr"] if torch.is_tensor(g["lr"]) else float(g["lr"]), g["betas"], g["eps"], g["weight_decay"],
-                g["clip_norm"] if g["clip_grad"] else 0.0, g["maximize"], g.get("seed", 0)) for g in self.param_groups]
-        old = plan.counters.advance() if plan.host else 0.0
-        if isinstance(old, float):
-            if not plan.one_step:
-                plan.table["set"], plan.one_step, self._set_key = plan.group_of, True, None
-            pairs = [(gi, old + 1) for gi in range(len(key))]
-        else:
-            steps = dict(zip(plan.host, old))
-            of = [(gi, steps.get(i, 0.0) + 1) for i, gi in enumerate(plan.group_of)]
-            pairs = sorted(set(of))
-            index = {pair: k for k, pair in enumerate(pairs)}
-            plan.table["set"], plan.one_step, self._set_key = [index[pair] for pair in of], False, None
-        sets = self._sets
-        if self._set_key is None or any([torch.is_tensor(k[0]) for k in key]) or self._set_key != key:
-            sets = self._sets = (L.AdamwSet * len(pairs))()
-            for s, (gi, _) in zip(sets, pairs):
-                lr, (b1, b2), eps, wd, clip_norm, maximize, seed = key[gi]
-                if torch.is_tensor(lr) and lr.is_cuda and self.param_groups[gi]["capturable"]:
-                    if lr.dtype is not torch.float32 or lr.numel() != 1 or lr.device != plan.device:
-                        raise ValueError(f"{self._name}: lr on the device must be one fp32 value on {plan.device}")
-                    s.lr_dev, lr = lr.data_ptr(), 0.0
-                s.lr, s.weight_decay, s.beta1, s.beta2, s.eps, s.clip_norm = float(lr), wd, b1, b2, eps, clip_norm
-                s.maximize, s.seed = bool(maximize), seed & 0xFFFFFFFF
-            self._set_key = key
-        for s, (_, step) in zip(sets, pairs):
-            s.step = int(step)
-        return sets
+        """The hyper-parameters of the step, a set per group."""
+        key = [(g["lr"], g["betas"], g["eps"], g["weight_decay"], g["clip_norm"] if g["clip_grad"] else 0.0, g["maximize"], g.get("seed", 0))
+               for g in self.param_groups]
+        if plan.set_key is not None and not any([torch.is_tensor(k[0]) for k in key]) and plan.set_key == key:
+            return
+        plan.sets = (L.AdamwSet * len(key))()
+        for s, group, (lr, (b1, b2), eps, wd, clip_norm, maximize, seed) in zip(plan.sets, self.param_groups, key):
+            if torch.is_tensor(lr) and lr.is_cuda and group["capturable"]:
+                if lr.dtype is not torch.float32 or lr.numel() != 1 or lr.device != plan.device:
+                    raise ValueError(f"{self._name}: lr on the device must be one fp32 value on {plan.device}")
+                s.lr_dev, lr = lr.data_ptr(), 0.0
+            s.lr, s.weight_decay, s.beta1, s.beta2, s.eps, s.clip_norm = float(lr), wd, b1, b2, eps, clip_norm
+            s.maximize, s.seed = bool(maximize), seed & 0xFFFFFFFF
+        plan.call.sets, plan.call.n_sets = plan.sets, len(key)
+        plan.set_key = key
 
 
 class AdamW_CUDA(_AdamWFamily):
@@ -402,71 +383,77 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     together; returns ``norm`` (fp32, on the device), as ``torch.nn.utils.clip_grad_norm_`` does.
 
     Gradients may be fp32, bf16 and fp16, mixed; the norm is summed up in fp32 and more whatever their type.  One that is given twice
-    counts and is scaled once.  Three launches and no synchronisation (``error_if_nonfinite`` waits for the norm); the gradients are
-    written only where the norm exceeds ``max_norm``, and not read again for ``max_norm = inf``."""
+    counts and is scaled once.  Two or three launches and no synchronisation (``error_if_nonfinite`` waits for the norm); the gradients are
+    written only where the norm exceeds ``max_norm``."""
     if float(norm_type) != 2.0:
         raise ValueError(f"clip_grad_norm_: only the 2-norm is supported, got norm_type={norm_type}")
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"clip_grad_norm_: invalid max_norm: {max_norm}")
-    grads = [g for g in [p.grad for p in ([parameters] if torch.is_tensor(parameters) else parameters)] if g is not None]
+    grads = [p.grad for p in ([parameters] if torch.is_tensor(parameters) else parameters)]
+    if any([g is None for g in grads]):
+        grads = [g for g in grads if g is not None]
     if not grads:
         return torch.tensor(0.0)
-    device = grads[0].device
-    if device.type != "cuda":
+    at = grads[0].get_device()
+    if at < 0:
         raise RuntimeError("clip_grad_norm_: gradients must live on a CUDA device (there is no CPU path)")
-    for g in grads:
-        if g.device != device:
-            raise RuntimeError(f"clip_grad_norm_: all gradients must live on one device, got {device} and {g.device}")
-        if g.layout is not torch.strided:
-            raise RuntimeError("Sparse gradients not supported")
-        if g.dtype not in TYPES:
-            raise RuntimeError(f"clip_grad_norm_: gradients must be fp32, bf16 or fp16, got {g.dtype}")
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _clip(grads, max_norm, error_if_nonfinite, device)
-    return _clip(grads, max_norm, error_if_nonfinite, device)
+    if not all([g.get_device() == at for g in grads]):
+        raise RuntimeError("clip_grad_norm_: all gradients must live on one device")
+    types = list(map(TYPES.get, map(_dtype, grads)))
+    if None in types:
+        raise RuntimeError(f"clip_grad_norm_: gradients must be fp32, bf16 or fp16, got {grads[types.index(None)].dtype}")
+    if at != torch._C._cuda_getDevice():
+        with torch.cuda.device(at):
+            return _clip(grads, types, max_norm, error_if_nonfinite)
+    return _clip(grads, types, max_norm, error_if_nonfinite)
 
 
-def _clip(grads, max_norm, error_if_nonfinite, device):
-    if not all([g.is_contiguous() for g in grads]):
+def _clip(grads, types, max_norm, error_if_nonfinite):
+    parts = grads
+    if any([g.layout is not torch.strided for g in grads]):
+        raise RuntimeError("Sparse gradients not supported")
+    if not all(map(_is_contiguous, grads)):
+        parts = [g if g.is_contiguous() or _dense(g) else g.detach().contiguous() for g in grads]
+    ptrs, sizes = list(map(_data_ptr, parts)), list(map(_numel, parts))
+    stream, call = current_stream_ptr(), L.lib.pylo_b200_clip_grads
+    floats = L.norm_floats(len(ptrs), sum(sizes))
+    norm = torch.empty(floats, dtype=torch.float32, device="cuda")
+    total = norm[1]
+
+    def run(ptrs, sizes, types, limit, distinct):
+        g, n, t = array("Q", ptrs), array("q", sizes), array("i", types)
+        return call(g.buffer_info()[0], n.buffer_info()[0], t.buffer_info()[0], len(ptrs), limit, norm.data_ptr(), floats, distinct, stream)
+
+    limit = math.inf if error_if_nonfinite else max_norm   # the norm is looked at before anything is scaled
+    code, distinct = run(ptrs, sizes, types, limit, 0), 0
+    if code == L.ERR_GRADS_NOT_IN_ORDER:
+        ptrs, sizes, types = _distinct(ptrs, sizes, types)
+        code, distinct = run(ptrs, sizes, types, limit, 1), 1
+    L.check(code, "clip_grads")
+    if error_if_nonfinite:
+        if not math.isfinite(float(total)):
+            raise RuntimeError("The total norm of order 2.0 for gradients from `parameters` is non-finite, so it cannot be clipped. To disable this "
+                               "error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
+        if max_norm < math.inf:
+            L.check(run(ptrs, sizes, types, max_norm, distinct), "clip_grads")
+    if parts is not grads and max_norm < math.inf:
         with torch.no_grad():
-            parts = [g.detach() if g.is_contiguous() or _dense(g) else g.detach().contiguous() for g in grads]
-    else:
-        parts = grads
-    table = np.zeros(len(parts), dtype=L.GRAD_DTYPE)
-    table["g"] = [g.data_ptr() for g in parts]
-    table["n"] = [g.numel() for g in parts]
-    table["type"] = [TYPES[g.dtype] for g in parts]
-    if len(parts) > 1:
-        table = _distinct(table)
-    stream, at, n = current_stream_ptr(), table.ctypes.data, len(table)
-    floats = L.lib.pylo_b200_grad_norm_scratch(at, n)
-    out = torch.empty(2 + max(floats, 0), dtype=torch.float32, device=device)
-    total = out[1]
-    L.check(L.lib.pylo_b200_grad_norm(at, n, out.data_ptr() + 8, out.data_ptr(), stream), "grad_norm")
-    if error_if_nonfinite and not math.isfinite(float(total)):
-        raise RuntimeError("The total norm of order 2.0 for gradients from `parameters` is non-finite, so it cannot be clipped. To disable this "
-                           "error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
-    if max_norm < math.inf:
-        L.check(L.lib.pylo_b200_grad_scale(at, n, total.data_ptr(), max_norm, stream), "grad_scale")
-        if parts is not grads:
-            with torch.no_grad():
-                for g, part in zip(grads, parts):
-                    if part.data_ptr() != g.data_ptr():
-                        g.copy_(part)
+            for g, part in zip(grads, parts):
+                if part is not g:
+                    g.copy_(part)
     return total
 
 
-def _distinct(table):
-    """The table with every gradient once; two that share only a part of their memory are refused."""
-    size = np.array([4, 2, 2], dtype=np.uint64)
-    order = np.argsort(table["g"], kind="stable")
-    g, end = table["g"][order], (table["g"] + table["n"].astype(np.uint64) * size[table["type"]])[order]
-    over = g[1:] < end[:-1]
-    if not over.any():
-        return table
-    twice = (g[1:] == g[:-1]) & (end[1:] == end[:-1])
+def _distinct(ptrs, sizes, types):
+    """Every gradient once, in the order given; two that share only a part of their memory are refused."""
+    g, n, t = np.array(ptrs, dtype=np.uint64), np.array(sizes, dtype=np.uint64), np.array(types)
+    order = np.argsort(g, kind="stable")
+    order = order[n[order] > 0]
+    first, end = g[order], (g + n * np.array([4, 2, 2], dtype=np.uint64)[t])[order]
+    over = first[1:] < end[:-1]
+    twice = over & (first[1:] == first[:-1]) & (end[1:] == end[:-1]) & (t[order][1:] == t[order][:-1])
     if (over & ~twice).any():
         raise ValueError("clip_grad_norm_: two gradients share a part of their memory")
-    return np.ascontiguousarray(table[np.sort(order[np.concatenate([[True], ~twice])])])
+    keep = np.sort(order[np.concatenate([[True], ~twice])]) if len(order) else order
+    return g[keep].tolist(), n[keep].tolist(), t[keep].tolist()

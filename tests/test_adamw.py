@@ -109,51 +109,64 @@ def check_codes(codes, scales, exact, err, parts, least):
 # ---------------------------------------------------------------------------------------------------------------------
 # without a GPU
 # ---------------------------------------------------------------------------------------------------------------------
+COUNT = np.zeros(1)
+
+
 def item(**kw):
     t = np.zeros(1, dtype=L.ADAMW_DTYPE)
-    for name, value in {**dict(p=256, g=256, m=256, v=256, n=4), **kw}.items():
+    for name, value in {**dict(p=256, g=256, m=256, v=256, n=4, step=COUNT.ctypes.data), **kw}.items():
         t[name] = value
     return t
 
 
+def a_call(t, s, **kw):
+    return L.AdamwCall(**{**dict(items=t.ctypes.data, n_items=len(t), sets=C.pointer(s), n_sets=1, bits=32), **kw})
+
+
 def a_set(**kw):
-    s = L.AdamwSet(lr=1e-3, weight_decay=0.0, beta1=0.9, beta2=0.99, eps=1e-8, step=1)
+    s = L.AdamwSet(lr=1e-3, weight_decay=0.0, beta1=0.9, beta2=0.99, eps=1e-8)
     for name, value in kw.items():
         setattr(s, name, value)
     return s
 
 
+def step(call, phases=L.ADAMW_STEP):
+    return L.lib.pylo_b200_adamw_step(C.byref(call), phases, None)
+
+
 @pytest.mark.parametrize("bad", [dict(n=-1), dict(n=2 ** 34 + 1), dict(set=1), dict(set=-1), dict(p_type=3), dict(g_type=-1), dict(p=0), dict(g=0), dict(m=0),
-                                 dict(v=0), dict(p_type=L.BF16, g_type=L.FP16), dict(p_type=L.FP16, g_type=L.BF16), dict(master=256)])
+                                 dict(v=0), dict(p_type=L.BF16, g_type=L.FP16), dict(p_type=L.FP16, g_type=L.BF16), dict(master=256), dict(step=0)])
 def test_items_are_checked_before_a_launch(bad):
     t, s = item(**bad), a_set()
-    assert L.lib.pylo_b200_adamw_step(t.ctypes.data, 1, C.byref(s), 1, 32, None, None) < 0
+    assert step(a_call(t, s)) < 0 and COUNT[0] == 0
 
 
-@pytest.mark.parametrize("bad", [dict(beta1=1.0), dict(beta1=-0.1), dict(beta2=1.0), dict(eps=-1.0), dict(step=0), dict(clip_norm=-1.0), dict(beta1=math.nan)])
+@pytest.mark.parametrize("bad", [dict(beta1=1.0), dict(beta1=-0.1), dict(beta2=1.0), dict(eps=-1.0), dict(clip_norm=-1.0), dict(beta1=math.nan), dict(clip_norm=1.0)])
 def test_sets_are_checked_before_a_launch(bad):
-    t, s = item(), a_set(**bad)
-    assert L.lib.pylo_b200_adamw_step(t.ctypes.data, 1, C.byref(s), 1, 32, None, None) < 0
+    t, s = item(), a_set(**bad)   # the last: no place for the norm
+    assert step(a_call(t, s)) < 0 and COUNT[0] == 0
 
 
 def test_calls_are_checked_before_a_launch():
-    t, s = item(), a_set()
-    call = L.lib.pylo_b200_adamw_step
-    assert call(None, 1, C.byref(s), 1, 32, None, None) < 0 and call(t.ctypes.data, 1, None, 1, 32, None, None) < 0
-    assert call(t.ctypes.data, 1, C.byref(s), 1, 16, None, None) < 0 and call(t.ctypes.data, -1, C.byref(s), 1, 32, None, None) < 0
-    assert call(t.ctypes.data, 1, C.byref(s), 1, 8, None, None) < 0   # no scales
-    assert call(t.ctypes.data, 0, C.byref(s), 1, 32, None, None) == 0 and call(item(n=0, p=0).ctypes.data, 1, C.byref(s), 1, 32, None, None) == 0
-    assert L.lib.pylo_b200_adamw_advance(None, 1, None) < 0
-    g = np.zeros(1, dtype=L.GRAD_DTYPE)
-    g["g"], g["n"] = 256, 5
-    out = C.c_void_p(256)
-    assert L.lib.pylo_b200_grad_norm_scratch(g.ctypes.data, 1) == 1 and L.lib.pylo_b200_grad_norm_scratch(None, 1) == -1
-    assert L.lib.pylo_b200_grad_norm(g.ctypes.data, 1, None, out, None) < 0 and L.lib.pylo_b200_grad_norm(g.ctypes.data, 1, out, None, None) < 0
-    assert L.lib.pylo_b200_grad_scale(g.ctypes.data, 1, None, 1.0, None) < 0 and L.lib.pylo_b200_grad_scale(g.ctypes.data, 1, out, -1.0, None) < 0
-    for name, value in (("type", 3), ("n", -1), ("g", 0)):
-        b = g.copy()
-        b[name] = value
-        assert L.lib.pylo_b200_grad_norm(b.ctypes.data, 1, out, out, None) < 0 and L.lib.pylo_b200_grad_scale(b.ctypes.data, 1, out, 1.0, None) < 0
+    t, s, none = item(), a_set(), item(n=0, p=0)
+    assert L.lib.pylo_b200_adamw_step(None, L.ADAMW_STEP, None) < 0 and step(a_call(t, s), 4) < 0
+    for bad in (dict(items=None), dict(n_items=-1), dict(n_sets=-1), dict(n_sets=0), dict(sets=None), dict(bits=16), dict(bits=8)):   # the last: no scales
+        assert step(a_call(t, s, **bad)) < 0, bad
+    assert step(a_call(t, s), L.ADAMW_NORM) < 0 and step(a_call(t, s, norm=256, norm_floats=2), L.ADAMW_NORM) < 0   # no place for the norm
+    assert step(a_call(t, s, n_items=0)) == 0 and COUNT[0] == 0
+    assert step(a_call(none, s)) == 0 and COUNT[0] == 1   # a tensor without elements takes its step too
+    COUNT[0] = 0
+
+
+def test_gradients_are_checked_before_a_launch():
+    g, n, t = np.array([512, 1024], dtype=np.uint64), np.array([128, 5]), np.array([L.FP32, L.BF16], dtype=np.int32)
+    call = lambda g=g, n=n, t=t, count=2, limit=1.0, norm=256, floats=100, distinct=0: L.lib.pylo_b200_clip_grads(
+        g.ctypes.data if g is not None else None, n.ctypes.data if n is not None else None, t.ctypes.data if t is not None else None, count, limit, norm, floats,
+        distinct, None)
+    for bad in (dict(g=None), dict(n=None), dict(t=None), dict(count=-1), dict(limit=-1.0), dict(limit=math.nan), dict(norm=None), dict(floats=3), dict(n=np.array([128, -1])),
+                dict(t=np.array([0, 3], dtype=np.int32)), dict(t=np.array([-1, 0], dtype=np.int32)), dict(g=np.array([512, 0], dtype=np.uint64))):
+        assert call(**bad) == -1, bad
+    assert call(g=g[::-1].copy()) == L.ERR_GRADS_NOT_IN_ORDER and call(n=np.array([129, 5])) == L.ERR_GRADS_NOT_IN_ORDER
 
 
 def test_there_is_no_path_without_a_gpu():
@@ -179,15 +192,14 @@ def test_clipping_refuses_what_it_does_not_do():
 
 
 def test_gradients_that_overlap():
-    t = np.zeros(3, dtype=L.GRAD_DTYPE)
-    t["g"], t["n"] = [1024, 512, 1024], [64, 128, 64]
-    assert A._distinct(t)["g"].tolist() == [1024, 512]
-    t["n"] = [64, 129, 64]
+    ptrs, types = [1024, 512, 1024], [L.FP32] * 3
+    assert A._distinct(ptrs, [64, 128, 64], types) == ([1024, 512], [64, 128], [L.FP32] * 2)
+    assert A._distinct([1024, 512, 0], [64, 128, 0], types)[0] == [1024, 512]
+    for sizes in ([64, 129, 64], [64, 128, 65]):
+        with pytest.raises(ValueError, match="memory"):
+            A._distinct(ptrs, sizes, types)
     with pytest.raises(ValueError, match="memory"):
-        A._distinct(t)
-    t["n"] = [64, 128, 65]
-    with pytest.raises(ValueError, match="memory"):
-        A._distinct(t)
+        A._distinct(ptrs, [64, 128, 128], [L.FP32, L.FP32, L.BF16])
 
 
 @pytest.mark.parametrize("n", [0, 1, 255, 256, 1000])
@@ -619,6 +631,36 @@ def test_another_memory_behind_a_parameter(cls):
         y.step()
     assert torch.equal(a[0], b[0])
     assert x.state[a[0]]["step"] == 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", [optim.AdamW_CUDA, optim.AdamW8bit_CUDA])
+def test_states_that_are_taken_away_or_set_anew(cls):
+    """A step goes by what the state holds now: cleared, it begins anew; a count or a tensor set by hand counts."""
+    a, b = params_of([(300,), (20,)], torch.float32, 1), params_of([(300,), (20,)], torch.float32, 1)
+    x, y = cls(a), cls(b)
+
+    def both(t):
+        set_grads(a, torch.float32, t)
+        for p, q in zip(a, b):
+            q.grad = p.grad.clone()
+        x.step()
+        y.step()
+
+    both(0)
+    x.state.clear()
+    y = cls(b)
+    both(1)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and float(x.state[a[0]]["step"]) == 1
+    x.state[a[0]] = {k: v.clone() for k, v in x.state[a[0]].items()}
+    x.state[a[1]]["step"] = 7
+    y.state[b[1]]["step"].fill_(7)
+    both(2)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and float(x.state[a[1]]["step"]) == 8
+    x.state.pop(a[1])
+    y.state.pop(b[1])
+    both(3)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and float(x.state[a[0]]["step"]) == 3 and float(x.state[a[1]]["step"]) == 1
 
 
 @pytest.mark.gpu
