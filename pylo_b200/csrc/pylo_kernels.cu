@@ -2534,21 +2534,7 @@ __global__ void __launch_bounds__(MIX_OUT * MIX_GROUPS) k_velo_mix(const pylo_ve
 // ================================================================================================
 // C ABI
 // ================================================================================================
-// Opt a kernel in to more than 48 KB of dynamic shared memory, once per device (the attribute belongs to the
-// device's copy of the function); flags[] is the caller's per-kernel record.
-template <class K>
-static int allow_dynamic_smem(K kernel, int bytes, bool (&flags)[PYLO_MAX_DEVICES]) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return (int)e;
-  if (dev >= 0 && dev < PYLO_MAX_DEVICES && flags[dev]) return 0;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return (int)e;
-  if (dev >= 0 && dev < PYLO_MAX_DEVICES) flags[dev] = true;
-  return 0;
-}
-
-// The same for clusters of more than eight CTAs.
+// As allow_dynamic_smem, for clusters of more than eight CTAs.
 template <class K>
 static int allow_wide_clusters(K kernel, bool (&flags)[PYLO_MAX_DEVICES]) {
   int dev = 0;

@@ -38,6 +38,12 @@ struct PlainLaunches {
 // 6 x 4096 x 4096 VeLO parameters: 921 us after the state sweep's ring, 755 us without).  Such a kernel has itself and the next
 // launch of its thread made plainly.
 inline thread_local bool t_plain_next = false;
+// For the launches of one scope: kernels that stream through memory and do not mind.  What they are followed by still does.
+struct AnyCache {
+  bool next;
+  AnyCache() : next(t_plain_next) { t_plain_next = false; }
+  ~AnyCache() { t_plain_next = next; }
+};
 template <class... P, class... A>
 static void launch_clusters(void (*kernel)(P...), dim3 grid, dim3 block, int cluster, size_t smem, cudaStream_t stream, A&&... args) {
   cudaLaunchAttribute attr[2];
@@ -65,6 +71,20 @@ static void launch_clusters(void (*kernel)(P...), dim3 grid, dim3 block, int clu
 template <class... P, class... A>
 static void launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
   launch_clusters(kernel, grid, block, 0, smem, stream, static_cast<A&&>(args)...);
+}
+
+// Opt a kernel in to more than 48 KB of dynamic shared memory, once per device (the attribute belongs to the
+// device's copy of the function); flags[] is the caller's per-kernel record.
+template <class K>
+static int allow_dynamic_smem(K kernel, int bytes, bool (&flags)[PYLO_MAX_DEVICES]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (dev >= 0 && dev < PYLO_MAX_DEVICES && flags[dev]) return 0;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return (int)e;
+  if (dev >= 0 && dev < PYLO_MAX_DEVICES) flags[dev] = true;
+  return 0;
 }
 
 #define CHECK_ARG(cond) \
