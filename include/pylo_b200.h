@@ -522,7 +522,7 @@ int pylo_b200_advance_steps(double* const* steps, int n, double* first, int* equ
 #define PYLO_ADAMW_BLOCK 256 /* elements that share a scale in the 8-bit states */
 /* One parameter tensor (contiguous).  32-bit states: m, v fp32[n].  8-bit: m and v hold the codes [n] of the first moment and of the ROOT of the
  * second, OCP e4m3 (torch.float8_e4m3fn), m_scale and v_scale an e8m0 power of two per PYLO_ADAMW_BLOCK elements [ceil(n / 256)]: a value is
- * code * scale. */
+ * code * scale.  master, m and v begin on 16-byte boundaries; p and g may begin anywhere. */
 typedef struct pylo_adamw_item {
   void* p;
   const void* g;

@@ -231,7 +231,8 @@ class _AdamWFamily(Optimizer):
                 raise ValueError(f"{self._name}: state {name!r} has shape {tuple(x.shape)}, the parameter's needs {tuple(shape)}")
             if x.dtype is not dtype and (dtype.itemsize == 1 or not x.dtype.is_floating_point):
                 raise ValueError(f"{self._name}: state {name!r} is {x.dtype}, not {dtype}")
-            st[name] = x.to(device=dev, dtype=dtype).contiguous()
+            x = x.to(device=dev, dtype=dtype).contiguous()
+            st[name] = x.clone() if x.data_ptr() % 16 else x   # the kernels want it on a boundary
 
     def _build(self, plist, group_of, flags, capturing):
         dev = plist[0].device if plist else None

@@ -135,7 +135,8 @@ def step(call, phases=L.ADAMW_STEP):
 
 
 @pytest.mark.parametrize("bad", [dict(n=-1), dict(n=2 ** 34 + 1), dict(set=1), dict(set=-1), dict(p_type=3), dict(g_type=-1), dict(p=0), dict(g=0), dict(m=0),
-                                 dict(v=0), dict(p_type=L.BF16, g_type=L.FP16), dict(p_type=L.FP16, g_type=L.BF16), dict(master=256), dict(step=0)])
+                                 dict(v=0), dict(p_type=L.BF16, g_type=L.FP16), dict(p_type=L.FP16, g_type=L.BF16), dict(master=256), dict(step=0), dict(m=264), dict(v=260),
+                                 dict(p_type=L.BF16, g_type=L.BF16, master=264)])
 def test_items_are_checked_before_a_launch(bad):
     t, s = item(**bad), a_set()
     assert step(a_call(t, s)) < 0 and COUNT[0] == 0
@@ -659,6 +660,9 @@ def test_states_that_are_taken_away_or_set_anew(cls):
     assert all(torch.equal(p, q) for p, q in zip(a, b)) and float(x.state[a[1]]["step"]) == 8
     x.state.pop(a[1])
     y.state.pop(b[1])
+    moment = x.state[a[0]]["exp_avg"]
+    odd = torch.empty(moment.numel() + 1, dtype=moment.dtype, device="cuda")[1:]
+    x.state[a[0]]["exp_avg"] = odd.copy_(moment)   # on no boundary
     both(3)
     assert all(torch.equal(p, q) for p, q in zip(a, b)) and float(x.state[a[0]]["step"]) == 3 and float(x.state[a[1]]["step"]) == 1
 
