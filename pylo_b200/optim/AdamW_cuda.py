@@ -14,6 +14,7 @@ import ctypes as C
 import math
 from array import array
 from collections import OrderedDict
+from itertools import chain
 from operator import attrgetter, is_, itemgetter
 
 import numpy as np
@@ -24,7 +25,9 @@ from .. import _lib as L
 from ..plan import current_stream_ptr, with_gradients
 from ._common import optimizer_step
 
-_numel, _data_ptr, _is_contiguous, _dtype = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.is_contiguous, attrgetter("dtype")   # for map: less per tensor
+# for map(): a loop of Python's own is a large part of a small model's step
+_numel, _data_ptr, _is_contiguous, _get_device = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.get_device
+_dtype, _grad = attrgetter("dtype"), attrgetter("grad")
 _moment_and_step = itemgetter("exp_avg", "step")
 
 TYPES = {torch.float32: L.FP32, torch.bfloat16: L.BF16, torch.float16: L.FP16}
@@ -81,7 +84,7 @@ class _Plan:
         # the table holds the addresses of these tensors: they stay alive with it, and it is good for them only
         self.params, self.every_state = params, list(state.values())
         self.states = states = [state[p] for p in params]
-        self.moments_and_steps = [x for st in states for x in _moment_and_step(st)]
+        self.moments_and_steps = list(chain.from_iterable(map(_moment_and_step, states)))
         self.table = t = np.zeros(len(params), dtype=L.ADAMW_DTYPE)
         t["p"], t["n"], t["p_type"] = self.p_ptrs, self.numels, [TYPES[d] for d in self.p_dtypes]
         ptr = lambda name: [st[name].data_ptr() if name in st else 0 for st in states]
@@ -97,13 +100,12 @@ class _Plan:
         self.sets, self.set_key, self.norm = None, None, None
 
     def good_for(self, params, group_of, flags, state):
-        same = lambda new, old: len(new) == len(old) and all(map(is_, new, old))
-        if not (same(params, self.params) and list(map(_data_ptr, params)) == self.p_ptrs and list(map(_numel, params)) == self.numels
-                and list(map(_dtype, params)) == self.p_dtypes and group_of == self.group_of and flags == self.flags
-                and same(state.values(), self.every_state)):
+        if not (len(params) == len(self.params) and all(map(is_, params, self.params)) and list(map(_data_ptr, params)) == self.p_ptrs
+                and list(map(_numel, params)) == self.numels and list(map(_dtype, params)) == self.p_dtypes and group_of == self.group_of
+                and flags == self.flags and len(state) == len(self.every_state) and all(map(is_, state.values(), self.every_state))):
             return False
         try:
-            return same([x for st in self.states for x in _moment_and_step(st)], self.moments_and_steps)
+            return all(map(is_, chain.from_iterable(map(_moment_and_step, self.states)), self.moments_and_steps))
         except KeyError:
             return False
 
@@ -312,7 +314,9 @@ class _AdamWFamily(Optimizer):
                 L.check(L.lib.pylo_b200_adamw_step(plan.call_ref, L.ADAMW_NORM, stream), "adamw_step")
                 torch.distributed.all_reduce(norm[:1], group=self.process_group)  # each rank holds its own tensors' share
                 phases = L.ADAMW_STEP
-        L.check(L.lib.pylo_b200_adamw_step(plan.call_ref, phases, stream), "adamw_step")
+        code = L.lib.pylo_b200_adamw_step(plan.call_ref, phases, stream)
+        if code:
+            L.check(code, "adamw_step")
         del copies
 
     def _fill_sets(self, plan):
@@ -391,7 +395,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"clip_grad_norm_: invalid max_norm: {max_norm}")
-    grads = [p.grad for p in ([parameters] if torch.is_tensor(parameters) else parameters)]
+    grads = list(map(_grad, [parameters] if torch.is_tensor(parameters) else parameters))
     if any([g is None for g in grads]):
         grads = [g for g in grads if g is not None]
     if not grads:
@@ -399,7 +403,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     at = grads[0].get_device()
     if at < 0:
         raise RuntimeError("clip_grad_norm_: gradients must live on a CUDA device (there is no CPU path)")
-    if not all([g.get_device() == at for g in grads]):
+    if any([d != at for d in map(_get_device, grads)]):
         raise RuntimeError("clip_grad_norm_: all gradients must live on one device")
     types = list(map(TYPES.get, map(_dtype, grads)))
     if None in types:
@@ -412,11 +416,16 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
 
 def _clip(grads, types, max_norm, error_if_nonfinite):
     parts = grads
-    if any([g.layout is not torch.strided for g in grads]):
-        raise RuntimeError("Sparse gradients not supported")
+    try:
+        ptrs = list(map(_data_ptr, grads))
+    except RuntimeError:
+        if any([g.layout is not torch.strided for g in grads]):
+            raise RuntimeError("Sparse gradients not supported") from None
+        raise
     if not all(map(_is_contiguous, grads)):
         parts = [g if g.is_contiguous() or _dense(g) else g.detach().contiguous() for g in grads]
-    ptrs, sizes = list(map(_data_ptr, parts)), list(map(_numel, parts))
+        ptrs = list(map(_data_ptr, parts))
+    sizes = list(map(_numel, parts))
     stream, call = current_stream_ptr(), L.lib.pylo_b200_clip_grads
     floats = L.norm_floats(len(ptrs), sum(sizes))
     norm = torch.empty(floats, dtype=torch.float32, device="cuda")
@@ -431,7 +440,8 @@ def _clip(grads, types, max_norm, error_if_nonfinite):
     if code == L.ERR_GRADS_NOT_IN_ORDER:
         ptrs, sizes, types = _distinct(ptrs, sizes, types)
         code, distinct = run(ptrs, sizes, types, limit, 1), 1
-    L.check(code, "clip_grads")
+    if code:
+        L.check(code, "clip_grads")
     if error_if_nonfinite:
         if not math.isfinite(float(total)):
             raise RuntimeError("The total norm of order 2.0 for gradients from `parameters` is non-finite, so it cannot be clipped. To disable this "
