@@ -552,7 +552,8 @@ typedef struct pylo_adamw_call {
   int32_t bits;        /* of the states: 32 or 8 */
   int32_t pad_;
 } pylo_adamw_call;
-int pylo_b200_sizeof_adamw_item(void);
+/* bytes of an item (0), a set (1), a call (2) */
+int pylo_b200_sizeof_adamw(int what);
 /* PYLO_ADAMW_NORM: the norm of all items' gradients.  PYLO_ADAMW_STEP: p *= 1 - lr wd; m = beta1 m + (1 - beta1) g;
  * v = beta2 v + (1 - beta2) g^2; p -= lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps).  Either phase or both in one call (then
  * norm[0] and norm[1] are not written if there are few partial sums); by themselves where norm[0] has to be summed over ranks in between. */

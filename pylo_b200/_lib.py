@@ -179,7 +179,7 @@ def _load():
         "pylo_b200_velo_rnn": [C.POINTER(VeloRnn), C.POINTER(VeloLoss), vp],
         "pylo_b200_velo_loss_features": [vp, vp, vp, vp, vp, vp, vp],
         "pylo_b200_step": [C.POINTER(StepPlan), C.POINTER(StepParams), i32, vp],
-        "pylo_b200_sizeof_adamw_item": [],
+        "pylo_b200_sizeof_adamw": [i32],
         "pylo_b200_adamw_step": [C.POINTER(AdamwCall), i32, vp],
         "pylo_b200_clip_grads": [vp, vp, vp, i32, f32, vp, C.c_int64, i32, vp],
         "pylo_b200_advance_steps": [vp, i32, C.POINTER(C.c_double), C.POINTER(C.c_int)],
@@ -191,7 +191,7 @@ def _load():
     if lib.pylo_b200_abi_version() != ABI_VERSION:
         raise ImportError("libpylo_b200.so was built from a different ABI version; rebuild it")
     if (lib.pylo_b200_sizeof_desc() != DESC_DTYPE.itemsize or lib.pylo_b200_sizeof_params() != C.sizeof(StepParams)
-            or lib.pylo_b200_sizeof_adamw_item() != ADAMW_DTYPE.itemsize):
+            or [lib.pylo_b200_sizeof_adamw(k) for k in range(3)] != [ADAMW_DTYPE.itemsize, C.sizeof(AdamwSet), C.sizeof(AdamwCall)]):
         raise ImportError("descriptor layout mismatch between the Python binding and libpylo_b200.so")
     return lib, sorted(sigs)
 

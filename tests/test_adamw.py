@@ -18,7 +18,7 @@ HALF = {torch.float32: H32, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11
 TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -25}   # half of the smallest step (or all of it)
 ROOTS = [(math.isqrt(q << 64) & 0xFFFFFFFF) | 1 for q in (2, 3, 5, 7, 11, 13, 17, 19, 23, 29, 31, 37, 41, 43, 47, 53)]
 LR, BETAS, EPS, WD = 1e-2, (0.9, 0.95), 1e-8, 0.1
-SIZES = [(1,), (7,), (256,), (257,), (3, 341), (64, 128), (40_003,)]
+SIZES = [(1,), (), (7,), (256,), (257,), (3, 341), (64, 128), (40_003,)]
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -911,6 +911,40 @@ def test_clipping_in_a_graph():
         check_clip([g], [new], norm, 1.0)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", [optim.AdamW_CUDA, optim.AdamW8bit_CUDA])
+def test_elements_behind_the_first_four_billion_bytes(cls):
+    """One tensor of more than 2^31 elements: its last ones get the step that a tensor of them alone gets (in 8 bits as far as the random rounding
+    goes, which takes an element's place into account), and count in the norm."""
+    if torch.cuda.get_device_properties(0).total_memory < 100 << 30:
+        pytest.skip("needs 60 GB")
+    n, k = 2 ** 31 + 2 ** 20, 2 ** 20 + 300
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda", dtype=torch.bfloat16))
+    p.grad = torch.zeros_like(p)
+    p.grad[-k:] = tensors([(k,)], torch.bfloat16, 1)[0]
+    p.data[-k:] = tensors([(k,)], torch.bfloat16, 2)[0]
+    q = torch.nn.Parameter(p.detach()[-k:].clone())
+    q.grad = p.grad[-k:].clone()
+    exact = math.sqrt(float(q.grad.double().square().sum()))
+    assert abs(float(optim.clip_grad_norm_(p, math.inf)) - exact) <= exact * 40 * H32
+    x, y = cls([p]), cls([q])
+    x.step()
+    y.step()
+    assert torch.equal(p[-k:], q) and not p[:-k].any()
+    st, want = x.state[p], y.state[q]
+    if cls is optim.AdamW_CUDA:
+        assert all(torch.equal(st[name][-k:], want[name]) for name in ("exp_avg", "exp_avg_sq"))
+    else:
+        assert (n - k) % 256 == 212   # blocks lie otherwise
+        for name in ("exp_avg", "exp_avg_sq_root"):
+            a, b = A.from_blocks(st[name][-k - 212:], st[name + "_scale"][(n - k) // 256:])[212:], A.from_blocks(want[name], want[name + "_scale"])
+            each = want[name + "_scale"].float().repeat_interleave(256)[:k]
+            # both within a step of a code: 2^-3 of the value (8 / 7 of the larger code at most), or 2^-9 of a scale (the largest value over 128 at most)
+            assert bool(((a - b).abs() <= 2.3 * 2.0 ** -3 * torch.maximum(a.abs(), b.abs()) + 4 * 2.0 ** -9 * torch.maximum(each, a.abs().amax() * 2.0 ** -7)).all())
+    del x, y, p, q, st, want
+    torch.cuda.empty_cache()
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------------------------------------------------
@@ -937,6 +971,32 @@ def test_a_training_loop(cls):
         assert any(not torch.equal(p, o) for p, o in zip(model.parameters(), old))
         for p in model.parameters():
             assert ("master" in opt.state[p]) == (p.dtype is torch.bfloat16)
+
+
+@pytest.mark.gpu
+def test_beside_a_learned_optimizer():
+    """Matrices through AdafacLO, vectors through AdamW, the gradients of both clipped together: each as by itself."""
+    from pylo_b200 import models
+
+    torch.manual_seed(1)
+    net = models.MetaMLP()
+    shapes = [(96, 64), (96,), (40, 96), (40,)]
+    a, b = params_of(shapes, torch.float32, 1), params_of(shapes, torch.float32, 1)
+    learned, plain = optim.AdafacLO_CUDA(a[::2], network=net), optim.AdamW8bit_CUDA(a[1::2])
+    alone, other = optim.AdafacLO_CUDA(b[::2], network=net), optim.AdamW8bit_CUDA(b[1::2])
+    for t in range(3):
+        set_grads(a, torch.float32, t)
+        for p, q in zip(a, b):
+            q.grad = p.grad.clone()
+        optim.clip_grad_norm_(a, 0.5)
+        plain.step()
+        learned.step()
+        optim.clip_grad_norm_(b, 0.5)
+        torch.cuda.synchronize()
+        alone.step()
+        torch.cuda.synchronize()
+        other.step()
+        assert all(torch.equal(p, q) for p, q in zip(a, b)), t
 
 
 @pytest.mark.gpu
