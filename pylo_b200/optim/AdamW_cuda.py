@@ -234,7 +234,7 @@ class _AdamWFamily(Optimizer):
             if x.dtype is not dtype and (dtype.itemsize == 1 or not x.dtype.is_floating_point):
                 raise ValueError(f"{self._name}: state {name!r} is {x.dtype}, not {dtype}")
             x = x.to(device=dev, dtype=dtype).contiguous()
-            st[name] = x.clone() if x.data_ptr() % 16 else x   # the kernels want it on a boundary
+            st[name] = x.clone() if x.data_ptr() % 16 and dtype is not _SCALES else x   # the kernels want all but scales on a boundary
 
     def _build(self, plist, group_of, flags, capturing):
         dev = plist[0].device if plist else None

@@ -636,6 +636,41 @@ def test_another_memory_behind_a_parameter(cls):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("cls", [optim.AdamW_CUDA, optim.AdamW8bit_CUDA])
+def test_states_in_the_callers_memory(cls):
+    """State tensors set before the first step, views into buffers of the caller's, are the ones that are updated."""
+    a, b = params_of([(300,), (1000,)], torch.bfloat16, 1), params_of([(300,), (1000,)], torch.bfloat16, 1)
+    x, y = cls(a, master_weights=True), cls(b, master_weights=True)
+    set_grads(b, torch.bfloat16, 2)
+    y.step()
+    buffers = {}
+    for p, q in zip(a, b):
+        p.grad = q.grad.clone()
+        x.state[p] = {}
+        for name, v in y.state[q].items():
+            if name == "step":
+                continue
+            room = torch.zeros(v.numel() * v.dtype.itemsize + 64, dtype=torch.uint8, device="cuda")
+            at = 3 if name.endswith("scale") else 16
+            view = room[at:at + v.numel() * v.dtype.itemsize].view(v.dtype).view(v.shape)
+            if name == "master":
+                view.copy_(p.detach())
+            elif at == 3:
+                view.view(torch.uint8).fill_(1)   # the least scale
+            x.state[p][name], buffers[p, name] = view, (room, at)
+    x.step()
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+        for name, v in y.state[q].items():
+            if name == "step":
+                continue
+            room, at = buffers[p, name]
+            n = v.numel() * v.dtype.itemsize
+            assert torch.equal(room[at:at + n], v.contiguous().view(-1).view(torch.uint8)), name
+            assert not room[:at].any() and not room[at + n:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", [optim.AdamW_CUDA, optim.AdamW8bit_CUDA])
 def test_states_that_are_taken_away_or_set_anew(cls):
     """A step goes by what the state holds now: cleared, it begins anew; a count or a tensor set by hand counts."""
     a, b = params_of([(300,), (20,)], torch.float32, 1), params_of([(300,), (20,)], torch.float32, 1)
