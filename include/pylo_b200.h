@@ -537,7 +537,7 @@ typedef struct pylo_adamw_item {
   int32_t pad_;
 } pylo_adamw_item;
 typedef struct pylo_adamw_set {
-  double lr, weight_decay, beta1, beta2, eps;
+  double lr, weight_decay, beta1, beta2, eps; /* eps > 0 with 8-bit states */
   double clip_norm;    /* > 0: gradients times clip_norm / max(norm, clip_norm), norm the root of call.norm[0] */
   const float* lr_dev; /* DEVICE scalar that stands for lr, or NULL */
   uint32_t seed;       /* of the random rounding of 8-bit states, which depends on seed, step and an element's place in its tensor only */
@@ -563,9 +563,9 @@ int pylo_b200_adamw_step(const pylo_adamw_call* call, int phases, void* stream);
 
 /* n_items gradients (contiguous; g, n, types: HOST arrays): norm[0] = sum of squares of all elements, norm[1] = its root, the same sums in
  * the same order on every call; then all elements times min(1, max_norm / (norm[1] + 1e-6)): nothing is written where that is 1, nor read for
- * max_norm = INFINITY.  norm: DEVICE, norm_floats as above.  distinct: the caller knows that no two share memory; else they have to come in
- * the order of their addresses, or the call is refused with PYLO_ERR_GRADS_NOT_IN_ORDER. */
-#define PYLO_ERR_GRADS_NOT_IN_ORDER (-5)
+ * max_norm = INFINITY.  norm: DEVICE, norm_floats as above.  distinct: the caller knows that no two share memory; else that is looked at, and
+ * the call refused with PYLO_ERR_GRADS_OVERLAP if two do, or if more than 1024 come in another order than that of their addresses. */
+#define PYLO_ERR_GRADS_OVERLAP (-5)
 int pylo_b200_clip_grads(void* const* g, const int64_t* n, const int32_t* types, int n_items, float max_norm, float* norm, int64_t norm_floats,
                          int distinct, void* stream);
 

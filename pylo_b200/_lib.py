@@ -57,7 +57,7 @@ ADAMW_DTYPE = np.dtype(
     + [("n", np.int64)] + [(name, np.int32) for name in ("p_type", "g_type", "set", "pad_")]
 )
 ADAMW_NORM, ADAMW_STEP = 1, 2
-ERR_GRADS_NOT_IN_ORDER = -5
+ERR_GRADS_OVERLAP = -5
 
 
 class AdamwSet(C.Structure):

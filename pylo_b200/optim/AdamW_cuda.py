@@ -151,6 +151,8 @@ class _AdamWFamily(Optimizer):
                                   ("clip_norm", group["clip_norm"], group["clip_norm"] > 0)):
             if not fine:
                 raise ValueError(f"{self._name}: invalid {name}: {value}")
+        if self._bits == 8 and group["eps"] == 0:
+            raise ValueError(f"{self._name}: eps must be positive (a second moment below the smallest normal number counts as zero)")
         if group.get("amsgrad"):
             raise ValueError(f"{self._name}: amsgrad is not supported")
 
@@ -173,9 +175,10 @@ class _AdamWFamily(Optimizer):
                 group.setdefault(name, value)
             self._check(group)
         for p, st in self.state.items():
-            for name, value in st.items():
+            for name, value in st.items() if isinstance(st, dict) else ():
                 if isinstance(value, _Kept):
-                    st[name] = value.value.detach().to(p.device if name != "step" else value.value.device, copy=True)
+                    own = torch.is_tensor(p) and name != "step"   # entries of no parameter stay as they are
+                    st[name] = value.value.detach().to(p.device if own else value.value.device, copy=True)
         self._reset()
 
     def load_state_dict(self, state_dict):
@@ -196,23 +199,33 @@ class _AdamWFamily(Optimizer):
         finally:
             self._optimizer_load_state_dict_pre_hooks = hooks
 
-    def _init_state(self, p, st, group):
-        """Make what a parameter's state lacks, and bring what it has into the form the kernels take."""
+    def _init_state(self, p, st, group, capturing):
+        """Make what a parameter's state lacks, and bring what it has into the form the kernels take.  Not in a capture, which would do it
+        again on every replay."""
         dev, n = p.device, p.numel()
         capturable = group["capturable"]
+
+        def changes():
+            if capturing:
+                raise RuntimeError(f"{self._name}: run a step before the one that is captured: a captured step would make its states anew on every replay")
+
         step, kind = st.get("step", 0.0), torch.float32 if capturable else torch.float64
         if not torch.is_tensor(step) or step.is_cuda != bool(capturable) or step.dim() != 0 or step.dtype is not kind:
+            changes()
             step = torch.tensor(float(step), dtype=kind, device=dev if capturable else "cpu")
-        elif capturable:
+        elif capturable and step.device != dev:
+            changes()
             step = step.to(dev)
         st["step"] = step
         if self._bits == 32:
             if "exp_avg_sq_root" in st:
+                changes()
                 st["exp_avg_sq"] = from_blocks(st.pop("exp_avg_sq_root"), st.pop("exp_avg_sq_root_scale")).square_()
                 st["exp_avg"] = from_blocks(st["exp_avg"], st.pop("exp_avg_scale"))
             wanted = {"exp_avg": (torch.float32, p.shape), "exp_avg_sq": (torch.float32, p.shape)}
         else:
             if "exp_avg_sq" in st:
+                changes()
                 st["exp_avg_sq_root"], st["exp_avg_sq_root_scale"] = to_blocks(st.pop("exp_avg_sq").to(torch.float32).sqrt())
                 st["exp_avg"], st["exp_avg_scale"] = to_blocks(st["exp_avg"])
             each = (blocks_of(n),)
@@ -221,20 +234,25 @@ class _AdamWFamily(Optimizer):
         if group["master_weights"] and p.dtype is not torch.float32:
             wanted["master"] = (torch.float32, p.shape)
             if "master" not in st:
+                changes()
                 st["master"] = p.detach().to(torch.float32).contiguous()
         else:
             st.pop("master", None)
         for name, (dtype, shape) in wanted.items():
             x = st.get(name)
             if x is None:
+                changes()
                 zero = 1 if dtype is _SCALES else 0   # the least scale there is
                 x = torch.full(shape, zero, dtype=torch.uint8, device=dev).view(dtype) if dtype.itemsize == 1 else torch.zeros(shape, dtype=dtype, device=dev)
             if tuple(x.shape) != tuple(shape):
                 raise ValueError(f"{self._name}: state {name!r} has shape {tuple(x.shape)}, the parameter's needs {tuple(shape)}")
             if x.dtype is not dtype and (dtype.itemsize == 1 or not x.dtype.is_floating_point):
                 raise ValueError(f"{self._name}: state {name!r} is {x.dtype}, not {dtype}")
-            x = x.to(device=dev, dtype=dtype).contiguous()
-            st[name] = x.clone() if x.data_ptr() % 16 and dtype is not _SCALES else x   # the kernels want all but scales on a boundary
+            y = x.to(device=dev, dtype=dtype).contiguous()
+            y = y.clone() if y.data_ptr() % 16 and dtype is not _SCALES else y   # the kernels want all but scales on a boundary
+            if y is not x:
+                changes()
+            st[name] = y
 
     def _build(self, plist, group_of, flags, capturing):
         dev = plist[0].device if plist else None
@@ -254,11 +272,8 @@ class _AdamWFamily(Optimizer):
         order = np.argsort(at)
         if len(at) and np.any(at[order][1:] < end[order][:-1]):
             raise ValueError(f"{self._name}: two parameters share memory")
-        states = [self.state[p] for p in plist]
-        if capturing and not all([len(st) for st in states]):
-            raise RuntimeError(f"{self._name}: run a step before the one that is captured: a captured step would make its states anew on every replay")
-        for p, st, gi in zip(plist, states, group_of):
-            self._init_state(p, st, self.param_groups[gi])
+        for p, gi in zip(plist, group_of):
+            self._init_state(p, self.state[p], self.param_groups[gi], capturing)
         return _Plan(plist, group_of, flags, self.state, self._bits)
 
     # ------------------------------------------------------------------ step
@@ -437,7 +452,7 @@ def _clip(grads, types, max_norm, error_if_nonfinite):
 
     limit = math.inf if error_if_nonfinite else max_norm   # the norm is looked at before anything is scaled
     code, distinct = run(ptrs, sizes, types, limit, 0), 0
-    if code == L.ERR_GRADS_NOT_IN_ORDER:
+    if code == L.ERR_GRADS_OVERLAP:
         ptrs, sizes, types = _distinct(ptrs, sizes, types)
         code, distinct = run(ptrs, sizes, types, limit, 1), 1
     if code:

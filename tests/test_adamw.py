@@ -154,6 +154,7 @@ def test_calls_are_checked_before_a_launch():
     for bad in (dict(items=None), dict(n_items=-1), dict(n_sets=-1), dict(n_sets=0), dict(sets=None), dict(bits=16), dict(bits=8)):   # the last: no scales
         assert step(a_call(t, s, **bad)) < 0, bad
     assert step(a_call(t, s), L.ADAMW_NORM) < 0 and step(a_call(t, s, norm=256, norm_floats=2), L.ADAMW_NORM) < 0   # no place for the norm
+    assert step(a_call(item(m_scale=256, v_scale=256), a_set(eps=0.0), bits=8)) < 0   # a root of zero is possible
     assert step(a_call(t, s, n_items=0)) == 0 and COUNT[0] == 0
     assert step(a_call(none, s)) == 0 and COUNT[0] == 1   # a tensor without elements takes its step too
     COUNT[0] = 0
@@ -167,7 +168,11 @@ def test_gradients_are_checked_before_a_launch():
     for bad in (dict(g=None), dict(n=None), dict(t=None), dict(count=-1), dict(limit=-1.0), dict(limit=math.nan), dict(norm=None), dict(floats=3), dict(n=np.array([128, -1])),
                 dict(t=np.array([0, 3], dtype=np.int32)), dict(t=np.array([-1, 0], dtype=np.int32)), dict(g=np.array([512, 0], dtype=np.uint64))):
         assert call(**bad) == -1, bad
-    assert call(g=g[::-1].copy()) == L.ERR_GRADS_NOT_IN_ORDER and call(n=np.array([129, 5])) == L.ERR_GRADS_NOT_IN_ORDER
+    assert call(n=np.array([129, 5])) == L.ERR_GRADS_OVERLAP and call(g=np.array([1024, 512], dtype=np.uint64), n=np.array([5, 300])) == L.ERR_GRADS_OVERLAP
+    many = 1025
+    apart = (np.arange(many, 0, -1) * 4096).astype(np.uint64)   # no two share memory, but there are too many to find out
+    assert call(g=apart, n=np.ones(many, dtype=np.int64), t=np.zeros(many, dtype=np.int32), count=many) == L.ERR_GRADS_OVERLAP
+    assert call(g=apart, n=np.ones(many, dtype=np.int64), t=np.zeros(many, dtype=np.int32), count=many, floats=0) in (-1, L.ERR_GRADS_OVERLAP)
 
 
 def test_there_is_no_path_without_a_gpu():
@@ -402,13 +407,13 @@ def test_a_root_that_is_not_zero_stays_so():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
-@pytest.mark.parametrize("count", [43, 44, 45, 400, 430])
+@pytest.mark.parametrize("count", [12, 179, 231, 690])   # a launch takes 180 (8-bit) or 224 of a kind; one kind, or three
 def test_many_tensors_and_many_sets(bits, count):
     """More tensors and more sets of hyper-parameters than a launch takes, steps that differ, tensors without elements and without
     gradients: the same as one optimizer for each tensor, to the last bit."""
     cls = optim.AdamW_CUDA if bits == 32 else optim.AdamW8bit_CUDA
     shapes = [(i % 7 * 61,) if i % 5 else (3, i + 1) for i in range(count)]
-    kinds = [torch.float32, torch.bfloat16, torch.float16]
+    kinds = [torch.float32, torch.bfloat16, torch.float16] if count % 10 == 0 else [torch.float32] * 3
     make = lambda: [torch.nn.Parameter(tensors([s], kinds[i % 3], i)[0]) for i, s in enumerate(shapes)]
     a, b = make(), make()
     group = lambda ps, k: dict(params=ps, lr=1e-3 * (k + 1), weight_decay=0.01 * k, betas=(0.8 + 0.01 * k, 0.9))
@@ -572,6 +577,10 @@ def test_what_is_refused(cls):
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(eps=-1e-8), dict(weight_decay=-1.0), dict(clip_norm=0.0)):
         with pytest.raises(ValueError):
             cls([p], **bad)
+
+    if cls is optim.AdamW8bit_CUDA:
+        with pytest.raises(ValueError, match="eps"):
+            cls([p], eps=0.0)
 
     def refused(params, match, error=RuntimeError):
         for q in params:
@@ -806,6 +815,31 @@ def test_captures_that_are_refused(cls):
 
 
 @pytest.mark.gpu
+def test_states_are_not_converted_in_a_capture():
+    """Loaded states of the other width would be converted on every replay: refused, and possible after a step."""
+    a = params_of([(300,)], torch.float32, 1)
+    set_grads(a, torch.float32, 2)
+    x = optim.AdamW_CUDA(a)
+    x.step()
+    y = optim.AdamW8bit_CUDA(a, capturable=True)
+    y.load_state_dict(x.state_dict())
+    for group in y.param_groups:
+        group["capturable"] = True
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="run a step before"):
+        with torch.cuda.graph(graph):
+            torch.ones(1, device="cuda").add_(1)
+            y.step()
+    y.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float(y.state[a[0]]["step"]) == 3
+
+
+@pytest.mark.gpu
 def test_two_graphs_of_two_optimizers_run_beside_each_other():
     """Each has its own norm's workspace."""
     runs = []
@@ -870,10 +904,11 @@ def test_clipping(kinds, odd, max_norm):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("count", [44, 45, 1537, 3200])
-def test_clipping_of_many_gradients(count):
+@pytest.mark.parametrize("backwards", [False, True])
+@pytest.mark.parametrize("count", [44, 801, 1024, 1025, 3200])
+def test_clipping_of_many_gradients(count, backwards):
     flat = torch.randn(count * 37, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
-    grads = [flat[37 * i:37 * i + 30 + i % 8] for i in range(count)]
+    grads = [flat[37 * i:37 * i + 30 + i % 8] for i in range(count)][::-1 if backwards else 1]
     before = [g.clone() for g in grads]
     gaps = flat.clone()
     check_clip(grads, before, optim.clip_grad_norm_(with_grads(grads), 0.5), 0.5)
