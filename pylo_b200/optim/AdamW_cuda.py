@@ -410,19 +410,18 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"clip_grad_norm_: invalid max_norm: {max_norm}")
-    grads = list(map(_grad, [parameters] if torch.is_tensor(parameters) else parameters))
-    if any([g is None for g in grads]):
-        grads = [g for g in grads if g is not None]
+    grads = [g for g in map(_grad, [parameters] if torch.is_tensor(parameters) else parameters) if g is not None]
     if not grads:
         return torch.tensor(0.0)
     at = grads[0].get_device()
     if at < 0:
         raise RuntimeError("clip_grad_norm_: gradients must live on a CUDA device (there is no CPU path)")
-    if any([d != at for d in map(_get_device, grads)]):
+    if set(map(_get_device, grads)) != {at}:
         raise RuntimeError("clip_grad_norm_: all gradients must live on one device")
-    types = list(map(TYPES.get, map(_dtype, grads)))
-    if None in types:
-        raise RuntimeError(f"clip_grad_norm_: gradients must be fp32, bf16 or fp16, got {grads[types.index(None)].dtype}")
+    dtypes = list(map(_dtype, grads))
+    if not TYPES.keys() >= set(dtypes):
+        raise RuntimeError(f"clip_grad_norm_: gradients must be fp32, bf16 or fp16, got {next(d for d in dtypes if d not in TYPES)}")
+    types = list(map(TYPES.__getitem__, dtypes))
     if at != torch._C._cuda_getDevice():
         with torch.cuda.device(at):
             return _clip(grads, types, max_norm, error_if_nonfinite)
@@ -444,11 +443,11 @@ def _clip(grads, types, max_norm, error_if_nonfinite):
     stream, call = current_stream_ptr(), L.lib.pylo_b200_clip_grads
     floats = L.norm_floats(len(ptrs), sum(sizes))
     norm = torch.empty(floats, dtype=torch.float32, device="cuda")
-    total = norm[1]
+    at = norm.data_ptr()
 
     def run(ptrs, sizes, types, limit, distinct):
         g, n, t = array("Q", ptrs), array("q", sizes), array("i", types)
-        return call(g.buffer_info()[0], n.buffer_info()[0], t.buffer_info()[0], len(ptrs), limit, norm.data_ptr(), floats, distinct, stream)
+        return call(g.buffer_info()[0], n.buffer_info()[0], t.buffer_info()[0], len(ptrs), limit, at, floats, distinct, stream)
 
     limit = math.inf if error_if_nonfinite else max_norm   # the norm is looked at before anything is scaled
     code, distinct = run(ptrs, sizes, types, limit, 0), 0
@@ -457,6 +456,7 @@ def _clip(grads, types, max_norm, error_if_nonfinite):
         code, distinct = run(ptrs, sizes, types, limit, 1), 1
     if code:
         L.check(code, "clip_grads")
+    total = norm[1]
     if error_if_nonfinite:
         if not math.isfinite(float(total)):
             raise RuntimeError("The total norm of order 2.0 for gradients from `parameters` is non-finite, so it cannot be clipped. To disable this "
