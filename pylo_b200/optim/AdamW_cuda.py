@@ -15,7 +15,7 @@ import math
 from array import array
 from collections import OrderedDict
 from itertools import chain
-from operator import attrgetter, is_, itemgetter
+from operator import attrgetter, is_
 
 import numpy as np
 import torch
@@ -28,7 +28,6 @@ from ._common import optimizer_step
 # for map(): a loop of Python's own is a large part of a small model's step
 _numel, _data_ptr, _is_contiguous, _get_device = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.get_device
 _dtype, _grad = attrgetter("dtype"), attrgetter("grad")
-_moment_and_step = itemgetter("exp_avg", "step")
 
 TYPES = {torch.float32: L.FP32, torch.bfloat16: L.BF16, torch.float16: L.FP16}
 _CODES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -84,7 +83,7 @@ class _Plan:
         # the table holds the addresses of these tensors: they stay alive with it, and it is good for them only
         self.params, self.every_state = params, list(state.values())
         self.states = states = [state[p] for p in params]
-        self.moments_and_steps = list(chain.from_iterable(map(_moment_and_step, states)))
+        self.tensors = list(chain.from_iterable(map(dict.values, states)))
         self.table = t = np.zeros(len(params), dtype=L.ADAMW_DTYPE)
         t["p"], t["n"], t["p_type"] = self.p_ptrs, self.numels, [TYPES[d] for d in self.p_dtypes]
         ptr = lambda name: [st[name].data_ptr() if name in st else 0 for st in states]
@@ -104,10 +103,8 @@ class _Plan:
                 and list(map(_numel, params)) == self.numels and list(map(_dtype, params)) == self.p_dtypes and group_of == self.group_of
                 and flags == self.flags and len(state) == len(self.every_state) and all(map(is_, state.values(), self.every_state))):
             return False
-        try:
-            return all(map(is_, chain.from_iterable(map(_moment_and_step, self.states)), self.moments_and_steps))
-        except KeyError:
-            return False
+        tensors = list(chain.from_iterable(map(dict.values, self.states)))
+        return len(tensors) == len(self.tensors) and all(map(is_, tensors, self.tensors))
 
     def look_at(self, grads):
         """Put the gradients' addresses and types into the table; returns the copies that stand in for some of them."""
@@ -313,6 +310,9 @@ class _AdamWFamily(Optimizer):
             raise RuntimeError(f"{self._name}: a step can be captured into a graph only with capturable=True")
         plan = self._plan
         if plan is None or not plan.good_for(plist, group_of, flags, self.state):
+            for p, g in zip(plist, grads):
+                if g.shape != p.shape:   # of a parameter whose memory was exchanged since
+                    raise RuntimeError(f"{self._name}: a gradient has shape {tuple(g.shape)}, its parameter {tuple(p.shape)}")
             plan = self._plan = self._build(plist, group_of, flags, capturing)
         stream = current_stream_ptr()
         copies = plan.look_at(grads)

@@ -604,6 +604,11 @@ def test_what_is_refused(cls):
     opt = cls([p])
     p.grad = torch.zeros_like(p)
     opt.step()
+    whole, p.data = p.data, p.data[:4]   # at the same address
+    with pytest.raises(RuntimeError, match="gradient has shape"):
+        opt.step()
+    p.data = whole
+    opt.step()
     opt.state[p]["exp_avg"] = opt.state[p]["exp_avg"][:4]
     with pytest.raises(ValueError, match="shape"):
         opt.step()
@@ -709,6 +714,17 @@ def test_states_that_are_taken_away_or_set_anew(cls):
     x.state[a[0]]["exp_avg"] = odd.copy_(moment)   # on no boundary
     both(3)
     assert all(torch.equal(p, q) for p, q in zip(a, b)) and float(x.state[a[0]]["step"]) == 3 and float(x.state[a[1]]["step"]) == 1
+    for k, name in enumerate(n for n in y.state[b[0]] if n != "step"):   # each of them by another tensor, what was there gone
+        x.state[a[0]][name] = y.state[b[0]][name].clone()
+        gone = [torch.full((301,), 255, dtype=torch.uint8, device="cuda") for _ in range(64)]   # over the memory that was given back
+        both(4 + k)
+        assert all(torch.equal(p, q) for p, q in zip(a, b)), name
+        del gone
+    x.state[a[1]].popitem()   # the last of all: made anew
+    last = list(y.state[b[1]])[-1]
+    y.state[b[1]].pop(last)
+    both(20)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and last in x.state[a[1]]
 
 
 @pytest.mark.gpu
