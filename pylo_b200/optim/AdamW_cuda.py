@@ -421,7 +421,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     dtypes = list(map(_dtype, grads))
     if not TYPES.keys() >= set(dtypes):
         raise RuntimeError(f"clip_grad_norm_: gradients must be fp32, bf16 or fp16, got {next(d for d in dtypes if d not in TYPES)}")
-    types = list(map(TYPES.__getitem__, dtypes))
+    types = array("i", map(TYPES.__getitem__, dtypes))
     if at != torch._C._cuda_getDevice():
         with torch.cuda.device(at):
             return _clip(grads, types, max_norm, error_if_nonfinite)
@@ -431,29 +431,27 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
 def _clip(grads, types, max_norm, error_if_nonfinite):
     parts = grads
     try:
-        ptrs = list(map(_data_ptr, grads))
+        if not all(map(_is_contiguous, grads)):
+            parts = [g if g.is_contiguous() or _dense(g) else g.detach().contiguous() for g in grads]
+        ptrs = array("Q", map(_data_ptr, parts))
     except RuntimeError:
         if any([g.layout is not torch.strided for g in grads]):
             raise RuntimeError("Sparse gradients not supported") from None
         raise
-    if not all(map(_is_contiguous, grads)):
-        parts = [g if g.is_contiguous() or _dense(g) else g.detach().contiguous() for g in grads]
-        ptrs = list(map(_data_ptr, parts))
-    sizes = list(map(_numel, parts))
-    stream, call = current_stream_ptr(), L.lib.pylo_b200_clip_grads
+    sizes = array("q", map(_numel, parts))
+    stream = current_stream_ptr()
     floats = L.norm_floats(len(ptrs), sum(sizes))
     norm = torch.empty(floats, dtype=torch.float32, device="cuda")
     at = norm.data_ptr()
 
-    def run(ptrs, sizes, types, limit, distinct):
-        g, n, t = array("Q", ptrs), array("q", sizes), array("i", types)
-        return call(g.buffer_info()[0], n.buffer_info()[0], t.buffer_info()[0], len(ptrs), limit, at, floats, distinct, stream)
+    def run(limit, distinct):
+        return L.lib.pylo_b200_clip_grads(ptrs.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], len(ptrs), limit, at, floats, distinct, stream)
 
     limit = math.inf if error_if_nonfinite else max_norm   # the norm is looked at before anything is scaled
-    code, distinct = run(ptrs, sizes, types, limit, 0), 0
+    code, distinct = run(limit, 0), 0
     if code == L.ERR_GRADS_OVERLAP:
-        ptrs, sizes, types = _distinct(ptrs, sizes, types)
-        code, distinct = run(ptrs, sizes, types, limit, 1), 1
+        ptrs, sizes, types = (array(kind, x) for kind, x in zip("Qqi", _distinct(ptrs, sizes, types)))
+        code, distinct = run(limit, 1), 1
     if code:
         L.check(code, "clip_grads")
     total = norm[1]
@@ -462,7 +460,7 @@ def _clip(grads, types, max_norm, error_if_nonfinite):
             raise RuntimeError("The total norm of order 2.0 for gradients from `parameters` is non-finite, so it cannot be clipped. To disable this "
                                "error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
         if max_norm < math.inf:
-            L.check(run(ptrs, sizes, types, max_norm, distinct), "clip_grads")
+            L.check(run(max_norm, distinct), "clip_grads")
     if parts is not grads and max_norm < math.inf:
         with torch.no_grad():
             for g, part in zip(grads, parts):
@@ -473,7 +471,7 @@ def _clip(grads, types, max_norm, error_if_nonfinite):
 
 def _distinct(ptrs, sizes, types):
     """Every gradient once, in the order given; two that share only a part of their memory are refused."""
-    g, n, t = np.array(ptrs, dtype=np.uint64), np.array(sizes, dtype=np.uint64), np.array(types)
+    g, n, t = np.array(ptrs, dtype=np.uint64), np.array(sizes, dtype=np.uint64), np.array(types, dtype=np.int64)
     order = np.argsort(g, kind="stable")
     order = order[n[order] > 0]
     first, end = g[order], (g + n * np.array([4, 2, 2], dtype=np.uint64)[t])[order]

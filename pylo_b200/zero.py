@@ -464,11 +464,11 @@ class StagedShardedStep(_GradIntake):
 def sharded_optimizer(cls, shard: ShardedStep, **kwargs):
     """Build ``cls`` over the tensors this rank owns, wired for the exchanges its family needs.
 
-    * CELO2 / ELO_CELO2 / ELO with ``clip_grad``: the global gradient norm is the sum over ranks
+    * CELO2 / ELO_CELO2 / ELO / AdamW (either width) with ``clip_grad``: the global gradient norm is the sum over ranks
       (one scalar all-reduce per step).
     * VeLO: the per-tensor LSTM inputs of all tensors are summed over ranks ([T, 30] floats) and every
       rank runs the LSTM for all T tensors; pass the same ``loss`` on every rank.
-    * AdafacLO needs nothing.
+    * AdafacLO, and AdamW without ``clip_grad``, need nothing.
     Call ``shard.gather()`` after ``optimizer.step()``.
     """
     params = [shard.params[i] for i in shard.owned]

@@ -1108,3 +1108,40 @@ def test_through_a_sharded_step(cls):
     new.load_state_dict(full)
     set_grads(b, torch.float32, 5)
     new.step()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", [optim.AdamW_CUDA, optim.AdamW8bit_CUDA])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_norm_that_is_summed_over_ranks(cls, capturable, monkeypatch):
+    """Two optimizers with half of the tensors each, the exchange of their sums of squares played by hand: each rank's sum is that of its own
+    gradients, the step goes by both."""
+    shapes = [(300, 200), (77,), (1000,), (5, 5)]
+    params = params_of(shapes, torch.float32, 1)
+    set_grads(params, torch.float32, 2)
+    old = [p.detach().clone() for p in params]
+    squares = [float(p.grad.double().square().sum()) for p in params]
+    norm = math.sqrt(sum(squares))
+    said = []
+    for mine in ((0, 1), (2, 3)):
+        opt = cls([params[i] for i in mine], lr=LR, betas=BETAS, eps=EPS, weight_decay=WD, clip_grad=True, clip_norm=0.5, capturable=capturable)
+        opt._sharded = True
+        own, rest = (sum(squares[i] for i in range(4) if (i in mine) == side) for side in (True, False))
+
+        def exchange(t, group=None):
+            said.append(abs(float(t) - own) <= own * 80 * H32)   # a sum of squares: twice a norm's error
+            t.add_(rest)
+
+        monkeypatch.setattr(torch.distributed, "is_initialized", lambda: True)
+        monkeypatch.setattr(torch.distributed, "all_reduce", exchange)
+        opt.step()
+        monkeypatch.undo()
+        for i in mine:
+            z = torch.zeros(shapes[i], device="cuda")
+            if cls is optim.AdamW_CUDA and not capturable:
+                st = opt.state[params[i]]
+                check_32(params[i].detach(), st["exp_avg"], st["exp_avg_sq"], (old[i], z, z), params[i].grad, 1, gs=0.5 / norm, gs_err=40 * H32)
+            else:
+                pe, _, _, upd = exact_step(old[i], params[i].grad.double() * 0.5 / norm, z, z, 1)
+                close(params[i].detach(), pe, upd * 200 * H32 + old[i].double().abs() * 4 * H32)   # 16 + 2 x 40 of the norm, the device's own factors
+    assert said == [True, True]
