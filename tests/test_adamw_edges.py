@@ -1,0 +1,73 @@
+"""AdamW and clipping where it is easy to go wrong: codes that hang on one rounding, memory that is exchanged under the same tensors,
+arguments at the ends of their ranges."""
+
+import pytest
+import torch
+
+from pylo_b200 import optim
+from pylo_b200.optim import AdamW_cuda as A
+from test_adamw import BETAS, EPS, LR, WD, random_parts
+
+WIDTHS = [optim.AdamW_CUDA, optim.AdamW8bit_CUDA]
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the 8-bit step, operation by operation
+# ---------------------------------------------------------------------------------------------------------------------
+def written_out(m, u, g, betas=BETAS):
+    """New moments and roots in fp32, every operation rounded by itself (on the CPU)."""
+    b1, b2 = betas
+    return b1 * m + (1 - b1) * g, torch.sqrt(b2 * (u * u) + (1 - b2) * (g * g))
+
+
+def encoded(x, parts, least):
+    """Values of the codes, and the scales' bytes, of finite fp32 values: the sum of a float's bits and random ones, cut off."""
+    n = x.numel()
+    b = torch.zeros(-(-n // 256) * 256)
+    b[:n] = x
+    b = b.view(-1, 256)
+    e = (b.abs().amax(1).view(torch.int32) >> 23).clamp(min=8)
+    t = (b.abs().double() * torch.exp2((141 - 127 - e).double())[:, None]).float()   # rounded once, where it is subnormal
+    bits = torch.zeros(b.numel(), dtype=torch.int64)
+    bits[:n] = (parts * 2 ** 24).long()
+    code = ((t.view(torch.int32).long() << 4) + bits.view(-1, 256)) >> 24
+    code = torch.maximum(code, (b != 0) * least)
+    value = code.to(torch.uint8).view(torch.float8_e4m3fn).float() * torch.where(b < 0, -1.0, 1.0)
+    return value.view(-1)[:n], (e - 7).to(torch.uint8)
+
+
+def one_step_8(m, u, g, t=10, seed=3, **kw):
+    """One step of AdamW8bit_CUDA from moments and roots (fp32 on the CPU) that are rounded to codes first: (optimizer's state, parameter,
+    the moments and roots that the codes stood for)."""
+    p = torch.nn.Parameter(torch.zeros(g.numel(), device="cuda"))
+    p.grad = g.to("cuda", torch.float32)
+    opt = optim.AdamW8bit_CUDA([p], **{**dict(lr=LR, betas=BETAS, eps=EPS, weight_decay=WD, seed=seed), **kw})
+    st = {"step": torch.tensor(t - 1.0, dtype=torch.float64)}
+    old = []
+    for name, x in (("exp_avg", m), ("exp_avg_sq_root", u)):
+        codes, scales = A.to_blocks(x)
+        old.append(A.from_blocks(codes, scales))
+        st[name], st[name + "_scale"] = codes.cuda(), scales.cuda()
+    opt.state[p] = st
+    opt.step()
+    return opt.state[p], p.detach().cpu(), old
+
+
+def check_written_out(st, name, want, n, t, seed, first, least):
+    value, scale = encoded(want, random_parts(n, seed, t, first), least)
+    assert torch.equal(st[name + "_scale"].cpu().view(torch.uint8), scale)
+    assert torch.equal(st[name].cpu().float(), value)
+
+
+@pytest.mark.gpu
+def test_moments_that_cancel_have_the_codes_of_the_operations_written_out():
+    """b1 m + (1 - b1) g where both are as large: what is left is their roundings, and one rounding more or less is another code or scale."""
+    n = 256 * 64 + 77
+    gen = torch.Generator().manual_seed(1)
+    m0, u0 = torch.randn(n, generator=gen), torch.rand(n, generator=gen)
+    m0 = A.from_blocks(*A.to_blocks(m0))
+    g = -9 * m0 * (1 + 1e-6 * torch.randn(n, generator=gen))
+    st, _, (m, u) = one_step_8(m0, u0, g)
+    want, _ = written_out(m, u, g)
+    assert want.abs().max() < 1e-4
+    check_written_out(st, "exp_avg", want, n, 10, 3, 8, 0)
