@@ -71,3 +71,36 @@ def test_moments_that_cancel_have_the_codes_of_the_operations_written_out():
     want, _ = written_out(m, u, g)
     assert want.abs().max() < 1e-4
     check_written_out(st, "exp_avg", want, n, 10, 3, 8, 0)
+
+
+def near_powers():
+    """Gradients whose root of v, from nothing, is within a few last places of a power of two: on its other side is another scale."""
+    blocks = []
+    for k in range(-40, 12):
+        at = (torch.tensor(2.0 ** k, dtype=torch.float64) / (1 - BETAS[1]) ** 0.5).float()
+        g = torch.zeros(17, 256)
+        g[:, 0] = (at.view(torch.int32) + torch.arange(-8, 9, dtype=torch.int32)).view(torch.float32)
+        blocks.append(g.view(-1))
+    return torch.cat(blocks)
+
+
+def many_sizes():
+    """Blocks of gradients from 1 down to where squares have few bits or none, wide blocks and narrow ones."""
+    gen = torch.Generator().manual_seed(4)
+    block = torch.arange(400)
+    size = 10.0 ** -(block % 25)[:, None]
+    wide = 10.0 ** (-8 * torch.rand(400, 256, generator=gen) * (block % 2)[:, None])
+    return (torch.randn(400, 256, generator=gen) * size * wide).view(-1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", [near_powers, many_sizes, lambda: torch.randn(1 << 23, generator=torch.Generator().manual_seed(5))],
+                         ids=["near powers of two", "many sizes", "many"])
+def test_roots_have_the_codes_of_the_operations_written_out(what):
+    g = what()
+    u0 = torch.zeros_like(g) if what is near_powers else g.abs() * torch.rand(g.numel(), generator=torch.Generator().manual_seed(6))
+    st, p, (m, u) = one_step_8(g / 3, u0, g)
+    want_m, want_u = written_out(m, u, g)
+    check_written_out(st, "exp_avg", want_m, g.numel(), 10, 3, 8, 0)
+    check_written_out(st, "exp_avg_sq_root", want_u, g.numel(), 10, 3, 0, 1)
+    assert bool(p.isfinite().all())
