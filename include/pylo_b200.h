@@ -537,7 +537,7 @@ typedef struct pylo_adamw_item {
   int32_t pad_;
 } pylo_adamw_item;
 typedef struct pylo_adamw_set {
-  double lr, weight_decay, beta1, beta2, eps; /* eps > 0 with 8-bit states */
+  double lr, weight_decay, beta1, beta2, eps; /* eps >= 2^-126 in fp32 with 8-bit states */
   double clip_norm;    /* > 0: gradients times clip_norm / max(norm, clip_norm), norm the root of call.norm[0] */
   const float* lr_dev; /* DEVICE scalar that stands for lr, or NULL */
   uint32_t seed;       /* of the random rounding of 8-bit states, which depends on seed, step and an element's place in its tensor only */

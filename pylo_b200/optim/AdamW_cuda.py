@@ -148,8 +148,8 @@ class _AdamWFamily(Optimizer):
                                   ("clip_norm", group["clip_norm"], group["clip_norm"] > 0)):
             if not fine:
                 raise ValueError(f"{self._name}: invalid {name}: {value}")
-        if self._bits == 8 and group["eps"] == 0:
-            raise ValueError(f"{self._name}: eps must be positive (a second moment below the smallest normal number counts as zero)")
+        if self._bits == 8 and group["eps"] < 2.0 ** -126:
+            raise ValueError(f"{self._name}: eps must be positive, 2^-126 at least (the step's reciprocal takes a smaller one for zero)")
         if group.get("amsgrad"):
             raise ValueError(f"{self._name}: amsgrad is not supported")
 

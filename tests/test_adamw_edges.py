@@ -6,6 +6,7 @@ import torch
 
 from pylo_b200 import optim
 from pylo_b200.optim import AdamW_cuda as A
+import test_adamw as T
 from test_adamw import BETAS, EPS, LR, WD, random_parts
 
 WIDTHS = [optim.AdamW_CUDA, optim.AdamW8bit_CUDA]
@@ -104,3 +105,33 @@ def test_roots_have_the_codes_of_the_operations_written_out(what):
     check_written_out(st, "exp_avg", want_m, g.numel(), 10, 3, 8, 0)
     check_written_out(st, "exp_avg_sq_root", want_u, g.numel(), 10, 3, 0, 1)
     assert bool(p.isfinite().all())
+
+
+@pytest.mark.parametrize("eps", [1e-40, 1.1e-38, 5e-324])
+def test_an_eps_that_is_no_normal_number_is_refused_with_8_bits(eps):
+    t = T.item(m_scale=256, v_scale=256)
+    assert T.step(T.a_call(t, T.a_set(eps=eps), bits=8)) < 0
+    assert T.COUNT[0] == 0
+    if torch.cuda.is_available():
+        with pytest.raises(ValueError, match="eps"):
+            optim.AdamW8bit_CUDA([torch.nn.Parameter(torch.zeros(3, device="cuda"))], eps=eps)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eps", [2.0 ** -126, 1e-30, 1e-20, 1e-15, 1e-8])
+def test_an_eps_that_is_smaller_than_roots(eps):
+    """Gradients whose squares are no normal numbers, beside ones of 1 and none at all: the update goes by their roots, not by eps alone."""
+    g = torch.zeros(5, 256)
+    g[0] = torch.linspace(1, 2, 256) * 1e-20
+    g[1, :128] = 1.0
+    g[1, 128:] = torch.linspace(1, 2, 128) * 1e-21
+    g[2, ::3] = -3e-19
+    g[3] = torch.logspace(-22, 0, 256)
+    g = g.view(-1)
+    zero = torch.zeros_like(g)
+    st, p, _ = one_step_8(zero, zero, g, t=1, eps=eps, weight_decay=0.0)
+    m, u = (x.double() for x in written_out(zero, zero, g))
+    want = -LR / (1 - BETAS[0]) * m / (u / (1 - BETAS[1]) ** 0.5 + eps)
+    # the factors' roundings: lr / bc1, 1 / root of bc2, product and sum, reciprocal (one place off), quotient, product, result: two half steps each at most
+    assert bool(((p.double() - want).abs() <= want.abs() * 16 * 2.0 ** -24 + 2.0 ** -149).all())
+    assert bool((p[g == 0] == 0).all())
