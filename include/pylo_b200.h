@@ -538,7 +538,7 @@ typedef struct pylo_adamw_item {
 } pylo_adamw_item;
 typedef struct pylo_adamw_set {
   double lr, weight_decay, beta1, beta2, eps; /* eps >= 2^-126 in fp32 with 8-bit states */
-  double clip_norm;    /* > 0: gradients times clip_norm / max(norm, clip_norm), norm the root of call.norm[0] */
+  double clip_norm;    /* > 0: gradients times clip_norm / max(norm, clip_norm), norm the root of call.norm[0]; 0, or infinite as fp32: as they are */
   const float* lr_dev; /* DEVICE scalar that stands for lr, or NULL */
   uint32_t seed;       /* of the random rounding of 8-bit states, which depends on seed, step and an element's place in its tensor only */
   int32_t maximize;

@@ -290,7 +290,7 @@ class _AdamWFamily(Optimizer):
             plist += ps
             grads += gs
             group_of += [gi] * len(ps)
-        clip = any([g["clip_grad"] for g in groups])
+        clip = any([g["clip_grad"] and g["clip_norm"] < math.inf for g in groups])
         if plist or clip:
             at = plist[0].get_device() if plist else -1
             if at >= 0 and at != torch._C._cuda_getDevice():
@@ -358,7 +358,7 @@ class AdamW_CUDA(_AdamWFamily):
     ``master_weights``: the state of a bf16 or fp16 parameter holds an fp32 copy (``master``), made from it in its first step,
     which the steps update; the parameter is its rounded value.  ``clip_grad``, ``clip_norm``: gradients are scaled by
     ``clip_norm / max(norm, clip_norm)`` within the step, with the norm over the gradients of all groups (they are left as
-    they are in memory).  ``capturable``: the step count lives on the device, as may ``lr``, and a step can be captured into a graph."""
+    they are in memory; ``clip_norm = inf`` clips nothing).  ``capturable``: the step count lives on the device, as may ``lr``, and a step can be captured into a graph."""
 
     _name = "AdamW_CUDA"
 

@@ -1,6 +1,8 @@
 """AdamW and clipping where it is easy to go wrong: codes that hang on one rounding, memory that is exchanged under the same tensors,
 arguments at the ends of their ranges."""
 
+import math
+
 import pytest
 import torch
 
@@ -135,3 +137,42 @@ def test_an_eps_that_is_smaller_than_roots(eps):
     # the factors' roundings: lr / bc1, 1 / root of bc2, product and sum, reciprocal (one place off), quotient, product, result: two half steps each at most
     assert bool(((p.double() - want).abs() <= want.abs() * 16 * 2.0 ** -24 + 2.0 ** -149).all())
     assert bool((p[g == 0] == 0).all())
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# clipping
+# ---------------------------------------------------------------------------------------------------------------------
+def test_a_set_without_a_limit_needs_no_norm():
+    t = T.item(n=0)   # nothing is launched
+    T.COUNT[0] = 0
+    assert T.step(T.a_call(t, T.a_set(clip_norm=1.0))) < 0
+    for none in (0.0, math.inf, 1e39):
+        assert T.step(T.a_call(t, T.a_set(clip_norm=none))) == 0
+    T.COUNT[0] = 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", WIDTHS)
+@pytest.mark.parametrize("mixed", [False, True])
+@pytest.mark.parametrize("clip_norm", [math.inf, 1e39, 1.7e308])
+def test_an_infinite_clipping_norm_clips_nothing(cls, clip_norm, mixed):
+    res = []
+    for clip in (False, True):
+        params = T.params_of([(700,), (30, 40)], torch.float32, 1)
+        groups = [dict(params=params[:1], clip_norm=0.1), dict(params=params[1:], clip_grad=clip)] if mixed else params
+        opt = cls(groups, clip_grad=clip or mixed, clip_norm=clip_norm)
+        for t in range(2):
+            T.set_grads(params, torch.float32, 2 + t)
+            opt.step()
+        res.append(params)
+    assert all(torch.equal(x, y) for x, y in zip(*res)) and bool(res[0][0].isfinite().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", WIDTHS)
+def test_a_clipping_norm_too_small_for_a_float_clips(cls):
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = cls([p], clip_grad=True, clip_norm=1e-60)
+    opt.step()
+    assert not opt.state[p]["exp_avg"].float().any()   # 2^-149 / norm is below half of the smallest float
