@@ -78,12 +78,15 @@ class _Plan:
 
     def __init__(self, params, group_of, flags, state, bits):
         self.device = params[0].device if params else torch.device("cuda", torch.cuda.current_device())
+        self.at = params[0].get_device() if params else -1
         self.p_ptrs, self.numels, self.p_dtypes = [p.data_ptr() for p in params], [p.numel() for p in params], [p.dtype for p in params]
         self.group_of, self.flags = group_of, flags
         # the table holds the addresses of these tensors: they stay alive with it, and it is good for them only
         self.params, self.every_state = params, list(state.values())
         self.states = states = [state[p] for p in params]
         self.tensors = list(chain.from_iterable(map(dict.values, states)))
+        self.state_ptrs = list(map(_data_ptr, self.tensors))
+        self.matrices = [k for k, x in enumerate(self.tensors) if x.dim() > 1]   # whose strides can change and nothing else
         self.table = t = np.zeros(len(params), dtype=L.ADAMW_DTYPE)
         t["p"], t["n"], t["p_type"] = self.p_ptrs, self.numels, [TYPES[d] for d in self.p_dtypes]
         ptr = lambda name: [st[name].data_ptr() if name in st else 0 for st in states]
@@ -99,14 +102,18 @@ class _Plan:
         self.sets, self.set_key, self.norm = None, None, None
 
     def good_for(self, params, group_of, flags, state):
+        """Whether the table says where everything is.  A tensor's memory can be exchanged under the same object (``x.data = y``, ``x.set_(y)``,
+        ``x.share_memory_()``), so that objects and addresses are both looked at."""
         if not (len(params) == len(self.params) and all(map(is_, params, self.params)) and list(map(_data_ptr, params)) == self.p_ptrs
-                and list(map(_numel, params)) == self.numels and list(map(_dtype, params)) == self.p_dtypes and group_of == self.group_of
+                and list(map(_numel, params)) == self.numels and list(map(_dtype, params)) == self.p_dtypes and all(map(_is_contiguous, params))
+                and group_of == self.group_of
                 and flags == self.flags and len(state) == len(self.every_state) and all(map(is_, state.values(), self.every_state))):
             return False
         tensors = list(chain.from_iterable(map(dict.values, self.states)))
-        return len(tensors) == len(self.tensors) and all(map(is_, tensors, self.tensors))
+        return (len(tensors) == len(self.tensors) and all(map(is_, tensors, self.tensors)) and list(map(_data_ptr, tensors)) == self.state_ptrs
+                and all([_is_contiguous(tensors[k]) for k in self.matrices]))
 
-    def look_at(self, grads):
+    def look_at(self, grads, name):
         """Put the gradients' addresses and types into the table; returns the copies that stand in for some of them."""
         try:
             ptrs = list(map(_data_ptr, grads))
@@ -122,6 +129,12 @@ class _Plan:
             self.table["g_type"] = [TYPES[g.dtype] for g in copies]
             self.g_dtypes = dtypes if all([c is g for c, g in zip(copies, grads)]) else None
         if ptrs != self.g_ptrs:
+            # no gradient of another device or size can be assigned to a parameter, but either's memory can be exchanged
+            if set(map(_get_device, grads)) - {self.at}:
+                raise RuntimeError(f"{name}: all gradients must live on {self.device}")
+            if list(map(_numel, grads)) != self.numels:
+                shapes = next((tuple(g.shape), tuple(p.shape)) for g, p in zip(grads, self.params) if g.numel() != p.numel())
+                raise RuntimeError(f"{name}: a gradient has shape {shapes[0]}, its parameter {shapes[1]}")
             self.table["g"] = ptrs
             self.g_ptrs = ptrs
         return copies
@@ -315,7 +328,7 @@ class _AdamWFamily(Optimizer):
                     raise RuntimeError(f"{self._name}: a gradient has shape {tuple(g.shape)}, its parameter {tuple(p.shape)}")
             plan = self._plan = self._build(plist, group_of, flags, capturing)
         stream = current_stream_ptr()
-        copies = plan.look_at(grads)
+        copies = plan.look_at(grads, self._name)
         self._fill_sets(plan)
         phases = L.ADAMW_STEP
         if clip:

@@ -176,3 +176,148 @@ def test_a_clipping_norm_too_small_for_a_float_clips(cls):
     opt = cls([p], clip_grad=True, clip_norm=1e-60)
     opt.step()
     assert not opt.state[p]["exp_avg"].float().any()   # 2^-149 / norm is below half of the smallest float
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# memory that is exchanged under the same tensors
+# ---------------------------------------------------------------------------------------------------------------------
+def moved(x, how):
+    """Other memory with the same values behind a tensor."""
+    new = x.detach().clone()
+    if how == "data":
+        x.data = new
+    elif how == "set_":
+        x.set_(new)
+    else:   # the storage grows, and moves
+        x.untyped_storage().resize_(x.untyped_storage().nbytes() + (1 << 20))
+
+
+def a_plan(bits):
+    """The host's table over parameters in the host's memory: nothing can be launched with it, but everything looked at."""
+    params = [torch.nn.Parameter(torch.ones(6, 6)), torch.nn.Parameter(torch.ones(40))]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    state = {}
+    for p in params:
+        n = -(-p.numel() // 256)
+        st = {"step": torch.tensor(3.0, dtype=torch.float64)}
+        if bits == 32:
+            st.update(exp_avg=torch.zeros(p.shape), exp_avg_sq=torch.zeros(p.shape))
+        else:
+            for name in ("exp_avg", "exp_avg_sq_root"):
+                st[name] = torch.zeros(p.shape, dtype=torch.uint8).view(torch.float8_e4m3fn)
+                st[name + "_scale"] = torch.ones(n, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+        state[p] = st
+    flags = [(False, False)]
+    plan = A._Plan(params, [0, 0], flags, state, bits)
+    assert plan.good_for(params, [0, 0], flags, state)
+    return plan, params, flags, state
+
+
+@pytest.mark.parametrize("how", ["data", "set_", "storage"])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_whose_memory_was_exchanged_is_noticed(bits, how):
+    for name in list(a_plan(bits)[3].values())[0]:
+        for k in (0, 1):
+            plan, params, flags, state = a_plan(bits)
+            moved(state[params[k]][name], how)
+            assert not plan.good_for(params, [0, 0], flags, state), name
+    plan, params, flags, state = a_plan(bits)
+    state[params[0]]["step"].share_memory_()
+    assert not plan.good_for(params, [0, 0], flags, state)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_strides_that_were_exchanged_are_noticed(bits):
+    plan, params, flags, state = a_plan(bits)
+    params[0].data = params[0].data.t()
+    assert not plan.good_for(params, [0, 0], flags, state)
+    for name in ("exp_avg", "exp_avg_sq" if bits == 32 else "exp_avg_sq_root"):
+        plan, params, flags, state = a_plan(bits)
+        state[params[0]][name].data = state[params[0]][name].data.t()
+        assert not plan.good_for(params, [0, 0], flags, state)
+
+
+def test_gradients_of_another_device_or_size_are_refused():
+    plan, params, *_ = a_plan(32)
+    look = lambda: plan.look_at([p.grad for p in params], "name")
+    look()
+    params[0].grad.data = torch.ones(3)
+    with pytest.raises(RuntimeError, match="gradient has shape"):
+        look()
+    params[0].grad.data = torch.ones(6, 6)
+    look()
+    plan.at = 0   # as if the parameters were on a GPU
+    params[1].grad.data = torch.ones(40)
+    with pytest.raises(RuntimeError, match="must live on"):
+        look()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", WIDTHS)
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("how", ["data", "set_", "storage"])
+def test_a_step_goes_by_the_memory_that_states_have_now(cls, capturable, how):
+    shapes = [(40, 40), (300,)]
+    a, b = T.params_of(shapes, torch.bfloat16, 1), T.params_of(shapes, torch.bfloat16, 1)
+    x, y = (cls(ps, master_weights=True, capturable=capturable) for ps in (a, b))
+
+    def both(t):
+        T.set_grads(a, torch.bfloat16, t)
+        for p, q in zip(a, b):
+            q.grad = p.grad.clone()
+        x.step()
+        y.step()
+        assert all(torch.equal(p, q) for p, q in zip(a, b)), t
+
+    both(0)
+    for k, name in enumerate(list(x.state[a[0]])):
+        kept = [x.state[p][name].detach().clone() for p in a]
+        if how == "storage" and name == "step" and not capturable:
+            x.state[a[0]][name].share_memory_()
+        else:
+            for p in a:
+                moved(x.state[p][name], how)
+        gone = [torch.full((64, 64), 255, dtype=torch.uint8, device="cuda") for _ in range(64)]   # over what was given back
+        both(1 + k)
+        if not name.endswith("scale"):   # the new memory is updated
+            assert not any(torch.equal(x.state[p][name].float(), z.float()) for p, z in zip(a, kept)), name
+        del gone
+    # values that come with the other memory count
+    x.state[a[0]]["exp_avg"].data = torch.zeros_like(x.state[a[0]]["exp_avg"])
+    y.state[b[0]]["exp_avg"] = torch.zeros_like(y.state[b[0]]["exp_avg"])
+    both(20)
+    # moments that were moved to the host come back
+    x.state[a[0]]["exp_avg"].data = x.state[a[0]]["exp_avg"].data.cpu()
+    both(21)
+    assert x.state[a[0]]["exp_avg"].is_cuda
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", WIDTHS)
+def test_a_parameter_whose_strides_were_exchanged_is_refused(cls):
+    p = torch.nn.Parameter(torch.randn(8, 8, device="cuda"))
+    opt = cls([p])
+    p.grad = torch.ones_like(p)
+    opt.step()
+    p.data = p.data.t()
+    with pytest.raises(RuntimeError, match="contiguous"):
+        opt.step()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", WIDTHS)
+def test_a_gradient_that_was_moved_to_the_host_is_refused(cls):
+    p, q = T.params_of([(30,), (7,)], torch.float32, 1)
+    opt = cls([p, q])
+    T.set_grads([p, q], torch.float32, 2)
+    opt.step()
+    q.grad.data = q.grad.data.cpu()
+    with pytest.raises(RuntimeError, match="must live on"):
+        opt.step()
+    q.grad.data = torch.ones(3, device="cuda")
+    with pytest.raises(RuntimeError, match="gradient has shape"):
+        opt.step()
+    q.grad.data = torch.ones(7, device="cuda")
+    opt.step()
+    assert float(opt.state[q]["step"]) == 2
