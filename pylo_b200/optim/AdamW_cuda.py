@@ -37,9 +37,10 @@ def blocks_of(n: int) -> int:
     return -(-n // L.ADAMW_BLOCK)
 
 
-def to_blocks(x: torch.Tensor):
+def to_blocks(x: torch.Tensor, least: int = 0):
     """(codes, scales) of the 8-bit states for the values of a tensor: e4m3 codes of its shape, rounded to nearest, and a power of
-    two for every 256 of its elements that brings the largest magnitude into [128, 256)."""
+    two for every 256 of its elements that brings the largest magnitude into [128, 256).  ``least = 1``, for roots: one that is not
+    zero gets the smallest code at least, as a step gives it (a moment over a root of zero would be divided by eps alone)."""
     flat = x.detach().to(torch.float32).contiguous().view(-1)
     n = flat.numel()
     b = torch.zeros(blocks_of(n) * L.ADAMW_BLOCK, dtype=torch.float32, device=x.device)
@@ -49,6 +50,8 @@ def to_blocks(x: torch.Tensor):
     most = finite.abs().amax(1) if len(b) else b.new_zeros(0)
     scale = ((most.view(torch.int32) >> 23).clamp(min=8) - 7)
     codes = (finite / (scale << 23).view(torch.float32)[:, None]).to(_CODES).view(torch.uint8)
+    if least:
+        codes = torch.where(finite > 0, codes.clamp(min=least), codes)
     codes = torch.where(b.isfinite(), codes, 0x7F).view(_CODES)
     return codes.view(-1)[:n].view(x.shape), scale.to(torch.uint8).view(_SCALES)
 
@@ -236,7 +239,7 @@ class _AdamWFamily(Optimizer):
         else:
             if "exp_avg_sq" in st:
                 changes()
-                st["exp_avg_sq_root"], st["exp_avg_sq_root_scale"] = to_blocks(st.pop("exp_avg_sq").to(torch.float32).sqrt())
+                st["exp_avg_sq_root"], st["exp_avg_sq_root_scale"] = to_blocks(st.pop("exp_avg_sq").to(torch.float32).sqrt(), least=1)
                 st["exp_avg"], st["exp_avg_scale"] = to_blocks(st["exp_avg"])
             each = (blocks_of(n),)
             wanted = {"exp_avg": (_CODES, p.shape), "exp_avg_scale": (_SCALES, each),

@@ -321,3 +321,35 @@ def test_a_gradient_that_was_moved_to_the_host_is_refused(cls):
     q.grad.data = torch.ones(7, device="cuda")
     opt.step()
     assert float(opt.state[q]["step"]) == 2
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# states of 32 bits that become ones of 8
+# ---------------------------------------------------------------------------------------------------------------------
+def test_roots_that_are_not_zero_get_a_code():
+    x = torch.logspace(-30, 0, 700)
+    x[::7] = 0
+    x[5], x[6] = math.nan, math.inf
+    codes, scales = A.to_blocks(x, least=1)
+    assert torch.equal(codes.float() == 0, x == 0) and bool(codes.float()[5:7].isnan().all())
+    nearest = A.to_blocks(x)
+    assert torch.equal(scales.view(torch.uint8), nearest[1].view(torch.uint8))
+    other = nearest[0].float() != 0
+    assert torch.equal(codes.view(torch.uint8)[other], nearest[0].view(torch.uint8)[other])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("g", [0.0, 1e-6])
+def test_the_first_step_from_converted_states_is_no_jump(g):
+    """One old gradient of 1 among many of 1e-6: the small roots' codes are what keeps their moments from being divided by eps alone."""
+    a, b = (torch.nn.Parameter(torch.zeros(512, device="cuda")) for _ in range(2))
+    x, y = optim.AdamW_CUDA([a], lr=1.0, weight_decay=0.0), optim.AdamW8bit_CUDA([b], lr=1.0, weight_decay=0.0)
+    v = torch.full((512,), 1e-12, device="cuda")
+    v[::256] = 1.0
+    x.state[a] = {"step": torch.tensor(1000.0, dtype=torch.float64), "exp_avg": torch.full((512,), 1e-6, device="cuda"), "exp_avg_sq": v}
+    y.load_state_dict(x.state_dict())
+    for p, opt in ((a, x), (b, y)):
+        p.grad = torch.full((512,), g, device="cuda")
+        opt.step()
+    # the moment's nearest code is 2^-4 of it away at most, a root's too where it has one of its own
+    assert bool((b.abs() <= a.abs() * (1 + 2.0 ** -4) / (1 - 2.0 ** -4) * (1 + 1e-5)).all())
