@@ -354,7 +354,8 @@ class _AdamWFamily(Optimizer):
         """The hyper-parameters of the step, a set per group."""
         key = [(g["lr"], g["betas"], g["eps"], g["weight_decay"], g["clip_norm"] if g["clip_grad"] else 0.0, g["maximize"], g.get("seed", 0))
                for g in self.param_groups]
-        if plan.set_key is not None and not any([torch.is_tensor(k[0]) for k in key]) and plan.set_key == key:
+        tensors = any([torch.is_tensor(k[0]) for k in key])   # whose value, not the object, is the learning rate: looked at anew in every step
+        if not tensors and plan.set_key == key:
             return
         plan.sets = (L.AdamwSet * len(key))()
         for s, group, (lr, (b1, b2), eps, wd, clip_norm, maximize, seed) in zip(plan.sets, self.param_groups, key):
@@ -365,7 +366,7 @@ class _AdamWFamily(Optimizer):
             s.lr, s.weight_decay, s.beta1, s.beta2, s.eps, s.clip_norm = float(lr), wd, b1, b2, eps, clip_norm
             s.maximize, s.seed = bool(maximize), seed & 0xFFFFFFFF
         plan.call.sets, plan.call.n_sets = plan.sets, len(key)
-        plan.set_key = key
+        plan.set_key = None if tensors else key
 
 
 class AdamW_CUDA(_AdamWFamily):

@@ -353,3 +353,32 @@ def test_the_first_step_from_converted_states_is_no_jump(g):
         opt.step()
     # the moment's nearest code is 2^-4 of it away at most, a root's too where it has one of its own
     assert bool((b.abs() <= a.abs() * (1 + 2.0 ** -4) / (1 - 2.0 ** -4) * (1 + 1e-5)).all())
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# a learning rate on the device that is replaced by a number
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", WIDTHS)
+def test_a_number_in_the_place_of_a_learning_rate_on_the_device(cls):
+    """The tensor has no say any more, also where the number is what it said, and the step can be captured."""
+    p = torch.nn.Parameter(torch.zeros(100, device="cuda"))
+    p.grad = torch.ones_like(p)
+    lr = torch.tensor(0.25, device="cuda")
+    opt = cls([p], lr=lr, weight_decay=0.0, capturable=True)
+    opt.step()
+    opt.param_groups[0]["lr"] = 0.25
+    opt.step()
+    lr.fill_(100.0)
+    before = p.detach().clone()
+    opt.step()
+    assert bool(((p - before).abs() < 1).all())
+    opt.param_groups[0]["lr"] = lr
+    opt.step()
+    opt.param_groups[0]["lr"] = 0.5
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    before = p.detach().clone()
+    graph.replay()
+    assert bool(((p - before).abs() < 1).all())
