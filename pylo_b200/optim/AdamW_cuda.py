@@ -102,7 +102,7 @@ class _Plan:
         self.g_ptrs, self.g_dtypes = None, None
         self.call = L.AdamwCall(items=t.ctypes.data, n_items=len(params), bits=bits, norm_floats=L.norm_floats(len(params), sum(self.numels)))
         self.call_ref = C.byref(self.call)
-        self.sets, self.set_key, self.norm = None, None, None
+        self.sets, self.set_key, self.norm, self.norm_stream = None, None, None, None
 
     def good_for(self, params, group_of, flags, state):
         """Whether the table says where everything is.  A tensor's memory can be exchanged under the same object (``x.data = y``, ``x.set_(y)``,
@@ -337,9 +337,10 @@ class _AdamWFamily(Optimizer):
         if clip:
             phases = L.ADAMW_NORM | L.ADAMW_STEP
             norm = plan.norm
-            if norm is None or capturing:   # a captured step has a buffer of its own, from the graph's memory
+            # a stream has a buffer of its own, which goes back to that stream's memory; a captured step has one from the graph's
+            if norm is None or capturing or stream != plan.norm_stream:
                 norm = torch.empty(plan.call.norm_floats, dtype=torch.float32, device=plan.device)
-                plan.norm = None if capturing else norm
+                plan.norm, plan.norm_stream = None if capturing else norm, stream
                 plan.call.norm = norm.data_ptr()
             if self.process_group is not None or (self._sharded and torch.distributed.is_initialized()):
                 L.check(L.lib.pylo_b200_adamw_step(plan.call_ref, L.ADAMW_NORM, stream), "adamw_step")

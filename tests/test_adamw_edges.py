@@ -382,3 +382,29 @@ def test_a_number_in_the_place_of_a_learning_rate_on_the_device(cls):
     before = p.detach().clone()
     graph.replay()
     assert bool(((p - before).abs() < 1).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", WIDTHS)
+def test_a_clipped_steps_workspace_is_its_streams_own(cls):
+    """A buffer of another stream's memory would be given back to that stream while this one still reads it."""
+    p = T.params_of([(500, 300)], torch.float32, 1)[0]
+    T.set_grads([p], torch.float32, 2)
+    opt = cls([p], clip_grad=True, clip_norm=0.1)
+    opt.step()
+    one = opt._plan.norm
+    opt.step()
+    assert opt._plan.norm is one
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+        assert opt._plan.norm.data_ptr() != one.data_ptr() and opt._plan.call.norm == opt._plan.norm.data_ptr()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    opt = cls([p], clip_grad=True, clip_norm=0.1, capturable=True)
+    opt.step()
+    with torch.cuda.graph(graph):
+        opt.step()
+    opt.step()
+    assert opt._plan.norm is not None
