@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define PYLO_B200_ABI_VERSION 20
+#define PYLO_B200_ABI_VERSION 21
 
 /* optimizer families (which feature set / network geometry a launch uses) */
 #define PYLO_FAM_ADAFAC 0 /* AdafacLO_CUDA, ELO_CUDA: 28+11 features, 39-32-32-2 */
@@ -568,6 +568,9 @@ int pylo_b200_adamw_step(const pylo_adamw_call* call, int phases, void* stream);
 #define PYLO_ERR_GRADS_OVERLAP (-5)
 int pylo_b200_clip_grads(void* const* g, const int64_t* n, const int32_t* types, int n_items, float max_norm, float* norm, int64_t norm_floats,
                          int distinct, void* stream);
+/* The same, with norm[1] in root[0] (DEVICE) too: what is kept of the call need not hold on to the workspace. */
+int pylo_b200_clip_grads_to(void* const* g, const int64_t* n, const int32_t* types, int n_items, float max_norm, float* root, float* norm,
+                            int64_t norm_floats, int distinct, void* stream);
 
 #ifdef __cplusplus
 }

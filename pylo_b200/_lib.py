@@ -17,7 +17,7 @@ TILE_ELEMS = 16384
 A_COLS = 1024
 PREP_TABLE = 2048  # table entries (rows x hidden units) per item of pylo_b200_prep_apply
 WFOLD_STRIDE = 4800
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 FAM_ADAFAC, FAM_CELO2, FAM_VELO = 0, 1, 2
 MODE_FAST2D, MODE_GENERIC, MODE_VEC1D, MODE_KERNEL = 0, 1, 2, 3
@@ -182,6 +182,7 @@ def _load():
         "pylo_b200_sizeof_adamw": [i32],
         "pylo_b200_adamw_step": [C.POINTER(AdamwCall), i32, vp],
         "pylo_b200_clip_grads": [vp, vp, vp, i32, f32, vp, C.c_int64, i32, vp],
+        "pylo_b200_clip_grads_to": [vp, vp, vp, i32, f32, vp, vp, C.c_int64, i32, vp],
         "pylo_b200_advance_steps": [vp, i32, C.POINTER(C.c_double), C.POINTER(C.c_int)],
     }
     for name, argtypes in sigs.items():

@@ -421,8 +421,9 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     together; returns ``norm`` (fp32, on the device), as ``torch.nn.utils.clip_grad_norm_`` does.
 
     Gradients may be fp32, bf16 and fp16, mixed; the norm is summed up in fp32 and more whatever their type.  One that is given twice
-    counts and is scaled once.  Two or three launches and no synchronisation (``error_if_nonfinite`` waits for the norm); the gradients are
-    written only where the norm exceeds ``max_norm``."""
+    counts and is scaled once.  A launch for the norm and one for the scaling per type and 800 gradients, one between them where there are
+    many partial sums; no synchronisation (``error_if_nonfinite`` waits for the norm).  The gradients are written only where the norm
+    exceeds ``max_norm``."""
     if float(norm_type) != 2.0:
         raise ValueError(f"clip_grad_norm_: only the 2-norm is supported, got norm_type={norm_type}")
     max_norm = float(max_norm)
@@ -459,11 +460,14 @@ def _clip(grads, types, max_norm, error_if_nonfinite):
     sizes = array("q", map(_numel, parts))
     stream = current_stream_ptr()
     floats = L.norm_floats(len(ptrs), sum(sizes))
-    norm = torch.empty(floats, dtype=torch.float32, device="cuda")
-    at = norm.data_ptr()
+    device = grads[0].device
+    total = torch.empty_strided((), (), dtype=torch.float32, device=device)   # by itself: who keeps it keeps no workspace
+    norm = torch.empty(floats, dtype=torch.float32, device=device)
+    to, at = total.data_ptr(), norm.data_ptr()
 
     def run(limit, distinct):
-        return L.lib.pylo_b200_clip_grads(ptrs.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], len(ptrs), limit, at, floats, distinct, stream)
+        return L.lib.pylo_b200_clip_grads_to(ptrs.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], len(ptrs), limit, to, at, floats, distinct,
+                                             stream)
 
     limit = math.inf if error_if_nonfinite else max_norm   # the norm is looked at before anything is scaled
     code, distinct = run(limit, 0), 0
@@ -472,7 +476,6 @@ def _clip(grads, types, max_norm, error_if_nonfinite):
         code, distinct = run(limit, 1), 1
     if code:
         L.check(code, "clip_grads")
-    total = norm[1]
     if error_if_nonfinite:
         if not math.isfinite(float(total)):
             raise RuntimeError("The total norm of order 2.0 for gradients from `parameters` is non-finite, so it cannot be clipped. To disable this "

@@ -3,9 +3,11 @@ arguments at the ends of their ranges."""
 
 import math
 
+import numpy as np
 import pytest
 import torch
 
+from pylo_b200 import _lib as L
 from pylo_b200 import optim
 from pylo_b200.optim import AdamW_cuda as A
 import test_adamw as T
@@ -408,3 +410,34 @@ def test_a_clipped_steps_workspace_is_its_streams_own(cls):
         opt.step()
     opt.step()
     assert opt._plan.norm is not None
+
+
+def test_a_place_for_the_norm_is_needed():
+    g, n, t = np.array([512], dtype=np.uint64), np.array([8]), np.array([L.FP32], dtype=np.int32)
+    call = lambda root, norm, floats: L.lib.pylo_b200_clip_grads_to(g.ctypes.data, n.ctypes.data, t.ctypes.data, 1, 1.0, root, norm, floats, 0, None)
+    assert call(None, 256, 100) == -1 and call(256, None, 100) == -1 and call(256, 512, 2) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm", [0.1, math.inf])
+@pytest.mark.parametrize("shapes", [[(30,)], [(700, 900), (5,)], [(3000, 3000)]])   # few partial sums, and more than a launch adds up itself
+def test_the_norm_that_is_returned_keeps_nothing_else(shapes, max_norm):
+    grads = T.tensors(shapes, torch.float32, 1)
+    before = [g.clone() for g in grads]
+    norm = optim.clip_grad_norm_(T.with_grads(grads), max_norm)
+    assert norm.untyped_storage().nbytes() == 4
+    T.check_clip(grads, before, norm, max_norm)
+    again = optim.clip_grad_norm_(T.with_grads(before), max_norm, error_if_nonfinite=True)
+    assert again.untyped_storage().nbytes() == 4 and torch.equal(again, norm)
+
+
+@pytest.mark.gpu
+def test_both_forms_of_the_native_call_say_the_same():
+    g = T.tensors([(5000,)], torch.float32, 1)[0]
+    ptrs, n, t = np.array([g.data_ptr()], dtype=np.uint64), np.array([5000]), np.array([L.FP32], dtype=np.int32)
+    for limit in (math.inf, 1e9):   # neither writes to the gradient
+        norm, root, other = torch.zeros(100, device="cuda"), torch.zeros(1, device="cuda"), torch.zeros(100, device="cuda")
+        L.check(L.lib.pylo_b200_clip_grads(ptrs.ctypes.data, n.ctypes.data, t.ctypes.data, 1, limit, norm.data_ptr(), 100, 0, None), "clip_grads")
+        L.check(L.lib.pylo_b200_clip_grads_to(ptrs.ctypes.data, n.ctypes.data, t.ctypes.data, 1, limit, root.data_ptr(), other.data_ptr(), 100, 0, None), "clip_grads_to")
+        torch.cuda.synchronize()
+        assert torch.equal(norm[:2], other[:2]) and torch.equal(root, norm[1:2]) and float(root) > 0
