@@ -416,6 +416,19 @@ def _dense(g: torch.Tensor) -> bool:
     return True
 
 
+def _as_runs(grads):
+    """The gradients as runs of memory: themselves, or copies, one for all that are the same elements."""
+    copies, parts = {}, []
+    for g in grads:
+        if not (g.is_contiguous() or _dense(g)):
+            same = (g.data_ptr(), g.dtype, g.shape, g.stride())
+            if same not in copies:
+                copies[same] = g.detach().contiguous()
+            g = copies[same]
+        parts.append(g)
+    return parts
+
+
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scale the gradients of ``parameters`` in place by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` the 2-norm of all of them
     together; returns ``norm`` (fp32, on the device), as ``torch.nn.utils.clip_grad_norm_`` does.
@@ -451,7 +464,7 @@ def _clip(grads, types, max_norm, error_if_nonfinite):
     parts = grads
     try:
         if not all(map(_is_contiguous, grads)):
-            parts = [g if g.is_contiguous() or _dense(g) else g.detach().contiguous() for g in grads]
+            parts = _as_runs(grads)
         ptrs = array("Q", map(_data_ptr, parts))
     except RuntimeError:
         if any([g.layout is not torch.strided for g in grads]):

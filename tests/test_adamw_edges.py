@@ -441,3 +441,16 @@ def test_both_forms_of_the_native_call_say_the_same():
         L.check(L.lib.pylo_b200_clip_grads_to(ptrs.ctypes.data, n.ctypes.data, t.ctypes.data, 1, limit, root.data_ptr(), other.data_ptr(), 100, 0, None), "clip_grads_to")
         torch.cuda.synchronize()
         assert torch.equal(norm[:2], other[:2]) and torch.equal(root, norm[1:2]) and float(root) > 0
+
+
+@pytest.mark.gpu
+def test_a_strided_gradient_that_is_given_twice_counts_once():
+    base = torch.randn(20, 30, device="cuda")
+    z, y = base[:, ::2], torch.randn(7, device="cuda")
+    params = T.with_grads([z, y])
+    before, hidden = [z.clone(), y.clone()], base[:, 1::2].clone()
+    other = torch.nn.Parameter(torch.zeros(20, 15, device="cuda"))   # another parameter with the same gradient
+    other.grad = base[:, ::2]
+    norm = optim.clip_grad_norm_(params + params[:1] + [other], 0.3)
+    T.check_clip([z, y], before, norm, 0.3)
+    assert torch.equal(base[:, 1::2], hidden)
