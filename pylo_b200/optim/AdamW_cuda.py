@@ -416,11 +416,13 @@ def _dense(g: torch.Tensor) -> bool:
     return True
 
 
-def _as_runs(grads):
+def _as_runs(grads, scaled):
     """The gradients as runs of memory: themselves, or copies, one for all that are the same elements."""
     copies, parts = {}, []
     for g in grads:
         if not (g.is_contiguous() or _dense(g)):
+            if scaled and any([stride == 0 and n > 1 for stride, n in zip(g.stride(), g.shape)]):
+                raise RuntimeError(f"clip_grad_norm_: a gradient's elements share memory (shape {tuple(g.shape)}, strides {g.stride()})")
             same = (g.data_ptr(), g.dtype, g.shape, g.stride())
             if same not in copies:
                 copies[same] = g.detach().contiguous()
@@ -464,7 +466,7 @@ def _clip(grads, types, max_norm, error_if_nonfinite):
     parts = grads
     try:
         if not all(map(_is_contiguous, grads)):
-            parts = _as_runs(grads)
+            parts = _as_runs(grads, max_norm < math.inf)
         ptrs = array("Q", map(_data_ptr, parts))
     except RuntimeError:
         if any([g.layout is not torch.strided for g in grads]):

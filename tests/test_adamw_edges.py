@@ -454,3 +454,12 @@ def test_a_strided_gradient_that_is_given_twice_counts_once():
     norm = optim.clip_grad_norm_(params + params[:1] + [other], 0.3)
     T.check_clip([z, y], before, norm, 0.3)
     assert torch.equal(base[:, 1::2], hidden)
+
+
+@pytest.mark.gpu
+def test_an_expanded_gradient_is_refused_before_anything_is_scaled():
+    grads = [torch.ones(7, device="cuda"), torch.randn(1, 4, device="cuda").expand(5, 4)]
+    with pytest.raises(RuntimeError, match="share memory"):
+        optim.clip_grad_norm_(T.with_grads(grads), 0.1)
+    assert bool((grads[0] == 1).all())
+    T.check_clip(grads, [g.clone() for g in grads], optim.clip_grad_norm_(T.with_grads(grads), math.inf), math.inf)   # its norm alone
