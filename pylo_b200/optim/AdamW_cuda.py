@@ -30,6 +30,7 @@ _numel, _data_ptr, _is_contiguous, _get_device = torch.Tensor.numel, torch.Tenso
 _dtype, _grad = attrgetter("dtype"), attrgetter("grad")
 
 TYPES = {torch.float32: L.FP32, torch.bfloat16: L.BF16, torch.float16: L.FP16}
+_STATES = ("step", "master", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale")
 _CODES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
@@ -87,9 +88,10 @@ class _Plan:
         # the table holds the addresses of these tensors: they stay alive with it, and it is good for them only
         self.params, self.every_state = params, list(state.values())
         self.states = states = [state[p] for p in params]
-        self.tensors = list(chain.from_iterable(map(dict.values, states)))
+        self.values = list(chain.from_iterable(map(dict.values, states)))
+        self.tensors = [st[name] for st in states for name in _STATES if name in st]   # a state may hold other things too
         self.state_ptrs = list(map(_data_ptr, self.tensors))
-        self.matrices = [k for k, x in enumerate(self.tensors) if x.dim() > 1]   # whose strides can change and nothing else
+        self.matrices = [x for x in self.tensors if x.dim() > 1]   # whose strides can change and nothing else
         self.table = t = np.zeros(len(params), dtype=L.ADAMW_DTYPE)
         t["p"], t["n"], t["p_type"] = self.p_ptrs, self.numels, [TYPES[d] for d in self.p_dtypes]
         ptr = lambda name: [st[name].data_ptr() if name in st else 0 for st in states]
@@ -112,9 +114,9 @@ class _Plan:
                 and group_of == self.group_of
                 and flags == self.flags and len(state) == len(self.every_state) and all(map(is_, state.values(), self.every_state))):
             return False
-        tensors = list(chain.from_iterable(map(dict.values, self.states)))
-        return (len(tensors) == len(self.tensors) and all(map(is_, tensors, self.tensors)) and list(map(_data_ptr, tensors)) == self.state_ptrs
-                and all([_is_contiguous(tensors[k]) for k in self.matrices]))
+        values = list(chain.from_iterable(map(dict.values, self.states)))
+        return (len(values) == len(self.values) and all(map(is_, values, self.values)) and list(map(_data_ptr, self.tensors)) == self.state_ptrs
+                and all(map(_is_contiguous, self.matrices)))
 
     def look_at(self, grads, name):
         """Put the gradients' addresses and types into the table; returns the copies that stand in for some of them."""

@@ -463,3 +463,51 @@ def test_an_expanded_gradient_is_refused_before_anything_is_scaled():
         optim.clip_grad_norm_(T.with_grads(grads), 0.1)
     assert bool((grads[0] == 1).all())
     T.check_clip(grads, [g.clone() for g in grads], optim.clip_grad_norm_(T.with_grads(grads), math.inf), math.inf)   # its norm alone
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# what a state may hold, and sharded steps
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", WIDTHS)
+def test_a_state_may_hold_other_things(cls):
+    a, b = T.params_of([(30, 20)], torch.float32, 1), T.params_of([(30, 20)], torch.float32, 1)
+    x, y = cls(a), cls(b)
+    for t in range(3):
+        T.set_grads(a + b, torch.float32, 2 + t)
+        b[0].grad = a[0].grad.clone()
+        x.step()
+        y.step()
+        x.state[a[0]]["note"] = t
+        x.state[a[0]]["mask"] = torch.ones(3, 4).t().to_sparse()
+        new = cls(a)
+        new.load_state_dict(x.state_dict())
+        assert new.state[a[0]]["note"] == t
+        x = new
+    x.step()
+    y.step()
+    assert torch.equal(a[0], b[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", WIDTHS)
+@pytest.mark.parametrize("kind", ["staged", "fused"])
+def test_through_the_steps_that_overlap_their_exchange(cls, kind):
+    """One rank of one: hooks and layout, no exchange."""
+    from pylo_b200.zero import FusedShardedStep, StagedShardedStep
+
+    shapes = [(72, 48), (48,), (30, 200), (7,)]
+    shard = StagedShardedStep(shapes, "cuda", blocks=2) if kind == "staged" else FusedShardedStep(shapes, "cuda", push="copies")
+    other = [torch.nn.Parameter(p.detach().clone()) for p in shard.params]
+    x = cls(shard.param_groups() if kind == "staged" else shard.param_groups(groups=2), clip_grad=True, clip_norm=0.5)
+    x.after_group = shard.after_group
+    x._sharded = True
+    y = cls(other, clip_grad=True, clip_norm=0.5)
+    for t in range(3):
+        T.set_grads(shard.params, torch.float32, t)
+        for p, q in zip(shard.params, other):
+            q.grad = p.grad.clone()
+        x.step()
+        shard.finish()
+        y.step()
+    assert all(torch.equal(p, q) for p, q in zip(shard.params, other))
