@@ -5,7 +5,8 @@ update and the state keys (``step``, ``exp_avg``, ``exp_avg_sq``) of ``torch.opt
 Parameters are fp32, bf16 or fp16, those of 16 bits with or without an fp32 copy in the state (``master_weights``).
 
 A step is one native call and one launch over the tensors of all param groups (one per combination of types and two hundred
-tensors), one or two more before it where gradients are clipped by their global norm.  Nothing of it waits for the device.
+tensors); where gradients are clipped by their global norm, one more before it per type of theirs, and one where there are many.
+Nothing of it waits for the device.
 """
 
 from __future__ import annotations
