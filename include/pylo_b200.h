@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define PYLO_B200_ABI_VERSION 21
+#define PYLO_B200_ABI_VERSION 22
 
 /* optimizer families (which feature set / network geometry a launch uses) */
 #define PYLO_FAM_ADAFAC 0 /* AdafacLO_CUDA, ELO_CUDA: 28+11 features, 39-32-32-2 */
@@ -571,6 +571,87 @@ int pylo_b200_clip_grads(void* const* g, const int64_t* n, const int32_t* types,
 /* The same, with norm[1] in root[0] (DEVICE) too: what is kept of the call need not hold on to the workspace. */
 int pylo_b200_clip_grads_to(void* const* g, const int64_t* n, const int32_t* types, int n_items, float max_norm, float* root, float* norm,
                             int64_t norm_floats, int distinct, void* stream);
+
+/* ---- Operators of a model's training step beside the optimizer: layer norm, distillation, the gated feed-forward block ----------------
+ * Arguments are HOST structs whose pointers are DEVICE memory; types are PYLO_FP32, PYLO_BF16, PYLO_FP16.  No call allocates: workspaces
+ * are the caller's, need not be cleared, and belong to one call at a time. */
+
+/* Layer norm of rows: y = (x - mean) rstd weight + bias with rstd = 1 / sqrt(variance + eps).  Width up to 32768. */
+typedef struct pylo_norm {
+  const void* x;                 /* [rows][width], rows x_stride elements apart */
+  const void *weight, *bias;     /* [width] or NULL; bias only beside a weight */
+  void* y;                       /* out [rows][width], contiguous (forward) */
+  float *mean, *rstd;            /* [rows]: written forward unless NULL, read backward */
+  const void* dy;                /* backward: [rows][width], rows dy_stride elements apart */
+  void *dx, *dweight, *dbias;    /* out (backward), contiguous; each may be NULL */
+  float* work;                   /* backward, where dweight or dbias is wanted */
+  int64_t work_floats, rows, x_stride, dy_stride;
+  int32_t width, type;
+  int32_t weight_type;           /* of weight, bias, dweight, dbias: type or PYLO_FP32 */
+  float eps;
+} pylo_norm;
+int pylo_b200_layer_norm(const pylo_norm* n, void* stream);
+int pylo_b200_layer_norm_backward(const pylo_norm* n, void* stream);
+/* floats of work (host only; depends on the current device) */
+int64_t pylo_b200_layer_norm_workspace(int64_t rows, int width);
+
+/* Distillation from a teacher's largest logits.  With p = softmax(teacher / temperature) over a row's top entries and q =
+ * softmax(logits / temperature) over all classes, a row's loss is temperature^2 sum_k p_k (log p_k - log q_{ids_k}); its gradient
+ * temperature (q_j - sum of the p_k with ids_k = j).  Ids outside of [0, vocab) are padding; rows without an entry, and rows of weight 0,
+ * count for nothing and have a gradient of zero. */
+#define PYLO_DISTILL_LOSS 1
+#define PYLO_DISTILL_GRAD 2
+#define PYLO_REDUCE_NONE 0 /* row_loss alone: weight * loss */
+#define PYLO_REDUCE_SUM 1
+#define PYLO_REDUCE_MEAN 2 /* over the sum of the weights that count; 0 where that is 0 */
+typedef struct pylo_distill {
+  const void* logits;            /* [rows][vocab], rows stride elements apart */
+  const void* teacher;           /* [rows][top] */
+  const void* ids;               /* [rows][top], int32 or int64 */
+  const float* weights;          /* [rows], or NULL: 1 */
+  float* loss;                   /* out [1] (SUM, MEAN) */
+  float* row_loss;               /* out [rows], or NULL */
+  float* stat;                   /* [rows][2]: written with the loss unless NULL, read for a gradient alone */
+  float* inv;                    /* [1]: 1 / sum of the weights; written with the loss unless NULL, read for a gradient alone (MEAN) */
+  void* grad;                    /* out [rows][vocab], contiguous, of the logits' type */
+  const float* upstream;         /* gradient of the loss: [1], or (NONE) [rows]; NULL: 1 */
+  void* work;                    /* with the loss; 16-byte aligned */
+  int64_t work_bytes, rows, stride;
+  int32_t vocab, top, type, teacher_type;   /* top up to 1024 */
+  int32_t ids_bytes;             /* 4 or 8 */
+  int32_t reduction;
+  float temperature;             /* > 0 */
+  float scale;                   /* another factor of the gradient */
+} pylo_distill;
+/* what: PYLO_DISTILL_LOSS, or PYLO_DISTILL_GRAD from an earlier call's stat and inv, or both at once. */
+int pylo_b200_distill(const pylo_distill* d, int what, void* stream);
+int64_t pylo_b200_distill_workspace(int64_t rows, int vocab);
+
+/* The gated feed-forward block: h = act(x w_gate^T) * (x w_up^T), y = h w_down^T, with its gradients.  PYLO_BF16 or PYLO_FP16 throughout,
+ * products on the tensor cores with fp32 sums.  Matrices are row-major with rows ld elements apart; operands (x, dy and the weights) begin
+ * on 16-byte boundaries and have ld % 8 = 0, results may lie anywhere. */
+#define PYLO_ACT_SILU 0
+#define PYLO_ACT_GELU 1      /* with the error function */
+#define PYLO_ACT_GELU_TANH 2
+#define PYLO_ACT_RELU 3
+typedef struct pylo_ffn {
+  const void *x, *w_gate, *w_up, *w_down;   /* [rows][width], [hidden][width] twice, [out][hidden] */
+  void* y;                                  /* out [rows][out] (forward) */
+  const void* dy;                           /* [rows][out] (backward) */
+  void *dx, *dw_gate, *dw_up, *dw_down;     /* out (backward), shaped like what they are gradients of, contiguous; each may be NULL */
+  void* kept;                               /* written forward, read backward: pylo_b200_gated_ffn_kept bytes, 256-byte aligned */
+  void* work;                               /* backward: pylo_b200_gated_ffn_workspace bytes, 256-byte aligned */
+  int64_t rows, ld_x, ld_gate, ld_up, ld_down, ld_dy;
+  int32_t width, hidden, out, type, activation;
+  int32_t keep;                             /* forward: 0 if no backward pass follows (kept then holds h alone) */
+  int *status, *host_status;                /* [1], or NULL: gets a bit where a kernel's bounded wait ran out (results are incomplete then) */
+} pylo_ffn;
+int64_t pylo_b200_gated_ffn_kept(int64_t rows, int hidden, int keep);
+int64_t pylo_b200_gated_ffn_workspace(int64_t rows, int hidden);
+int pylo_b200_gated_ffn(const pylo_ffn* f, void* stream);
+int pylo_b200_gated_ffn_backward(const pylo_ffn* f, void* stream);
+/* bytes of pylo_norm (0), pylo_distill (1), pylo_ffn (2) */
+int pylo_b200_sizeof_layers(int what);
 
 #ifdef __cplusplus
 }

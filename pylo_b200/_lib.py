@@ -17,7 +17,7 @@ TILE_ELEMS = 16384
 A_COLS = 1024
 PREP_TABLE = 2048  # table entries (rows x hidden units) per item of pylo_b200_prep_apply
 WFOLD_STRIDE = 4800
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 FAM_ADAFAC, FAM_CELO2, FAM_VELO = 0, 1, 2
 MODE_FAST2D, MODE_GENERIC, MODE_VEC1D, MODE_KERNEL = 0, 1, 2, 3
@@ -131,6 +131,34 @@ class StepPlan(C.Structure):
                                        "small_rows", "small_cols", "n_kernel", "n_mats", "small_networks", "factor_threads", "pad_")]
 
 
+class Norm(C.Structure):
+    """pylo_norm: layer norm of rows, forward or backward."""
+    _fields_ = [(name, C.c_void_p) for name in ("x", "weight", "bias", "y", "mean", "rstd", "dy", "dx", "dweight", "dbias", "work")] + [
+        (name, C.c_int64) for name in ("work_floats", "rows", "x_stride", "dy_stride")] + [
+        (name, C.c_int32) for name in ("width", "type", "weight_type")] + [("eps", C.c_float)]
+
+
+class Distill(C.Structure):
+    """pylo_distill: the loss against a teacher's largest logits, and its gradient."""
+    _fields_ = [(name, C.c_void_p) for name in ("logits", "teacher", "ids", "weights", "loss", "row_loss", "stat", "inv", "grad", "upstream", "work")] + [
+        (name, C.c_int64) for name in ("work_bytes", "rows", "stride")] + [
+        (name, C.c_int32) for name in ("vocab", "top", "type", "teacher_type", "ids_bytes", "reduction")] + [
+        ("temperature", C.c_float), ("scale", C.c_float)]
+
+
+class Ffn(C.Structure):
+    """pylo_ffn: the gated feed-forward block, forward or backward."""
+    _fields_ = [(name, C.c_void_p) for name in ("x", "w_gate", "w_up", "w_down", "y", "dy", "dx", "dw_gate", "dw_up", "dw_down", "kept", "work")] + [
+        (name, C.c_int64) for name in ("rows", "ld_x", "ld_gate", "ld_up", "ld_down", "ld_dy")] + [
+        (name, C.c_int32) for name in ("width", "hidden", "out", "type", "activation", "keep")] + [("status", C.c_void_p), ("host_status", C.c_void_p)]
+
+
+DISTILL_LOSS, DISTILL_GRAD = 1, 2
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
+ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU = 0, 1, 2, 3
+NORM_MOST, DISTILL_MOST_TOP = 32768, 1024   # elements of a row of layer norm, entries of a teacher
+
+
 class PyloLibError(RuntimeError):
     pass
 
@@ -184,15 +212,27 @@ def _load():
         "pylo_b200_clip_grads": [vp, vp, vp, i32, f32, vp, C.c_int64, i32, vp],
         "pylo_b200_clip_grads_to": [vp, vp, vp, i32, f32, vp, vp, C.c_int64, i32, vp],
         "pylo_b200_advance_steps": [vp, i32, C.POINTER(C.c_double), C.POINTER(C.c_int)],
+        "pylo_b200_sizeof_layers": [i32],
+        "pylo_b200_layer_norm": [C.POINTER(Norm), vp],
+        "pylo_b200_layer_norm_backward": [C.POINTER(Norm), vp],
+        "pylo_b200_layer_norm_workspace": [C.c_int64, i32],
+        "pylo_b200_distill": [C.POINTER(Distill), i32, vp],
+        "pylo_b200_distill_workspace": [C.c_int64, i32],
+        "pylo_b200_gated_ffn": [C.POINTER(Ffn), vp],
+        "pylo_b200_gated_ffn_backward": [C.POINTER(Ffn), vp],
+        "pylo_b200_gated_ffn_kept": [C.c_int64, i32, i32],
+        "pylo_b200_gated_ffn_workspace": [C.c_int64, i32],
     }
     for name, argtypes in sigs.items():
         fn = getattr(lib, name)  # AttributeError if a declared symbol is missing
         fn.argtypes = argtypes
-        fn.restype = C.c_int64 if name in ("pylo_b200_workspace_bytes", "pylo_b200_newton_schulz_workspace") else C.c_int
+        fn.restype = C.c_int64 if name in ("pylo_b200_workspace_bytes", "pylo_b200_newton_schulz_workspace", "pylo_b200_layer_norm_workspace",
+                                           "pylo_b200_distill_workspace", "pylo_b200_gated_ffn_kept", "pylo_b200_gated_ffn_workspace") else C.c_int
     if lib.pylo_b200_abi_version() != ABI_VERSION:
         raise ImportError("libpylo_b200.so was built from a different ABI version; rebuild it")
     if (lib.pylo_b200_sizeof_desc() != DESC_DTYPE.itemsize or lib.pylo_b200_sizeof_params() != C.sizeof(StepParams)
-            or [lib.pylo_b200_sizeof_adamw(k) for k in range(3)] != [ADAMW_DTYPE.itemsize, C.sizeof(AdamwSet), C.sizeof(AdamwCall)]):
+            or [lib.pylo_b200_sizeof_adamw(k) for k in range(3)] != [ADAMW_DTYPE.itemsize, C.sizeof(AdamwSet), C.sizeof(AdamwCall)]
+            or [lib.pylo_b200_sizeof_layers(k) for k in range(3)] != [C.sizeof(Norm), C.sizeof(Distill), C.sizeof(Ffn)]):
         raise ImportError("descriptor layout mismatch between the Python binding and libpylo_b200.so")
     return lib, sorted(sigs)
 

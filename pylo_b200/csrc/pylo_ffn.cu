@@ -1,0 +1,722 @@
+// The gated feed-forward block on the tensor cores, forward and backward.
+//
+//   g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T
+//   dh = dy Wd;  dg = dh P with P = u act'(g), du = dh Q with Q = act(g)
+//   dx = dg Wg + du Wu;  dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+//
+// Four launches of one product kernel, C = sum_k A(m, k) B(n, k) over 16-bit operands with fp32 sums, whose epilogues differ:
+//   gate    both projections of a tile of h at once: half of a tile's columns are rows of Wg, the other half the same rows of Wu, so g and u
+//           meet in one thread's registers, which makes h, P and Q of them; g and u themselves reach no memory
+//   plain   y = h Wd^T
+//   back    dh = dy Wd, which reaches no memory either: dg and du of P and Q
+//   plain   dx (a contraction of two parts), dWg, dWu, dWd side by side in one launch
+// No operand is transposed: 16-bit operands may be read with the contraction index as rows ("MN-major"), as dx and the weights' gradients
+// need them.
+//
+// What is kept for the backward pass: h in 16 bits, which the forward pass needs in memory anyway, P and Q with 24 (16 significant bits, an fp32
+// value's upper three bytes, rounded; in two planes, so that rows stay aligned): 8 bytes per element of h, what g, u, act(g) and h take in 16 bits.
+// With P and Q in 16 bits, dg and du would be rounded twice on their way into dx, dWg and dWu: an error of 1.7 instead of 1.4 times that of the
+// result's own rounding.
+//
+// A CTA has ten warps: one lane issues the copies (TMA, 128-byte swizzle), one the products, eight warps run the epilogue.  Every wait is bounded;
+// one that runs out ends the CTA's work in order and sets a bit of the caller's status word.
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include "pylo_common.cuh"
+#include "pylo_launch.cuh"
+
+#define FF_BM 128               // rows of a CTA's tile
+#define FF_BK 64                // terms per stage
+#define FF_BOX 8192             // bytes of a box: 64 x 64 elements
+#define FF_STAGES 6             // of 32 KB
+#define FF_EPI_WARPS 8
+#define FF_THREADS ((FF_EPI_WARPS + 2) * 32)
+#define FF_SPIN_LIMIT (1 << 22)
+#define FF_GROUP 4              // products of a launch
+#define FF_BAND 8               // rows of tiles that are taken together, so that what is in flight shares operands in the L2 cache
+enum { FF_PLAIN = 0, FF_GATE = 1, FF_BACK = 2 };
+
+// ------------------------------------------------------------------------------------------------
+// tensor cores and barriers
+// ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t ff_cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t ff_cluster_size() { uint32_t n; asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n)); return n; }
+__device__ __forceinline__ void cluster_sync() {   // all threads of the cluster's CTAs; orders accesses to all memory
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address of another CTA's copy of a shared variable
+__device__ __forceinline__ uint32_t nf_at_rank(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ bool ff_elect() {
+  uint32_t pred;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(pred));
+  return pred != 0;
+}
+__device__ __forceinline__ void ff_init(uint64_t* bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ bool ff_try(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+  return ok;
+}
+// false if the wait ran out, here or in another warp of the CTA
+__device__ __forceinline__ bool ff_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  for (int it = 0; it < FF_SPIN_LIMIT; ++it) {
+    if (ff_try(bar, parity)) return true;
+    if ((it & 63) == 63 && *abort) return false;
+  }
+  *abort = 1;
+  return false;
+}
+template <bool PAIR>
+__device__ __forceinline__ void ff_arrive(uint64_t* bar) {   // a pair's: at the first CTA's barrier
+  if constexpr (PAIR) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(nf_at_rank(bar, 0)) : "memory");
+  else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void ff_expect(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void ff_copy(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  if constexpr (PAIR)   // the barrier may be the other CTA's
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void ff_commit(uint64_t* bar) {
+  if constexpr (PAIR)   // arrives at the barriers of both CTAs
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)), "h"((uint16_t)3) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void ff_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (PAIR)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Descriptor of a 128-byte-swizzled operand of 64 x 64 boxes.  K-major: rows of 64 k, groups of eight rows 1024 bytes apart, boxes one behind
+// the other.  MN-major: rows are k and hold 64 mn, groups of eight k 1024 bytes apart, boxes of 64 mn FF_BOX apart.
+__device__ __forceinline__ uint64_t ff_desc(uint32_t saddr, int mn) {
+  return (uint64_t)((saddr >> 4) & 0x3fff) | ((uint64_t)(mn ? FF_BOX >> 4 : 1) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// fp32 sums of products of two operands of one 16-bit type (bf16 or fp16)
+__device__ __forceinline__ uint32_t ff_idesc(uint32_t m, uint32_t n, int a_mn, int b_mn, bool bf16) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+__device__ __forceinline__ void ff_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ff_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// 32 columns of a warp's 32 rows, a row per lane
+__device__ __forceinline__ void ff_ld32(uint32_t taddr, float (&f)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr) : "memory");
+#pragma unroll
+  for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(r[j]);
+}
+
+// ------------------------------------------------------------------------------------------------
+// 16-bit elements, two in a word
+// ------------------------------------------------------------------------------------------------
+template <bool BF>
+__device__ __forceinline__ uint32_t ff_pack(float a, float b) {
+  if constexpr (BF) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+// an fp32 value rounded to its upper three bytes (NaN stays NaN, what rounds beyond the largest becomes infinite)
+__device__ __forceinline__ uint32_t ff_round24(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return v != v ? b | 0x400000u : b + 0x7f + ((b >> 8) & 1);
+}
+
+// ------------------------------------------------------------------------------------------------
+// the product kernel
+// ------------------------------------------------------------------------------------------------
+// What is kept of a tile of h: planes [rows][ld]
+struct ff_kept {
+  uint16_t *h, *p_hi, *q_hi;
+  uint8_t *p_lo, *q_lo;
+};
+struct ff_product {
+  CUtensorMap A[2], B[2];   // the two parts of the contraction; GATE: B is Wg, Wu
+  void* C;                  // PLAIN: [M][ldc]
+  long long ldc;
+  int M, N, K;              // of each part; GATE, BACK: N = hidden
+  int parts;                // of the contraction: 1 or 2
+  int a_mn, b_mn;           // the operand's rows are the contraction index
+  int tiles_m, tiles_n, tile0;   // tile0: tiles of the products before this one
+};
+struct ff_args {
+  ff_product p[FF_GROUP];
+  ff_kept kept;             // GATE: written, BACK: read
+  uint16_t *dg, *du;        // BACK
+  long long ld;             // of kept, dg, du
+  int n, tiles, activation, keep;
+  int *status, *host_status;
+};
+
+template <bool PAIR>
+struct FfSmem {
+  // per stage: A (128 x 64), B (128 x 64; of a pair one half of the tile's 256)
+  unsigned char st[FF_STAGES][4 * FF_BOX];
+  unsigned char out[FF_EPI_WARPS][4096];   // per epilogue warp: 32 rows of 32 elements on their way
+  uint64_t full[FF_STAGES], empty[FF_STAGES], ready[2], free[2], sums;
+  uint32_t tmem;
+  volatile int abort;
+};
+
+// A warp's block of 32 rows x 64 bytes (32 x 16 bit) or 32 x 32 bytes (32 x 8 bit) between rows per lane and rows of four (two) lanes: 16-byte
+// pieces, spread over the banks.
+__device__ __forceinline__ uint4* ff_at64(unsigned char* s, int row, int piece) { return reinterpret_cast<uint4*>(s + row * 64 + 16 * (piece ^ ((row >> 1) & 3))); }
+__device__ __forceinline__ uint4* ff_at32(unsigned char* s, int row, int piece) { return reinterpret_cast<uint4*>(s + row * 32 + 16 * (piece ^ ((row >> 2) & 1))); }
+
+// 32 x 32 elements of 16 bits from a row per lane to memory; rows and columns beyond the matrix are left out
+__device__ __forceinline__ void ff_store16(unsigned char* s, const uint32_t (&w)[16], uint16_t* dst, long long ld, int rows, int cols) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) *ff_at64(s, lane, q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+  __syncwarp();
+  if ((((uintptr_t)dst | (uintptr_t)(2 * ld)) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (lane >> 2) + 8 * i, c = 8 * (lane & 3);
+      if (r < rows && c < cols) {
+        const uint4 v = *ff_at64(s, r, lane & 3);
+        uint16_t* const to = dst + r * ld + c;
+        if (c + 8 <= cols) *reinterpret_cast<uint4*>(to) = v;
+        else {
+          const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (c + j < cols) to[j] = (uint16_t)(e[j >> 1] >> (16 * (j & 1)));
+        }
+      }
+    }
+  } else if (lane < cols) {   // rows that begin anywhere: a row at a time
+    for (int r = 0; r < 32 && r < rows; ++r)
+      dst[r * ld + lane] = reinterpret_cast<const uint16_t*>(ff_at64(s, r, lane >> 3))[lane & 7];
+  }
+}
+// the same for a plane of bytes, whose rows are aligned and have room for whole pieces
+__device__ __forceinline__ void ff_store8(unsigned char* s, const uint32_t (&w)[8], uint8_t* dst, long long ld, int rows, int cols) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 2; ++q) *ff_at32(s, lane, q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = (lane >> 1) + 16 * i, c = 16 * (lane & 1);
+    if (r < rows && c < cols) *reinterpret_cast<uint4*>(dst + r * ld + c) = *ff_at32(s, r, lane & 1);
+  }
+}
+// 32 columns in 24 bits, as two planes
+__device__ __forceinline__ void ff_store24(unsigned char* s, const float (&v)[32], uint16_t* hi, uint8_t* lo, long long ld, int rows, int cols) {
+  uint32_t h[16], l[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = ff_round24(v[4 * j + i]);
+    h[2 * j] = __byte_perm(b[0], b[1], 0x7632);
+    h[2 * j + 1] = __byte_perm(b[2], b[3], 0x7632);
+    l[j] = __byte_perm(__byte_perm(b[0], b[1], 0x0051), __byte_perm(b[2], b[3], 0x0051), 0x5410);
+  }
+  ff_store16(s, h, hi, ld, rows, cols);
+  ff_store8(s, l, lo, ld, rows, cols);
+}
+struct ff_raw24 { uint4 hi[4], lo[2]; };
+__device__ __forceinline__ void ff_fetch24(ff_raw24& r, const uint16_t* hi, const uint8_t* lo, long long ld, int rows, int cols) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = (lane >> 2) + 8 * i, c = 8 * (lane & 3);
+    r.hi[i] = row < rows && c < cols ? __ldg(reinterpret_cast<const uint4*>(hi + row * ld + c)) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = (lane >> 1) + 16 * i, c = 16 * (lane & 1);
+    r.lo[i] = row < rows && c < cols ? __ldg(reinterpret_cast<const uint4*>(lo + row * ld + c)) : make_uint4(0, 0, 0, 0);
+  }
+}
+__device__ __forceinline__ void ff_turn24(unsigned char* s, const ff_raw24& r, float (&v)[32]) {   // to a row per lane
+  const int lane = threadIdx.x & 31;
+  uint32_t h[16], l[8];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *ff_at64(s, (lane >> 2) + 8 * i, lane & 3) = r.hi[i];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) *ff_at32(s + 2048, (lane >> 1) + 16 * i, lane & 1) = r.lo[i];
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(h + 4 * q) = *ff_at64(s, lane, q);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) *reinterpret_cast<uint4*>(l + 4 * q) = *ff_at32(s + 2048, lane, q);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {   // an fp32 value's upper half, and the byte below
+    v[4 * j] = __uint_as_float((h[2 * j] << 16) | ((l[j] << 8) & 0xff00u));
+    v[4 * j + 1] = __uint_as_float((h[2 * j] & 0xffff0000u) | (l[j] & 0xff00u));
+    v[4 * j + 2] = __uint_as_float((h[2 * j + 1] << 16) | ((l[j] >> 8) & 0xff00u));
+    v[4 * j + 3] = __uint_as_float((h[2 * j + 1] & 0xffff0000u) | ((l[j] >> 16) & 0xff00u));
+  }
+}
+
+// act(g) and its slope
+__device__ __forceinline__ void ff_act(int activation, float g, float& a, float& slope) {
+  if (activation == PYLO_ACT_SILU) {
+    const float s = __fdividef(1.0f, 1.0f + __expf(-g));
+    a = g * s;
+    slope = fmaf(a, 1.0f - s, s);
+  } else if (activation == PYLO_ACT_GELU) {
+    const float phi = 0.5f + 0.5f * erff(g * 0.70710678118654752f);
+    a = g * phi;
+    slope = fmaf(g * 0.3989422804014327f, __expf(-0.5f * g * g), phi);
+  } else if (activation == PYLO_ACT_GELU_TANH) {
+    const float k = 0.7978845608028654f, t = tanhf(k * fmaf(0.044715f * g * g, g, g));
+    a = 0.5f * g * (1.0f + t);
+    slope = 0.5f * (1.0f + t) + 0.5f * g * (1.0f - t * t) * k * fmaf(3.0f * 0.044715f * g, g, 1.0f);
+  } else {
+    a = g > 0.f ? g : g != g ? g : 0.f;
+    slope = g > 0.f ? 1.0f : 0.f;
+  }
+}
+
+// PAIR: two CTAs on two SMs share a tile of 256 x 256 (each has its own 128 rows of A and one half of B's columns, and the tensor cores of both
+// read both halves); persistent, with two accumulators, so that one tile's epilogue runs beside the next one's products.
+// Otherwise the CTAs of a cluster (1, 2, 4 or 8) share one tile of 128 x 128, each with its part of the contraction; the first adds their sums up
+// through distributed shared memory, in rank order.
+template <bool PAIR, int EPI, bool BF>
+__global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_constant__ ff_args a) {
+  extern __shared__ unsigned char ff_dyn[];
+  using Smem = FfSmem<PAIR>;
+  constexpr int BN = PAIR ? 256 : 128, TILE_M = PAIR ? 256 : 128, OUT_N = EPI == FF_GATE ? BN / 2 : BN;
+  constexpr uint32_t STAGE = 4 * FF_BOX;
+  Smem& sm = *reinterpret_cast<Smem*>(ff_dyn + ((1024 - (smem_addr(ff_dyn) & 1023)) & 1023));   // at the same place in all CTAs of a cluster
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int rank = (int)ff_cluster_rank(), ctas = (int)ff_cluster_size();
+  if (tid == 0) {
+    for (int s = 0; s < FF_STAGES; ++s) { ff_init(&sm.full[s], 1); ff_init(&sm.empty[s], 1); }
+    for (int s = 0; s < 2; ++s) { ff_init(&sm.ready[s], 1); ff_init(&sm.free[s], (PAIR ? 2 : 1) * FF_EPI_WARPS); }
+    ff_init(&sm.sums, ctas > 1 ? (ctas - 1) * FF_EPI_WARPS : 1);
+    sm.abort = 0;
+  }
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)), "r"(512) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)), "r"(512) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+  ff_fence_before();
+  __syncthreads();
+  cluster_sync();   // the other CTAs' barriers exist
+  ff_fence_after();
+  pdl_begin();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+  const int step = (int)gridDim.x / ctas, first = (int)blockIdx.x / ctas;
+  // the product a tile belongs to and its place there: bands of FF_BAND rows of tiles, column by column
+  auto locate = [&](int tile, int& tm, int& tn) -> const ff_product& {
+    int k = 0;
+    while (k + 1 < a.n && tile >= a.p[k + 1].tile0) ++k;
+    const ff_product& p = a.p[k];
+    const int r = tile - p.tile0, band = r / (FF_BAND * p.tiles_n), at = r - band * FF_BAND * p.tiles_n, high = min(FF_BAND, p.tiles_m - band * FF_BAND);
+    tn = at / high;
+    tm = band * FF_BAND + at - tn * high;
+    return p;
+  };
+  // this CTA's share of the contraction, in stages
+  auto share = [&](const ff_product& p, int& kb0, int& kb1) {
+    const int per_part = (p.K + FF_BK - 1) / FF_BK, n = per_part * p.parts, per = PAIR ? n : (n + ctas - 1) / ctas;
+    kb0 = PAIR ? 0 : min(rank * per, n);
+    kb1 = PAIR ? n : min(kb0 + per, n);
+    return per_part;
+  };
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- copies
+    if (ff_elect()) {
+      asm volatile("fence.proxy.async;" ::: "memory");   // what earlier kernels stored is read through the async proxy
+      uint32_t n = 0;
+      bool dead = false;
+      for (int tile = first; tile < a.tiles && !dead && !sm.abort; tile += step) {
+        int tm, tn, kb0, kb1;
+        const ff_product& p = locate(tile, tm, tn);
+        const int per_part = share(p, kb0, kb1);
+        for (int kb = kb0; kb < kb1; ++kb, ++n) {
+          const uint32_t s = n % FF_STAGES, use = n / FF_STAGES;
+          if (use > 0 && !ff_wait(&sm.empty[s], (use - 1) & 1, &sm.abort)) { dead = true; break; }
+          // boxes that reach beyond the matrix are filled with zeros and count in full; of a pair the first CTA's barrier takes the bytes of both
+          if (!PAIR || rank == 0) ff_expect(&sm.full[s], (PAIR ? 2 : 1) * STAGE);
+          const uint32_t bar = PAIR ? nf_at_rank(&sm.full[s], 0) : smem_addr(&sm.full[s]);
+          const int part = kb >= per_part, k = (kb - part * per_part) * FF_BK;
+          uint32_t dst = smem_addr(sm.st[s]);
+#pragma unroll
+          for (int u = 0; u < 2; ++u, dst += FF_BOX) {
+            const int mn = tm * TILE_M + (PAIR ? rank * FF_BM : 0) + 64 * u;
+            ff_copy<PAIR>(dst, &p.A[part], bar, p.a_mn ? mn : k, p.a_mn ? k : mn);
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u, dst += FF_BOX) {
+            int mn = tn * OUT_N + (PAIR ? rank * 128 : 0) + 64 * u, which = part;
+            if constexpr (EPI == FF_GATE) {   // the first half of a tile's columns are Wg's, the second Wu's
+              which = PAIR ? rank : u;
+              mn = tn * OUT_N + (PAIR ? 64 * u : 0);
+            }
+            ff_copy<PAIR>(dst, &p.B[which], bar, p.b_mn ? mn : k, p.b_mn ? k : mn);
+          }
+        }
+      }
+      // the CTA must not end while a copy into its shared memory is in flight: normally the issuing lane has waited for every stage; after an
+      // abort wait (bounded) for the stages filled last
+      if ((!PAIR || rank == 0) && (dead || sm.abort))
+        for (uint32_t f = n > FF_STAGES ? n - FF_STAGES : 0; f < n; ++f)
+          for (int it = 0; it < FF_SPIN_LIMIT; ++it)
+            if (ff_try(&sm.full[f % FF_STAGES], (f / FF_STAGES) & 1)) break;
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- products (of a pair the first CTA issues them)
+    if ((!PAIR || rank == 0) && ff_elect()) {
+      uint32_t n = 0, c = 0;
+      bool dead = false;
+      for (int tile = first; tile < a.tiles && !dead && !sm.abort; tile += step, ++c) {
+        int tm, tn, kb0, kb1;
+        const ff_product& p = locate(tile, tm, tn);
+        share(p, kb0, kb1);
+        const uint32_t idesc = ff_idesc(TILE_M, BN, p.a_mn, p.b_mn, BF), acc = tmem + (c & 1) * 256;
+        const uint64_t a_step = (p.a_mn ? 2048 : 32) >> 4, b_step = (p.b_mn ? 2048 : 32) >> 4;   // 16 terms further
+        if (c >= 2) {   // the tile before the last has left its accumulator
+          if (!ff_wait(&sm.free[c & 1], ((c >> 1) - 1) & 1, &sm.abort)) break;
+          ff_fence_after();
+        }
+        for (int kb = kb0; kb < kb1; ++kb, ++n) {
+          const uint32_t s = n % FF_STAGES;
+          if (!ff_wait(&sm.full[s], (n / FF_STAGES) & 1, &sm.abort)) { dead = true; break; }
+          ff_fence_after();
+          const uint64_t da = ff_desc(smem_addr(sm.st[s]), p.a_mn), db = ff_desc(smem_addr(sm.st[s]) + 2 * FF_BOX, p.b_mn);
+#pragma unroll
+          for (int ks = 0; ks < FF_BK / 16; ++ks) ff_mma<PAIR>(acc, da + ks * a_step, db + ks * b_step, idesc, kb > kb0 || ks > 0);
+          ff_commit<PAIR>(&sm.empty[s]);
+        }
+        if (!dead) ff_commit<PAIR>(&sm.ready[c & 1]);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- epilogue: a warp's 32 rows, half of the tile's columns, 32 at a time
+    const int quarter = warp & 3, half = (warp - 2) >> 2, e = warp - 2;
+    const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
+    unsigned char* const stage = sm.out[e];
+    uint32_t c = 0;
+    for (int tile = first; tile < a.tiles && !sm.abort; tile += step, ++c) {
+      int tm, tn, kb0, kb1;
+      const ff_product& p = locate(tile, tm, tn);
+      share(p, kb0, kb1);
+      const int m0 = tm * TILE_M + (PAIR ? rank * FF_BM : 0) + quarter * 32, rows = p.M - m0;
+      if (!ff_wait(&sm.ready[c & 1], (c >> 1) & 1, &sm.abort)) break;
+      ff_fence_after();
+      const uint32_t acc = t_lane + (c & 1) * 256;
+      bool leave = false;
+      if constexpr (!PAIR) {
+        // this CTA's sums, where another one has the tile: the stages are free, all products being done
+        if (rank > 0) {
+          for (int q = 0; q < 2; ++q) {   // GATE: 32 columns of either half, else 64 columns of one
+            const int block = EPI == FF_GATE ? half + 2 * q : 2 * half + q;
+            float v[32];
+            ff_ld32(acc + 32 * block, v);
+            const bool none = kb0 == kb1;   // no share: nothing has been written there
+            float4* const box = reinterpret_cast<float4*>(sm.st) + (block * 4 + quarter) * 256 + lane;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) box[32 * j] = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          }
+          __syncwarp();
+          if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(nf_at_rank(&sm.sums, 0)) : "memory");
+          leave = true;
+        } else if (ctas > 1) {
+          if (!ff_wait(&sm.sums, 0, &sm.abort)) break;
+          asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        }
+      }
+      // 32 columns of the tile's sums
+      auto tile_sums = [&](int block, float (&v)[32]) {
+        ff_ld32(acc + 32 * block, v);
+        if constexpr (!PAIR) {
+          for (int r = 1; r < ctas; ++r) {
+            const uint32_t src = nf_at_rank(reinterpret_cast<float4*>(sm.st) + (block * 4 + quarter) * 256 + lane, r);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float4 o;
+              asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w) : "r"(src + 512 * j) : "memory");
+              v[4 * j] += o.x; v[4 * j + 1] += o.y; v[4 * j + 2] += o.z; v[4 * j + 3] += o.w;
+            }
+          }
+        }
+      };
+      if (!leave && rows > 0) {
+        constexpr int BLOCKS = OUT_N / 64;   // of 32 columns for this warp
+#pragma unroll 1
+        for (int q = 0; q < BLOCKS; ++q) {
+          const int block = half * BLOCKS + q, n0 = tn * OUT_N + 32 * block, cols = p.N - n0;
+          const long long at = (long long)m0 * a.ld + n0;
+          if (cols <= 0) break;
+          if constexpr (EPI == FF_PLAIN) {
+            float v[32];
+            tile_sums(block, v);
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = ff_pack<BF>(v[2 * j], v[2 * j + 1]);
+            ff_store16(stage, w, (uint16_t*)p.C + (long long)m0 * p.ldc + n0, p.ldc, rows, cols);
+          } else if constexpr (EPI == FF_GATE) {
+            float g[32], u[32], q_[32];
+            tile_sums(block, g);
+            tile_sums(block + OUT_N / 32, u);
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float slope[2], h[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                ff_act(a.activation, g[2 * j + i], q_[2 * j + i], slope[i]);
+                h[i] = q_[2 * j + i] * u[2 * j + i];
+                u[2 * j + i] *= slope[i];
+              }
+              w[j] = ff_pack<BF>(h[0], h[1]);
+            }
+            ff_store16(stage, w, a.kept.h + at, a.ld, rows, cols);
+            if (a.keep) {
+              ff_store24(stage, u, a.kept.p_hi + at, a.kept.p_lo + at, a.ld, rows, cols);
+              ff_store24(stage, q_, a.kept.q_hi + at, a.kept.q_lo + at, a.ld, rows, cols);
+            }
+          } else {
+            ff_raw24 rp, rq;
+            ff_fetch24(rp, a.kept.p_hi + at, a.kept.p_lo + at, a.ld, rows, cols);
+            ff_fetch24(rq, a.kept.q_hi + at, a.kept.q_lo + at, a.ld, rows, cols);
+            float v[32], f[32];
+            tile_sums(block, v);
+            uint32_t w[16];
+            ff_turn24(stage, rp, f);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = ff_pack<BF>(v[2 * j] * f[2 * j], v[2 * j + 1] * f[2 * j + 1]);
+            ff_store16(stage, w, a.dg + at, a.ld, rows, cols);
+            ff_turn24(stage, rq, f);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = ff_pack<BF>(v[2 * j] * f[2 * j], v[2 * j + 1] * f[2 * j + 1]);
+            ff_store16(stage, w, a.du + at, a.ld, rows, cols);
+          }
+        }
+      }
+      ff_fence_before();
+      __syncwarp();
+      if (lane == 0) ff_arrive<PAIR>(&sm.free[c & 1]);
+    }
+  }
+  ff_fence_before();
+  __syncthreads();
+  cluster_sync();   // no CTA leaves while another may reach into its shared memory
+  if (tid == 0 && sm.abort) {
+    if (a.status) atomicOr(a.status, 16);
+    if (a.host_status) *reinterpret_cast<volatile int*>(a.host_status) = 16;
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// host
+// ------------------------------------------------------------------------------------------------
+typedef CUresult (*FfEncode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static FfEncode ff_encode() {
+  static FfEncode fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
+    return (FfEncode)p;
+  }();
+  return fn;
+}
+// [rows][cols] of 16-bit elements, boxes of 64 x 64; what a box reaches beyond the matrix reads as zero
+static int ff_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int type) {
+  FfEncode fn = ff_encode();
+  if (!fn) return -5;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {64, 64}, unit[2] = {1, 1};
+  return fn(map, type == PYLO_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, unit,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -5;
+}
+
+// Encoding a tensor map wants the device's context to be the thread's current one, which a thread that has only asked for the device (autograd's, at its
+// first backward pass) need not have.
+static int ff_begin() {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaSetDevice(dev);
+  return (int)e;
+}
+static int64_t ff_ld(int hidden) { return ((int64_t)hidden + 15) / 16 * 16; }   // of h and what is made like it
+static int64_t ff_plane(int64_t rows, int hidden, int bytes) { return (rows * ff_ld(hidden) * bytes + 255) / 256 * 256; }
+static ff_kept ff_planes(void* base, int64_t rows, int hidden) {
+  char* p = (char*)base;
+  const int64_t two = ff_plane(rows, hidden, 2), one = ff_plane(rows, hidden, 1);
+  return {(uint16_t*)p, (uint16_t*)(p + two), (uint16_t*)(p + 2 * two), (uint8_t*)(p + 3 * two), (uint8_t*)(p + 3 * two + one)};
+}
+
+static bool ff_pairs(const ff_args& a, int epi) {
+  return false;
+}
+template <bool PAIR, int EPI, bool BF>
+static int ff_go(ff_args& a, cudaStream_t s) {
+  constexpr int TILE_M = PAIR ? 256 : 128, TILE_N = (PAIR ? 256 : 128) / (EPI == FF_GATE ? 2 : 1);
+  int64_t tiles = 0;
+  int longest = 1;
+  for (int k = 0; k < a.n; ++k) {
+    ff_product& p = a.p[k];
+    p.tiles_m = (p.M + TILE_M - 1) / TILE_M;
+    p.tiles_n = (p.N + TILE_N - 1) / TILE_N;
+    p.tile0 = (int)tiles;
+    tiles += (int64_t)p.tiles_m * p.tiles_n;
+    const int blocks = (p.K + FF_BK - 1) / FF_BK * p.parts;
+    if (blocks > longest) longest = blocks;
+  }
+  if (tiles > (1 << 27)) return -1;
+  a.tiles = (int)tiles;
+  if (!tiles) return 0;
+  static bool configured[PYLO_MAX_DEVICES] = {};
+  constexpr int SMEM = (int)sizeof(FfSmem<PAIR>) + 1024;
+  if (int rc = allow_dynamic_smem(k_ffn_product<PAIR, EPI, BF>, SMEM, configured)) return rc;
+  int cluster = 2, grid;
+  if constexpr (PAIR) {
+    const int pairs = sm_count() / 2;
+    grid = 2 * (int)(tiles < pairs ? tiles : pairs);
+  } else {
+    // the CTAs that share a tile: as long as all run at once and each has four stages of the contraction at least
+    cluster = 1;
+    while (cluster < 8 && tiles * cluster * 2 <= sm_count() && longest >= cluster * 2 * 4) cluster *= 2;
+    grid = (int)tiles * cluster;
+  }
+  launch_clusters(k_ffn_product<PAIR, EPI, BF>, grid, FF_THREADS, cluster, SMEM, s, a);
+  return launch_status();
+}
+template <int EPI>
+static int ff_run(ff_args& a, int type, cudaStream_t s) {
+  if (ff_pairs(a, EPI)) return type == PYLO_BF16 ? ff_go<true, EPI, true>(a, s) : ff_go<true, EPI, false>(a, s);
+  return type == PYLO_BF16 ? ff_go<false, EPI, true>(a, s) : ff_go<false, EPI, false>(a, s);
+}
+static bool ff_operand(const void* p, int64_t ld, int64_t cols) { return p && ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld >= cols; }
+static bool ff_good(const pylo_ffn* f) {
+  return f && f->rows >= 0 && f->rows <= (1 << 30) && f->width > 0 && f->hidden > 0 && f->out > 0 && f->width <= (1 << 24) && f->hidden <= (1 << 24) &&
+         f->out <= (1 << 24) && (f->type == PYLO_BF16 || f->type == PYLO_FP16) && f->activation >= PYLO_ACT_SILU && f->activation <= PYLO_ACT_RELU;
+}
+static ff_product ff_of(void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, int parts, int a_mn, int b_mn) {
+  ff_product p = {};
+  p.C = C; p.ldc = ldc; p.M = (int)M; p.N = (int)N; p.K = (int)K; p.parts = parts; p.a_mn = a_mn; p.b_mn = b_mn;
+  return p;
+}
+
+extern "C" {
+
+int64_t pylo_b200_gated_ffn_kept(int64_t rows, int hidden, int keep) {
+  if (rows <= 0 || hidden <= 0) return 0;
+  return ff_plane(rows, hidden, 2) * (keep ? 3 : 1) + ff_plane(rows, hidden, 1) * (keep ? 2 : 0);
+}
+int64_t pylo_b200_gated_ffn_workspace(int64_t rows, int hidden) { return rows <= 0 || hidden <= 0 ? 0 : 2 * ff_plane(rows, hidden, 2); }
+
+int pylo_b200_gated_ffn(const pylo_ffn* f, void* stream) {
+  CHECK_ARG(ff_good(f));
+  if (f->rows == 0) return 0;
+  CHECK_ARG(ff_operand(f->x, f->ld_x, f->width) && ff_operand(f->w_gate, f->ld_gate, f->width) && ff_operand(f->w_up, f->ld_up, f->width) &&
+            ff_operand(f->w_down, f->ld_down, f->hidden) && f->y && f->kept && ((uintptr_t)f->kept & 255) == 0);
+  if (int rc = ff_begin()) return rc;
+  const ff_kept kept = ff_planes(f->kept, f->rows, f->hidden);
+  const int64_t ld = ff_ld(f->hidden);
+  ff_args a = {};
+  a.kept = kept; a.ld = ld; a.n = 1; a.activation = f->activation; a.keep = f->keep; a.status = f->status; a.host_status = f->host_status;
+  a.p[0] = ff_of(nullptr, 0, f->rows, f->hidden, f->width, 1, 0, 0);
+  if (int rc = ff_map(&a.p[0].A[0], f->x, f->rows, f->width, f->ld_x, f->type)) return rc;
+  if (int rc = ff_map(&a.p[0].B[0], f->w_gate, f->hidden, f->width, f->ld_gate, f->type)) return rc;
+  if (int rc = ff_map(&a.p[0].B[1], f->w_up, f->hidden, f->width, f->ld_up, f->type)) return rc;
+  if (int rc = ff_run<FF_GATE>(a, f->type, (cudaStream_t)stream)) return rc;
+  a.p[0] = ff_of(f->y, f->out, f->rows, f->out, f->hidden, 1, 0, 0);
+  if (int rc = ff_map(&a.p[0].A[0], kept.h, f->rows, f->hidden, ld, f->type)) return rc;
+  if (int rc = ff_map(&a.p[0].B[0], f->w_down, f->out, f->hidden, f->ld_down, f->type)) return rc;
+  return ff_run<FF_PLAIN>(a, f->type, (cudaStream_t)stream);
+}
+
+int pylo_b200_gated_ffn_backward(const pylo_ffn* f, void* stream) {
+  CHECK_ARG(ff_good(f) && f->rows > 0);
+  const bool inner = f->dx || f->dw_gate || f->dw_up;
+  CHECK_ARG(ff_operand(f->dy, f->ld_dy, f->out) && f->kept && ((uintptr_t)f->kept & 255) == 0);
+  CHECK_ARG(!inner || (ff_operand(f->w_down, f->ld_down, f->hidden) && f->work && ((uintptr_t)f->work & 255) == 0));
+  CHECK_ARG(!f->dx || (ff_operand(f->w_gate, f->ld_gate, f->width) && ff_operand(f->w_up, f->ld_up, f->width)));
+  CHECK_ARG(!(f->dw_gate || f->dw_up) || ff_operand(f->x, f->ld_x, f->width));
+  if (int rc = ff_begin()) return rc;
+  const ff_kept kept = ff_planes(f->kept, f->rows, f->hidden);
+  const int64_t ld = ff_ld(f->hidden);
+  ff_args a = {};
+  a.kept = kept; a.ld = ld; a.activation = f->activation; a.status = f->status; a.host_status = f->host_status;
+  a.dg = (uint16_t*)f->work;
+  a.du = (uint16_t*)((char*)f->work + ff_plane(f->rows, f->hidden, 2));
+  if (inner) {   // dh (m: rows, n: hidden, k: out), Wd's rows being the contraction index
+    a.n = 1;
+    a.p[0] = ff_of(nullptr, 0, f->rows, f->hidden, f->out, 1, 0, 1);
+    if (int rc = ff_map(&a.p[0].A[0], f->dy, f->rows, f->out, f->ld_dy, f->type)) return rc;
+    if (int rc = ff_map(&a.p[0].B[0], f->w_down, f->out, f->hidden, f->ld_down, f->type)) return rc;
+    if (int rc = ff_run<FF_BACK>(a, f->type, (cudaStream_t)stream)) return rc;
+  }
+  a.n = 0;
+  if (f->dx) {
+    ff_product& p = a.p[a.n++] = ff_of(f->dx, f->width, f->rows, f->width, f->hidden, 2, 0, 1);
+    if (int rc = ff_map(&p.A[0], a.dg, f->rows, f->hidden, ld, f->type)) return rc;
+    if (int rc = ff_map(&p.A[1], a.du, f->rows, f->hidden, ld, f->type)) return rc;
+    if (int rc = ff_map(&p.B[0], f->w_gate, f->hidden, f->width, f->ld_gate, f->type)) return rc;
+    if (int rc = ff_map(&p.B[1], f->w_up, f->hidden, f->width, f->ld_up, f->type)) return rc;
+  }
+  for (int k = 0; k < 2; ++k)
+    if (void* const out = k ? f->dw_up : f->dw_gate) {
+      ff_product& p = a.p[a.n++] = ff_of(out, f->width, f->hidden, f->width, f->rows, 1, 1, 1);
+      if (int rc = ff_map(&p.A[0], k ? a.du : a.dg, f->rows, f->hidden, ld, f->type)) return rc;
+      if (int rc = ff_map(&p.B[0], f->x, f->rows, f->width, f->ld_x, f->type)) return rc;
+    }
+  if (f->dw_down) {
+    ff_product& p = a.p[a.n++] = ff_of(f->dw_down, f->hidden, f->out, f->hidden, f->rows, 1, 1, 1);
+    if (int rc = ff_map(&p.A[0], f->dy, f->rows, f->out, f->ld_dy, f->type)) return rc;
+    if (int rc = ff_map(&p.B[0], kept.h, f->rows, f->hidden, ld, f->type)) return rc;
+  }
+  return a.n ? ff_run<FF_PLAIN>(a, f->type, (cudaStream_t)stream) : 0;
+}
+
+int pylo_b200_sizeof_layers(int what) {
+  return what == 0 ? (int)sizeof(pylo_norm) : what == 1 ? (int)sizeof(pylo_distill) : what == 2 ? (int)sizeof(pylo_ffn) : -1;
+}
+
+}  // extern "C"

@@ -1,0 +1,436 @@
+"""What a model's training step needs beside the optimizer, where the gradients come from: layer norm, the gated feed-forward block and the
+loss of a distillation from a teacher's largest logits, each with its gradients.
+
+Functions that autograd differentiates once, and modules that hold their parameters.  They take CUDA tensors of fp32, bf16 or fp16 (the
+feed-forward block: bf16 or fp16), run on the current stream of the tensors' device, wait for nothing, and leave their arguments as they are.
+A call can be captured into a CUDA graph, forward and backward, ``gated_ffn`` after one that is not; as with any other operator, no result of an
+earlier pass over the same parameters may be alive when a backward pass is captured (autograd would make the capture wait for that pass's stream).
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+
+TYPES = {torch.float32: L.FP32, torch.bfloat16: L.BF16, torch.float16: L.FP16}
+ACTIVATIONS = {"silu": L.ACT_SILU, "gelu": L.ACT_GELU, "gelu_tanh": L.ACT_GELU_TANH, "relu": L.ACT_RELU}
+REDUCTIONS = {"none": L.REDUCE_NONE, "sum": L.REDUCE_SUM, "mean": L.REDUCE_MEAN}
+
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _call(function, what, device, *args):
+    """A function of the library on the current stream of a device."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        code = function(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = function(*args, _raw_stream(index))
+    if code:
+        L.check(code, what)
+
+
+def _on(device, function, *args):
+    """What a function of the library that asks the current device says for ``device``."""
+    if device.index == torch.cuda.current_device():
+        return function(*args)
+    with torch.cuda.device(device):
+        return function(*args)
+
+
+def _check(name, t, device=None, types=TYPES):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} has to be a tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} has to be a CUDA tensor, it is on {t.device}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.dtype not in types:
+        raise TypeError(f"{name} is {t.dtype}, supported are {', '.join(str(d).split('.')[1] for d in types)}")
+
+
+def _rows(t):
+    """A tensor as rows of its last dimension, whose elements follow one another: a view where there is one, else a copy."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 else t.contiguous()
+
+
+def _graph(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# layer norm
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def _norm_forward(x, weight, bias, eps, keep):
+    n, width = x.shape
+    y = torch.empty((n, width), dtype=x.dtype, device=x.device)
+    stat = torch.empty((2, n), dtype=torch.float32, device=x.device) if keep else None
+    if n:
+        w = L.Norm(x=x.data_ptr(), weight=None if weight is None else weight.data_ptr(), bias=None if bias is None else bias.data_ptr(),
+                   y=y.data_ptr(), rows=n, x_stride=x.stride(0), width=width, type=TYPES[x.dtype],
+                   weight_type=TYPES[x.dtype if weight is None else weight.dtype], eps=eps)
+        if keep:
+            w.mean = stat.data_ptr()
+            w.rstd = w.mean + 4 * n
+        _call(L.lib.pylo_b200_layer_norm, "layer_norm", x.device, C.byref(w))
+    return y, stat
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, weight, bias, eps):
+        y, stat = _norm_forward(rows, weight, bias, eps, True)
+        ctx.save_for_backward(rows, weight, stat)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        rows, weight, stat = ctx.saved_tensors
+        n, width = rows.shape
+        dy = _rows(dy)
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        dx = torch.empty((n, width), dtype=rows.dtype, device=rows.device) if need_x else None
+        dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w else None
+        db = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_b else None
+        columns = need_w or need_b
+        w = L.Norm(x=rows.data_ptr(), dy=dy.data_ptr(), weight=None if weight is None else weight.data_ptr(), mean=stat.data_ptr(),
+                   rstd=stat.data_ptr() + 4 * n, dx=dx.data_ptr() if need_x else None, dweight=dw.data_ptr() if need_w else None,
+                   dbias=db.data_ptr() if need_b else None, rows=n, x_stride=rows.stride(0), dy_stride=dy.stride(0), width=width,
+                   type=TYPES[rows.dtype], weight_type=TYPES[rows.dtype if weight is None else weight.dtype])
+        if columns:
+            w.work_floats = _on(rows.device, L.lib.pylo_b200_layer_norm_workspace, n, width)
+            work = torch.empty(w.work_floats, dtype=torch.float32, device=rows.device)
+            w.work = work.data_ptr()
+        if n or columns:
+            _call(L.lib.pylo_b200_layer_norm_backward, "layer_norm backward", rows.device, C.byref(w))
+        return dx, dw, db, None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last dimension: ``(x - mean) / sqrt(variance + eps) * weight + bias``, of ``x``'s type.
+
+    ``weight`` and ``bias`` are vectors of ``x``'s type or fp32, and their gradients are of that type; a bias needs a weight beside it.  Means,
+    variances and the sums of the gradients are fp32, each result is rounded once.  Rows of up to 32768 elements, of any stride."""
+    _check("x", x)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("x needs a last dimension of at least one element")
+    width = x.shape[-1]
+    if width > L.NORM_MOST:
+        raise ValueError(f"x has rows of {width} elements: {L.NORM_MOST} are supported")
+    if not (isinstance(eps, (int, float)) and 0.0 <= eps < math.inf):
+        raise ValueError(f"eps has to be a finite number >= 0, got {eps!r}")
+    if weight is None and bias is not None:
+        raise ValueError("a bias needs a weight beside it")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        _check(name, t, x.device)
+        if t.shape != (width,):
+            raise ValueError(f"{name} has the shape {tuple(t.shape)}, x has rows of {width} elements")
+        if t.dtype not in (x.dtype, torch.float32) or t.dtype != weight.dtype:
+            raise TypeError(f"weight and bias have to be both of x's type or both float32, {name} is {t.dtype}")
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    rows = _rows(x)
+    y = _LayerNorm.apply(rows, weight, bias, float(eps)) if _graph(x, weight, bias) else _norm_forward(rows, weight, bias, float(eps), False)[0]
+    return y if x.dim() == 2 else y.view(x.shape)
+
+
+class LayerNorm(torch.nn.Module):
+    """:func:`layer_norm` with its parameters, as ``torch.nn.LayerNorm`` over the last dimension."""
+
+    def __init__(self, width: int, eps: float = 1e-5, bias: bool = True, device=None, dtype=None):
+        super().__init__()
+        self.eps = eps
+        self.weight = torch.nn.Parameter(torch.ones(width, device=device, dtype=dtype))
+        self.bias = torch.nn.Parameter(torch.zeros(width, device=device, dtype=dtype)) if bias else None
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+    def extra_repr(self):
+        return f"{self.weight.numel()}, eps={self.eps}, bias={self.bias is not None}"
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the gated feed-forward block
+# ---------------------------------------------------------------------------------------------------------------------
+
+_reported = None   # a word in pinned memory that a kernel sets when one of its waits ran out
+
+
+def _status_word():
+    global _reported
+    if _reported is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("gated_ffn has to run once before it is captured into a CUDA graph")
+        word = torch.zeros(1, dtype=torch.int32).pin_memory()
+        _reported = (word, word.numpy(), word.data_ptr())
+    if _reported[1][0]:
+        raise L.PyloLibError("gated_ffn: a wait in a kernel of an earlier call ran out, its results are incomplete (clear_status() to go on)")
+    return _reported[2]
+
+
+def check_status():
+    """Waits for the current device and raises if a kernel of an earlier :func:`gated_ffn` reported a wait that ran out.  Without it, the
+    next call does."""
+    torch.cuda.synchronize()
+    if _reported is not None:
+        _status_word()
+
+
+def clear_status():
+    """Forget what :func:`check_status` raises for."""
+    if _reported is not None:
+        torch.cuda.synchronize()
+        _reported[1][0] = 0
+
+
+def _operand(t):
+    """Rows as the copies to the tensor cores need them, on 16-byte boundaries: (tensor, elements between rows)."""
+    rows, cols = t.shape
+    if t.stride(1) == 1 and t.data_ptr() % 16 == 0:
+        if rows == 1:
+            return t, -(-cols // 8) * 8
+        if t.stride(0) % 8 == 0 and t.stride(0) >= cols:
+            return t, t.stride(0)
+    out = torch.empty((rows, -(-cols // 8) * 8), dtype=t.dtype, device=t.device)
+    out[:, :cols] = t
+    return out[:, :cols], out.stride(0)
+
+
+def _ffn_struct(x, w_gate, w_up, w_down, activation):
+    """The call's struct with its operands, and what has to stay alive until it is made."""
+    n, width = x.shape
+    (x, ld_x), (w_gate, ld_gate), (w_up, ld_up), (w_down, ld_down) = map(_operand, (x, w_gate, w_up, w_down))
+    f = L.Ffn(x=x.data_ptr(), w_gate=w_gate.data_ptr(), w_up=w_up.data_ptr(), w_down=w_down.data_ptr(), rows=n, ld_x=ld_x, ld_gate=ld_gate, ld_up=ld_up,
+              ld_down=ld_down, width=width, hidden=w_gate.shape[0], out=w_down.shape[0], type=TYPES[x.dtype], activation=activation,
+              host_status=_status_word())
+    return f, (x, w_gate, w_up, w_down)
+
+
+def _ffn_forward(rows, w_gate, w_up, w_down, activation, keep):
+    """(y, the rows as they are saved for the backward pass, what else is)"""
+    y = torch.empty((rows.shape[0], w_down.shape[0]), dtype=rows.dtype, device=rows.device)
+    if not rows.shape[0]:
+        return y, rows, None
+    f, alive = _ffn_struct(rows, w_gate, w_up, w_down, activation)
+    kept = torch.empty(L.lib.pylo_b200_gated_ffn_kept(f.rows, f.hidden, keep), dtype=torch.uint8, device=rows.device)
+    f.y, f.kept, f.keep = y.data_ptr(), kept.data_ptr(), keep
+    _call(L.lib.pylo_b200_gated_ffn, "gated_ffn", rows.device, C.byref(f))
+    return y, alive[0], kept
+
+
+class _GatedFFN(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, w_gate, w_up, w_down, activation):
+        y, rows, kept = _ffn_forward(rows, w_gate, w_up, w_down, activation, 1)
+        ctx.save_for_backward(rows, w_gate, w_up, w_down, kept)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        rows, w_gate, w_up, w_down, kept = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        like = dict(dtype=rows.dtype, device=rows.device)
+        make = torch.empty if kept is not None else torch.zeros
+        grads = [make(shape, **like) if wanted else None for wanted, shape in zip(need, (rows.shape, w_gate.shape, w_up.shape, w_down.shape))]
+        if kept is not None:
+            dy, ld = _operand(_rows(dy))
+            f, alive = _ffn_struct(rows, w_gate, w_up, w_down, ctx.activation)
+            work = torch.empty(L.lib.pylo_b200_gated_ffn_workspace(f.rows, f.hidden), dtype=torch.uint8, device=rows.device)
+            f.dy, f.ld_dy, f.kept, f.work = dy.data_ptr(), ld, kept.data_ptr(), work.data_ptr()
+            f.dx, f.dw_gate, f.dw_up, f.dw_down = (None if g is None else g.data_ptr() for g in grads)
+            _call(L.lib.pylo_b200_gated_ffn_backward, "gated_ffn backward", rows.device, C.byref(f))
+        return *grads, None
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """The gated feed-forward block ``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T``.
+
+    ``x`` is ``[..., width]``, ``w_gate`` and ``w_up`` are ``[hidden, width]``, ``w_down`` is ``[out, hidden]``; all are bf16 or all fp16.
+    ``activation``: ``"silu"``, ``"gelu"`` (with the error function), ``"gelu_tanh"`` or ``"relu"``.  Sums are fp32; the hidden values, and backward
+    their gradients, are rounded to the type once, where they become operands of the next product.  Sizes and strides are free; matrices whose rows do
+    not begin on 16-byte boundaries are copied first.  For a backward pass 8 bytes are kept per hidden value."""
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError(f"activation is {activation!r}, supported are {', '.join(ACTIVATIONS)}")
+    _check("x", x, types=(torch.bfloat16, torch.float16))
+    for name, t in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
+        _check(name, t, x.device, (x.dtype,))
+        if t.dim() != 2:
+            raise ValueError(f"{name} has to be a matrix, got the shape {tuple(t.shape)}")
+    if x.dim() == 0 or w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[-1] or w_down.shape[1] != w_gate.shape[0]:
+        raise ValueError(f"the shapes do not fit together: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, w_down {tuple(w_down.shape)}")
+    if min(*w_gate.shape, *w_down.shape) == 0 or max(*w_gate.shape, *w_down.shape) > 1 << 24 or math.prod(x.shape[:-1]) > 1 << 30:
+        raise ValueError("sizes from 1 to 2^24 and up to 2^30 rows are supported")
+    rows = _rows(x)
+    y = _GatedFFN.apply(rows, w_gate, w_up, w_down, code) if _graph(x, w_gate, w_up, w_down) else _ffn_forward(rows, w_gate, w_up, w_down, code, 0)[0]
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
+
+
+class GatedFFN(torch.nn.Module):
+    """:func:`gated_ffn` with its parameters, initialised as ``torch.nn.Linear`` without biases."""
+
+    def __init__(self, width: int, hidden: int, out: int | None = None, activation: str = "silu", device=None, dtype=torch.bfloat16):
+        super().__init__()
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"activation is {activation!r}, supported are {', '.join(ACTIVATIONS)}")
+        self.activation = activation
+        make = lambda rows, cols: torch.nn.Parameter(torch.empty(rows, cols, device=device, dtype=dtype).uniform_(-cols ** -0.5, cols ** -0.5))
+        self.w_gate, self.w_up, self.w_down = make(hidden, width), make(hidden, width), make(width if out is None else out, hidden)
+
+    def forward(self, x):
+        return gated_ffn(x, self.w_gate, self.w_up, self.w_down, self.activation)
+
+    def extra_repr(self):
+        return f"{self.w_gate.shape[1]}, {self.w_gate.shape[0]}, out={self.w_down.shape[0]}, activation={self.activation!r}"
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# distillation from a teacher's largest logits
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def _distill_arguments(logits, teacher_logits, teacher_ids, temperature, weights, reduction):
+    """Checked arguments: (logits' rows, teacher, ids, weights, code of the reduction)."""
+    _check("logits", logits)
+    _check("teacher_logits", teacher_logits, logits.device)
+    _check("teacher_ids", teacher_ids, logits.device, (torch.int64, torch.int32))
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"reduction is {reduction!r}, supported are {', '.join(REDUCTIONS)}")
+    if not (isinstance(temperature, (int, float)) and 2.0 ** -60 <= temperature <= 2.0 ** 60):
+        raise ValueError(f"temperature has to be a positive number from 2^-60 to 2^60, got {temperature!r}")
+    if logits.dim() == 0 or not 1 <= logits.shape[-1] <= 1 << 30:
+        raise ValueError("logits need a last dimension of 1 to 2^30 classes")
+    lead = logits.shape[:-1]
+    if teacher_logits.dim() == 0 or teacher_logits.shape != teacher_ids.shape or teacher_logits.shape[:-1] != lead:
+        raise ValueError(f"teacher_logits {tuple(teacher_logits.shape)} and teacher_ids {tuple(teacher_ids.shape)} have to be alike and to begin as logits do, {tuple(lead)}")
+    if not 1 <= teacher_logits.shape[-1] <= L.DISTILL_MOST_TOP:
+        raise ValueError(f"a teacher gives 1 to {L.DISTILL_MOST_TOP} entries, got {teacher_logits.shape[-1]}")
+    if weights is not None:
+        _check("weights", weights, logits.device, (*TYPES, torch.bool))
+        if weights.shape != lead:
+            raise ValueError(f"weights have the shape {tuple(weights.shape)}, the rows of logits {tuple(lead)}")
+    if torch.is_grad_enabled() and (teacher_logits.requires_grad or (weights is not None and weights.requires_grad)):
+        raise ValueError("teacher_logits and weights are constants here: detach them")
+    rows = _rows(logits.detach())
+    if rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]:
+        rows = rows.contiguous()
+    if weights is not None:
+        weights = weights.detach().to(torch.float32).contiguous()
+    return rows, teacher_logits.detach().contiguous(), teacher_ids.contiguous(), weights, REDUCTIONS[reduction]
+
+
+def _distill_struct(rows, teacher, ids, weights, temperature, reduction):
+    n, vocab = rows.shape
+    return L.Distill(logits=rows.data_ptr(), teacher=teacher.data_ptr(), ids=ids.data_ptr(), weights=None if weights is None else weights.data_ptr(),
+                     rows=n, stride=vocab if n == 1 else rows.stride(0), vocab=vocab, top=ids.shape[-1], type=TYPES[rows.dtype],
+                     teacher_type=TYPES[teacher.dtype], ids_bytes=ids.element_size(), reduction=reduction, temperature=temperature, scale=1.0)
+
+
+def _distill_forward(rows, teacher, ids, weights, temperature, reduction, lead, keep):
+    n, vocab = rows.shape
+    device = rows.device
+    d = _distill_struct(rows, teacher, ids, weights, temperature, reduction)
+    loss = torch.empty(lead if reduction == L.REDUCE_NONE else (), dtype=torch.float32, device=device)
+    stat = torch.empty((n, 2), dtype=torch.float32, device=device) if keep else None
+    inv = torch.empty(1, dtype=torch.float32, device=device) if keep and reduction == L.REDUCE_MEAN else None
+    d.work_bytes = _on(device, L.lib.pylo_b200_distill_workspace, n, vocab)
+    work = torch.empty(d.work_bytes // 8, dtype=torch.float64, device=device)
+    d.work = work.data_ptr()
+    if reduction == L.REDUCE_NONE:
+        d.row_loss = loss.data_ptr()
+    else:
+        d.loss = loss.data_ptr()
+    if keep:
+        d.stat = stat.data_ptr()
+        d.inv = None if inv is None else inv.data_ptr()
+    _call(L.lib.pylo_b200_distill, "distillation_loss", device, C.byref(d), L.DISTILL_LOSS)
+    return loss, stat, inv
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, rows, teacher, ids, weights, temperature, reduction):
+        loss, stat, inv = _distill_forward(rows, teacher, ids, weights, temperature, reduction, logits.shape[:-1], True)
+        ctx.save_for_backward(rows, teacher, ids, weights, stat, inv)
+        ctx.temperature, ctx.reduction, ctx.shape = temperature, reduction, logits.shape
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, upstream):
+        rows, teacher, ids, weights, stat, inv = ctx.saved_tensors
+        grad = torch.empty(ctx.shape, dtype=rows.dtype, device=rows.device)
+        upstream = upstream.to(torch.float32).contiguous()
+        d = _distill_struct(rows, teacher, ids, weights, ctx.temperature, ctx.reduction)
+        d.stat, d.grad, d.upstream = stat.data_ptr(), grad.data_ptr(), upstream.data_ptr()
+        d.inv = None if inv is None else inv.data_ptr()
+        _call(L.lib.pylo_b200_distill, "distillation_loss backward", rows.device, C.byref(d), L.DISTILL_GRAD)
+        return grad, None, None, None, None, None, None
+
+
+def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor, temperature: float = 1.0,
+                      weights: torch.Tensor | None = None, reduction: str = "mean") -> torch.Tensor:
+    """The divergence of a student's distribution from that of a teacher's largest logits, times ``temperature ** 2``, in fp32.
+
+    ``logits`` are ``[..., classes]``; ``teacher_logits`` and ``teacher_ids`` (int64 or int32) are ``[..., K]``, K up to 1024: the teacher's
+    distribution is the softmax over its K entries.  An id outside of ``[0, classes)`` is padding, whatever stands beside it; one that is given
+    twice counts twice.  ``weights`` (``[...]``, a mask or numbers): a row of weight 0 is not looked at and gets a gradient of 0, as does a row
+    without any entry.  ``reduction``: ``"mean"`` over the sum of the weights that count (0 where that is 0), ``"sum"``, or ``"none"`` (weighted rows).
+    Only ``logits`` are differentiated."""
+    rows, teacher, ids, w, code = _distill_arguments(logits, teacher_logits, teacher_ids, temperature, weights, reduction)
+    if _graph(logits):
+        return _Distillation.apply(logits, rows, teacher, ids, w, float(temperature), code)
+    return _distill_forward(rows, teacher, ids, w, float(temperature), code, logits.shape[:-1], False)[0]
+
+
+def distillation_loss_and_grad(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor, temperature: float = 1.0,
+                               weights: torch.Tensor | None = None, reduction: str = "mean", scale: float | torch.Tensor = 1.0):
+    """:func:`distillation_loss` and ``scale`` times its gradient in one pass over the logits, for ``logits.backward(grad)``: ``(loss, grad)``.
+
+    ``reduction`` is ``"mean"`` or ``"sum"``; ``scale`` a number or a one-element fp32 tensor on the device, such as a loss scale (the
+    loss itself is not scaled)."""
+    rows, teacher, ids, w, code = _distill_arguments(logits, teacher_logits, teacher_ids, temperature, weights, reduction)
+    if code == L.REDUCE_NONE:
+        raise ValueError("reduction has to be 'mean' or 'sum'")
+    d = _distill_struct(rows, teacher, ids, w, float(temperature), code)
+    if isinstance(scale, torch.Tensor):
+        _check("scale", scale, logits.device, (torch.float32,))
+        if scale.numel() != 1:
+            raise ValueError("scale has to have one element")
+        d.upstream = scale.data_ptr()
+    else:
+        d.scale = float(scale)
+    device = rows.device
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    d.work_bytes = _on(device, L.lib.pylo_b200_distill_workspace, *rows.shape)
+    work = torch.empty(d.work_bytes // 8, dtype=torch.float64, device=device)
+    d.loss, d.grad, d.work = loss.data_ptr(), grad.data_ptr(), work.data_ptr()
+    _call(L.lib.pylo_b200_distill, "distillation_loss_and_grad", device, C.byref(d), L.DISTILL_LOSS | L.DISTILL_GRAD)
+    return loss, grad
+
+
+class DistillationLoss(torch.nn.Module):
+    """:func:`distillation_loss` with its options."""
+
+    def __init__(self, temperature: float = 1.0, reduction: str = "mean"):
+        super().__init__()
+        self.temperature, self.reduction = temperature, reduction
+
+    def forward(self, logits, teacher_logits, teacher_ids, weights=None):
+        return distillation_loss(logits, teacher_logits, teacher_ids, self.temperature, weights, self.reduction)
