@@ -75,10 +75,11 @@ __device__ __forceinline__ bool ff_wait(uint64_t* bar, uint32_t parity, volatile
   *abort = 1;
   return false;
 }
+// The accumulator has been read (and nothing else is passed on with it: a release would wait for the warp's stores).  A pair's: at the first CTA's barrier
 template <bool PAIR>
-__device__ __forceinline__ void ff_arrive(uint64_t* bar) {   // a pair's: at the first CTA's barrier
-  if constexpr (PAIR) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(nf_at_rank(bar, 0)) : "memory");
-  else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+__device__ __forceinline__ void ff_arrive(uint64_t* bar) {
+  if constexpr (PAIR) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(nf_at_rank(bar, 0)) : "memory");
+  else asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 __device__ __forceinline__ void ff_expect(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
@@ -480,8 +481,15 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
           }
         }
       };
+      constexpr int BLOCKS = OUT_N / 64;   // of 32 columns for this warp
+      int left = BLOCKS;                   // of them to be read; behind the last, the accumulator is free
+      auto read = [&] {
+        if (--left > 0) return;
+        ff_fence_before();
+        __syncwarp();
+        if (lane == 0) ff_arrive<PAIR>(&sm.free[c & 1]);
+      };
       if (!leave && rows > 0) {
-        constexpr int BLOCKS = OUT_N / 64;   // of 32 columns for this warp
 #pragma unroll 1
         for (int q = 0; q < BLOCKS; ++q) {
           const int block = half * BLOCKS + q, n0 = tn * OUT_N + 32 * block, cols = p.N - n0;
@@ -490,6 +498,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
           if constexpr (EPI == FF_PLAIN) {
             float v[32];
             tile_sums(block, v);
+            read();
             uint32_t w[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[j] = ff_pack<BF>(v[2 * j], v[2 * j + 1]);
@@ -498,6 +507,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
             float g[32], u[32], q_[32];
             tile_sums(block, g);
             tile_sums(block + OUT_N / 32, u);
+            read();
             uint32_t w[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -521,6 +531,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
             ff_fetch24(rq, a.kept.q_hi + at, a.kept.q_lo + at, a.ld, rows, cols);
             float v[32], f[32];
             tile_sums(block, v);
+            read();
             uint32_t w[16];
             ff_turn24(stage, rp, f);
 #pragma unroll
@@ -533,9 +544,10 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
           }
         }
       }
-      ff_fence_before();
-      __syncwarp();
-      if (lane == 0) ff_arrive<PAIR>(&sm.free[c & 1]);
+      if (left > 0) {   // nothing of the tile, or not all of it, lies in the matrix
+        left = 1;
+        read();
+      }
     }
   }
   ff_fence_before();
@@ -591,8 +603,37 @@ static ff_kept ff_planes(void* base, int64_t rows, int hidden) {
   return {(uint16_t*)p, (uint16_t*)(p + two), (uint16_t*)(p + 2 * two), (uint8_t*)(p + 3 * two), (uint8_t*)(p + 3 * two + one)};
 }
 
-static bool ff_pairs(const ff_args& a, int epi) {
-  return false;
+// Which form a product takes.  Pairs where their tiles fill the GPU more than half (74 run at once): rows x 1024 by 1024 x 4096, both projections,
+// 512 rows (64 tiles) 17 us and 22 in tiles of 128 x 128, 256 rows (32) 16 and 13.
+static bool ff_pairs(const ff_product& p, int epi) {
+  const int64_t n = (p.N + (epi == FF_GATE ? 127 : 255)) / (epi == FF_GATE ? 128 : 256);
+  return (int64_t)((p.M + 255) / 256) * n >= 48;
+}
+// Clusters of so many CTAs that run at once: one CTA fills an SM, and not every group of SMs that a cluster has to stay in is a multiple of it.
+template <class K>
+static int ff_active(K kernel, int cluster, int smem) {
+  static int known[PYLO_MAX_DEVICES][4] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int at = cluster == 1 ? 0 : cluster == 2 ? 1 : cluster == 4 ? 2 : 3;
+  if (dev >= 0 && dev < PYLO_MAX_DEVICES && known[dev][at]) return known[dev][at];
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = 8 * 148;
+  cfg.blockDim = FF_THREADS;
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    n = sm_count() / cluster;
+  }
+  if (dev >= 0 && dev < PYLO_MAX_DEVICES) known[dev][at] = n;
+  return n;
 }
 template <bool PAIR, int EPI, bool BF>
 static int ff_go(ff_args& a, cudaStream_t s) {
@@ -619,18 +660,34 @@ static int ff_go(ff_args& a, cudaStream_t s) {
     const int pairs = sm_count() / 2;
     grid = 2 * (int)(tiles < pairs ? tiles : pairs);
   } else {
-    // the CTAs that share a tile: as long as all run at once and each has four stages of the contraction at least
-    cluster = 1;
-    while (cluster < 8 && tiles * cluster * 2 <= sm_count() && longest >= cluster * 2 * 4) cluster *= 2;
+    // how many CTAs share a tile, by the time that is to be expected: 0.15 us a stage, and what a tile costs besides
+    float best = 0.f;
+    for (int c = 1; c <= 8; c *= 2) {
+      const int64_t at_once = ff_active(k_ffn_product<PAIR, EPI, BF>, c, SMEM), waves = (tiles + at_once - 1) / at_once;
+      const float t = (float)waves * (0.15f * (float)((longest + c - 1) / c) + (c > 1 ? 4.0f + 0.3f * (float)c : 3.0f));
+      if (c == 1 || t < best) { best = t; cluster = c; }
+    }
     grid = (int)tiles * cluster;
   }
   launch_clusters(k_ffn_product<PAIR, EPI, BF>, grid, FF_THREADS, cluster, SMEM, s, a);
   return launch_status();
 }
+// The products of a that take pairs in one launch, the others in one each
 template <int EPI>
-static int ff_run(ff_args& a, int type, cudaStream_t s) {
-  if (ff_pairs(a, EPI)) return type == PYLO_BF16 ? ff_go<true, EPI, true>(a, s) : ff_go<true, EPI, false>(a, s);
-  return type == PYLO_BF16 ? ff_go<false, EPI, true>(a, s) : ff_go<false, EPI, false>(a, s);
+static int ff_run(const ff_args& all, int type, cudaStream_t s) {
+  ff_args a = all;
+  a.n = 0;
+  for (int k = 0; k < all.n; ++k)
+    if (ff_pairs(all.p[k], EPI)) a.p[a.n++] = all.p[k];
+  if (a.n)
+    if (int rc = type == PYLO_BF16 ? ff_go<true, EPI, true>(a, s) : ff_go<true, EPI, false>(a, s)) return rc;
+  for (int k = 0; k < all.n; ++k)
+    if (!ff_pairs(all.p[k], EPI)) {
+      a.n = 1;
+      a.p[0] = all.p[k];
+      if (int rc = type == PYLO_BF16 ? ff_go<false, EPI, true>(a, s) : ff_go<false, EPI, false>(a, s)) return rc;
+    }
+  return 0;
 }
 static bool ff_operand(const void* p, int64_t ld, int64_t cols) { return p && ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld >= cols; }
 static bool ff_good(const pylo_ffn* f) {
