@@ -27,28 +27,67 @@ constexpr int RW_VEC = 16 / (int)sizeof(T);   // elements of 16 bytes
 // N neighbouring elements: 16 bytes, or one element
 template <class T, int N>
 struct RwPiece {
-  static_assert(N * sizeof(T) == 16 || N == 1, "16 bytes or one element");
-  struct alignas(N * sizeof(T)) Raw { T v[N]; };
-  Raw raw;
+  static_assert(N * sizeof(T) == 16, "16 bytes or one element");
+  uint32_t w[4];   // two 16-bit elements in each, or one of 32
   __device__ __forceinline__ void load(const T* p) {   // read once: not kept in the L1 cache
-    if constexpr (N == 1) raw.v[0] = *p;   // (__ldg of 16-bit types is assembly that the compiler may move out of a branch, to where p is not valid)
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+  }
+  __device__ __forceinline__ void store(T* p) const { __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3])); }
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (std::is_same_v<T, float>) return __uint_as_float(w[j]);
+    else if constexpr (std::is_same_v<T, __half>) {
+      const __half2 h = *reinterpret_cast<const __half2*>(&w[j >> 1]);
+      return j & 1 ? __high2float(h) : __low2float(h);
+    } else return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+  }
+  __device__ __forceinline__ T one(int j) const {
+    if constexpr (std::is_same_v<T, float>) return __uint_as_float(w[j]);
     else {
-      uint4 u;
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
-      raw = *reinterpret_cast<Raw*>(&u);
+      const uint16_t h = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+      return *reinterpret_cast<const T*>(&h);
     }
   }
-  __device__ __forceinline__ void zero() {
+  template <class F>
+  __device__ __forceinline__ void make(F&& f) {   // element j from f(j), rounded
 #pragma unroll
-    for (int j = 0; j < N; ++j) raw.v[j] = rw_to<T>(0.f);
-  }
-  __device__ __forceinline__ float at(int j) const { return rw_float(raw.v[j]); }
-  __device__ __forceinline__ void set(int j, float x) { raw.v[j] = rw_to<T>(x); }
-  __device__ __forceinline__ void store(T* p) const {
-    if constexpr (N == 1) *p = raw.v[0];
-    else __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&raw));
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, float>) w[i] = __float_as_uint(f(i));
+      else if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(f(2 * i), f(2 * i + 1));
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f(2 * i), f(2 * i + 1));
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
   }
 };
+template <class T>
+struct RwPiece<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }   // (__ldg of 16-bit types is assembly that the compiler may move out of a branch, to where p is not valid)
+  __device__ __forceinline__ void store(T* p) const { *p = v; }
+  __device__ __forceinline__ float at(int) const { return rw_float(v); }
+  template <class F>
+  __device__ __forceinline__ void make(F&& f) { v = rw_to<T>(f(0)); }
+};
+
+// the largest of some pieces' elements that are numbers
+template <class T, int N, int U>
+__device__ __forceinline__ float rw_most(const RwPiece<T, N> (&v)[U]) {
+  if constexpr (std::is_same_v<T, float>) {
+    float most = v[0].at(0);
+#pragma unroll
+    for (int j = 1; j < N * U; ++j) most = fmaxf(most, v[j / N].at(j % N));
+    return most;
+  } else {   // two at a time
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    T2 most = *reinterpret_cast<const T2*>(&v[0].w[0]);
+#pragma unroll
+    for (int j = 1; j < 4 * U; ++j) most = __hmax2(most, *reinterpret_cast<const T2*>(&v[j / 4].w[j % 4]));
+    return fmaxf(rw_float(most.x), rw_float(most.y));
+  }
+}
 
 __device__ __forceinline__ float rw_warp_sum(float v) {   // in every lane, in an order of its own
 #pragma unroll
@@ -73,18 +112,6 @@ __device__ __forceinline__ float rw_sum(float v, float* buf) {
   }
   return v;
 }
-template <bool BLOCK>
-__device__ __forceinline__ float rw_max(float v, float* buf) {
-  v = rw_warp_max(v);
-  if constexpr (BLOCK) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (lane == 0) buf[warp] = v;
-    __syncthreads();
-    v = rw_warp_max(lane < (int)(blockDim.x >> 5) ? buf[lane] : -CUDART_INF_F);
-  }
-  return v;
-}
-
 // ------------------------------------------------------------------------------------------------
 // Layer norm.  m = mean x, r = 1 / sqrt(mean (x - m)^2 + eps), xh = (x - m) r:
 //   y = xh w + b;   dx = r (q - mean q - xh mean(q xh)) with q = dy w;   dw = sum over rows dy xh, db = sum over rows dy
@@ -125,7 +152,7 @@ __global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS) k_layer_norm(co
     for (int i = 0; i < NV; ++i) {
       const int c = (t + i * threads) * VN;
       if (c < width && r < a.rows) v[i].load(x + r * a.x_stride + c);
-      else v[i].zero();
+      else v[i].make([](int) { return 0.f; });
     }
   };
   fetch(row);
@@ -155,13 +182,12 @@ __global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS) k_layer_norm(co
       const int c = (t + i * threads) * VN;
       if (c < width) {
         RwPiece<T, VN> o;
-#pragma unroll
-        for (int j = 0; j < VN; ++j) {
+        o.make([&](int j) {
           float q = f[i * VN + j] * rstd;
           if (a.weight) q *= rw_float(((const W*)a.weight)[c + j]);
           if (a.bias) q += rw_float(((const W*)a.bias)[c + j]);
-          o.set(j, q);
-        }
+          return q;
+        });
         o.store(out + c);
       }
     }
@@ -190,7 +216,7 @@ __global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS) k_layer_norm_ba
     for (int i = 0; i < NV; ++i) {
       const int c = (t + i * threads) * VN;
       if (c < width) { vx[i].load(x + c); vd[i].load(dy + c); }
-      else { vx[i].zero(); vd[i].zero(); }
+      else { vx[i].make([](int) { return 0.f; }); vd[i].make([](int) { return 0.f; }); }
     }
     const float mean = a.mean[row], rstd = a.rstd[row];
     float q[E], s1 = 0.f, s2 = 0.f;
@@ -218,8 +244,7 @@ __global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS) k_layer_norm_ba
       const int c = (t + i * threads) * VN;
       if (c < width) {
         RwPiece<T, VN> o;
-#pragma unroll
-        for (int j = 0; j < VN; ++j) o.set(j, rstd * (q[i * VN + j] - s1 - (vx[i].at(j) - mean) * rstd * s2));
+        o.make([&](int j) { return rstd * (q[i * VN + j] - s1 - (vx[i].at(j) - mean) * rstd * s2); });
         o.store(out + c);
       }
     }
@@ -321,7 +346,7 @@ static bool rw_type(int type) { return type == PYLO_FP32 || type == PYLO_BF16 ||
 // An id outside of [0, V) is padding, whatever the teacher's logit beside it is; a row whose entries are all padding or -inf has no
 // teacher and the weight zero.  Rows of weight zero are not read, whatever they hold: their loss and gradient are zero.
 //
-// One pass over a row with a running maximum and sum per thread; exponents to base 2 of values that are scaled by log2(e) / T.  The
+// One pass over a row with a running maximum and sum per thread; powers of two of values that are scaled by log2(e) / T.  The
 // gradient reads the row again (in the call that makes both, out of the L2 cache: the rows that are being worked on fit it).  The K
 // columns with a teacher's entry are written a second time, behind a barrier, with what their entries add up to.
 // ------------------------------------------------------------------------------------------------
@@ -356,42 +381,104 @@ __device__ __forceinline__ int dt_id(const DtArgs& a, long long i) {
   return id >= 0 && id < a.vocab ? (int)id : -1;
 }
 
-template <class T, bool BLOCK, int DO>
-__global__ void __launch_bounds__(BLOCK ? 512 : DT_WARP_THREADS) k_distill(const DtArgs a) {
+// 2^x; what is below 2^-126 is 0
+__device__ __forceinline__ float dt_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// What the gradient of every row is multiplied by
+__device__ __forceinline__ float dt_factor(const DtArgs& a) {
+  float factor = a.scale * a.temperature;
+  if (a.weight_sums) {   // in the same order in every CTA
+    double w = 0.0;
+    for (int i = 0; i < a.n_sums; ++i) w += a.weight_sums[i];
+    factor = w != 0.0 ? (float)(factor / w) : 0.f;
+  } else if (a.inv) factor *= *a.inv;
+  if (a.upstream && !a.per_row) factor *= *a.upstream;
+  return factor;
+}
+// A teacher's K entries by a warp: ids (-1 for padding), probabilities and their logarithms to base 2; whether there are any
+__device__ __forceinline__ bool dt_teacher(const DtArgs& a, long long row, int* id, float* p, float* lp) {
+  const int lane = threadIdx.x & 31, K = a.top;
+  float most = -CUDART_INF_F, sum = 0.f;
+  bool any = false;
+  for (int k = lane; k < K; k += 32) {
+    id[k] = dt_id(a, row * K + k);
+    const float z = id[k] >= 0 ? dt_any(a.teacher, a.teacher_type, row * K + k) * a.c : -CUDART_INF_F;
+    lp[k] = z;
+    most = fmaxf(most, z);
+    any |= !(z == -CUDART_INF_F);
+  }
+  any = __any_sync(0xffffffffu, any);
+  if (!any) return false;
+  most = rw_warp_max(most);
+  for (int k = lane; k < K; k += 32) sum += dt_exp2(lp[k] - most);
+  const float log_sum = log2f(rw_warp_sum(sum));
+  for (int k = lane; k < K; k += 32) {
+    lp[k] = lp[k] - most - log_sum;
+    p[k] = dt_exp2(lp[k]);
+  }
+  __syncwarp();
+  return true;
+}
+// The loss of a row to base 2, without the student's sum: sum of p (log p - s), by a warp
+template <class T>
+__device__ __forceinline__ float dt_cross(const DtArgs& a, const T* s, const int* id, const float* p, const float* lp, float m) {
+  float sum = 0.f;
+  for (int k = threadIdx.x & 31; k < a.top; k += 32)
+    if (!(p[k] == 0.f)) sum = fmaf(p[k], lp[k] - fmaf(rw_float(s[id[k] < 0 ? 0 : id[k]]), a.c, -m), sum);   // (p > 0 has an id)
+  return rw_warp_sum(sum);
+}
+// The columns of the teacher's entries, once more; a class that several entries name takes them all, in their order
+template <class T>
+__device__ __forceinline__ void dt_columns(const DtArgs& a, const T* s, T* grad, const int* id, const float* p, float f, float total, float m, int t, int threads) {
+  for (int k = t; k < a.top; k += threads) {
+    const int at = id[k];
+    if (at < 0) continue;
+    const float v = rw_float(s[at]);
+    float sum = 0.f;
+    bool first = true;   // of the entries with this id
+    for (int j = 0; j < a.top; ++j)
+      if (id[j] == at) {
+        first &= j >= k;
+        sum += p[j];
+      }
+    if (first) grad[at] = rw_to<T>(f * (total * dt_exp2(fmaf(v, a.c, -m)) - sum));
+  }
+}
+
+// Where a row's 16-byte pieces lie, and the element before or behind them that is thread t's
+template <class T>
+struct DtRow {
+  const T* s;
+  int head, pieces, edge;   // edge: -1 for none
+  __device__ __forceinline__ DtRow(const T* s_, int V, int t) : s(s_) {
+    constexpr int VN = RW_VEC<T>;
+    head = min(V, (int)((16 - ((uintptr_t)s & 15)) & 15) / (int)sizeof(T));
+    pieces = (V - head) / VN;
+    const int tail = head + pieces * VN;
+    edge = t < head ? t : tail + t - head < V ? tail + t - head : -1;
+    static_assert(2 * (VN - 1) <= 32, "a thread per element outside of the pieces");
+  }
+};
+
+// Short rows: a warp each.
+template <class T, int DO>
+__global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs a) {
   pdl_begin();
   extern __shared__ __align__(16) unsigned char dt_raw[];
-  __shared__ float s_buf[6][32];
-  constexpr int VN = RW_VEC<T>;
-  const int t = BLOCK ? threadIdx.x : threadIdx.x & 31, threads = BLOCK ? blockDim.x : 32;
-  const int group = BLOCK ? 0 : threadIdx.x >> 5, groups = BLOCK ? 1 : DT_WARP_THREADS / 32, K = a.top, V = a.vocab;
-  int* const s_id = (int*)dt_raw + (size_t)group * 2 * K;
-  float* const s_p = (float*)(s_id + K);
-  auto sync = [] { if constexpr (BLOCK) __syncthreads(); else __syncwarp(); };
-  float factor = a.scale * a.temperature;
-  if constexpr (DO & DT_GRAD) {
-    if (a.weight_sums) {   // in the same order in every CTA
-      double w = 0.0;
-      for (int i = 0; i < a.n_sums; ++i) w += a.weight_sums[i];
-      factor = w != 0.0 ? (float)(factor / w) : 0.f;
-    } else if (a.inv) factor *= *a.inv;
-    if (a.upstream && !a.per_row) factor *= *a.upstream;
-  }
+  __shared__ double s_sums[2][DT_WARP_THREADS / 32];
+  constexpr int VN = RW_VEC<T>, GROUPS = DT_WARP_THREADS / 32;
+  const int t = threadIdx.x & 31, group = threadIdx.x >> 5, V = a.vocab;
+  int* const id = (int*)dt_raw + (size_t)group * 3 * a.top;
+  float* const p = (float*)(id + a.top);
+  float* const lp = p + a.top;
+  const float factor = DO & DT_GRAD ? dt_factor(a) : 0.f;
   double loss_sum = 0.0, weight_sum = 0.0;
-  for (long long row = (long long)blockIdx.x * groups + group; row < a.rows; row += (long long)gridDim.x * groups) {
-    // ---------------------------------------------------------------- the teacher
+  for (long long row = (long long)blockIdx.x * GROUPS + group; row < a.rows; row += (long long)gridDim.x * GROUPS) {
     const float weight = a.weights ? a.weights[row] : 1.0f;
-    float zmax = -CUDART_INF_F;
-    bool any = false;
-    if (weight != 0.f)
-      for (int k = t; k < K; k += threads) {
-        const int id = dt_id(a, row * K + k);
-        const float z = id >= 0 ? dt_any(a.teacher, a.teacher_type, row * K + k) * a.c : -CUDART_INF_F;
-        s_id[k] = id;
-        s_p[k] = z;
-        zmax = fmaxf(zmax, z);
-        any |= !(z == -CUDART_INF_F);
-      }
-    if constexpr (BLOCK) any = __syncthreads_or(any); else any = __any_sync(0xffffffffu, any);
+    const bool any = weight != 0.f && dt_teacher(a, row, id, p, lp);
     T* const grad = DO & DT_GRAD ? (T*)a.grad + row * V : nullptr;
     if (!any) {
       if constexpr (DO & DT_LOSS) {
@@ -399,75 +486,44 @@ __global__ void __launch_bounds__(BLOCK ? 512 : DT_WARP_THREADS) k_distill(const
         if (t == 0 && a.stat) a.stat[row] = make_float2(0.f, 0.f);
       }
       if constexpr (DO & DT_GRAD)
-        for (int j = t; j < V; j += threads) grad[j] = rw_to<T>(0.f);
+        for (int j = t; j < V; j += 32) grad[j] = rw_to<T>(0.f);
       continue;
     }
-    zmax = rw_max<BLOCK>(zmax, s_buf[0]);
-    float zsum = 0.f;
-    for (int k = t; k < K; k += threads) zsum += exp2f(s_p[k] - zmax);
-    zsum = rw_sum<BLOCK>(zsum, s_buf[1]);
-    const float zlog = log2f(zsum);
-
-    // ---------------------------------------------------------------- the student: 16 bytes at a time between the row's first and last boundary
-    const T* const s = (const T*)a.logits + row * a.stride;
-    const int head = min(V, (int)((16 - ((uintptr_t)s & 15)) & 15) / (int)sizeof(T)), pieces = (V - head) / VN, tail = head + pieces * VN;
-    const int edge = t < head ? t : tail + t - head;   // an element before the first boundary or behind the last
-    const bool has_edge = edge < V && (t < head || t - head < V - tail);
-    static_assert(2 * (VN - 1) <= 32, "a thread per element outside of the pieces");
+    const DtRow<T> r((const T*)a.logits + row * a.stride, V, t);
+    const T* const body = r.s + r.head;
     float m = -CUDART_INF_F, total = 0.f;   // scaled maximum; sum of powers relative to it
     if constexpr (DO & DT_LOSS) {
-      constexpr int U = 4;
       auto add = [&](const float (&v)[VN]) {
-        float mx = v[0];
+        float most = v[0];
 #pragma unroll
-        for (int j = 1; j < VN; ++j) mx = fmaxf(mx, v[j]);
-        const float up = fmaxf(m, mx * a.c), ref = up == -CUDART_INF_F ? 0.f : up;
+        for (int j = 1; j < VN; ++j) most = fmaxf(most, v[j]);
+        const float up = fmaxf(m, most * a.c), ref = up == -CUDART_INF_F ? 0.f : up;
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < VN; ++j) sum += exp2f(fmaf(v[j], a.c, -ref));
-        total = fmaf(total, exp2f(m - ref), sum);
+        for (int j = 0; j < VN; ++j) sum += dt_exp2(fmaf(v[j], a.c, -ref));
+        total = fmaf(total, dt_exp2(m - ref), sum);
         m = up;
       };
-      const T* const body = s + head;
-      int i = t;
-      for (; i + (U - 1) * threads < pieces; i += U * threads) {
-        RwPiece<T, VN> v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u].load(body + (long long)(i + u * threads) * VN);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float f[VN];
-#pragma unroll
-          for (int j = 0; j < VN; ++j) f[j] = v[u].at(j);
-          add(f);
-        }
-      }
-      for (; i < pieces; i += threads) {
+      float f[VN];
+      for (int i = t; i < r.pieces; i += 32) {
         RwPiece<T, VN> v;
         v.load(body + (long long)i * VN);
-        float f[VN];
 #pragma unroll
         for (int j = 0; j < VN; ++j) f[j] = v.at(j);
         add(f);
       }
-      if (has_edge) {
-        float f[VN];
-        f[0] = rw_float(s[edge]);
+      if (r.edge >= 0) {
+        f[0] = rw_float(r.s[r.edge]);
 #pragma unroll
         for (int j = 1; j < VN; ++j) f[j] = -CUDART_INF_F;
         add(f);
       }
-      const float all = rw_max<BLOCK>(m, s_buf[2]), ref = all == -CUDART_INF_F ? 0.f : all;
-      total = rw_sum<BLOCK>(total * exp2f(m - ref), s_buf[3]);
+      const float all = rw_warp_max(m), ref = all == -CUDART_INF_F ? 0.f : all;
+      total = rw_warp_sum(total * dt_exp2(m - ref));
       m = ref;
-      float sum = 0.f;
-      for (int k = t; k < K; k += threads) {
-        const float lp = s_p[k] - zmax - zlog, p = exp2f(lp);
-        if (!(p == 0.f)) sum = fmaf(p, lp - fmaf(rw_float(s[s_id[k] < 0 ? 0 : s_id[k]]), a.c, -m), sum);   // (p > 0 has an id)
-      }
-      sum = rw_sum<BLOCK>(sum, s_buf[4]);
+      const float cross = dt_cross(a, r.s, id, p, lp, m);
       if (t == 0) {
-        const float loss = weight * a.temperature * a.temperature * DT_LN2 * (sum + log2f(total));
+        const float loss = weight * a.temperature * a.temperature * DT_LN2 * (cross + log2f(total));
         if (a.row_loss) a.row_loss[row] = loss;
         if (a.stat) a.stat[row] = make_float2(m, 1.0f / total);
         loss_sum += loss;
@@ -478,62 +534,183 @@ __global__ void __launch_bounds__(BLOCK ? 512 : DT_WARP_THREADS) k_distill(const
       const float2 st = a.stat[row];
       m = st.x;
       total = st.y;
-      sync();   // the teacher's entries are there
     }
-
-    // ---------------------------------------------------------------- the gradient
     if constexpr (DO & DT_GRAD) {
       const float f = factor * weight * (a.upstream && a.per_row ? a.upstream[row] : 1.0f), g = f * total;
-      T* const out = grad + head;
-      const T* const body = s + head;
-      const bool aligned = ((uintptr_t)out & 15) == 0;
-      auto one = [&](float v) { return g * exp2f(fmaf(v, a.c, -m)); };
-      constexpr int U = 4;
-      for (int i = t; i < pieces; i += U * threads) {
-        RwPiece<T, VN> v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (i + u * threads < pieces) v[u].load(body + (long long)(i + u * threads) * VN);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (i + u * threads < pieces) {
-            RwPiece<T, VN> o;
-#pragma unroll
-            for (int j = 0; j < VN; ++j) o.set(j, one(v[u].at(j)));
-            T* const to = out + (long long)(i + u * threads) * VN;
-            if (aligned) o.store(to);
-            else
-#pragma unroll
-              for (int j = 0; j < VN; ++j) to[j] = o.raw.v[j];
-          }
-      }
-      if (has_edge) grad[edge] = rw_to<T>(one(rw_float(s[edge])));
-      sync();   // behind it, the columns of the teacher's entries are written again
-      for (int k = t; k < K; k += threads) {
-        const int id = s_id[k];
-        if (id < 0) continue;
-        float p = 0.f;
-        bool first = true;   // of the entries with this id
-        for (int j = 0; j < K; ++j)
-          if (s_id[j] == id) {
-            first &= j >= k;
-            p += exp2f(s_p[j] - zmax - zlog);
-          }
-        if (first) grad[id] = rw_to<T>(fmaf(-f, p, one(rw_float(s[id]))));
-      }
+      for (int i = t; i < V; i += 32) grad[i] = rw_to<T>(g * dt_exp2(fmaf(rw_float(r.s[i]), a.c, -m)));
+      __syncwarp();   // behind it, the columns of the teacher's entries are written again
+      dt_columns(a, r.s, grad, id, p, f, total, m, t, 32);
     }
-    sync();   // the next row's teacher takes the place of this one's
+    __syncwarp();   // the next row's teacher takes the place of this one's
   }
   if constexpr (DO & DT_LOSS) {
-    __shared__ double s_sums[2][DT_WARP_THREADS / 32];
     if (t == 0) { s_sums[0][group] = loss_sum; s_sums[1][group] = weight_sum; }
     __syncthreads();
     if (threadIdx.x == 0) {
-      double2 p = make_double2(0.0, 0.0);
-      for (int g = 0; g < groups; ++g) { p.x += s_sums[0][g]; p.y += s_sums[1][g]; }
-      a.part[blockIdx.x] = p;
+      double2 sums = make_double2(0.0, 0.0);
+      for (int g = 0; g < GROUPS; ++g) { sums.x += s_sums[0][g]; sums.y += s_sums[1][g]; }
+      a.part[blockIdx.x] = sums;
     }
   }
+}
+
+// Long rows: a CTA each.  Eight warps stream through the logits, each thread with four pieces of 16 bytes on their way while it works on four
+// others, the next row's first ones behind this row's last; a ninth warp has the teacher's entries and the row's loss, so that nothing of the stream
+// waits for them.  One barrier per row and pass: what the warps leave for one another lies in two buffers that take turns.
+#define DL_STREAM 256
+#define DL_THREADS (DL_STREAM + 32)
+#define DL_CTAS 4   // of an SM
+#define DL_U 4
+template <class T, int DO>
+__global__ void __launch_bounds__(DL_THREADS, DL_CTAS) k_distill_long(const DtArgs a) {
+  pdl_begin();
+  extern __shared__ __align__(16) unsigned char dt_raw[];
+  __shared__ float2 s_part[2][DL_STREAM / 32];
+  __shared__ int s_any[2];
+  constexpr int VN = RW_VEC<T>, U = DL_U, SPAN = U * DL_STREAM;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, K = a.top, V = a.vocab;
+  const bool streams = warp < DL_STREAM / 32;
+  const float c = a.c, factor = DO & DT_GRAD ? dt_factor(a) : 0.f;
+  double loss_sum = 0.0, weight_sum = 0.0;
+  RwPiece<T, VN> next[U];
+  const T* const logits = (const T*)a.logits;
+  // pieces i, i + DL_STREAM, ... of a row; beyond its last -inf, which adds nothing
+  auto fetch = [&](const T* body, int pieces, int i) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u * DL_STREAM < pieces) next[u].load(body + (long long)(i + u * DL_STREAM) * VN);
+      else next[u].make([](int) { return -CUDART_INF_F; });
+    }
+  };
+  auto place = [&](long long row) { return DtRow<T>(logits + (row < a.rows ? row : 0) * a.stride, streams && row < a.rows ? V : 0, t); };
+  auto outside = [&](const DtRow<T>& r) { return streams && r.edge >= 0 ? rw_float(r.s[r.edge]) : -CUDART_INF_F; };
+  DtRow<T> coming = place(blockIdx.x);
+  fetch(coming.s + coming.head, coming.pieces, t);
+  float weight = a.weights && blockIdx.x < a.rows ? a.weights[blockIdx.x] : 1.0f, edge = outside(coming);
+  int buf = 0;
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const long long row1 = row + gridDim.x;
+    const DtRow<T> r = coming;
+    const float w = weight, mine = edge;
+    coming = place(row1);
+    edge = outside(coming);
+    if (a.weights && row1 < a.rows) weight = a.weights[row1];
+    const T* const body = r.s + r.head;
+    T* const grad = DO & DT_GRAD ? (T*)a.grad + row * V : nullptr;
+    float2 st = make_float2(0.f, 0.f);
+    if constexpr (!(DO & DT_LOSS)) st = a.stat[row];
+    auto zeros = [&] {
+      if (streams)
+        for (int j = t; j < V; j += DL_STREAM) grad[j] = rw_to<T>(0.f);
+    };
+    if (w == 0.f || (!(DO & DT_LOSS) && st.y == 0.f)) {   // (a row without a teacher has left 0 there)
+      if constexpr (DO & DT_LOSS) {
+        if (t == 0 && a.row_loss) a.row_loss[row] = 0.f;
+        if (t == 0 && a.stat) a.stat[row] = make_float2(0.f, 0.f);
+      }
+      if constexpr (DO & DT_GRAD) zeros();
+      fetch(coming.s + coming.head, coming.pieces, t);
+      continue;
+    }
+    int* const id = (int*)dt_raw + (size_t)buf * 3 * K;
+    float* const p = (float*)(id + K);
+    float* const lp = p + K;
+    const float f = DO & DT_GRAD ? factor * w * (a.upstream && a.per_row ? a.upstream[row] : 1.0f) : 0.f;
+    // a row's pieces, from those that have been fetched on; behind the last, those of what comes next are
+    auto sweep = [&](const T* then, int then_pieces, auto&& work) {
+      int i = t;
+      do {
+        RwPiece<T, VN> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = next[u];
+        const bool last = i + SPAN >= r.pieces;
+        fetch(last ? then : body, last ? then_pieces : r.pieces, last ? t : i + SPAN);
+        work(v, i);
+      } while ((i += SPAN) < r.pieces);
+    };
+    // this thread's part of the gradient, from powers relative to m
+    auto gradient = [&](float m, float total) {
+      const float g = f * total;
+      T* const out = grad + r.head;
+      const bool aligned = ((uintptr_t)out & 15) == 0;
+      sweep(coming.s + coming.head, coming.pieces, [&](const RwPiece<T, VN> (&v)[U], int i) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (i + u * DL_STREAM < r.pieces) {
+            RwPiece<T, VN> o;
+            o.make([&](int j) { return g * dt_exp2(fmaf(v[u].at(j), c, -m)); });
+            T* const to = out + (long long)(i + u * DL_STREAM) * VN;
+            if (aligned) o.store(to);
+            else
+#pragma unroll
+              for (int j = 0; j < VN; ++j) to[j] = o.one(j);
+          }
+      });
+      if (r.edge >= 0) grad[r.edge] = rw_to<T>(g * dt_exp2(fmaf(mine, c, -m)));
+    };
+    if (!streams) {
+      const bool any = dt_teacher(a, row, id, p, lp);
+      if (lane == 0) s_any[buf] = any;
+    } else if constexpr (DO & DT_LOSS) {
+      float m = -CUDART_INF_F, total = 0.f;   // scaled maximum; sum of powers relative to it
+      const bool again = DO & DT_GRAD;
+      sweep(again ? body : coming.s + coming.head, again ? r.pieces : coming.pieces, [&](const RwPiece<T, VN> (&v)[U], int) {
+        const float up = fmaxf(m, rw_most(v) * c), ref = up == -CUDART_INF_F ? 0.f : up;
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < U * VN; ++j) sum[j & 1] += dt_exp2(fmaf(v[j / VN].at(j % VN), c, -ref));
+        total = fmaf(total, dt_exp2(m - ref), sum[0] + sum[1]);
+        m = up;
+      });
+      if (r.edge >= 0) {
+        const float up = fmaxf(m, mine * c), ref = up == -CUDART_INF_F ? 0.f : up;
+        total = fmaf(total, dt_exp2(m - ref), dt_exp2(fmaf(mine, c, -ref)));
+        m = up;
+      }
+      const float all = rw_warp_max(m), ref = all == -CUDART_INF_F ? 0.f : all;
+      total = rw_warp_sum(total * dt_exp2(m - ref));
+      if (lane == 0) s_part[buf][warp] = make_float2(all, total);
+    }
+    if constexpr (!(DO & DT_LOSS))
+      if (streams) gradient(st.x, st.y);
+    __syncthreads();
+    if constexpr (DO & DT_LOSS) {
+      float m = -CUDART_INF_F, total = 0.f;
+#pragma unroll
+      for (int i = 0; i < DL_STREAM / 32; ++i) m = fmaxf(m, s_part[buf][i].x);
+      m = m == -CUDART_INF_F ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < DL_STREAM / 32; ++i) {
+        const float2 q = s_part[buf][i];
+        total += q.y * dt_exp2((q.x == -CUDART_INF_F ? 0.f : q.x) - m);
+      }
+      st = make_float2(m, 1.0f / total);
+      const bool any = s_any[buf];
+      if (!streams) {
+        const float cross = any ? dt_cross(a, r.s, id, p, lp, m) : 0.f;
+        if (lane == 0) {
+          const float loss = any ? w * a.temperature * a.temperature * DT_LN2 * (cross + log2f(total)) : 0.f;
+          if (a.row_loss) a.row_loss[row] = loss;
+          if (a.stat) a.stat[row] = any ? st : make_float2(0.f, 0.f);
+          loss_sum += loss;
+          weight_sum += any ? w : 0.f;
+        }
+      } else if constexpr (DO & DT_GRAD) {
+        if (any) gradient(st.x, st.y);
+        else {
+          zeros();
+          fetch(coming.s + coming.head, coming.pieces, t);
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(DL_STREAM) : "memory");   // the streaming warps
+        if (any) dt_columns(a, r.s, grad, id, p, f, st.y, st.x, t, DL_STREAM);
+      }
+    } else if (streams) {
+      dt_columns(a, r.s, grad, id, p, f, st.y, st.x, t, DL_STREAM);
+    }
+    buf ^= 1;
+  }
+  if constexpr (DO & DT_LOSS)
+    if (t == DL_STREAM) a.part[blockIdx.x] = make_double2(loss_sum, weight_sum);
 }
 
 // The weights that count, before the gradient is scaled by their sum: a row's is zero if it has no teacher.
@@ -574,18 +751,17 @@ __global__ void __launch_bounds__(NT) k_distill_total(const double2* __restrict_
 }
 
 // CTAs of a call, which is also the number of its partial sums
-static int dt_threads(int vocab) { return vocab <= DT_WARP_VOCAB ? DT_WARP_THREADS : vocab <= 8192 ? 256 : 512; }
 static int dt_ctas(long long rows, int vocab) {
-  const int t = dt_threads(vocab), per = vocab <= DT_WARP_VOCAB ? DT_WARP_THREADS / 32 : 1;
-  const long long n = (rows + per - 1) / per, most = (long long)sm_count() * (1024 / t);
+  const bool is_short = vocab <= DT_WARP_VOCAB;
+  const long long n = is_short ? (rows + DT_WARP_THREADS / 32 - 1) / (DT_WARP_THREADS / 32) : rows, most = (long long)sm_count() * (is_short ? 8 : DL_CTAS);
   return (int)(n < most ? n : most);
 }
 static int dt_weight_ctas(long long rows) { return (int)(rows < 64 * NT ? (rows + NT - 1) / NT : 64); }
 template <class T, int DO>
 static int dt_run(const DtArgs& a, cudaStream_t s) {
-  const int t = dt_threads(a.vocab), ctas = dt_ctas(a.rows, a.vocab);
-  if (a.vocab <= DT_WARP_VOCAB) launch(k_distill<T, false, DO>, ctas, t, (size_t)8 * a.top * (DT_WARP_THREADS / 32), s, a);
-  else launch(k_distill<T, true, DO>, ctas, t, (size_t)8 * a.top, s, a);
+  const int ctas = dt_ctas(a.rows, a.vocab);
+  if (a.vocab <= DT_WARP_VOCAB) launch(k_distill_short<T, DO>, ctas, DT_WARP_THREADS, (size_t)12 * a.top * (DT_WARP_THREADS / 32), s, a);
+  else launch(k_distill_long<T, DO>, ctas, DL_THREADS, (size_t)24 * a.top, s, a);
   return launch_status();
 }
 template <int DO>
