@@ -5,6 +5,7 @@
 // the latency of its launches.  A row belongs to a warp where it is short, else to a CTA; the CTAs are as many as run at once and go
 // from row to row.  Everything is computed in fp32 from the elements' own type and rounded once, where it is stored.
 #include <cuda_bf16.h>
+#include <limits.h>
 
 #include "pylo_common.cuh"
 #include "pylo_launch.cuh"
@@ -72,23 +73,28 @@ struct RwPiece<T, 1> {
   __device__ __forceinline__ void make(F&& f) { v = rw_to<T>(f(0)); }
 };
 
-// the largest of some pieces' elements that are numbers
-template <class T, int N, int U>
-__device__ __forceinline__ float rw_most(const RwPiece<T, N> (&v)[U]) {
-  if constexpr (std::is_same_v<T, float>) {
-    float most = v[0].at(0);
-#pragma unroll
-    for (int j = 1; j < N * U; ++j) most = fmaxf(most, v[j / N].at(j % N));
-    return most;
-  } else {   // two at a time
+// the largest of a piece's elements that are numbers
+template <class T, int N>
+__device__ __forceinline__ float rw_most(const RwPiece<T, N>& v) {
+  if constexpr (std::is_same_v<T, float>) return fmaxf(fmaxf(v.at(0), v.at(1)), fmaxf(v.at(2), v.at(3)));
+  else {   // two at a time
     using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
-    T2 most = *reinterpret_cast<const T2*>(&v[0].w[0]);
-#pragma unroll
-    for (int j = 1; j < 4 * U; ++j) most = __hmax2(most, *reinterpret_cast<const T2*>(&v[j / 4].w[j % 4]));
+    const T2* const q = reinterpret_cast<const T2*>(v.w);
+    const T2 most = __hmax2(__hmax2(q[0], q[1]), __hmax2(q[2], q[3]));
     return fmaxf(rw_float(most.x), rw_float(most.y));
   }
 }
 
+__device__ __forceinline__ void rw_cluster_sync() {   // all threads of the cluster's CTAs; orders accesses to all memory
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address of another CTA's copy of a shared variable
+__device__ __forceinline__ uint32_t rw_at_rank(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+  return a;
+}
 __device__ __forceinline__ float rw_warp_sum(float v) {   // in every lane, in an order of its own
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -398,53 +404,80 @@ __device__ __forceinline__ float dt_factor(const DtArgs& a) {
   if (a.upstream && !a.per_row) factor *= *a.upstream;
   return factor;
 }
-// A teacher's K entries by a warp: ids (-1 for padding), probabilities and their logarithms to base 2; whether there are any
-__device__ __forceinline__ bool dt_teacher(const DtArgs& a, long long row, int* id, float* p, float* lp) {
-  const int lane = threadIdx.x & 31, K = a.top;
+// A teacher's entry: its class, the probability and its logarithm to base 2, and what its column takes: of several entries of one class the first
+// takes what all of them add up to, in their order.  id: ~class for those that leave the column alone; padding is DT_PADDING with p = 0.
+#define DT_PADDING INT_MIN
+struct DtEntry { int id; float p, lp, column; };
+static __host__ __device__ __forceinline__ int dt_slots(int top) {   // of the table of classes: a power of two, half full at most
+  int n = 64;
+  while (n < 2 * top) n *= 2;
+  return n;
+}
+// A row's K entries, by a warp; slots: dt_slots(K) words.  False if there are none
+__device__ __forceinline__ bool dt_teacher(const DtArgs& a, long long row, DtEntry* e, int* slots) {
+  const int lane = threadIdx.x & 31, K = a.top, n = dt_slots(K);
   float most = -CUDART_INF_F, sum = 0.f;
   bool any = false;
+  for (int i = lane; i < n; i += 32) slots[i] = -1;
+  __syncwarp();
+  bool twice = false;   // a class that has an entry already
   for (int k = lane; k < K; k += 32) {
-    id[k] = dt_id(a, row * K + k);
-    const float z = id[k] >= 0 ? dt_any(a.teacher, a.teacher_type, row * K + k) * a.c : -CUDART_INF_F;
-    lp[k] = z;
+    const int id = dt_id(a, row * K + k);
+    const float z = id >= 0 ? dt_any(a.teacher, a.teacher_type, row * K + k) * a.c : -CUDART_INF_F;
+    e[k].id = id >= 0 ? id : DT_PADDING;
+    e[k].lp = z;
     most = fmaxf(most, z);
     any |= !(z == -CUDART_INF_F);
+    if (id >= 0)
+      for (unsigned at = (unsigned)id * 2654435761u;; ++at) {   // ends: half of the slots stay free
+        const int found = atomicCAS(&slots[(at ^ at >> 16) & (n - 1)], -1, id);
+        twice |= found == id;
+        if (found == -1 || found == id) break;
+      }
   }
-  any = __any_sync(0xffffffffu, any);
-  if (!any) return false;
+  if (!__any_sync(0xffffffffu, any)) return false;
+  twice = __any_sync(0xffffffffu, twice);
   most = rw_warp_max(most);
-  for (int k = lane; k < K; k += 32) sum += dt_exp2(lp[k] - most);
+  for (int k = lane; k < K; k += 32) sum += dt_exp2(e[k].lp - most);
   const float log_sum = log2f(rw_warp_sum(sum));
   for (int k = lane; k < K; k += 32) {
-    lp[k] = lp[k] - most - log_sum;
-    p[k] = dt_exp2(lp[k]);
+    const float lp = e[k].lp - most - log_sum, p = dt_exp2(lp);
+    e[k].lp = lp;
+    e[k].p = p;
+    e[k].column = p;
   }
   __syncwarp();
+  if (twice) {
+    for (int k = lane; k < K; k += 32) {
+      const int id = e[k].id;
+      float all = 0.f;
+      for (int j = 0; j < K; ++j)
+        if (e[j].id == id || e[j].id == ~id) {   // (the other lanes are at work on them)
+          if (j < k && id >= 0) { e[k].id = ~id; break; }
+          all += e[j].p;
+        }
+      e[k].column = all;
+    }
+    __syncwarp();
+  }
   return true;
 }
 // The loss of a row to base 2, without the student's sum: sum of p (log p - s), by a warp
 template <class T>
-__device__ __forceinline__ float dt_cross(const DtArgs& a, const T* s, const int* id, const float* p, const float* lp, float m) {
+__device__ __forceinline__ float dt_cross(const DtArgs& a, const T* s, const DtEntry* e, float m) {
   float sum = 0.f;
-  for (int k = threadIdx.x & 31; k < a.top; k += 32)
-    if (!(p[k] == 0.f)) sum = fmaf(p[k], lp[k] - fmaf(rw_float(s[id[k] < 0 ? 0 : id[k]]), a.c, -m), sum);   // (p > 0 has an id)
+  for (int k = threadIdx.x & 31; k < a.top; k += 32) {
+    const DtEntry q = e[k];
+    if (!(q.p == 0.f)) sum = fmaf(q.p, q.lp - fmaf(rw_float(s[q.id < 0 ? ~q.id : q.id]), a.c, -m), sum);
+  }
   return rw_warp_sum(sum);
 }
-// The columns of the teacher's entries, once more; a class that several entries name takes them all, in their order
+// The columns of the teacher's entries among lo to hi, once more
 template <class T>
-__device__ __forceinline__ void dt_columns(const DtArgs& a, const T* s, T* grad, const int* id, const float* p, float f, float total, float m, int t, int threads) {
+__device__ __forceinline__ void dt_columns(const DtArgs& a, const T* s, T* grad, const DtEntry* e, float f, float total, float m, int t, int threads, int lo, int hi) {
   for (int k = t; k < a.top; k += threads) {
-    const int at = id[k];
-    if (at < 0) continue;
-    const float v = rw_float(s[at]);
-    float sum = 0.f;
-    bool first = true;   // of the entries with this id
-    for (int j = 0; j < a.top; ++j)
-      if (id[j] == at) {
-        first &= j >= k;
-        sum += p[j];
-      }
-    if (first) grad[at] = rw_to<T>(f * (total * dt_exp2(fmaf(v, a.c, -m)) - sum));
+    const DtEntry q = e[k];
+    if (q.id >= lo && q.id < hi) grad[q.id] = rw_to<T>(f * (total * dt_exp2(fmaf(rw_float(s[q.id]), a.c, -m)) - q.column));
   }
 }
 
@@ -471,14 +504,13 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs 
   __shared__ double s_sums[2][DT_WARP_THREADS / 32];
   constexpr int VN = RW_VEC<T>, GROUPS = DT_WARP_THREADS / 32;
   const int t = threadIdx.x & 31, group = threadIdx.x >> 5, V = a.vocab;
-  int* const id = (int*)dt_raw + (size_t)group * 3 * a.top;
-  float* const p = (float*)(id + a.top);
-  float* const lp = p + a.top;
+  DtEntry* const e = (DtEntry*)dt_raw + group * a.top;
+  int* const slots = (int*)((DtEntry*)dt_raw + GROUPS * a.top) + group * dt_slots(a.top);
   const float factor = DO & DT_GRAD ? dt_factor(a) : 0.f;
   double loss_sum = 0.0, weight_sum = 0.0;
   for (long long row = (long long)blockIdx.x * GROUPS + group; row < a.rows; row += (long long)gridDim.x * GROUPS) {
     const float weight = a.weights ? a.weights[row] : 1.0f;
-    const bool any = weight != 0.f && dt_teacher(a, row, id, p, lp);
+    const bool any = weight != 0.f && dt_teacher(a, row, e, slots);
     T* const grad = DO & DT_GRAD ? (T*)a.grad + row * V : nullptr;
     if (!any) {
       if constexpr (DO & DT_LOSS) {
@@ -521,7 +553,7 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs 
       const float all = rw_warp_max(m), ref = all == -CUDART_INF_F ? 0.f : all;
       total = rw_warp_sum(total * dt_exp2(m - ref));
       m = ref;
-      const float cross = dt_cross(a, r.s, id, p, lp, m);
+      const float cross = dt_cross(a, r.s, e, m);
       if (t == 0) {
         const float loss = weight * a.temperature * a.temperature * DT_LN2 * (cross + log2f(total));
         if (a.row_loss) a.row_loss[row] = loss;
@@ -539,7 +571,7 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs 
       const float f = factor * weight * (a.upstream && a.per_row ? a.upstream[row] : 1.0f), g = f * total;
       for (int i = t; i < V; i += 32) grad[i] = rw_to<T>(g * dt_exp2(fmaf(rw_float(r.s[i]), a.c, -m)));
       __syncwarp();   // behind it, the columns of the teacher's entries are written again
-      dt_columns(a, r.s, grad, id, p, f, total, m, t, 32);
+      dt_columns(a, r.s, grad, e, f, total, m, t, 32, 0, V);
     }
     __syncwarp();   // the next row's teacher takes the place of this one's
   }
@@ -554,163 +586,258 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs 
   }
 }
 
-// Long rows: a CTA each.  Eight warps stream through the logits, each thread with four pieces of 16 bytes on their way while it works on four
-// others, the next row's first ones behind this row's last; a ninth warp has the teacher's entries and the row's loss, so that nothing of the stream
-// waits for them.  One barrier per row and pass: what the warps leave for one another lies in two buffers that take turns.
-#define DL_STREAM 256
-#define DL_THREADS (DL_STREAM + 32)
-#define DL_CTAS 4   // of an SM
+// Long rows: a CTA each, or a cluster's, each CTA with its part of the row.  STREAM threads go through the logits, each with DL_U pieces of
+// 16 bytes on their way, the next row's first ones behind this row's last; one more warp has the teacher's entries and the row's loss, so that
+// nothing of the stream waits for them.  One barrier per row and pass: what the warps leave for one another lies in two buffers that take turns.
+//
+// A cluster shares a row where there are too few rows for all CTAs.
 #define DL_U 4
-template <class T, int DO>
-__global__ void __launch_bounds__(DL_THREADS, DL_CTAS) k_distill_long(const DtArgs a) {
-  pdl_begin();
+#define DL_MOST_SHARE 8
+__host__ __device__ constexpr int dl_ctas(int stream) { return stream == 128 ? 7 : stream == 256 ? 4 : 2; }   // of an SM
+__device__ __forceinline__ uint64_t dt_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void dt_unpair(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t dt_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t dt_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t dt_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+template <class T, int DO, int STREAM>
+__global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(const DtArgs a) {
   extern __shared__ __align__(16) unsigned char dt_raw[];
-  __shared__ float2 s_part[2][DL_STREAM / 32];
+  __shared__ float2 s_part[2][DL_MOST_SHARE * STREAM / 32];
   __shared__ int s_any[2];
-  constexpr int VN = RW_VEC<T>, U = DL_U, SPAN = U * DL_STREAM;
+  constexpr int VN = RW_VEC<T>, U = DL_U, SPAN = U * STREAM, PARTS = STREAM / 32;
+  constexpr float LOWEST = -3.0e38f;   // in the place of a maximum of -inf
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, K = a.top, V = a.vocab;
-  const bool streams = warp < DL_STREAM / 32;
+  const bool streams = warp < STREAM / 32;
+  uint32_t rank, share;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(share));
+  if (DO == DT_LOSS || DO == (DT_LOSS | DT_GRAD))
+    if (share > 1) rw_cluster_sync();   // the others are running
+  pdl_begin();
+  const long long groups = gridDim.x / share;
   const float c = a.c, factor = DO & DT_GRAD ? dt_factor(a) : 0.f;
+  const uint64_t cc = dt_pair(c, c);
   double loss_sum = 0.0, weight_sum = 0.0;
   RwPiece<T, VN> next[U];
-  const T* const logits = (const T*)a.logits;
-  // pieces i, i + DL_STREAM, ... of a row; beyond its last -inf, which adds nothing
+  // A row, and what of it is this CTA's: `pieces` of 16 bytes from body on, elements lo to hi, thread t's element outside of the pieces (or -1)
+  struct Row { const T *s, *body; int at, pieces, lo, hi, edge; };
+  auto place = [&](long long row) {
+    Row r;
+    r.s = (const T*)a.logits + (row < a.rows ? row : 0) * a.stride;
+    const int head = min(V, (int)((16 - ((uintptr_t)r.s & 15)) & 15) / (int)sizeof(T)), all = (V - head) / VN, tail = head + all * VN;
+    const int per = (all + (int)share - 1) / (int)share, p0 = min((int)rank * per, all);
+    r.pieces = row < a.rows && streams ? min(per, all - p0) : 0;
+    r.at = head + p0 * VN;
+    r.body = r.s + r.at;
+    r.lo = rank == 0 ? 0 : r.at;
+    r.hi = rank == share - 1 ? V : min(r.at + per * VN, tail);
+    r.edge = t < head ? t : tail + t - head < V ? tail + t - head : -1;
+    if (!streams || row >= a.rows || r.edge < r.lo || r.edge >= r.hi) r.edge = -1;
+    return r;
+  };
+  static_assert(2 * (VN - 1) <= STREAM, "a thread per element outside of the pieces");
+  // pieces i, i + STREAM, ...; beyond the last -inf, which adds nothing
   auto fetch = [&](const T* body, int pieces, int i) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (i + u * DL_STREAM < pieces) next[u].load(body + (long long)(i + u * DL_STREAM) * VN);
+      if (i + u * STREAM < pieces) next[u].load(body + (long long)(i + u * STREAM) * VN);
       else next[u].make([](int) { return -CUDART_INF_F; });
     }
   };
-  auto place = [&](long long row) { return DtRow<T>(logits + (row < a.rows ? row : 0) * a.stride, streams && row < a.rows ? V : 0, t); };
-  auto outside = [&](const DtRow<T>& r) { return streams && r.edge >= 0 ? rw_float(r.s[r.edge]) : -CUDART_INF_F; };
-  DtRow<T> coming = place(blockIdx.x);
-  fetch(coming.s + coming.head, coming.pieces, t);
-  float weight = a.weights && blockIdx.x < a.rows ? a.weights[blockIdx.x] : 1.0f, edge = outside(coming);
+  Row coming = place(blockIdx.x / share);
+  fetch(coming.body, coming.pieces, t);
+  float weight = a.weights && blockIdx.x / share < a.rows ? a.weights[blockIdx.x / share] : 1.0f;
+  float edge = coming.edge >= 0 ? rw_float(coming.s[coming.edge]) : -CUDART_INF_F;
+  float2 ahead = make_float2(0.f, 0.f);
+  if constexpr (!(DO & DT_LOSS))
+    if (blockIdx.x / share < a.rows) ahead = a.stat[blockIdx.x / share];
   int buf = 0;
-  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const long long row1 = row + gridDim.x;
-    const DtRow<T> r = coming;
+  for (long long row = blockIdx.x / share; row < a.rows; row += groups) {
+    const Row r = coming;
     const float w = weight, mine = edge;
-    coming = place(row1);
-    edge = outside(coming);
-    if (a.weights && row1 < a.rows) weight = a.weights[row1];
-    const T* const body = r.s + r.head;
+    coming = place(row + groups);
+    edge = coming.edge >= 0 ? rw_float(coming.s[coming.edge]) : -CUDART_INF_F;
+    if (a.weights && row + groups < a.rows) weight = a.weights[row + groups];
     T* const grad = DO & DT_GRAD ? (T*)a.grad + row * V : nullptr;
-    float2 st = make_float2(0.f, 0.f);
-    if constexpr (!(DO & DT_LOSS)) st = a.stat[row];
+    float2 st = ahead;
+    if constexpr (!(DO & DT_LOSS))
+      if (row + groups < a.rows) ahead = a.stat[row + groups];
     auto zeros = [&] {
       if (streams)
-        for (int j = t; j < V; j += DL_STREAM) grad[j] = rw_to<T>(0.f);
+        for (int j = r.lo + t; j < r.hi; j += STREAM) grad[j] = rw_to<T>(0.f);
     };
     if (w == 0.f || (!(DO & DT_LOSS) && st.y == 0.f)) {   // (a row without a teacher has left 0 there)
       if constexpr (DO & DT_LOSS) {
-        if (t == 0 && a.row_loss) a.row_loss[row] = 0.f;
-        if (t == 0 && a.stat) a.stat[row] = make_float2(0.f, 0.f);
+        if (t == 0 && rank == 0 && a.row_loss) a.row_loss[row] = 0.f;
+        if (t == 0 && rank == 0 && a.stat) a.stat[row] = make_float2(0.f, 0.f);
       }
       if constexpr (DO & DT_GRAD) zeros();
-      fetch(coming.s + coming.head, coming.pieces, t);
+      fetch(coming.body, coming.pieces, t);
       continue;
     }
-    int* const id = (int*)dt_raw + (size_t)buf * 3 * K;
-    float* const p = (float*)(id + K);
-    float* const lp = p + K;
+    DtEntry* const e = (DtEntry*)dt_raw + buf * K;
     const float f = DO & DT_GRAD ? factor * w * (a.upstream && a.per_row ? a.upstream[row] : 1.0f) : 0.f;
-    // a row's pieces, from those that have been fetched on; behind the last, those of what comes next are
+    // this CTA's pieces, from those that have been fetched on: work(piece, its number); each one's place is taken by the one SPAN further at once,
+    // behind the last ones by those of what comes next
     auto sweep = [&](const T* then, int then_pieces, auto&& work) {
+      const int blocks = (r.pieces + SPAN - 1) / SPAN;
+      const T* ahead = r.body + (long long)(t + SPAN) * VN;
       int i = t;
-      do {
-        RwPiece<T, VN> v[U];
+      for (int k = 2; k < blocks; ++k, i += SPAN, ahead += SPAN * VN)
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = next[u];
-        const bool last = i + SPAN >= r.pieces;
-        fetch(last ? then : body, last ? then_pieces : r.pieces, last ? t : i + SPAN);
-        work(v, i);
-      } while ((i += SPAN) < r.pieces);
+        for (int u = 0; u < U; ++u) {
+          const RwPiece<T, VN> v = next[u];
+          next[u].load(ahead + u * STREAM * VN);
+          work(v, i + u * STREAM);
+        }
+      if (blocks > 1) {   // the last ones may be fewer
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const RwPiece<T, VN> v = next[u];
+          if (i + SPAN + u * STREAM < r.pieces) next[u].load(ahead + u * STREAM * VN);
+          else next[u].make([](int) { return -CUDART_INF_F; });
+          work(v, i + u * STREAM);
+        }
+        i += SPAN;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const RwPiece<T, VN> v = next[u];
+        if (t + u * STREAM < then_pieces) next[u].load(then + (long long)(t + u * STREAM) * VN);
+        else next[u].make([](int) { return -CUDART_INF_F; });
+        if (i + u * STREAM < r.pieces) work(v, i + u * STREAM);
+      }
     };
     // this thread's part of the gradient, from powers relative to m
     auto gradient = [&](float m, float total) {
       const float g = f * total;
-      T* const out = grad + r.head;
-      const bool aligned = ((uintptr_t)out & 15) == 0;
-      sweep(coming.s + coming.head, coming.pieces, [&](const RwPiece<T, VN> (&v)[U], int i) {
+      const uint64_t gg = dt_pair(g, g), mm = dt_pair(-m, -m);
+      T* const out = grad + r.at;
+      auto go = [&](auto aligned) {
+        sweep(coming.body, coming.pieces, [&](const RwPiece<T, VN>& v, int i) {
+          float x[VN];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (i + u * DL_STREAM < r.pieces) {
-            RwPiece<T, VN> o;
-            o.make([&](int j) { return g * dt_exp2(fmaf(v[u].at(j), c, -m)); });
-            T* const to = out + (long long)(i + u * DL_STREAM) * VN;
-            if (aligned) o.store(to);
-            else
-#pragma unroll
-              for (int j = 0; j < VN; ++j) to[j] = o.one(j);
+          for (int j = 0; j < VN; j += 2) {
+            dt_unpair(dt_fma2(dt_pair(v.at(j), v.at(j + 1)), cc, mm), x[j], x[j + 1]);
+            dt_unpair(dt_mul2(gg, dt_pair(dt_exp2(x[j]), dt_exp2(x[j + 1]))), x[j], x[j + 1]);
           }
-      });
+          RwPiece<T, VN> o;
+          o.make([&](int j) { return x[j]; });
+          T* const to = out + (long long)i * VN;
+          if constexpr (decltype(aligned)::value) o.store(to);
+          else
+#pragma unroll
+            for (int j = 0; j < VN; ++j) to[j] = o.one(j);
+        });
+      };
+      if (((uintptr_t)out & 15) == 0) go(std::true_type());
+      else go(std::false_type());
       if (r.edge >= 0) grad[r.edge] = rw_to<T>(g * dt_exp2(fmaf(mine, c, -m)));
     };
     if (!streams) {
-      const bool any = dt_teacher(a, row, id, p, lp);
+      const bool any = dt_teacher(a, row, e, (int*)((DtEntry*)dt_raw + 2 * K));
       if (lane == 0) s_any[buf] = any;
     } else if constexpr (DO & DT_LOSS) {
-      float m = -CUDART_INF_F, total = 0.f;   // scaled maximum; sum of powers relative to it
+      float m = LOWEST, total = 0.f;   // scaled maximum; sum of powers relative to it
+      uint64_t mm = dt_pair(-m, -m), sum = dt_pair(0.f, 0.f);
+      auto raise = [&](float to) {
+        const float by = dt_exp2(m - to);
+        sum = dt_mul2(sum, dt_pair(by, by));
+        m = to;
+        mm = dt_pair(-m, -m);
+      };
       const bool again = DO & DT_GRAD;
-      sweep(again ? body : coming.s + coming.head, again ? r.pieces : coming.pieces, [&](const RwPiece<T, VN> (&v)[U], int) {
-        const float up = fmaxf(m, rw_most(v) * c), ref = up == -CUDART_INF_F ? 0.f : up;
-        float sum[2] = {0.f, 0.f};
+      sweep(again ? r.body : coming.body, again ? r.pieces : coming.pieces, [&](const RwPiece<T, VN>& v, int) {
+        const float most = rw_most(v) * c;
+        if (most > m) raise(most);
 #pragma unroll
-        for (int j = 0; j < U * VN; ++j) sum[j & 1] += dt_exp2(fmaf(v[j / VN].at(j % VN), c, -ref));
-        total = fmaf(total, dt_exp2(m - ref), sum[0] + sum[1]);
-        m = up;
+        for (int j = 0; j < VN; j += 2) {
+          float x, y;
+          dt_unpair(dt_fma2(dt_pair(v.at(j), v.at(j + 1)), cc, mm), x, y);
+          sum = dt_add2(sum, dt_pair(dt_exp2(x), dt_exp2(y)));
+        }
       });
       if (r.edge >= 0) {
-        const float up = fmaxf(m, mine * c), ref = up == -CUDART_INF_F ? 0.f : up;
-        total = fmaf(total, dt_exp2(m - ref), dt_exp2(fmaf(mine, c, -ref)));
-        m = up;
+        if (mine * c > m) raise(mine * c);
+        sum = dt_add2(sum, dt_pair(dt_exp2(fmaf(mine, c, -m)), 0.f));
       }
-      const float all = rw_warp_max(m), ref = all == -CUDART_INF_F ? 0.f : all;
-      total = rw_warp_sum(total * dt_exp2(m - ref));
-      if (lane == 0) s_part[buf][warp] = make_float2(all, total);
+      float other;
+      dt_unpair(sum, total, other);
+      total += other;
+      const float all = rw_warp_max(m);
+      total = rw_warp_sum(total * dt_exp2(m - all));
+      if (lane < (int)share) {
+        const uint32_t to = rw_at_rank(&s_part[buf][rank * PARTS + warp], lane);
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(all), "f"(total) : "memory");
+      }
     }
     if constexpr (!(DO & DT_LOSS))
       if (streams) gradient(st.x, st.y);
-    __syncthreads();
+    if ((DO & DT_LOSS) && share > 1) rw_cluster_sync();
+    else __syncthreads();
+    if constexpr (DO == DT_LOSS)
+      if (streams) { buf ^= 1; continue; }
     if constexpr (DO & DT_LOSS) {
-      float m = -CUDART_INF_F, total = 0.f;
+      const int parts = (int)share * PARTS;
+      constexpr int EACH = DL_MOST_SHARE * PARTS / 32;   // of a lane
+      float2 x[EACH];
+      float m = LOWEST, total = 0.f;
 #pragma unroll
-      for (int i = 0; i < DL_STREAM / 32; ++i) m = fmaxf(m, s_part[buf][i].x);
-      m = m == -CUDART_INF_F ? 0.f : m;
-#pragma unroll
-      for (int i = 0; i < DL_STREAM / 32; ++i) {
-        const float2 q = s_part[buf][i];
-        total += q.y * dt_exp2((q.x == -CUDART_INF_F ? 0.f : q.x) - m);
+      for (int i = 0; i < EACH; ++i) {
+        x[i] = lane + 32 * i < parts ? s_part[buf][lane + 32 * i] : make_float2(LOWEST, 0.f);
+        m = fmaxf(m, x[i].x);
       }
+      m = rw_warp_max(m);
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) total += x[i].y * dt_exp2(x[i].x - m);
+      total = rw_warp_sum(total);
+      m = m == LOWEST ? 0.f : m;   // (then all are -inf, and total is 0)
       st = make_float2(m, 1.0f / total);
       const bool any = s_any[buf];
       if (!streams) {
-        const float cross = any ? dt_cross(a, r.s, id, p, lp, m) : 0.f;
-        if (lane == 0) {
-          const float loss = any ? w * a.temperature * a.temperature * DT_LN2 * (cross + log2f(total)) : 0.f;
-          if (a.row_loss) a.row_loss[row] = loss;
-          if (a.stat) a.stat[row] = any ? st : make_float2(0.f, 0.f);
-          loss_sum += loss;
-          weight_sum += any ? w : 0.f;
+        if (rank == 0) {
+          const float cross = any ? dt_cross(a, r.s, e, m) : 0.f;
+          if (lane == 0) {
+            const float loss = any ? w * a.temperature * a.temperature * DT_LN2 * (cross + log2f(total)) : 0.f;
+            if (a.row_loss) a.row_loss[row] = loss;
+            if (a.stat) a.stat[row] = any ? st : make_float2(0.f, 0.f);
+            loss_sum += loss;
+            weight_sum += any ? w : 0.f;
+          }
         }
       } else if constexpr (DO & DT_GRAD) {
         if (any) gradient(st.x, st.y);
         else {
           zeros();
-          fetch(coming.s + coming.head, coming.pieces, t);
+          fetch(coming.body, coming.pieces, t);
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(DL_STREAM) : "memory");   // the streaming warps
-        if (any) dt_columns(a, r.s, grad, id, p, f, st.y, st.x, t, DL_STREAM);
+        asm volatile("bar.sync 1, %0;" ::"n"(STREAM) : "memory");   // the streaming warps
+        if (any) dt_columns(a, r.s, grad, e, f, st.y, st.x, t, STREAM, r.lo, r.hi);
       }
     } else if (streams) {
-      dt_columns(a, r.s, grad, id, p, f, st.y, st.x, t, DL_STREAM);
+      dt_columns(a, r.s, grad, e, f, st.y, st.x, t, STREAM, r.lo, r.hi);
     }
     buf ^= 1;
   }
   if constexpr (DO & DT_LOSS)
-    if (t == DL_STREAM) a.part[blockIdx.x] = make_double2(loss_sum, weight_sum);
+    if (t == STREAM && rank == 0) a.part[blockIdx.x / share] = make_double2(loss_sum, weight_sum);
 }
 
 // The weights that count, before the gradient is scaled by their sum: a row's is zero if it has no teacher.
@@ -750,23 +877,45 @@ __global__ void __launch_bounds__(NT) k_distill_total(const double2* __restrict_
   }
 }
 
-// CTAs of a call, which is also the number of its partial sums
-static int dt_ctas(long long rows, int vocab) {
-  const bool is_short = vocab <= DT_WARP_VOCAB;
-  const long long n = is_short ? (rows + DT_WARP_THREADS / 32 - 1) / (DT_WARP_THREADS / 32) : rows, most = (long long)sm_count() * (is_short ? 8 : DL_CTAS);
-  return (int)(n < most ? n : most);
+// Rows' groups of a call, one CTA or a cluster each, which is also the number of its partial sums
+// A call's form.  Threads that stream through a long row: few for short ones, so that more rows' latencies lie side by side, many for long ones, so
+// that (loss and gradient) the rows being worked on stay in the L2 cache between their two passes.  share: CTAs that share a row, until all have work.
+struct DtForm { int stream, share, ctas; };
+static DtForm dt_form(long long rows, int vocab, int type_bytes) {
+  if (vocab <= DT_WARP_VOCAB) {
+    const long long n = (rows + DT_WARP_THREADS / 32 - 1) / (DT_WARP_THREADS / 32), most = (long long)sm_count() * 8;
+    return {0, 1, (int)(n < most ? n : most)};
+  }
+  const long long bytes = (long long)vocab * type_bytes;
+  const int stream = bytes <= 16384 ? 128 : bytes <= 131072 ? 256 : 512;
+  const long long most = (long long)sm_count() * dl_ctas(stream);
+  int share = 1;
+  while (share < DL_MOST_SHARE && bytes >= share * 2 * 16384 && rows * share * 2 <= most) share *= 2;
+  return {stream, share, (int)(rows < most / share ? rows : most / share)};
 }
 static int dt_weight_ctas(long long rows) { return (int)(rows < 64 * NT ? (rows + NT - 1) / NT : 64); }
 template <class T, int DO>
-static int dt_run(const DtArgs& a, cudaStream_t s) {
-  const int ctas = dt_ctas(a.rows, a.vocab);
-  if (a.vocab <= DT_WARP_VOCAB) launch(k_distill_short<T, DO>, ctas, DT_WARP_THREADS, (size_t)12 * a.top * (DT_WARP_THREADS / 32), s, a);
-  else launch(k_distill_long<T, DO>, ctas, DL_THREADS, (size_t)24 * a.top, s, a);
+static int dt_run(const DtArgs& a, const DtForm& form, cudaStream_t s) {
+  const size_t slots = (size_t)4 * dt_slots(a.top), entries = sizeof(DtEntry) * a.top;
+#define DT_LONG(STREAM)                                                                                                    \
+  {                                                                                                                        \
+    launch_clusters(k_distill_long<T, DO, STREAM>, form.ctas * form.share, STREAM + 32, form.share, 2 * entries + slots, s, a); \
+    return launch_status();                                                                                                \
+  }
+  if (form.stream == 128) DT_LONG(128)
+  if (form.stream == 256) DT_LONG(256)
+  if (form.stream == 512) DT_LONG(512)
+#undef DT_LONG
+  const size_t smem = (entries + slots) * (DT_WARP_THREADS / 32);
+  static bool configured[PYLO_MAX_DEVICES] = {};
+  if (smem > 48 * 1024)
+    if (int rc = allow_dynamic_smem(k_distill_short<T, DO>, (int)(DT_WARP_THREADS / 32 * (sizeof(DtEntry) * DT_MOST_K + 4 * dt_slots(DT_MOST_K))), configured)) return rc;
+  launch(k_distill_short<T, DO>, form.ctas, DT_WARP_THREADS, smem, s, a);
   return launch_status();
 }
 template <int DO>
-static int dt_any_type(const DtArgs& a, int type, cudaStream_t s) {
-  return type == PYLO_FP32 ? dt_run<float, DO>(a, s) : type == PYLO_BF16 ? dt_run<__nv_bfloat16, DO>(a, s) : dt_run<__half, DO>(a, s);
+static int dt_any_type(const DtArgs& a, int type, const DtForm& form, cudaStream_t s) {
+  return type == PYLO_FP32 ? dt_run<float, DO>(a, form, s) : type == PYLO_BF16 ? dt_run<__nv_bfloat16, DO>(a, form, s) : dt_run<__half, DO>(a, form, s);
 }
 static bool dt_good(const pylo_distill* d) {
   return d && d->rows >= 0 && d->rows <= (1ll << 40) && d->vocab > 0 && d->vocab <= (1 << 30) && d->top > 0 && d->top <= DT_MOST_K && rw_type(d->type) &&
@@ -825,7 +974,8 @@ int pylo_b200_layer_norm_backward(const pylo_norm* n, void* stream) {
 
 int64_t pylo_b200_distill_workspace(int64_t rows, int vocab) {
   if (rows <= 0 || vocab <= 0) return 16;
-  return 16 * (int64_t)dt_ctas(rows, vocab) + 8 * (int64_t)dt_weight_ctas(rows);
+  const long long most = (long long)sm_count() * 8;   // groups of rows of whatever form
+  return 16 * (int64_t)(rows < most ? rows : most) + 8 * (int64_t)dt_weight_ctas(rows);
 }
 
 int pylo_b200_distill(const pylo_distill* d, int what, void* stream) {
@@ -836,20 +986,21 @@ int pylo_b200_distill(const pylo_distill* d, int what, void* stream) {
   CHECK_ARG(!grad || d->rows == 0 || (d->grad && (uintptr_t)d->grad % rw_bytes(d->type) == 0));
   CHECK_ARG(!grad || loss || d->rows == 0 || (d->stat && (!mean || d->inv)));
   DtArgs a = dt_args(d);
+  const DtForm form = d->rows ? dt_form(d->rows, d->vocab, (int)rw_bytes(d->type)) : DtForm{};
   if (d->rows) {
     a.part = (double2*)d->work;
     if (grad) a.scale = d->scale;
     if (grad && mean && loss) {
-      double* const sums = (double*)((char*)d->work + 16 * (size_t)dt_ctas(d->rows, d->vocab));
+      double* const sums = (double*)((char*)d->work + 16 * (size_t)form.ctas);
       a.weight_sums = sums;
       a.n_sums = dt_weight_ctas(d->rows);
       launch(k_distill_weights, a.n_sums, NT, 0, s, a, sums);
     } else if (grad && mean) a.inv = d->inv;
-    const int rc = !grad ? dt_any_type<DT_LOSS>(a, d->type, s) : loss ? dt_any_type<DT_LOSS | DT_GRAD>(a, d->type, s) : dt_any_type<DT_GRAD>(a, d->type, s);
+    const int rc = !grad ? dt_any_type<DT_LOSS>(a, d->type, form, s) : loss ? dt_any_type<DT_LOSS | DT_GRAD>(a, d->type, form, s) : dt_any_type<DT_GRAD>(a, d->type, form, s);
     if (rc) return rc;
   }
   if (loss && d->reduction != PYLO_REDUCE_NONE)
-    launch(k_distill_total, 1, NT, 0, s, (const double2*)d->work, d->rows ? dt_ctas(d->rows, d->vocab) : 0, (int)mean, 1.0f, d->loss, d->inv);
+    launch(k_distill_total, 1, NT, 0, s, (const double2*)d->work, form.ctas, (int)mean, 1.0f, d->loss, d->inv);
   return launch_status();
 }
 

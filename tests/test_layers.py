@@ -418,6 +418,9 @@ def test_distill_of_padded_masked_and_repeated_entries(T, vocab):
     ids[4, 7] = ids[4, 0]                          # the same class twice, three times
     ids[4, 9] = ids[4, 0]
     ids[5, :] = ids[5, 0]
+    ids[12], ids[13] = -1, -1                      # padding before and between class 0
+    ids[12, 3], ids[13, 2], ids[13, 5], ids[13, 6] = 0, 0, 0, 1
+    ids[14, :6] = torch.arange(6, device="cuda") * 64 % vocab   # neighbours in a table
     teacher[6, 3:] = -math.inf
     teacher[7] = -math.inf
     teacher[1, 5:] = math.nan                      # beside padding: not looked at
