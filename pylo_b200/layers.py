@@ -21,38 +21,45 @@ TYPES = {torch.float32: L.FP32, torch.bfloat16: L.BF16, torch.float16: L.FP16}
 ACTIVATIONS = {"silu": L.ACT_SILU, "gelu": L.ACT_GELU, "gelu_tanh": L.ACT_GELU_TANH, "relu": L.ACT_RELU}
 REDUCTIONS = {"none": L.REDUCE_NONE, "sum": L.REDUCE_SUM, "mean": L.REDUCE_MEAN}
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_Tensor = torch.Tensor
+_device_now, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_sizes = {}   # what the library says of a call's workspace
 
 
 def _call(function, what, device, *args):
-    """A function of the library on the current stream of a device."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        code = function(*args, _raw_stream(index))
+    """A function of the library on the current stream of a device (its number)."""
+    if device == _device_now():
+        code = function(*args, _raw_stream(device))
     else:
-        with torch.cuda.device(index):
-            code = function(*args, _raw_stream(index))
+        with torch.cuda.device(device):
+            code = function(*args, _raw_stream(device))
     if code:
         L.check(code, what)
 
 
-def _on(device, function, *args):
+def _size(name, device, *args):
     """What a function of the library that asks the current device says for ``device``."""
-    if device.index == torch.cuda.current_device():
-        return function(*args)
-    with torch.cuda.device(device):
-        return function(*args)
+    key = (name, device, args)
+    size = _sizes.get(key)
+    if size is None:
+        with torch.cuda.device(device):
+            size = getattr(L.lib, name)(*args)
+        if len(_sizes) > 4096:
+            _sizes.clear()
+        _sizes[key] = size
+    return size
 
 
 def _check(name, t, device=None, types=TYPES):
-    if not isinstance(t, torch.Tensor):
+    if isinstance(t, _Tensor) and t.is_cuda and (device is None or t.get_device() == device) and t.dtype in types:
+        return
+    if not isinstance(t, _Tensor):
         raise TypeError(f"{name} has to be a tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise ValueError(f"{name} has to be a CUDA tensor, it is on {t.device}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if t.dtype not in types:
-        raise TypeError(f"{name} is {t.dtype}, supported are {', '.join(str(d).split('.')[1] for d in types)}")
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
+    raise TypeError(f"{name} is {t.dtype}, supported are {', '.join(str(d).split('.')[1] for d in types)}")
 
 
 def _rows(t):
@@ -62,8 +69,27 @@ def _rows(t):
     return t if t.stride(1) == 1 else t.contiguous()
 
 
+def _like(t):
+    """An uninitialised contiguous tensor of the shape, type and device of ``t``."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _graph(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _once(backward):
+    """``once_differentiable``, whose contexts a plain backward pass does without."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -73,16 +99,15 @@ def _graph(*tensors):
 
 def _norm_forward(x, weight, bias, eps, keep):
     n, width = x.shape
-    y = torch.empty((n, width), dtype=x.dtype, device=x.device)
+    y = _like(x)
     stat = torch.empty((2, n), dtype=torch.float32, device=x.device) if keep else None
     if n:
-        w = L.Norm(x=x.data_ptr(), weight=None if weight is None else weight.data_ptr(), bias=None if bias is None else bias.data_ptr(),
-                   y=y.data_ptr(), rows=n, x_stride=x.stride(0), width=width, type=TYPES[x.dtype],
-                   weight_type=TYPES[x.dtype if weight is None else weight.dtype], eps=eps)
-        if keep:
-            w.mean = stat.data_ptr()
-            w.rstd = w.mean + 4 * n
-        _call(L.lib.pylo_b200_layer_norm, "layer_norm", x.device, C.byref(w))
+        mean = stat.data_ptr() if keep else None
+        kind = TYPES[x.dtype]
+        w = L.Norm(x=x.data_ptr(), weight=None if weight is None else weight.data_ptr(), bias=None if bias is None else bias.data_ptr(), y=y.data_ptr(),
+                   mean=mean, rstd=mean + 4 * n if keep else None, rows=n, x_stride=x.stride(0), width=width, type=kind,
+                   weight_type=kind if weight is None else TYPES[weight.dtype], eps=eps)
+        _call(L.lib.pylo_b200_layer_norm, "layer_norm", x.get_device(), C.byref(w))
     return y, stat
 
 
@@ -94,26 +119,27 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         rows, weight, stat = ctx.saved_tensors
         n, width = rows.shape
+        device = rows.get_device()
         dy = _rows(dy)
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        dx = torch.empty((n, width), dtype=rows.dtype, device=rows.device) if need_x else None
-        dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w else None
-        db = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_b else None
-        columns = need_w or need_b
-        w = L.Norm(x=rows.data_ptr(), dy=dy.data_ptr(), weight=None if weight is None else weight.data_ptr(), mean=stat.data_ptr(),
-                   rstd=stat.data_ptr() + 4 * n, dx=dx.data_ptr() if need_x else None, dweight=dw.data_ptr() if need_w else None,
-                   dbias=db.data_ptr() if need_b else None, rows=n, x_stride=rows.stride(0), dy_stride=dy.stride(0), width=width,
-                   type=TYPES[rows.dtype], weight_type=TYPES[rows.dtype if weight is None else weight.dtype])
-        if columns:
-            w.work_floats = _on(rows.device, L.lib.pylo_b200_layer_norm_workspace, n, width)
-            work = torch.empty(w.work_floats, dtype=torch.float32, device=rows.device)
-            w.work = work.data_ptr()
-        if n or columns:
-            _call(L.lib.pylo_b200_layer_norm_backward, "layer_norm backward", rows.device, C.byref(w))
+        dx = _like(rows) if need_x else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty_like(weight) if need_b else None
+        kind, mean = TYPES[rows.dtype], stat.data_ptr()
+        w = L.Norm(x=rows.data_ptr(), dy=dy.data_ptr(), weight=None if weight is None else weight.data_ptr(), mean=mean, rstd=mean + 4 * n,
+                   dx=dx.data_ptr() if need_x else None, dweight=dw.data_ptr() if need_w else None, dbias=db.data_ptr() if need_b else None, rows=n,
+                   x_stride=rows.stride(0), dy_stride=dy.stride(0), width=width, type=kind, weight_type=kind if weight is None else TYPES[weight.dtype])
+        if need_w or need_b:
+            size = _size("pylo_b200_layer_norm_workspace", device, n, width)
+            work = torch.empty(size, dtype=torch.float32, device=rows.device)
+            w.work, w.work_floats = work.data_ptr(), size
+        elif not n:
+            return dx, dw, db, None
+        _call(L.lib.pylo_b200_layer_norm_backward, "layer_norm backward", device, C.byref(w))
         return dx, dw, db, None
 
 
@@ -123,27 +149,29 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     ``weight`` and ``bias`` are vectors of ``x``'s type or fp32, and their gradients are of that type; a bias needs a weight beside it.  Means,
     variances and the sums of the gradients are fp32, each result is rounded once.  Rows of up to 32768 elements, of any stride."""
     _check("x", x)
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError("x needs a last dimension of at least one element")
-    width = x.shape[-1]
-    if width > L.NORM_MOST:
-        raise ValueError(f"x has rows of {width} elements: {L.NORM_MOST} are supported")
+    dim, device, dtype = x.dim(), x.get_device(), x.dtype
+    width = x.shape[-1] if dim else 0
+    if not 1 <= width <= L.NORM_MOST:
+        raise ValueError(f"x has to have rows of 1 to {L.NORM_MOST} elements, its shape is {tuple(x.shape)}")
     if not (isinstance(eps, (int, float)) and 0.0 <= eps < math.inf):
         raise ValueError(f"eps has to be a finite number >= 0, got {eps!r}")
-    if weight is None and bias is not None:
-        raise ValueError("a bias needs a weight beside it")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        _check(name, t, x.device)
-        if t.shape != (width,):
-            raise ValueError(f"{name} has the shape {tuple(t.shape)}, x has rows of {width} elements")
-        if t.dtype not in (x.dtype, torch.float32) or t.dtype != weight.dtype:
-            raise TypeError(f"weight and bias have to be both of x's type or both float32, {name} is {t.dtype}")
-    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    if weight is not None:
+        _check("weight", weight, device, (dtype, torch.float32))
+        if weight.shape != (width,):
+            raise ValueError(f"weight has the shape {tuple(weight.shape)}, x has rows of {width} elements")
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+    if bias is not None:
+        if weight is None:
+            raise ValueError("a bias needs a weight beside it")
+        _check("bias", bias, device, (weight.dtype,))
+        if bias.shape != (width,):
+            raise ValueError(f"bias has the shape {tuple(bias.shape)}, x has rows of {width} elements")
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
     rows = _rows(x)
     y = _LayerNorm.apply(rows, weight, bias, float(eps)) if _graph(x, weight, bias) else _norm_forward(rows, weight, bias, float(eps), False)[0]
-    return y if x.dim() == 2 else y.view(x.shape)
+    return y if dim == 2 else y.view(x.shape)
 
 
 class LayerNorm(torch.nn.Module):
@@ -227,7 +255,7 @@ def _ffn_forward(rows, w_gate, w_up, w_down, activation, keep):
     f, alive = _ffn_struct(rows, w_gate, w_up, w_down, activation)
     kept = torch.empty(L.lib.pylo_b200_gated_ffn_kept(f.rows, f.hidden, keep), dtype=torch.uint8, device=rows.device)
     f.y, f.kept, f.keep = y.data_ptr(), kept.data_ptr(), keep
-    _call(L.lib.pylo_b200_gated_ffn, "gated_ffn", rows.device, C.byref(f))
+    _call(L.lib.pylo_b200_gated_ffn, "gated_ffn", rows.get_device(), C.byref(f))
     return y, alive[0], kept
 
 
@@ -240,7 +268,7 @@ class _GatedFFN(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         rows, w_gate, w_up, w_down, kept = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -253,7 +281,7 @@ class _GatedFFN(torch.autograd.Function):
             work = torch.empty(L.lib.pylo_b200_gated_ffn_workspace(f.rows, f.hidden), dtype=torch.uint8, device=rows.device)
             f.dy, f.ld_dy, f.kept, f.work = dy.data_ptr(), ld, kept.data_ptr(), work.data_ptr()
             f.dx, f.dw_gate, f.dw_up, f.dw_down = (None if g is None else g.data_ptr() for g in grads)
-            _call(L.lib.pylo_b200_gated_ffn_backward, "gated_ffn backward", rows.device, C.byref(f))
+            _call(L.lib.pylo_b200_gated_ffn_backward, "gated_ffn backward", rows.get_device(), C.byref(f))
         return *grads, None
 
 
@@ -269,7 +297,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         raise ValueError(f"activation is {activation!r}, supported are {', '.join(ACTIVATIONS)}")
     _check("x", x, types=(torch.bfloat16, torch.float16))
     for name, t in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
-        _check(name, t, x.device, (x.dtype,))
+        _check(name, t, x.get_device(), (x.dtype,))
         if t.dim() != 2:
             raise ValueError(f"{name} has to be a matrix, got the shape {tuple(t.shape)}")
     if x.dim() == 0 or w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[-1] or w_down.shape[1] != w_gate.shape[0]:
@@ -307,8 +335,9 @@ class GatedFFN(torch.nn.Module):
 def _distill_arguments(logits, teacher_logits, teacher_ids, temperature, weights, reduction):
     """Checked arguments: (logits' rows, teacher, ids, weights, code of the reduction)."""
     _check("logits", logits)
-    _check("teacher_logits", teacher_logits, logits.device)
-    _check("teacher_ids", teacher_ids, logits.device, (torch.int64, torch.int32))
+    device = logits.get_device()
+    _check("teacher_logits", teacher_logits, device)
+    _check("teacher_ids", teacher_ids, device, (torch.int64, torch.int32))
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction is {reduction!r}, supported are {', '.join(REDUCTIONS)}")
     if not (isinstance(temperature, (int, float)) and 2.0 ** -60 <= temperature <= 2.0 ** 60):
@@ -321,7 +350,7 @@ def _distill_arguments(logits, teacher_logits, teacher_ids, temperature, weights
     if not 1 <= teacher_logits.shape[-1] <= L.DISTILL_MOST_TOP:
         raise ValueError(f"a teacher gives 1 to {L.DISTILL_MOST_TOP} entries, got {teacher_logits.shape[-1]}")
     if weights is not None:
-        _check("weights", weights, logits.device, (*TYPES, torch.bool))
+        _check("weights", weights, device, (*TYPES, torch.bool))
         if weights.shape != lead:
             raise ValueError(f"weights have the shape {tuple(weights.shape)}, the rows of logits {tuple(lead)}")
     if torch.is_grad_enabled() and (teacher_logits.requires_grad or (weights is not None and weights.requires_grad)):
@@ -329,9 +358,13 @@ def _distill_arguments(logits, teacher_logits, teacher_ids, temperature, weights
     rows = _rows(logits.detach())
     if rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]:
         rows = rows.contiguous()
-    if weights is not None:
+    if weights is not None and not (weights.dtype is torch.float32 and weights.is_contiguous()):
         weights = weights.detach().to(torch.float32).contiguous()
-    return rows, teacher_logits.detach().contiguous(), teacher_ids.contiguous(), weights, REDUCTIONS[reduction]
+    return rows, _contiguous(teacher_logits), _contiguous(teacher_ids), weights, REDUCTIONS[reduction]
+
+
+def _contiguous(t):
+    return t if t.is_contiguous() else t.detach().contiguous()
 
 
 def _distill_struct(rows, teacher, ids, weights, temperature, reduction):
@@ -342,45 +375,46 @@ def _distill_struct(rows, teacher, ids, weights, temperature, reduction):
 
 
 def _distill_forward(rows, teacher, ids, weights, temperature, reduction, lead, keep):
+    """(loss, a buffer that begins with the rows' statistics and has the sum of the weights behind them)"""
     n, vocab = rows.shape
-    device = rows.device
+    device = rows.get_device()
     d = _distill_struct(rows, teacher, ids, weights, temperature, reduction)
-    loss = torch.empty(lead if reduction == L.REDUCE_NONE else (), dtype=torch.float32, device=device)
-    stat = torch.empty((n, 2), dtype=torch.float32, device=device) if keep else None
-    inv = torch.empty(1, dtype=torch.float32, device=device) if keep and reduction == L.REDUCE_MEAN else None
-    d.work_bytes = _on(device, L.lib.pylo_b200_distill_workspace, n, vocab)
-    work = torch.empty(d.work_bytes // 8, dtype=torch.float64, device=device)
-    d.work = work.data_ptr()
+    loss = torch.empty(lead if reduction == L.REDUCE_NONE else (), dtype=torch.float32, device=rows.device)
+    work_bytes = _size("pylo_b200_distill_workspace", device, n, vocab)
+    stat_bytes = (8 * n + 4 + 15) // 16 * 16 if keep else 0
+    buffer = torch.empty(stat_bytes + work_bytes, dtype=torch.uint8, device=rows.device)
+    at = buffer.data_ptr()
+    d.work, d.work_bytes = at + stat_bytes, work_bytes
     if reduction == L.REDUCE_NONE:
         d.row_loss = loss.data_ptr()
     else:
         d.loss = loss.data_ptr()
     if keep:
-        d.stat = stat.data_ptr()
-        d.inv = None if inv is None else inv.data_ptr()
+        d.stat, d.inv = at, at + 8 * n
     _call(L.lib.pylo_b200_distill, "distillation_loss", device, C.byref(d), L.DISTILL_LOSS)
-    return loss, stat, inv
+    return loss, buffer
 
 
 class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, rows, teacher, ids, weights, temperature, reduction):
-        loss, stat, inv = _distill_forward(rows, teacher, ids, weights, temperature, reduction, logits.shape[:-1], True)
-        ctx.save_for_backward(rows, teacher, ids, weights, stat, inv)
+        loss, buffer = _distill_forward(rows, teacher, ids, weights, temperature, reduction, logits.shape[:-1], True)
+        ctx.save_for_backward(rows, teacher, ids, weights, buffer)
         ctx.temperature, ctx.reduction, ctx.shape = temperature, reduction, logits.shape
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, upstream):
-        rows, teacher, ids, weights, stat, inv = ctx.saved_tensors
-        grad = torch.empty(ctx.shape, dtype=rows.dtype, device=rows.device)
-        upstream = upstream.to(torch.float32).contiguous()
+        rows, teacher, ids, weights, buffer = ctx.saved_tensors
+        grad = _like(rows)
+        if upstream.dtype is not torch.float32 or not upstream.is_contiguous():
+            upstream = upstream.to(torch.float32).contiguous()
         d = _distill_struct(rows, teacher, ids, weights, ctx.temperature, ctx.reduction)
-        d.stat, d.grad, d.upstream = stat.data_ptr(), grad.data_ptr(), upstream.data_ptr()
-        d.inv = None if inv is None else inv.data_ptr()
-        _call(L.lib.pylo_b200_distill, "distillation_loss backward", rows.device, C.byref(d), L.DISTILL_GRAD)
-        return grad, None, None, None, None, None, None
+        d.stat, d.grad, d.upstream = buffer.data_ptr(), grad.data_ptr(), upstream.data_ptr()
+        d.inv = d.stat + 8 * d.rows
+        _call(L.lib.pylo_b200_distill, "distillation_loss backward", rows.get_device(), C.byref(d), L.DISTILL_GRAD)
+        return grad.view(ctx.shape), None, None, None, None, None, None
 
 
 def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor, temperature: float = 1.0,
@@ -409,20 +443,20 @@ def distillation_loss_and_grad(logits: torch.Tensor, teacher_logits: torch.Tenso
         raise ValueError("reduction has to be 'mean' or 'sum'")
     d = _distill_struct(rows, teacher, ids, w, float(temperature), code)
     if isinstance(scale, torch.Tensor):
-        _check("scale", scale, logits.device, (torch.float32,))
+        _check("scale", scale, logits.get_device(), (torch.float32,))
         if scale.numel() != 1:
             raise ValueError("scale has to have one element")
         d.upstream = scale.data_ptr()
     else:
         d.scale = float(scale)
-    device = rows.device
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-    d.work_bytes = _on(device, L.lib.pylo_b200_distill_workspace, *rows.shape)
-    work = torch.empty(d.work_bytes // 8, dtype=torch.float64, device=device)
+    device = rows.get_device()
+    loss = torch.empty((), dtype=torch.float32, device=rows.device)
+    grad = _like(rows)
+    d.work_bytes = _size("pylo_b200_distill_workspace", device, *rows.shape)
+    work = torch.empty(d.work_bytes, dtype=torch.uint8, device=rows.device)
     d.loss, d.grad, d.work = loss.data_ptr(), grad.data_ptr(), work.data_ptr()
     _call(L.lib.pylo_b200_distill, "distillation_loss_and_grad", device, C.byref(d), L.DISTILL_LOSS | L.DISTILL_GRAD)
-    return loss, grad
+    return loss, grad.view(logits.shape)
 
 
 class DistillationLoss(torch.nn.Module):
