@@ -576,7 +576,7 @@ int pylo_b200_clip_grads_to(void* const* g, const int64_t* n, const int32_t* typ
  * Arguments are HOST structs whose pointers are DEVICE memory; types are PYLO_FP32, PYLO_BF16, PYLO_FP16.  No call allocates: workspaces
  * are the caller's, need not be cleared, and belong to one call at a time. */
 
-/* Layer norm of rows: y = (x - mean) rstd weight + bias with rstd = 1 / sqrt(variance + eps).  Width up to 32768. */
+/* Layer norm of rows: y = (x - mean) rstd weight + bias with rstd = 1 / sqrt(variance + eps).  Width up to 16384. */
 typedef struct pylo_norm {
   const void* x;                 /* [rows][width], rows x_stride elements apart */
   const void *weight, *bias;     /* [width] or NULL; bias only beside a weight */

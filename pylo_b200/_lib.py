@@ -156,7 +156,7 @@ class Ffn(C.Structure):
 DISTILL_LOSS, DISTILL_GRAD = 1, 2
 REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
 ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU = 0, 1, 2, 3
-NORM_MOST, DISTILL_MOST_TOP = 32768, 1024   # elements of a row of layer norm, entries of a teacher
+NORM_MOST, DISTILL_MOST_TOP = 16384, 1024   # elements of a row of layer norm, entries of a teacher
 
 
 class PyloLibError(RuntimeError):

@@ -609,32 +609,6 @@ static bool ff_pairs(const ff_product& p, int epi) {
   const int64_t n = (p.N + (epi == FF_GATE ? 127 : 255)) / (epi == FF_GATE ? 128 : 256);
   return (int64_t)((p.M + 255) / 256) * n >= 48;
 }
-// Clusters of so many CTAs that run at once: one CTA fills an SM, and not every group of SMs that a cluster has to stay in is a multiple of it.
-template <class K>
-static int ff_active(K kernel, int cluster, int smem) {
-  static int known[PYLO_MAX_DEVICES][4] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const int at = cluster == 1 ? 0 : cluster == 2 ? 1 : cluster == 4 ? 2 : 3;
-  if (dev >= 0 && dev < PYLO_MAX_DEVICES && known[dev][at]) return known[dev][at];
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = cluster;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = 8 * 148;
-  cfg.blockDim = FF_THREADS;
-  cfg.dynamicSmemBytes = smem;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
-    cudaGetLastError();
-    n = sm_count() / cluster;
-  }
-  if (dev >= 0 && dev < PYLO_MAX_DEVICES) known[dev][at] = n;
-  return n;
-}
 template <bool PAIR, int EPI, bool BF>
 static int ff_go(ff_args& a, cudaStream_t s) {
   constexpr int TILE_M = PAIR ? 256 : 128, TILE_N = (PAIR ? 256 : 128) / (EPI == FF_GATE ? 2 : 1);
@@ -663,7 +637,7 @@ static int ff_go(ff_args& a, cudaStream_t s) {
     // how many CTAs share a tile, by the time that is to be expected: 0.15 us a stage, and what a tile costs besides
     float best = 0.f;
     for (int c = 1; c <= 8; c *= 2) {
-      const int64_t at_once = ff_active(k_ffn_product<PAIR, EPI, BF>, c, SMEM), waves = (tiles + at_once - 1) / at_once;
+      const int64_t at_once = active_clusters<k_ffn_product<PAIR, EPI, BF>>(FF_THREADS, c, SMEM), waves = (tiles + at_once - 1) / at_once;
       const float t = (float)waves * (0.15f * (float)((longest + c - 1) / c) + (c > 1 ? 4.0f + 0.3f * (float)c : 3.0f));
       if (c == 1 || t < best) { best = t; cluster = c; }
     }

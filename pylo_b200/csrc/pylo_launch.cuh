@@ -87,6 +87,35 @@ static int allow_dynamic_smem(K kernel, int bytes, bool (&flags)[PYLO_MAX_DEVICE
   return 0;
 }
 
+// Clusters of 2, 4 or 8 CTAs that run at once (of single CTAs for 1): not every group of SMs that a cluster has to stay in holds a multiple of it.
+template <auto KERNEL>
+static int active_clusters(int threads, int cluster, size_t smem) {
+  static int known[PYLO_MAX_DEVICES][4] = {};
+  static size_t known_smem[PYLO_MAX_DEVICES][4] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int at = cluster == 1 ? 0 : cluster == 2 ? 1 : cluster == 4 ? 2 : 3;
+  const bool kept = dev >= 0 && dev < PYLO_MAX_DEVICES;
+  if (kept && known[dev][at] && known_smem[dev][at] == smem) return known[dev][at];
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = cluster;
+  cfg.blockDim = threads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    n = sm_count() / cluster > 0 ? sm_count() / cluster : 1;
+  }
+  if (kept) { known[dev][at] = n; known_smem[dev][at] = smem; }
+  return n;
+}
+
 #define CHECK_ARG(cond) \
   do {                  \
     if (!(cond)) return -1; \

@@ -48,6 +48,13 @@ struct RwPiece {
       return *reinterpret_cast<const T*>(&h);
     }
   }
+  // What is computed from the elements behind this is not taken from what was computed before it, which would have to be kept
+  __device__ __forceinline__ void anew() { asm volatile("" : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3])); }
+  __device__ __forceinline__ uint64_t two(int j) const {   // elements j, j + 1
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(at(j)), "f"(at(j + 1)));
+    return r;
+  }
   template <class F>
   __device__ __forceinline__ void make(F&& f) {   // element j from f(j), rounded
 #pragma unroll
@@ -68,6 +75,7 @@ struct RwPiece<T, 1> {
   T v;
   __device__ __forceinline__ void load(const T* p) { v = *p; }   // (__ldg of 16-bit types is assembly that the compiler may move out of a branch, to where p is not valid)
   __device__ __forceinline__ void store(T* p) const { *p = v; }
+  __device__ __forceinline__ void anew() {}
   __device__ __forceinline__ float at(int) const { return rw_float(v); }
   template <class F>
   __device__ __forceinline__ void make(F&& f) { v = rw_to<T>(f(0)); }
@@ -95,6 +103,34 @@ __device__ __forceinline__ uint32_t rw_at_rank(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
   return a;
 }
+// two fp32 values, and operations on two at once
+__device__ __forceinline__ uint64_t rw_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void rw_unpair(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ float rw_both(uint64_t r) {   // their sum
+  float a, b;
+  rw_unpair(r, a, b);
+  return a + b;
+}
+__device__ __forceinline__ uint64_t rw_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t rw_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t rw_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 __device__ __forceinline__ float rw_warp_sum(float v) {   // in every lane, in an order of its own
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -105,240 +141,355 @@ __device__ __forceinline__ float rw_warp_max(float v) {
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-// Sums over the threads of a row, in every one of them.  buf: 32 floats of shared memory that all threads of the CTA have finished
-// reading by the barrier before the last: two calls in a row take two of them.
-template <bool BLOCK>
-__device__ __forceinline__ float rw_sum(float v, float* buf) {
-  v = rw_warp_sum(v);
-  if constexpr (BLOCK) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (lane == 0) buf[warp] = v;
-    __syncthreads();
-    v = rw_warp_sum(lane < (int)(blockDim.x >> 5) ? buf[lane] : 0.f);
-  }
-  return v;
-}
 // ------------------------------------------------------------------------------------------------
 // Layer norm.  m = mean x, r = 1 / sqrt(mean (x - m)^2 + eps), xh = (x - m) r:
 //   y = xh w + b;   dx = r (q - mean q - xh mean(q xh)) with q = dy w;   dw = sum over rows dy xh, db = sum over rows dy
 //
-// A row is read once and stays in registers, 32 elements of each thread at most, so that the variance is that of the differences
-// from the mean (a sum of squares less the mean's would lose what rows far off centre have).  The weights stay in registers from row
-// to row, the sums of their gradients too; they leave as one partial sum per CTA, and a second kernel adds those up in a fixed order.
+// A row is read once and stays in registers, 16 or 32 elements of each thread, so that the variance is that of the differences from the mean (a
+// sum of squares less the mean's would lose what rows far off centre have).  A row is a warp's, a CTA's, or a cluster's of two or four
+// CTAs; the next one is on its way while one is worked on.  The weights stay in registers from row to row, the sums of their
+// gradients too; those leave as one partial sum per CTA, and a second kernel adds them up in a fixed order.
 // ------------------------------------------------------------------------------------------------
-#define LN_ELEMS 32           // of a row per thread at most
 #define LN_WARP_THREADS 128   // of a CTA whose warps have a row each
-#define LN_MOST 32768         // elements of a row: 1024 threads
-
+#define LN_WARPS (LN_WARP_THREADS / 32)
+#define LN_MOST 16384         // elements of a row
+#define LN_MOST_SHARE 4
+// CTAs of so many threads on an SM, with E elements per thread: 64 to 128 registers forward, 100 to 168 backward
+__host__ __device__ constexpr int ln_ctas(int threads, int e, bool backward) {
+  return threads > 128 ? backward ? 1 : 512 / threads : e <= 8 ? backward ? 5 : 8 : backward ? 3 : 4;
+}
 struct LnArgs {
   const void *x, *dy, *weight, *bias;
   void *y;               // or dx, or NULL
   float *mean, *rstd;    // written forward (or NULL), read backward
-  float* part;           // [CTAs][2][width]: sums for dw, db; or NULL
+  float* part;           // [CTAs that begin rows][2][width]: sums for dw, db; or NULL
   long long rows, x_stride, dy_stride;
   int width;
   float eps;
 };
 
+// a vector's elements that are a thread's, NV pieces of VN, `gap` elements from one to the next
+template <class W, int VN, int NV>
+struct LnVector {
+  static constexpr int WN = VN == 1 ? 1 : RW_VEC<W>, PER = VN / WN;
+  RwPiece<W, WN> p[NV * PER];
+  __device__ __forceinline__ void load(const W* v, int first, int gap, int width) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        if (first + i * gap < width) p[i * PER + k].load(v + first + i * gap + k * WN);
+        else p[i * PER + k].make([](int) { return 0.f; });
+      }
+  }
+  __device__ __forceinline__ void anew() {
+#pragma unroll
+    for (int i = 0; i < NV * PER; ++i) p[i].anew();
+  }
+  __device__ __forceinline__ uint64_t two(int k) const {   // elements 2k, 2k + 1 of the thread's
+    if constexpr (VN == 1) return rw_pair(p[2 * k].at(0), p[2 * k + 1].at(0));
+    else return p[2 * k / WN].two(2 * k % WN);
+  }
+};
+template <class T, int VN, int NV>
+__device__ __forceinline__ uint64_t ln_two(const RwPiece<T, VN> (&v)[NV], int k) {
+  if constexpr (VN == 1) return rw_pair(v[2 * k].at(0), v[2 * k + 1].at(0));
+  else return v[2 * k / VN].two(2 * k % VN);
+}
+
+// Two sums over the threads of a row, in every one of them, in an order of its own.  buf: what the warps leave for one another; two take turns.
+template <bool BLOCK>
+__device__ __forceinline__ float2 ln_sums(float a, float b, float2* buf, uint32_t rank, uint32_t share) {
+  a = rw_warp_sum(a);
+  b = rw_warp_sum(b);
+  if constexpr (BLOCK) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if (share == 1) {
+      if (lane == 0) buf[warp] = make_float2(a, b);
+      __syncthreads();
+    } else {
+      if (lane < (int)share)
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(rw_at_rank(&buf[rank * warps + warp], lane)), "f"(a), "f"(b) : "memory");
+      rw_cluster_sync();
+    }
+    const float2 q = lane < (int)share * warps ? buf[lane] : make_float2(0.f, 0.f);
+    a = rw_warp_sum(q.x);
+    b = rw_warp_sum(q.y);
+  }
+  return make_float2(a, b);
+}
+
+// Which rows and which elements of them are a thread's
+template <bool BLOCK, int VN, int NV>
+struct LnPlace {
+  uint32_t rank = 0, share = 1;
+  int first, gap;          // elements first + i gap + j of a row
+  long long row, step;
+  __device__ __forceinline__ LnPlace() {
+    if constexpr (BLOCK) {
+      asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+      asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(share));
+      gap = blockDim.x * VN;
+      first = rank * gap * NV + threadIdx.x * VN;
+      row = blockIdx.x / share;
+      step = gridDim.x / share;
+    } else {
+      gap = 32 * VN;
+      first = (threadIdx.x & 31) * VN;
+      row = (long long)blockIdx.x * LN_WARPS + (threadIdx.x >> 5);
+      step = (long long)gridDim.x * LN_WARPS;
+    }
+  }
+  __device__ __forceinline__ bool in(int e, int width) const { return first + e / VN * gap < width; }   // whether the thread's element e is one of the row's
+  template <class T, class F>
+  __device__ __forceinline__ void store(T* out, int width, F&& f) const {   // elements 2k, 2k + 1 from f(k)
+    float keep = 0.f;   // the second of two, where pieces have one element
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float x[VN];
+      if constexpr (VN == 1) {
+        if (i & 1) x[0] = keep;
+        else rw_unpair(f(i / 2), x[0], keep);
+      } else
+        for (int j = 0; j < VN; j += 2) rw_unpair(f((i * VN + j) / 2), x[j], x[j + 1]);
+      if (first + i * gap < width) {
+        RwPiece<T, VN> o;
+        o.make([&](int j) { return x[j]; });
+        o.store(out + first + i * gap);
+      }
+    }
+  }
+};
+
 template <class T, class W, int VN, int E, int MOST>
-__global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS) k_layer_norm(const LnArgs a) {
-  pdl_begin();
+__global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS, ln_ctas(MOST, E, false)) k_layer_norm(const LnArgs a) {
   constexpr bool BLOCK = MOST > 0;   // a row is a CTA's, of so many threads at most
   constexpr int NV = E / VN;
-  __shared__ float s_buf[2][32];
-  const int t = BLOCK ? threadIdx.x : threadIdx.x & 31, threads = BLOCK ? blockDim.x : 32, width = a.width;
-  const long long step = BLOCK ? gridDim.x : (long long)gridDim.x * (LN_WARP_THREADS / 32);
-  long long row = BLOCK ? blockIdx.x : (long long)blockIdx.x * (LN_WARP_THREADS / 32) + (threadIdx.x >> 5);
+  __shared__ float2 s_buf[2][32];   // a part of the sums per lane
+  const LnPlace<BLOCK, VN, NV> at;
+  const int width = a.width;
+  if (at.share > 1) rw_cluster_sync();   // the others are running
+  pdl_begin();
   const float inv = 1.0f / (float)width;
   const T* const x = (const T*)a.x;
-  T* const y = (T*)a.y;
+  LnVector<W, VN, NV> weight, bias;
+  if (a.weight) weight.load((const W*)a.weight, at.first, at.gap, width);
+  if (a.bias) bias.load((const W*)a.bias, at.first, at.gap, width);
   RwPiece<T, VN> v[NV];
   auto fetch = [&](long long r) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * threads) * VN;
-      if (c < width && r < a.rows) v[i].load(x + r * a.x_stride + c);
+    for (int i = 0; i < NV; ++i)
+      if (at.first + i * at.gap < width && r < a.rows) v[i].load(x + r * a.x_stride + at.first + i * at.gap);
       else v[i].make([](int) { return 0.f; });
-    }
   };
-  fetch(row);
-  for (; row < a.rows; row += step) {
-    float f[E], sum = 0.f;
+  fetch(at.row);
+  for (long long row = at.row; row < a.rows; row += at.step) {
+    // elements two by two: of a piece, or (VN = 1) of two pieces
+    uint64_t f[E / 2], sum = rw_pair(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int k = 0; k < E / 2; ++k) sum = rw_add2(sum, f[k] = ln_two<T, VN, NV>(v, k));
+    fetch(row + at.step);
+    const float mean = ln_sums<BLOCK>(rw_both(sum), 0.f, s_buf[0], at.rank, at.share).x * inv;
+    const uint64_t off = rw_pair(-mean, -mean);
+    uint64_t sq = rw_pair(0.f, 0.f);
 #pragma unroll
-      for (int j = 0; j < VN; ++j) sum += f[i * VN + j] = v[i].at(j);
-    fetch(row + step);
-    const float mean = rw_sum<BLOCK>(sum, s_buf[0]) * inv;
-    float sq = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if ((t + i * threads) * VN < width)
-#pragma unroll
-        for (int j = 0; j < VN; ++j) {
-          const float d = f[i * VN + j] - mean;
-          f[i * VN + j] = d;
-          sq = fmaf(d, d, sq);
-        }
-    const float rstd = 1.0f / sqrtf(fmaf(rw_sum<BLOCK>(sq, s_buf[1]), inv, a.eps));
-    if (t == 0 && a.mean) { a.mean[row] = mean; a.rstd[row] = rstd; }
-    T* const out = y + row * width;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * threads) * VN;
-      if (c < width) {
-        RwPiece<T, VN> o;
-        o.make([&](int j) {
-          float q = f[i * VN + j] * rstd;
-          if (a.weight) q *= rw_float(((const W*)a.weight)[c + j]);
-          if (a.bias) q += rw_float(((const W*)a.bias)[c + j]);
-          return q;
-        });
-        o.store(out + c);
+    for (int k = 0; k < E / 2; ++k) {
+      if (VN > 1 && !at.in(2 * k, width)) continue;
+      f[k] = rw_add2(f[k], off);
+      uint64_t d = f[k];
+      if constexpr (VN == 1) {   // what lies behind the row does not differ from the mean
+        float lo, hi;
+        rw_unpair(d, lo, hi);
+        d = rw_pair(at.in(2 * k, width) ? lo : 0.f, at.in(2 * k + 1, width) ? hi : 0.f);
       }
+      sq = rw_fma2(d, d, sq);
     }
+    const float rstd = 1.0f / sqrtf(fmaf(ln_sums<BLOCK>(rw_both(sq), 0.f, s_buf[1], at.rank, at.share).x, inv, a.eps));
+    if (at.first == 0 && a.mean) { a.mean[row] = mean; a.rstd[row] = rstd; }
+    const uint64_t by = rw_pair(rstd, rstd);
+    at.store((T*)a.y + row * width, width, [&](int k) {
+      uint64_t q = rw_mul2(f[k], by);
+      if (a.weight) q = rw_mul2(q, weight.two(k));
+      return a.bias ? rw_add2(q, bias.two(k)) : q;
+    });
   }
 }
 
 template <class T, class W, int VN, int E, int MOST>
-__global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS) k_layer_norm_backward(const LnArgs a) {
-  pdl_begin();
-  constexpr bool BLOCK = MOST > 0;   // a row is a CTA's, of so many threads at most
-  constexpr int NV = E / VN, WARPS = LN_WARP_THREADS / 32;
-  __shared__ float s_buf[4][32];
+__global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS, ln_ctas(MOST, E, true)) k_layer_norm_backward(const LnArgs a) {
+  constexpr bool BLOCK = MOST > 0;
+  constexpr int NV = E / VN;
+  __shared__ float2 s_buf[2][32];   // a part of the sums per lane
   __shared__ float s_cols[BLOCK ? 1 : 2 * 32 * E];
-  const int t = BLOCK ? threadIdx.x : threadIdx.x & 31, threads = BLOCK ? blockDim.x : 32, width = a.width;
-  const long long step = BLOCK ? gridDim.x : (long long)gridDim.x * WARPS;
+  const LnPlace<BLOCK, VN, NV> at;
+  const int width = a.width;
+  if (at.share > 1) rw_cluster_sync();   // the others are running
+  pdl_begin();
   const float inv = 1.0f / (float)width;
-  float dw[E], db[E];
+  LnVector<W, VN, NV> weight;
+  if (a.weight) weight.load((const W*)a.weight, at.first, at.gap, width);
+  uint64_t dw2[E / 2], db2[E / 2];
 #pragma unroll
-  for (int j = 0; j < E; ++j) dw[j] = db[j] = 0.f;
-  int flip = 0;
-  for (long long row = BLOCK ? blockIdx.x : (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); row < a.rows; row += step, flip ^= 2) {
-    const T* const x = (const T*)a.x + row * a.x_stride;
-    const T* const dy = (const T*)a.dy + row * a.dy_stride;
-    RwPiece<T, VN> vx[NV], vd[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * threads) * VN;
-      if (c < width) { vx[i].load(x + c); vd[i].load(dy + c); }
-      else { vx[i].make([](int) { return 0.f; }); vd[i].make([](int) { return 0.f; }); }
-    }
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float q[E], s1 = 0.f, s2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * threads) * VN;
-      if (c < width)
-#pragma unroll
-        for (int j = 0; j < VN; ++j) {
-          const int e = i * VN + j;
-          const float d = vd[i].at(j), xh = (vx[i].at(j) - mean) * rstd;
-          dw[e] = fmaf(d, xh, dw[e]);
-          db[e] += d;
-          q[e] = a.weight ? d * rw_float(((const W*)a.weight)[c + j]) : d;
-          s1 += q[e];
-          s2 = fmaf(q[e], xh, s2);
-        }
-    }
-    if (a.y == nullptr) continue;
-    s1 = rw_sum<BLOCK>(s1, s_buf[flip]) * inv;
-    s2 = rw_sum<BLOCK>(s2, s_buf[flip + 1]) * inv;
-    T* const out = (T*)a.y + row * width;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * threads) * VN;
-      if (c < width) {
-        RwPiece<T, VN> o;
-        o.make([&](int j) { return rstd * (q[i * VN + j] - s1 - (vx[i].at(j) - mean) * rstd * s2); });
-        o.store(out + c);
-      }
-    }
-  }
-  if (a.part == nullptr) return;
-  float* const part = a.part + (long long)blockIdx.x * 2 * width;
-  if constexpr (BLOCK) {
+  for (int k = 0; k < E / 2; ++k) dw2[k] = db2[k] = rw_pair(0.f, 0.f);
+  RwPiece<T, VN> nx[NV], nd[NV];
+  float next_mean = 0.f, next_rstd = 0.f;
+  auto fetch = [&](long long r) {   // what lies behind the row has a gradient of zero
+    if (r >= a.rows) return;
+    next_mean = a.mean[r];
+    next_rstd = a.rstd[r];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < VN; ++j) {
-        const int c = (t + i * threads) * VN + j;
-        if (c < width) { part[c] = dw[i * VN + j]; part[width + c] = db[i * VN + j]; }
+      if (at.first + i * at.gap < width) {
+        nx[i].load((const T*)a.x + r * a.x_stride + at.first + i * at.gap);
+        nd[i].load((const T*)a.dy + r * a.dy_stride + at.first + i * at.gap);
       }
-  } else {
-    // the warps' sums, one warp after the other
-    for (int w = 0; w < WARPS; ++w) {
-      if ((int)(threadIdx.x >> 5) == w)
+  };
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) { nx[i].make([](int) { return 0.f; }); nd[i].make([](int) { return 0.f; }); }
+  fetch(at.row);
+  int flip = 0;
+#pragma unroll 1
+  for (long long row = at.row; row < a.rows; row += at.step, flip ^= 1) {
+    RwPiece<T, VN> vx[NV], vd[NV];
 #pragma unroll
-          for (int j = 0; j < VN; ++j) {
-            const int at = (t + i * 32) * VN + j;
-            s_cols[at] = w ? s_cols[at] + dw[i * VN + j] : dw[i * VN + j];
-            s_cols[32 * E + at] = w ? s_cols[32 * E + at] + db[i * VN + j] : db[i * VN + j];
-          }
-      __syncthreads();
+    for (int i = 0; i < NV; ++i) { vx[i] = nx[i]; vd[i] = nd[i]; }
+    if constexpr (sizeof(W) == 2 && VN > 1) weight.anew();   // its elements in fp32 would take twice the registers
+    // xh = x rstd - mean rstd, one rounding: what the mean's own rounding does to it is as large
+    const uint64_t r2 = rw_pair(next_rstd, next_rstd), off = rw_pair(-next_mean * next_rstd, -next_mean * next_rstd);
+    const float rstd = next_rstd;
+    fetch(row + at.step);
+    uint64_t t1 = rw_pair(0.f, 0.f), t2 = t1;
+#pragma unroll
+    for (int k = 0; k < E / 2; ++k) {
+      const uint64_t d = ln_two<T, VN, NV>(vd, k), xh = rw_fma2(ln_two<T, VN, NV>(vx, k), r2, off), q = a.weight ? rw_mul2(d, weight.two(k)) : d;
+      dw2[k] = rw_fma2(d, xh, dw2[k]);
+      db2[k] = rw_add2(d, db2[k]);
+      t1 = rw_add2(t1, q);
+      t2 = rw_fma2(q, xh, t2);
     }
-    for (int c = threadIdx.x; c < width; c += LN_WARP_THREADS) { part[c] = s_cols[c]; part[width + c] = s_cols[32 * E + c]; }
+    if (a.y == nullptr) continue;
+    const float2 sums = ln_sums<BLOCK>(rw_both(t1), rw_both(t2), s_buf[flip], at.rank, at.share);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) { vx[i].anew(); vd[i].anew(); }
+    if constexpr (sizeof(W) == 2 && VN > 1) weight.anew();
+    // rstd (q - s1 - xh s2)
+    const uint64_t s1 = rw_pair(-sums.x * inv * rstd, -sums.x * inv * rstd), s2 = rw_pair(-sums.y * inv, -sums.y * inv);
+    at.store((T*)a.y + row * width, width, [&](int k) {
+      const uint64_t d = ln_two<T, VN, NV>(vd, k), xh = rw_fma2(ln_two<T, VN, NV>(vx, k), r2, off), q = a.weight ? rw_mul2(d, weight.two(k)) : d;
+      return rw_fma2(rw_fma2(xh, s2, q), r2, s1);
+    });
+  }
+  float dw[E], db[E];
+#pragma unroll
+  for (int k = 0; k < E / 2; ++k) {
+    rw_unpair(dw2[k], dw[2 * k], dw[2 * k + 1]);
+    rw_unpair(db2[k], db[2 * k], db[2 * k + 1]);
+  }
+  if (a.part) {
+    float* const part = a.part + (long long)(BLOCK ? blockIdx.x / at.share : blockIdx.x) * 2 * width;
+    if constexpr (BLOCK) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VN; ++j) {
+          const int c = at.first + i * at.gap + j;
+          if (c < width) { part[c] = dw[i * VN + j]; part[width + c] = db[i * VN + j]; }
+        }
+    } else {
+      // the warps' sums, one warp after the other
+      for (int w = 0; w < LN_WARPS; ++w) {
+        if ((int)(threadIdx.x >> 5) == w)
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VN; ++j) {
+              const int c = at.first + i * at.gap + j;
+              s_cols[c] = w ? s_cols[c] + dw[i * VN + j] : dw[i * VN + j];
+              s_cols[32 * E + c] = w ? s_cols[32 * E + c] + db[i * VN + j] : db[i * VN + j];
+            }
+        __syncthreads();
+      }
+      for (int c = threadIdx.x; c < width; c += LN_WARP_THREADS) { part[c] = s_cols[c]; part[width + c] = s_cols[32 * E + c]; }
+    }
   }
 }
 
-// The partial sums of 32 columns by a CTA: eight rows of threads, each adding up every eighth partial, then those.
+// The partial sums of 32 columns by a CTA: sixteen rows of threads, each adding up every sixteenth partial, then those.
+#define LN_COLUMN_GROUPS 16
 template <class W>
-__global__ void __launch_bounds__(NT) k_layer_norm_columns(const float* __restrict__ part, int n, int width, W* dweight, W* dbias) {
+__global__ void __launch_bounds__(32 * LN_COLUMN_GROUPS) k_layer_norm_columns(const float* __restrict__ part, int n, int width, W* dweight, W* dbias) {
   pdl_begin();
-  __shared__ float s[8][33];
+  __shared__ float s[LN_COLUMN_GROUPS][33];
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   W* const out = blockIdx.y ? dbias : dweight;
   if (out == nullptr) return;
   const float* p = part + (blockIdx.y ? width : 0) + c;
   float sum = 0.f;
   if (c < width)
-    for (int i = g; i < n; i += 8) sum += p[(long long)i * 2 * width];
+#pragma unroll 8
+    for (int i = g; i < n; i += LN_COLUMN_GROUPS) sum += p[(long long)i * 2 * width];
   s[g][lane] = sum;
   __syncthreads();
   if (g == 0 && c < width) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) sum += s[i][lane];
+    for (int i = 1; i < LN_COLUMN_GROUPS; ++i) sum += s[i][lane];
     out[c] = rw_to<W>(sum);
   }
 }
 
-// CTAs of a call: as many as run at once, by rows of so many threads
-static int ln_threads(int width) { return width <= 32 * LN_ELEMS ? LN_WARP_THREADS : (width + 32 * LN_ELEMS - 1) / (32 * LN_ELEMS) * 32; }
-static long long ln_groups(long long rows, int width) { return width <= 32 * LN_ELEMS ? (rows + LN_WARP_THREADS / 32 - 1) / (LN_WARP_THREADS / 32) : rows; }
-static int ln_ctas(long long rows, int width, int resident) {
-  const int t = ln_threads(width), per = resident / t > 1 ? resident / t : 1;
-  const long long n = ln_groups(rows, width), most = (long long)sm_count() * per;
-  return (int)(n < most ? n : most);
+// A call's form: elements of a thread, the most threads of a CTA that the kernel is made for (0: a warp per row), its threads, CTAs that share a row,
+// groups of CTAs that begin with different rows
+struct LnForm { int elems, most, threads, share, groups; };
+static LnForm ln_form(long long rows, int width, bool wide, bool backward) {   // wide: 16-bit elements by 16 bytes
+  const int many = wide ? 32 : 16, few = wide ? 8 : 4;
+  LnForm f = {many, 0, LN_WARP_THREADS, 1, 0};
+  long long n = (rows + LN_WARPS - 1) / LN_WARPS;
+  if (width <= 32 * few) f.elems = few;
+  else if (wide && width <= 512) f.elems = 16;
+  else if (width > 32 * many) {
+    n = rows;
+    f.threads = (width + 32 * many - 1) / (32 * many) * 32;
+    const int most = backward ? 256 : 512;
+    while (f.threads > most) f.threads = (f.threads / 2 + 31) / 32 * 32, f.share *= 2;
+    f.most = f.threads <= 128 ? 128 : f.threads <= 256 ? 256 : 512;
+  }
+  long long at_once = (long long)sm_count() * ln_ctas(f.most, f.elems, backward) / f.share;
+  if (f.most && f.threads < 128) at_once = at_once * 128 / f.threads;
+  f.groups = (int)(n < at_once ? n : at_once);
+  return f;
 }
-#define LN_FORWARD 1024   // threads of an SM: forward, backward
-#define LN_BACKWARD 384
-
 template <class T, class W, int VN>
 static void ln_launch(const LnArgs& a, bool backward, cudaStream_t s) {
-  const int t = ln_threads(a.width), ctas = ln_ctas(a.rows, a.width, backward ? LN_BACKWARD : LN_FORWARD);
-  constexpr int FEW = VN > 1 ? RW_VEC<T> : 8;
-#define LN_GO(E, MOST) backward ? launch(k_layer_norm_backward<T, W, VN, E, MOST>, ctas, t, 0, s, a) : launch(k_layer_norm<T, W, VN, E, MOST>, ctas, t, 0, s, a)
-  if (a.width <= 32 * FEW) LN_GO(FEW, 0);
-  else if (a.width <= 32 * LN_ELEMS) LN_GO(LN_ELEMS, 0);
-  else if (t <= 256) LN_GO(LN_ELEMS, 256);
-  else LN_GO(LN_ELEMS, 1024);
+  constexpr bool WIDE = sizeof(T) == 2 && VN > 1;
+  constexpr int MANY = WIDE ? 32 : 16, FEW = WIDE ? 8 : 4;
+  const LnForm f = ln_form(a.rows, a.width, WIDE, backward);
+#define LN_GO(E, MOST)                                                                                                                   \
+  backward ? launch_clusters(k_layer_norm_backward<T, W, VN, E, MOST>, f.groups * f.share, f.threads, MOST ? f.share : 0, 0, s, a)       \
+           : launch_clusters(k_layer_norm<T, W, VN, E, MOST>, f.groups * f.share, f.threads, MOST ? f.share : 0, 0, s, a)
+  if (f.most == 128) LN_GO(MANY, 128);
+  else if (f.most == 256) LN_GO(MANY, 256);
+  else if (f.most == 512) launch_clusters(k_layer_norm<T, W, VN, MANY, 512>, f.groups * f.share, f.threads, f.share, 0, s, a);
+  else if (f.elems == FEW) LN_GO(FEW, 0);
+  else if (WIDE && f.elems == 16) LN_GO(16, 0);
+  else LN_GO(MANY, 0);
 #undef LN_GO
 }
+// 16 bytes at a time where every row begins on their boundary
+static bool ln_aligned(const pylo_norm* n, bool backward) {
+  const int vec = n->type == PYLO_FP32 ? 4 : 8;
+  uintptr_t p = (uintptr_t)n->x | (uintptr_t)n->weight | (backward ? (uintptr_t)n->dy | (uintptr_t)n->dx : (uintptr_t)n->y | (uintptr_t)n->bias);
+  return p % 16 == 0 && (n->width | n->x_stride | (backward ? n->dy_stride : 0)) % vec == 0;
+}
 template <class T, class W>
-static void ln_run(const LnArgs& a, bool backward, cudaStream_t s) {
-  // 16 bytes at a time where every row begins on their boundary
-  const bool aligned = ((uintptr_t)a.x | (uintptr_t)a.dy | (uintptr_t)a.y) % 16 == 0 &&
-                       (a.width | a.x_stride | (backward ? a.dy_stride : 0)) % RW_VEC<T> == 0;
+static void ln_run(const LnArgs& a, bool aligned, bool backward, cudaStream_t s) {
   aligned ? ln_launch<T, W, RW_VEC<T>>(a, backward, s) : ln_launch<T, W, 1>(a, backward, s);
 }
-static int ln_any(const LnArgs& a, int type, int weight_type, bool backward, cudaStream_t s) {
-  if (type == PYLO_FP32 && weight_type == PYLO_FP32) ln_run<float, float>(a, backward, s);
-  else if (type == PYLO_BF16 && weight_type == PYLO_BF16) ln_run<__nv_bfloat16, __nv_bfloat16>(a, backward, s);
-  else if (type == PYLO_FP16 && weight_type == PYLO_FP16) ln_run<__half, __half>(a, backward, s);
-  else if (type == PYLO_BF16 && weight_type == PYLO_FP32) ln_run<__nv_bfloat16, float>(a, backward, s);
-  else if (type == PYLO_FP16 && weight_type == PYLO_FP32) ln_run<__half, float>(a, backward, s);
+static int ln_any(const LnArgs& a, int type, int weight_type, bool aligned, bool backward, cudaStream_t s) {
+  if (type == PYLO_FP32 && weight_type == PYLO_FP32) ln_run<float, float>(a, aligned, backward, s);
+  else if (type == PYLO_BF16 && weight_type == PYLO_BF16) ln_run<__nv_bfloat16, __nv_bfloat16>(a, aligned, backward, s);
+  else if (type == PYLO_FP16 && weight_type == PYLO_FP16) ln_run<__half, __half>(a, aligned, backward, s);
+  else if (type == PYLO_BF16 && weight_type == PYLO_FP32) ln_run<__nv_bfloat16, float>(a, aligned, backward, s);
+  else if (type == PYLO_FP16 && weight_type == PYLO_FP32) ln_run<__half, float>(a, aligned, backward, s);
   else return -1;
   return launch_status();
 }
@@ -359,6 +510,7 @@ static bool rw_type(int type) { return type == PYLO_FP32 || type == PYLO_BF16 ||
 #define DT_MOST_K 1024
 #define DT_WARP_VOCAB 1024     // classes up to which a row is a warp's
 #define DT_WARP_THREADS 128
+#define DT_MOST_CTAS 8         // of an SM, in whatever form
 #define DT_LOG2E 1.4426950408889634
 #define DT_LN2 0.6931471805599453f
 enum { DT_LOSS = 1, DT_GRAD = 2 };
@@ -586,210 +738,239 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs 
   }
 }
 
-// Long rows: a CTA each, or a cluster's, each CTA with its part of the row.  STREAM threads go through the logits, each with DL_U pieces of
-// 16 bytes on their way, the next row's first ones behind this row's last; one more warp has the teacher's entries and the row's loss, so that
-// nothing of the stream waits for them.  One barrier per row and pass: what the warps leave for one another lies in two buffers that take turns.
+// Long rows: a CTA each, or a cluster's, each CTA with its part of the row.  STREAM threads go through the logits; each has a ring of pieces of 16 bytes
+// of its own in shared memory, which it fills by asynchronous copies and alone reads, so that what is on its way takes neither registers nor barriers, and
+// the next row's first pieces come behind this row's last.  In the call that makes loss and gradient a row's pieces stay in the ring between the two
+// passes (dt_form sees to it that they fit).  One more warp has the teacher's entries and the row's loss, so that nothing of the stream waits for them.
+// One barrier per row and pass: what the warps leave for one another lies in two buffers that take turns.
 //
-// A cluster shares a row where there are too few rows for all CTAs.
-#define DL_U 4
+// A cluster shares a row where there are too few rows for all CTAs, and where a row would not fit the ring.
 #define DL_MOST_SHARE 8
+#define DL_KEPT 8   // pieces of a row that stay in the ring of 12
 __host__ __device__ constexpr int dl_ctas(int stream) { return stream == 128 ? 7 : stream == 256 ? 4 : 2; }   // of an SM
-__device__ __forceinline__ uint64_t dt_pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
+__host__ __device__ constexpr int dl_ring(int what) { return what == (DT_LOSS | DT_GRAD) ? 12 : 8; }
+// all copies of this thread but the last n groups have arrived
+__device__ __forceinline__ void rw_arrived(int n) {
+  switch (n) {
+#define RW_CASE(N) case N: asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); break;
+    RW_CASE(1) RW_CASE(2) RW_CASE(3) RW_CASE(4) RW_CASE(5) RW_CASE(6) RW_CASE(7) RW_CASE(8) RW_CASE(9) RW_CASE(10) RW_CASE(11)
+#undef RW_CASE
+    default: asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
 }
-__device__ __forceinline__ void dt_unpair(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
-__device__ __forceinline__ uint64_t dt_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t dt_add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t dt_mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
+__device__ __forceinline__ void rw_copy(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void rw_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 template <class T, int DO, int STREAM>
 __global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(const DtArgs a) {
   extern __shared__ __align__(16) unsigned char dt_raw[];
   __shared__ float2 s_part[2][DL_MOST_SHARE * STREAM / 32];
   __shared__ int s_any[2];
-  constexpr int VN = RW_VEC<T>, U = DL_U, SPAN = U * STREAM, PARTS = STREAM / 32;
+  constexpr int VN = RW_VEC<T>, PARTS = STREAM / 32, RING = dl_ring(DO), STEP = STREAM * 16;
+  constexpr bool BOTH = DO == (DT_LOSS | DT_GRAD);
   constexpr float LOWEST = -3.0e38f;   // in the place of a maximum of -inf
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, K = a.top, V = a.vocab;
   const bool streams = warp < STREAM / 32;
+  DtEntry* const entries = (DtEntry*)(dt_raw + RING * STEP);
   uint32_t rank, share;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(share));
-  if (DO == DT_LOSS || DO == (DT_LOSS | DT_GRAD))
-    if (share > 1) rw_cluster_sync();   // the others are running
+  if ((DO & DT_LOSS) && share > 1) rw_cluster_sync();   // the others are running
   pdl_begin();
   const long long groups = gridDim.x / share;
   const float c = a.c, factor = DO & DT_GRAD ? dt_factor(a) : 0.f;
-  const uint64_t cc = dt_pair(c, c);
+  const uint64_t cc = rw_pair(c, c);
   double loss_sum = 0.0, weight_sum = 0.0;
-  RwPiece<T, VN> next[U];
-  // A row, and what of it is this CTA's: `pieces` of 16 bytes from body on, elements lo to hi, thread t's element outside of the pieces (or -1)
-  struct Row { const T *s, *body; int at, pieces, lo, hi, edge; };
+  // A row, and what of it is this CTA's: `pieces` of 16 bytes from element `at` on, elements lo to hi; of those pieces t, t + STREAM, ... are thread t's,
+  // `count` of them, from `from` on
+  struct Row { const T* s; const unsigned char* from; int at, pieces, lo, hi, count; };
   auto place = [&](long long row) {
     Row r;
-    r.s = (const T*)a.logits + (row < a.rows ? row : 0) * a.stride;
-    const int head = min(V, (int)((16 - ((uintptr_t)r.s & 15)) & 15) / (int)sizeof(T)), all = (V - head) / VN, tail = head + all * VN;
-    const int per = (all + (int)share - 1) / (int)share, p0 = min((int)rank * per, all);
-    r.pieces = row < a.rows && streams ? min(per, all - p0) : 0;
+    r.s = (const T*)a.logits + row * a.stride;
+    const int head = min(V, (int)((16 - ((uintptr_t)r.s & 15)) & 15) / (int)sizeof(T)), all = (V - head) / VN;
+    const int per = share > 1 ? (all + (int)share - 1) / (int)share : all, p0 = min((int)rank * per, all);
+    r.pieces = min(per, all - p0);
     r.at = head + p0 * VN;
-    r.body = r.s + r.at;
     r.lo = rank == 0 ? 0 : r.at;
-    r.hi = rank == share - 1 ? V : min(r.at + per * VN, tail);
-    r.edge = t < head ? t : tail + t - head < V ? tail + t - head : -1;
-    if (!streams || row >= a.rows || r.edge < r.lo || r.edge >= r.hi) r.edge = -1;
+    r.hi = rank == share - 1 ? V : r.at + r.pieces * VN;
+    r.count = streams && t < r.pieces ? (r.pieces - t + STREAM - 1) / STREAM : 0;
+    r.from = (const unsigned char*)(r.s + r.at) + 16 * t;
     return r;
   };
-  static_assert(2 * (VN - 1) <= STREAM, "a thread per element outside of the pieces");
-  // pieces i, i + STREAM, ...; beyond the last -inf, which adds nothing
-  auto fetch = [&](const T* body, int pieces, int i) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u * STREAM < pieces) next[u].load(body + (long long)(i + u * STREAM) * VN);
-      else next[u].make([](int) { return -CUDART_INF_F; });
+  auto weight_of = [&](long long row) { return a.weights ? a.weights[row] : 1.0f; };
+  // a row of weight 0, or (an earlier call has left 0 there) without a teacher
+  auto pass_over = [&](long long row) {
+    if constexpr (DO & DT_LOSS) {
+      if (t == 0 && rank == 0 && a.row_loss) a.row_loss[row] = 0.f;
+      if (t == 0 && rank == 0 && a.stat) a.stat[row] = make_float2(0.f, 0.f);
     }
-  };
-  Row coming = place(blockIdx.x / share);
-  fetch(coming.body, coming.pieces, t);
-  float weight = a.weights && blockIdx.x / share < a.rows ? a.weights[blockIdx.x / share] : 1.0f;
-  float edge = coming.edge >= 0 ? rw_float(coming.s[coming.edge]) : -CUDART_INF_F;
-  float2 ahead = make_float2(0.f, 0.f);
-  if constexpr (!(DO & DT_LOSS))
-    if (blockIdx.x / share < a.rows) ahead = a.stat[blockIdx.x / share];
-  int buf = 0;
-  for (long long row = blockIdx.x / share; row < a.rows; row += groups) {
-    const Row r = coming;
-    const float w = weight, mine = edge;
-    coming = place(row + groups);
-    edge = coming.edge >= 0 ? rw_float(coming.s[coming.edge]) : -CUDART_INF_F;
-    if (a.weights && row + groups < a.rows) weight = a.weights[row + groups];
-    T* const grad = DO & DT_GRAD ? (T*)a.grad + row * V : nullptr;
-    float2 st = ahead;
-    if constexpr (!(DO & DT_LOSS))
-      if (row + groups < a.rows) ahead = a.stat[row + groups];
-    auto zeros = [&] {
+    if constexpr (DO & DT_GRAD) {
+      const Row r = place(row);
+      T* const grad = (T*)a.grad + row * V;
       if (streams)
         for (int j = r.lo + t; j < r.hi; j += STREAM) grad[j] = rw_to<T>(0.f);
-    };
-    if (w == 0.f || (!(DO & DT_LOSS) && st.y == 0.f)) {   // (a row without a teacher has left 0 there)
-      if constexpr (DO & DT_LOSS) {
-        if (t == 0 && rank == 0 && a.row_loss) a.row_loss[row] = 0.f;
-        if (t == 0 && rank == 0 && a.stat) a.stat[row] = make_float2(0.f, 0.f);
-      }
-      if constexpr (DO & DT_GRAD) zeros();
-      fetch(coming.body, coming.pieces, t);
-      continue;
     }
-    DtEntry* const e = (DtEntry*)dt_raw + buf * K;
+  };
+  // the next row from `row` on that counts, its weight and (of an earlier call) its maximum and sum
+  struct Next { long long row; float w; float2 st; };
+  auto look = [&](long long row) {
+    Next n = {row, 0.f, make_float2(0.f, 1.f)};
+    if (row < a.rows) {
+      n.w = weight_of(row);
+      if constexpr (!(DO & DT_LOSS)) n.st = a.stat[row];
+    }
+    return n;
+  };
+  Next peeked = look(blockIdx.x / share);   // asked for a row ahead
+  auto find = [&] {
+    Next n = peeked;
+    while (n.row < a.rows && (n.w == 0.f || n.st.y == 0.f)) {
+      pass_over(n.row);
+      n = look(n.row + groups);
+    }
+    peeked = look(n.row + groups);
+    return n;
+  };
+  const uint32_t ring = smem_addr(dt_raw) + 16 * t;
+  uint32_t in = 0, out = 0;   // places of the ring, as offsets: where the next copy goes, where the next piece is
+  auto copy = [&](const unsigned char* from) {
+    rw_copy(ring + in, from);
+    in = in == (RING - 1) * STEP ? 0 : in + STEP;
+  };
+  auto take = [&] {
+    RwPiece<T, VN> v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]) : "r"(ring + out) : "memory");
+    out = out == (RING - 1) * STEP ? 0 : out + STEP;
+    return v;
+  };
+  Next now = find(), next = now;
+  Row r = place(now.row < a.rows ? now.row : 0), coming = r;
+  if (now.row >= a.rows) r.count = 0;
+  int on_way = min(RING, r.count);   // this row's pieces that have been asked for
+  for (int i = 0; i < on_way; ++i) { copy(r.from + i * STEP); rw_commit(); }
+  int buf = 0;
+  for (; now.row < a.rows; now = next, r = coming) {
+    const long long row = now.row;
+    next = find();
+    coming = place(next.row < a.rows ? next.row : 0);
+    if (next.row >= a.rows) coming.count = 0;
+    const float w = now.w;
+    float2 st = now.st;
+    DtEntry* const e = entries + buf * K;
+    T* const grad = DO & DT_GRAD ? (T*)a.grad + row * V : nullptr;
     const float f = DO & DT_GRAD ? factor * w * (a.upstream && a.per_row ? a.upstream[row] : 1.0f) : 0.f;
-    // this CTA's pieces, from those that have been fetched on: work(piece, its number); each one's place is taken by the one SPAN further at once,
-    // behind the last ones by those of what comes next
-    auto sweep = [&](const T* then, int then_pieces, auto&& work) {
-      const int blocks = (r.pieces + SPAN - 1) / SPAN;
-      const T* ahead = r.body + (long long)(t + SPAN) * VN;
-      int i = t;
-      for (int k = 2; k < blocks; ++k, i += SPAN, ahead += SPAN * VN)
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const RwPiece<T, VN> v = next[u];
-          next[u].load(ahead + u * STREAM * VN);
-          work(v, i + u * STREAM);
+    // an element before the row's first piece or behind its last
+    const int head = rank == 0 ? r.at : 0, edge = t < head ? t : r.at + r.pieces * VN + t - head;
+    const bool has_edge = streams && (t < head || (rank == share - 1 && edge < V));
+    const float edge_value = has_edge ? rw_float(r.s[edge]) : -CUDART_INF_F;
+    static_assert(2 * (VN - 1) <= STREAM, "a thread per element outside of the pieces");
+    // One pass over the row's pieces, each of which makes room for another: of this row, then of the next.  A piece was asked for `on_way` pieces before.
+    auto sweep = [&](auto&& work) {
+      const int rest = r.count - on_way;
+      const unsigned char* from = r.from + on_way * STEP;
+      if (on_way == RING)
+#pragma unroll 2
+        for (int k = 0; k < rest; ++k, from += STEP) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
+          const RwPiece<T, VN> v = take();
+          work(v);
+          copy(from);
+          rw_commit();
         }
-      if (blocks > 1) {   // the last ones may be fewer
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const RwPiece<T, VN> v = next[u];
-          if (i + SPAN + u * STREAM < r.pieces) next[u].load(ahead + u * STREAM * VN);
-          else next[u].make([](int) { return -CUDART_INF_F; });
-          work(v, i + u * STREAM);
-        }
-        i += SPAN;
+      from = coming.from;
+      const int most = min(on_way, coming.count);
+      for (int k = 0; k < on_way; ++k, from += STEP) {
+        if (on_way == RING) asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
+        else rw_arrived(0);
+        const RwPiece<T, VN> v = take();
+        work(v);
+        if (k < most) copy(from);
+        rw_commit();
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const RwPiece<T, VN> v = next[u];
-        if (t + u * STREAM < then_pieces) next[u].load(then + (long long)(t + u * STREAM) * VN);
-        else next[u].make([](int) { return -CUDART_INF_F; });
-        if (i + u * STREAM < r.pieces) work(v, i + u * STREAM);
+      // a next row that is longer than this one
+      for (int k = most; k < min(RING, coming.count); ++k, from += STEP) {
+        if (k == most) from = coming.from + k * STEP;
+        copy(from);
+        rw_commit();
       }
+      on_way = min(RING, coming.count);
     };
-    // this thread's part of the gradient, from powers relative to m
-    auto gradient = [&](float m, float total) {
+    // a piece of the gradient, from powers relative to m
+    auto gradient = [&](float m, float total, auto&& over) {
       const float g = f * total;
-      const uint64_t gg = dt_pair(g, g), mm = dt_pair(-m, -m);
-      T* const out = grad + r.at;
+      const uint64_t gg = rw_pair(g, g), mm = rw_pair(-m, -m);
+      T* to = grad + r.at + t * VN;
       auto go = [&](auto aligned) {
-        sweep(coming.body, coming.pieces, [&](const RwPiece<T, VN>& v, int i) {
+        over([&](const RwPiece<T, VN>& v) {
           float x[VN];
 #pragma unroll
           for (int j = 0; j < VN; j += 2) {
-            dt_unpair(dt_fma2(dt_pair(v.at(j), v.at(j + 1)), cc, mm), x[j], x[j + 1]);
-            dt_unpair(dt_mul2(gg, dt_pair(dt_exp2(x[j]), dt_exp2(x[j + 1]))), x[j], x[j + 1]);
+            rw_unpair(rw_fma2(v.two(j), cc, mm), x[j], x[j + 1]);
+            rw_unpair(rw_mul2(gg, rw_pair(dt_exp2(x[j]), dt_exp2(x[j + 1]))), x[j], x[j + 1]);
           }
           RwPiece<T, VN> o;
           o.make([&](int j) { return x[j]; });
-          T* const to = out + (long long)i * VN;
           if constexpr (decltype(aligned)::value) o.store(to);
           else
 #pragma unroll
             for (int j = 0; j < VN; ++j) to[j] = o.one(j);
+          to += STREAM * VN;
         });
       };
-      if (((uintptr_t)out & 15) == 0) go(std::true_type());
+      if (((uintptr_t)(grad + r.at) & 15) == 0) go(std::true_type());
       else go(std::false_type());
-      if (r.edge >= 0) grad[r.edge] = rw_to<T>(g * dt_exp2(fmaf(mine, c, -m)));
+      if (has_edge) grad[edge] = rw_to<T>(g * dt_exp2(fmaf(edge_value, c, -m)));
     };
     if (!streams) {
-      const bool any = dt_teacher(a, row, e, (int*)((DtEntry*)dt_raw + 2 * K));
+      const bool any = dt_teacher(a, row, e, (int*)(entries + 2 * K));
       if (lane == 0) s_any[buf] = any;
     } else if constexpr (DO & DT_LOSS) {
-      float m = LOWEST, total = 0.f;   // scaled maximum; sum of powers relative to it
-      uint64_t mm = dt_pair(-m, -m), sum = dt_pair(0.f, 0.f);
+      float m = LOWEST;   // scaled maximum
+      uint64_t mm = rw_pair(-m, -m), sum = rw_pair(0.f, 0.f);   // sums of powers relative to it
       auto raise = [&](float to) {
         const float by = dt_exp2(m - to);
-        sum = dt_mul2(sum, dt_pair(by, by));
+        sum = rw_mul2(sum, rw_pair(by, by));
         m = to;
-        mm = dt_pair(-m, -m);
+        mm = rw_pair(-m, -m);
       };
-      const bool again = DO & DT_GRAD;
-      sweep(again ? r.body : coming.body, again ? r.pieces : coming.pieces, [&](const RwPiece<T, VN>& v, int) {
+      auto add = [&](const RwPiece<T, VN>& v) {
         const float most = rw_most(v) * c;
         if (most > m) raise(most);
 #pragma unroll
         for (int j = 0; j < VN; j += 2) {
           float x, y;
-          dt_unpair(dt_fma2(dt_pair(v.at(j), v.at(j + 1)), cc, mm), x, y);
-          sum = dt_add2(sum, dt_pair(dt_exp2(x), dt_exp2(y)));
+          rw_unpair(rw_fma2(v.two(j), cc, mm), x, y);
+          sum = rw_add2(sum, rw_pair(dt_exp2(x), dt_exp2(y)));
         }
-      });
-      if (r.edge >= 0) {
-        if (mine * c > m) raise(mine * c);
-        sum = dt_add2(sum, dt_pair(dt_exp2(fmaf(mine, c, -m)), 0.f));
+      };
+      if constexpr (!BOTH) sweep(add);
+      else {
+        // the rest of the row, and as much of the next as there is room for (on_way: of the next from here on)
+        const uint32_t first = out;
+        for (int k = on_way; k < r.count; ++k) { copy(r.from + k * STEP); rw_commit(); }
+        on_way = min(RING - r.count, coming.count);
+        for (int k = 0; k < RING - r.count; ++k) {
+          if (k < on_way) copy(coming.from + k * STEP);
+          rw_commit();
+        }
+        for (int k = 0; k < r.count; ++k) {
+          rw_arrived(RING - 1 - k);
+          add(take());
+        }
+        out = first;
       }
-      float other;
-      dt_unpair(sum, total, other);
-      total += other;
-      const float all = rw_warp_max(m);
-      total = rw_warp_sum(total * dt_exp2(m - all));
+      if (has_edge) {
+        if (edge_value * c > m) raise(edge_value * c);
+        sum = rw_add2(sum, rw_pair(dt_exp2(fmaf(edge_value, c, -m)), 0.f));
+      }
+      const float all = rw_warp_max(m), total = rw_warp_sum(rw_both(sum) * dt_exp2(m - all));
       if (lane < (int)share) {
         const uint32_t to = rw_at_rank(&s_part[buf][rank * PARTS + warp], lane);
         asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(all), "f"(total) : "memory");
       }
     }
     if constexpr (!(DO & DT_LOSS))
-      if (streams) gradient(st.x, st.y);
+      if (streams) gradient(st.x, st.y, sweep);
     if ((DO & DT_LOSS) && share > 1) rw_cluster_sync();
     else __syncthreads();
     if constexpr (DO == DT_LOSS)
@@ -822,11 +1003,21 @@ __global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(c
             weight_sum += any ? w : 0.f;
           }
         }
-      } else if constexpr (DO & DT_GRAD) {
-        if (any) gradient(st.x, st.y);
+      } else if constexpr (BOTH) {
+        // the second pass: each piece makes room for one of the next row
+        auto again = [&](auto&& work) {
+          const int from = on_way;
+          on_way = min(from + r.count, coming.count);
+          for (int k = 0; k < r.count; ++k) {
+            work(take());
+            if (from + k < on_way) copy(coming.from + (from + k) * STEP);
+            rw_commit();
+          }
+        };
+        if (any) gradient(st.x, st.y, again);
         else {
-          zeros();
-          fetch(coming.body, coming.pieces, t);
+          again([](const RwPiece<T, VN>&) {});
+          for (int j = r.lo + t; j < r.hi; j += STREAM) grad[j] = rw_to<T>(0.f);
         }
         asm volatile("bar.sync 1, %0;" ::"n"(STREAM) : "memory");   // the streaming warps
         if (any) dt_columns(a, r.s, grad, e, f, st.y, st.x, t, STREAM, r.lo, r.hi);
@@ -836,6 +1027,7 @@ __global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(c
     }
     buf ^= 1;
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   if constexpr (DO & DT_LOSS)
     if (t == STREAM && rank == 0) a.part[blockIdx.x / share] = make_double2(loss_sum, weight_sum);
 }
@@ -878,29 +1070,35 @@ __global__ void __launch_bounds__(NT) k_distill_total(const double2* __restrict_
 }
 
 // Rows' groups of a call, one CTA or a cluster each, which is also the number of its partial sums
-// A call's form.  Threads that stream through a long row: few for short ones, so that more rows' latencies lie side by side, many for long ones, so
-// that (loss and gradient) the rows being worked on stay in the L2 cache between their two passes.  share: CTAs that share a row, until all have work.
-struct DtForm { int stream, share, ctas; };
-static DtForm dt_form(long long rows, int vocab, int type_bytes) {
-  if (vocab <= DT_WARP_VOCAB) {
-    const long long n = (rows + DT_WARP_THREADS / 32 - 1) / (DT_WARP_THREADS / 32), most = (long long)sm_count() * 8;
-    return {0, 1, (int)(n < most ? n : most)};
-  }
+// A call's form.  Threads that stream through a long row: few for short ones, so that more rows' latencies lie side by side.  share: CTAs that share a
+// row, until all have work, or (loss and gradient) until DL_KEPT pieces of a thread are its part of the row.
+struct DtForm { int stream, share; bool fits; };   // fits: into the rings
+static DtForm dt_form(long long rows, int vocab, int type_bytes, bool both) {
+  if (vocab <= DT_WARP_VOCAB) return {0, 1, true};
   const long long bytes = (long long)vocab * type_bytes;
-  const int stream = bytes <= 16384 ? 128 : bytes <= 131072 ? 256 : 512;
+  const int stream = bytes <= 16384 ? 128 : bytes <= (both ? 32768 : 131072) ? 256 : 512;
   const long long most = (long long)sm_count() * dl_ctas(stream);
   int share = 1;
-  while (share < DL_MOST_SHARE && bytes >= share * 2 * 16384 && rows * share * 2 <= most) share *= 2;
-  return {stream, share, (int)(rows < most / share ? rows : most / share)};
+  while (share < DL_MOST_SHARE && ((bytes >= share * 2 * 16384 && rows * share * 2 <= most) || (both && bytes > (long long)share * stream * 16 * DL_KEPT))) share *= 2;
+  return {stream, share, bytes <= (long long)share * stream * 16 * dl_ring(DT_LOSS | DT_GRAD)};
 }
+#define DT_FITS_ANYWAY 196608   // classes of any type, DL_MOST_SHARE rings of 12 pieces of 512 threads
 static int dt_weight_ctas(long long rows) { return (int)(rows < 64 * NT ? (rows + NT - 1) / NT : 64); }
+// Launches one pass; *groups: CTAs or clusters that begin with different rows, which is also the number of partial sums
 template <class T, int DO>
-static int dt_run(const DtArgs& a, const DtForm& form, cudaStream_t s) {
+static int dt_run(const DtArgs& a, const DtForm& form, int* groups, cudaStream_t s) {
   const size_t slots = (size_t)4 * dt_slots(a.top), entries = sizeof(DtEntry) * a.top;
-#define DT_LONG(STREAM)                                                                                                    \
-  {                                                                                                                        \
-    launch_clusters(k_distill_long<T, DO, STREAM>, form.ctas * form.share, STREAM + 32, form.share, 2 * entries + slots, s, a); \
-    return launch_status();                                                                                                \
+#define DT_LONG(STREAM)                                                                                                              \
+  {                                                                                                                                  \
+    constexpr int RING = dl_ring(DO) * STREAM * 16;                                                                                  \
+    const size_t smem = RING + 2 * entries + slots;                                                                                  \
+    static bool configured[PYLO_MAX_DEVICES] = {};                                                                                   \
+    if (int rc = allow_dynamic_smem(k_distill_long<T, DO, STREAM>, RING + (int)sizeof(DtEntry) * 2 * DT_MOST_K + 4 * dt_slots(DT_MOST_K), configured)) return rc; \
+    const long long most = form.share > 1 ? active_clusters<k_distill_long<T, DO, STREAM>>(STREAM + 32, form.share, smem)            \
+                                          : (long long)sm_count() * dl_ctas(STREAM);                                                 \
+    *groups = (int)(a.rows < most ? a.rows : most);                                                                                  \
+    launch_clusters(k_distill_long<T, DO, STREAM>, *groups * form.share, STREAM + 32, form.share, smem, s, a);                       \
+    return launch_status();                                                                                                          \
   }
   if (form.stream == 128) DT_LONG(128)
   if (form.stream == 256) DT_LONG(256)
@@ -910,12 +1108,14 @@ static int dt_run(const DtArgs& a, const DtForm& form, cudaStream_t s) {
   static bool configured[PYLO_MAX_DEVICES] = {};
   if (smem > 48 * 1024)
     if (int rc = allow_dynamic_smem(k_distill_short<T, DO>, (int)(DT_WARP_THREADS / 32 * (sizeof(DtEntry) * DT_MOST_K + 4 * dt_slots(DT_MOST_K))), configured)) return rc;
-  launch(k_distill_short<T, DO>, form.ctas, DT_WARP_THREADS, smem, s, a);
+  const long long n = (a.rows + DT_WARP_THREADS / 32 - 1) / (DT_WARP_THREADS / 32), most = (long long)sm_count() * DT_MOST_CTAS;
+  *groups = (int)(n < most ? n : most);
+  launch(k_distill_short<T, DO>, *groups, DT_WARP_THREADS, smem, s, a);
   return launch_status();
 }
 template <int DO>
-static int dt_any_type(const DtArgs& a, int type, const DtForm& form, cudaStream_t s) {
-  return type == PYLO_FP32 ? dt_run<float, DO>(a, form, s) : type == PYLO_BF16 ? dt_run<__nv_bfloat16, DO>(a, form, s) : dt_run<__half, DO>(a, form, s);
+static int dt_any_type(const DtArgs& a, int type, const DtForm& form, int* groups, cudaStream_t s) {
+  return type == PYLO_FP32 ? dt_run<float, DO>(a, form, groups, s) : type == PYLO_BF16 ? dt_run<__nv_bfloat16, DO>(a, form, groups, s) : dt_run<__half, DO>(a, form, groups, s);
 }
 static bool dt_good(const pylo_distill* d) {
   return d && d->rows >= 0 && d->rows <= (1ll << 40) && d->vocab > 0 && d->vocab <= (1 << 30) && d->top > 0 && d->top <= DT_MOST_K && rw_type(d->type) &&
@@ -935,7 +1135,8 @@ extern "C" {
 
 int64_t pylo_b200_layer_norm_workspace(int64_t rows, int width) {
   if (rows <= 0 || width <= 0 || width > LN_MOST) return 0;
-  return (int64_t)ln_ctas(rows, width, LN_BACKWARD) * 2 * width;
+  const int a = ln_form(rows, width, false, true).groups, b = ln_form(rows, width, true, true).groups;
+  return (int64_t)(a > b ? a : b) * 2 * width;
 }
 
 int pylo_b200_layer_norm(const pylo_norm* n, void* stream) {
@@ -945,37 +1146,43 @@ int pylo_b200_layer_norm(const pylo_norm* n, void* stream) {
   LnArgs a = {};
   a.x = n->x; a.weight = n->weight; a.bias = n->bias; a.y = n->y; a.mean = n->mean; a.rstd = n->rstd;
   a.rows = n->rows; a.x_stride = n->x_stride; a.width = n->width; a.eps = n->eps;
-  return ln_any(a, n->type, n->weight_type, false, (cudaStream_t)stream);
+  return ln_any(a, n->type, n->weight_type, ln_aligned(n, false), false, (cudaStream_t)stream);
 }
 
 int pylo_b200_layer_norm_backward(const pylo_norm* n, void* stream) {
   CHECK_ARG(n && n->rows >= 0 && n->width > 0 && n->width <= LN_MOST && rw_type(n->type));
   cudaStream_t s = (cudaStream_t)stream;
-  const bool columns = n->dweight || n->dbias;
-  const int ctas = n->rows ? ln_ctas(n->rows, n->width, LN_BACKWARD) : 0;
-  CHECK_ARG(!columns || ctas == 0 || (n->work && n->work_floats >= (int64_t)ctas * 2 * n->width));
-  if (ctas) {
+  const bool columns = n->dweight || n->dbias, aligned = ln_aligned(n, true);
+  const int groups = n->rows ? ln_form(n->rows, n->width, aligned && n->type != PYLO_FP32, true).groups : 0;
+  CHECK_ARG(!columns || groups == 0 || (n->work && n->work_floats >= (int64_t)groups * 2 * n->width));
+  if (groups) {
     CHECK_ARG(n->x && n->dy && n->mean && n->rstd && n->x_stride >= 0 && n->dy_stride >= 0);
     LnArgs a = {};
     a.x = n->x; a.dy = n->dy; a.weight = n->weight; a.y = n->dx; a.mean = n->mean; a.rstd = n->rstd; a.part = columns ? n->work : nullptr;
     a.rows = n->rows; a.x_stride = n->x_stride; a.dy_stride = n->dy_stride; a.width = n->width;
     if (n->dx || columns)
-      if (int rc = ln_any(a, n->type, n->weight_type, true, s)) return rc;
+      if (int rc = ln_any(a, n->type, n->weight_type, aligned, true, s)) return rc;
   }
   if (columns) {
     const dim3 grid((n->width + 31) / 32, n->dbias ? 2 : 1);
-    if (n->weight_type == PYLO_FP32) launch(k_layer_norm_columns<float>, grid, NT, 0, s, n->work, ctas, n->width, (float*)n->dweight, (float*)n->dbias);
-    else if (n->weight_type == PYLO_BF16) launch(k_layer_norm_columns<__nv_bfloat16>, grid, NT, 0, s, n->work, ctas, n->width, (__nv_bfloat16*)n->dweight, (__nv_bfloat16*)n->dbias);
-    else if (n->weight_type == PYLO_FP16) launch(k_layer_norm_columns<__half>, grid, NT, 0, s, n->work, ctas, n->width, (__half*)n->dweight, (__half*)n->dbias);
+#define LN_COLUMNS(W) launch(k_layer_norm_columns<W>, grid, 32 * LN_COLUMN_GROUPS, 0, s, n->work, groups, n->width, (W*)n->dweight, (W*)n->dbias)
+    if (n->weight_type == PYLO_FP32) LN_COLUMNS(float);
+    else if (n->weight_type == PYLO_BF16) LN_COLUMNS(__nv_bfloat16);
+    else if (n->weight_type == PYLO_FP16) LN_COLUMNS(__half);
     else return -1;
+#undef LN_COLUMNS
   }
   return launch_status();
 }
 
+// [partial sums of loss and weights][parts of the weights][a row's maximum and sum, where loss and gradient take two launches]
+static int64_t dt_part_bytes(int64_t rows) {
+  const int64_t most = (int64_t)sm_count() * DT_MOST_CTAS;
+  return 16 * (rows < most ? rows : most);
+}
 int64_t pylo_b200_distill_workspace(int64_t rows, int vocab) {
   if (rows <= 0 || vocab <= 0) return 16;
-  const long long most = (long long)sm_count() * 8;   // groups of rows of whatever form
-  return 16 * (int64_t)(rows < most ? rows : most) + 8 * (int64_t)dt_weight_ctas(rows);
+  return dt_part_bytes(rows) + 8 * (int64_t)dt_weight_ctas(rows) + (vocab > DT_FITS_ANYWAY ? 8 * rows : 0);
 }
 
 int pylo_b200_distill(const pylo_distill* d, int what, void* stream) {
@@ -986,21 +1193,29 @@ int pylo_b200_distill(const pylo_distill* d, int what, void* stream) {
   CHECK_ARG(!grad || d->rows == 0 || (d->grad && (uintptr_t)d->grad % rw_bytes(d->type) == 0));
   CHECK_ARG(!grad || loss || d->rows == 0 || (d->stat && (!mean || d->inv)));
   DtArgs a = dt_args(d);
-  const DtForm form = d->rows ? dt_form(d->rows, d->vocab, (int)rw_bytes(d->type)) : DtForm{};
+  int groups = 0;
   if (d->rows) {
+    const DtForm form = dt_form(d->rows, d->vocab, (int)rw_bytes(d->type), loss && grad);
     a.part = (double2*)d->work;
     if (grad) a.scale = d->scale;
     if (grad && mean && loss) {
-      double* const sums = (double*)((char*)d->work + 16 * (size_t)form.ctas);
+      double* const sums = (double*)((char*)d->work + dt_part_bytes(d->rows));
       a.weight_sums = sums;
       a.n_sums = dt_weight_ctas(d->rows);
       launch(k_distill_weights, a.n_sums, NT, 0, s, a, sums);
     } else if (grad && mean) a.inv = d->inv;
-    const int rc = !grad ? dt_any_type<DT_LOSS>(a, d->type, form, s) : loss ? dt_any_type<DT_LOSS | DT_GRAD>(a, d->type, form, s) : dt_any_type<DT_GRAD>(a, d->type, form, s);
+    int rc;
+    if (loss && grad && form.fits) rc = dt_any_type<DT_LOSS | DT_GRAD>(a, d->type, form, &groups, s);
+    else {
+      if (loss && grad && !a.stat) a.stat = (float2*)((char*)d->work + dt_part_bytes(d->rows) + 8 * (int64_t)dt_weight_ctas(d->rows));
+      rc = loss ? dt_any_type<DT_LOSS>(a, d->type, form, &groups, s) : 0;
+      int unused;
+      if (grad && !rc) rc = dt_any_type<DT_GRAD>(a, d->type, form, &unused, s);
+    }
     if (rc) return rc;
   }
   if (loss && d->reduction != PYLO_REDUCE_NONE)
-    launch(k_distill_total, 1, NT, 0, s, (const double2*)d->work, form.ctas, (int)mean, 1.0f, d->loss, d->inv);
+    launch(k_distill_total, 1, NT, 0, s, (const double2*)d->work, groups, (int)mean, 1.0f, d->loss, d->inv);
   return launch_status();
 }
 

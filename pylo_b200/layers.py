@@ -147,7 +147,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     """Layer norm over the last dimension: ``(x - mean) / sqrt(variance + eps) * weight + bias``, of ``x``'s type.
 
     ``weight`` and ``bias`` are vectors of ``x``'s type or fp32, and their gradients are of that type; a bias needs a weight beside it.  Means,
-    variances and the sums of the gradients are fp32, each result is rounded once.  Rows of up to 32768 elements, of any stride."""
+    variances and the sums of the gradients are fp32, each result is rounded once.  Rows of up to 16384 elements, of any stride."""
     _check("x", x)
     dim, device, dtype = x.dim(), x.get_device(), x.dtype
     width = x.shape[-1] if dim else 0

@@ -90,8 +90,8 @@ def check_norm(x, weight=None, bias=None, dy=None, eps=1e-5):
         near(got, *want[name], name)
 
 
-SHAPES = [(1, 1), (3, 7), (5, 8), (2, 128), (7, 129), (300, 33), (33, 1000), (9, 1001), (130, 256), (9, 1024), (6, 1025), (700, 768), (11, 4096), (5, 8192), (3, 8200), (2, 20001),
-          (2, 32768)]
+SHAPES = [(1, 1), (3, 7), (5, 8), (2, 128), (7, 129), (300, 33), (33, 1000), (9, 1001), (130, 256), (9, 1024), (6, 1025), (700, 768), (11, 4096), (5, 8192), (3, 8200), (2, 12001),
+          (2, 16384), (500, 2050), (200, 5001)]
 
 
 @gpu
@@ -400,7 +400,7 @@ def distill_inputs(rows, vocab, top, dtype, seed=0):
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, FP16])
 @pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (4, 2, 1), (256, 10, 10), (5, 7, 3), (37, 100, 100), (9, 1000, 17), (3, 1024, 64), (6, 1025, 64), (5, 5003, 128), (4, 32768, 1024),
-                                            (3, 50257, 64), (2, 128256, 128)])
+                                            (3, 50257, 64), (2, 128256, 128), (2, 400001, 16), (700, 2500, 7)])
 def test_distill(rows, vocab, top, dtype):
     logits, teacher, ids = distill_inputs(rows, vocab, top, dtype)
     check_distill(logits, teacher, ids, T=2.0, upstream=0.5)
