@@ -611,11 +611,9 @@ typedef struct pylo_distill {
   const float* weights;          /* [rows], or NULL: 1 */
   float* loss;                   /* out [1] (SUM, MEAN) */
   float* row_loss;               /* out [rows], or NULL */
-  float* stat;                   /* [rows][2]: written with the loss unless NULL, read for a gradient alone */
-  float* inv;                    /* [1]: 1 / sum of the weights; written with the loss unless NULL, read for a gradient alone (MEAN) */
   void* grad;                    /* out [rows][vocab], contiguous, of the logits' type */
   const float* upstream;         /* gradient of the loss: [1], or (NONE) [rows]; NULL: 1 */
-  void* work;                    /* with the loss; 16-byte aligned */
+  void* work;                    /* 16-byte aligned; a gradient alone reads what the call that made the loss of the same arguments has left there */
   int64_t work_bytes, rows, stride;
   int32_t vocab, top, type, teacher_type;   /* top up to 1024 */
   int32_t ids_bytes;             /* 4 or 8 */
@@ -623,9 +621,9 @@ typedef struct pylo_distill {
   float temperature;             /* > 0 */
   float scale;                   /* another factor of the gradient */
 } pylo_distill;
-/* what: PYLO_DISTILL_LOSS, or PYLO_DISTILL_GRAD from an earlier call's stat and inv, or both at once. */
+/* what: PYLO_DISTILL_LOSS, or PYLO_DISTILL_GRAD after it, or both at once. */
 int pylo_b200_distill(const pylo_distill* d, int what, void* stream);
-int64_t pylo_b200_distill_workspace(int64_t rows, int vocab);
+int64_t pylo_b200_distill_workspace(int64_t rows, int vocab, int top);
 
 /* The gated feed-forward block: h = act(x w_gate^T) * (x w_up^T), y = h w_down^T, with its gradients.  PYLO_BF16 or PYLO_FP16 throughout,
  * products on the tensor cores with fp32 sums.  Matrices are row-major with rows ld elements apart; operands (x, dy and the weights) begin

@@ -140,7 +140,7 @@ class Norm(C.Structure):
 
 class Distill(C.Structure):
     """pylo_distill: the loss against a teacher's largest logits, and its gradient."""
-    _fields_ = [(name, C.c_void_p) for name in ("logits", "teacher", "ids", "weights", "loss", "row_loss", "stat", "inv", "grad", "upstream", "work")] + [
+    _fields_ = [(name, C.c_void_p) for name in ("logits", "teacher", "ids", "weights", "loss", "row_loss", "grad", "upstream", "work")] + [
         (name, C.c_int64) for name in ("work_bytes", "rows", "stride")] + [
         (name, C.c_int32) for name in ("vocab", "top", "type", "teacher_type", "ids_bytes", "reduction")] + [
         ("temperature", C.c_float), ("scale", C.c_float)]
@@ -217,7 +217,7 @@ def _load():
         "pylo_b200_layer_norm_backward": [C.POINTER(Norm), vp],
         "pylo_b200_layer_norm_workspace": [C.c_int64, i32],
         "pylo_b200_distill": [C.POINTER(Distill), i32, vp],
-        "pylo_b200_distill_workspace": [C.c_int64, i32],
+        "pylo_b200_distill_workspace": [C.c_int64, i32, i32],
         "pylo_b200_gated_ffn": [C.POINTER(Ffn), vp],
         "pylo_b200_gated_ffn_backward": [C.POINTER(Ffn), vp],
         "pylo_b200_gated_ffn_kept": [C.c_int64, i32, i32],

@@ -520,11 +520,14 @@ struct DtArgs {
   const float* weights;     // [rows] or NULL
   float* row_loss;          // [rows]: weight * loss, or NULL
   float2* stat;             // [rows]: maximum (scaled), 1 / sum of powers; written with the loss, read for a gradient alone; or NULL
-  double2* part;            // [CTAs]: sums of weight * loss, of weights
+  double2* part;            // [CTAs or clusters]: sums of weight * loss, of weights
   void* grad;               // [rows][vocab]
   const float* upstream;    // of the loss: a scalar, or (per_row) [rows]; NULL: 1
   const float* inv;         // scalar: 1 / sum of the weights; NULL: 1, or
   const double* weight_sums;// [n_sums]: its parts
+  // of long rows, what their teachers come to (k_distill_teachers)
+  float4* teachers;         // [rows]: weight (0 where no entry counts), sum of p (log2 p - scaled logit), sum of p
+  int2* columns;            // [rows][top]: a class that an entry gives (the first of several; else -1), the bits of its probability; or NULL
   long long rows, stride;
   int vocab, top, teacher_type, wide_ids, n_sums, per_row;
   float c, temperature, scale;   // log2(e) / T, T, another factor of the gradient
@@ -565,27 +568,48 @@ static __host__ __device__ __forceinline__ int dt_slots(int top) {   // of the t
   while (n < 2 * top) n *= 2;
   return n;
 }
+// A warp's next 128 entries of a row, as they are in memory: asked for together, and ahead of their use
+struct DtPeek { int id[4]; float t[4]; };
+__device__ __forceinline__ DtPeek dt_peek(const DtArgs& a, long long row, int first) {
+  DtPeek p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int k = first + 32 * i + (threadIdx.x & 31);
+    p.id[i] = -1;
+    p.t[i] = 0.f;
+    if (k < a.top && row < a.rows) {
+      p.id[i] = dt_id(a, row * a.top + k);
+      p.t[i] = dt_any(a.teacher, a.teacher_type, row * a.top + k);
+    }
+  }
+  return p;
+}
 // A row's K entries, by a warp; slots: dt_slots(K) words.  False if there are none
-__device__ __forceinline__ bool dt_teacher(const DtArgs& a, long long row, DtEntry* e, int* slots) {
+__device__ __forceinline__ bool dt_teacher(const DtArgs& a, long long row, DtPeek peek, DtEntry* e, int* slots) {
   const int lane = threadIdx.x & 31, K = a.top, n = dt_slots(K);
   float most = -CUDART_INF_F, sum = 0.f;
   bool any = false;
   for (int i = lane; i < n; i += 32) slots[i] = -1;
   __syncwarp();
   bool twice = false;   // a class that has an entry already
-  for (int k = lane; k < K; k += 32) {
-    const int id = dt_id(a, row * K + k);
-    const float z = id >= 0 ? dt_any(a.teacher, a.teacher_type, row * K + k) * a.c : -CUDART_INF_F;
-    e[k].id = id >= 0 ? id : DT_PADDING;
-    e[k].lp = z;
-    most = fmaxf(most, z);
-    any |= !(z == -CUDART_INF_F);
-    if (id >= 0)
-      for (unsigned at = (unsigned)id * 2654435761u;; ++at) {   // ends: half of the slots stay free
-        const int found = atomicCAS(&slots[(at ^ at >> 16) & (n - 1)], -1, id);
-        twice |= found == id;
-        if (found == -1 || found == id) break;
-      }
+  for (int first = 0; first < K; first += 128) {
+    if (first) peek = dt_peek(a, row, first);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = first + 32 * i + lane, id = peek.id[i];
+      if (k >= K) break;
+      const float z = id >= 0 ? peek.t[i] * a.c : -CUDART_INF_F;
+      e[k].id = id >= 0 ? id : DT_PADDING;
+      e[k].lp = z;
+      most = fmaxf(most, z);
+      any |= !(z == -CUDART_INF_F);
+      if (id >= 0)
+        for (unsigned at = (unsigned)id * 2654435761u;; ++at) {   // ends: half of the slots stay free
+          const int found = atomicCAS(&slots[(at ^ at >> 16) & (n - 1)], -1, id);
+          twice |= found == id;
+          if (found == -1 || found == id) break;
+        }
+    }
   }
   if (!__any_sync(0xffffffffu, any)) return false;
   twice = __any_sync(0xffffffffu, twice);
@@ -618,19 +642,25 @@ __device__ __forceinline__ bool dt_teacher(const DtArgs& a, long long row, DtEnt
 template <class T>
 __device__ __forceinline__ float dt_cross(const DtArgs& a, const T* s, const DtEntry* e, float m) {
   float sum = 0.f;
-  for (int k = threadIdx.x & 31; k < a.top; k += 32) {
-    const DtEntry q = e[k];
-    if (!(q.p == 0.f)) sum = fmaf(q.p, q.lp - fmaf(rw_float(s[q.id < 0 ? ~q.id : q.id]), a.c, -m), sum);
+  for (int first = threadIdx.x & 31; first < a.top; first += 128) {
+    DtEntry q[4];
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      q[i].p = v[i] = 0.f;
+      if (first + 32 * i < a.top) q[i] = e[first + 32 * i];
+      if (!(q[i].p == 0.f)) v[i] = rw_float(s[q[i].id < 0 ? ~q[i].id : q[i].id]);   // all four on their way together
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!(q[i].p == 0.f)) sum = fmaf(q[i].p, q[i].lp - fmaf(v[i], a.c, -m), sum);
   }
   return rw_warp_sum(sum);
 }
-// The columns of the teacher's entries among lo to hi, once more
+// The column of a teacher's entry, once more
 template <class T>
-__device__ __forceinline__ void dt_columns(const DtArgs& a, const T* s, T* grad, const DtEntry* e, float f, float total, float m, int t, int threads, int lo, int hi) {
-  for (int k = t; k < a.top; k += threads) {
-    const DtEntry q = e[k];
-    if (q.id >= lo && q.id < hi) grad[q.id] = rw_to<T>(f * (total * dt_exp2(fmaf(rw_float(s[q.id]), a.c, -m)) - q.column));
-  }
+__device__ __forceinline__ void dt_column(T* grad, int id, float p, float logit, float f, float total, float m, float c) {
+  grad[id] = rw_to<T>(f * (total * dt_exp2(fmaf(logit, c, -m)) - p));
 }
 
 // Where a row's 16-byte pieces lie, and the element before or behind them that is thread t's
@@ -662,7 +692,7 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs 
   double loss_sum = 0.0, weight_sum = 0.0;
   for (long long row = (long long)blockIdx.x * GROUPS + group; row < a.rows; row += (long long)gridDim.x * GROUPS) {
     const float weight = a.weights ? a.weights[row] : 1.0f;
-    const bool any = weight != 0.f && dt_teacher(a, row, e, slots);
+    const bool any = weight != 0.f && dt_teacher(a, row, dt_peek(a, row, 0), e, slots);
     T* const grad = DO & DT_GRAD ? (T*)a.grad + row * V : nullptr;
     if (!any) {
       if constexpr (DO & DT_LOSS) {
@@ -723,7 +753,8 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs 
       const float f = factor * weight * (a.upstream && a.per_row ? a.upstream[row] : 1.0f), g = f * total;
       for (int i = t; i < V; i += 32) grad[i] = rw_to<T>(g * dt_exp2(fmaf(rw_float(r.s[i]), a.c, -m)));
       __syncwarp();   // behind it, the columns of the teacher's entries are written again
-      dt_columns(a, r.s, grad, e, f, total, m, t, 32, 0, V);
+      for (int k = t; k < a.top; k += 32)
+        if (e[k].id >= 0) dt_column(grad, e[k].id, e[k].column, rw_float(r.s[e[k].id]), f, total, m, a.c);
     }
     __syncwarp();   // the next row's teacher takes the place of this one's
   }
@@ -738,22 +769,57 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs 
   }
 }
 
-// Long rows: a CTA each, or a cluster's, each CTA with its part of the row.  STREAM threads go through the logits; each has a ring of pieces of 16 bytes
-// of its own in shared memory, which it fills by asynchronous copies and alone reads, so that what is on its way takes neither registers nor barriers, and
-// the next row's first pieces come behind this row's last.  In the call that makes loss and gradient a row's pieces stay in the ring between the two
-// passes (dt_form sees to it that they fit).  One more warp has the teacher's entries and the row's loss, so that nothing of the stream waits for them.
-// One barrier per row and pass: what the warps leave for one another lies in two buffers that take turns.
+// What the teachers of long rows come to, a warp for each row, before the rows themselves: in the kernel that streams through the logits a warp that did
+// this beside the stream was what the stream waited for (4096 x 128256 bf16 with 128 entries, loss and gradient: 733 us, 494 without it).
+template <class T>
+__global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_teachers(const DtArgs a, double* weight_sums) {
+  pdl_begin();
+  extern __shared__ __align__(16) unsigned char dt_raw[];
+  __shared__ double s_sums[DT_WARP_THREADS / 32];
+  constexpr int GROUPS = DT_WARP_THREADS / 32;
+  const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+  DtEntry* const e = (DtEntry*)dt_raw + group * a.top;
+  int* const slots = (int*)((DtEntry*)dt_raw + GROUPS * a.top) + group * dt_slots(a.top);
+  double weight_sum = 0.0;
+  for (long long row = (long long)blockIdx.x * GROUPS + group; row < a.rows; row += (long long)gridDim.x * GROUPS) {
+    const float weight = a.weights ? a.weights[row] : 1.0f;
+    const bool any = weight != 0.f && dt_teacher(a, row, dt_peek(a, row, 0), e, slots);
+    if (any) {
+      const float cross = dt_cross(a, (const T*)a.logits + row * a.stride, e, 0.f);
+      float sum = 0.f;
+      for (int k = lane; k < a.top; k += 32) sum += e[k].p;
+      sum = rw_warp_sum(sum);
+      if (a.columns)
+        for (int k = lane; k < a.top; k += 32) a.columns[row * a.top + k] = make_int2(e[k].id < 0 ? -1 : e[k].id, __float_as_int(e[k].column));
+      if (lane == 0) a.teachers[row] = make_float4(weight, cross, sum, 0.f);
+      weight_sum += weight;
+    } else if (lane == 0) a.teachers[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+    __syncwarp();
+  }
+  if (lane == 0) s_sums[group] = weight_sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int g = 1; g < GROUPS; ++g) weight_sum += s_sums[g];
+    weight_sums[blockIdx.x] = weight_sum;
+  }
+}
+
+// Long rows: a CTA each, or a cluster's, each CTA with its part of the row.  Each thread has a ring of pieces of 16 bytes of its own in shared memory,
+// which it fills by asynchronous copies and alone reads, so that what is on its way takes neither registers nor barriers, and the next row's first pieces
+// come behind this row's last.  In the call that makes loss and gradient a row's pieces stay in the ring between the two passes (dt_form sees to it that
+// they fit).  What the warps leave for one another lies in two buffers that take turns.
 //
 // A cluster shares a row where there are too few rows for all CTAs, and where a row would not fit the ring.
 #define DL_MOST_SHARE 8
-#define DL_KEPT 8   // pieces of a row that stay in the ring of 12
-__host__ __device__ constexpr int dl_ctas(int stream) { return stream == 128 ? 7 : stream == 256 ? 4 : 2; }   // of an SM
-__host__ __device__ constexpr int dl_ring(int what) { return what == (DT_LOSS | DT_GRAD) ? 12 : 8; }
+#define DL_KEPT 16   // pieces of a row that stay in the ring of 24
+__host__ __device__ constexpr int dl_ring(int what) { return what == (DT_LOSS | DT_GRAD) ? 24 : 16; }
+__host__ __device__ constexpr int dl_ctas(int stream, int what) { return 768 * 16 / dl_ring(what) / stream; }   // of an SM: 192 KB of rings
 // all copies of this thread but the last n groups have arrived
 __device__ __forceinline__ void rw_arrived(int n) {
   switch (n) {
 #define RW_CASE(N) case N: asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); break;
     RW_CASE(1) RW_CASE(2) RW_CASE(3) RW_CASE(4) RW_CASE(5) RW_CASE(6) RW_CASE(7) RW_CASE(8) RW_CASE(9) RW_CASE(10) RW_CASE(11)
+    RW_CASE(12) RW_CASE(13) RW_CASE(14) RW_CASE(15) RW_CASE(16) RW_CASE(17) RW_CASE(18) RW_CASE(19) RW_CASE(20) RW_CASE(21) RW_CASE(22) RW_CASE(23)
 #undef RW_CASE
     default: asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
@@ -762,16 +828,13 @@ __device__ __forceinline__ void rw_copy(uint32_t to, const void* from) { asm vol
 __device__ __forceinline__ void rw_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 template <class T, int DO, int STREAM>
-__global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(const DtArgs a) {
+__global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(const DtArgs a) {
   extern __shared__ __align__(16) unsigned char dt_raw[];
   __shared__ float2 s_part[2][DL_MOST_SHARE * STREAM / 32];
-  __shared__ int s_any[2];
   constexpr int VN = RW_VEC<T>, PARTS = STREAM / 32, RING = dl_ring(DO), STEP = STREAM * 16;
   constexpr bool BOTH = DO == (DT_LOSS | DT_GRAD);
   constexpr float LOWEST = -3.0e38f;   // in the place of a maximum of -inf
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, K = a.top, V = a.vocab;
-  const bool streams = warp < STREAM / 32;
-  DtEntry* const entries = (DtEntry*)(dt_raw + RING * STEP);
   uint32_t rank, share;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(share));
@@ -793,30 +856,27 @@ __global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(c
     r.at = head + p0 * VN;
     r.lo = rank == 0 ? 0 : r.at;
     r.hi = rank == share - 1 ? V : r.at + r.pieces * VN;
-    r.count = streams && t < r.pieces ? (r.pieces - t + STREAM - 1) / STREAM : 0;
+    r.count = t < r.pieces ? (r.pieces - t + STREAM - 1) / STREAM : 0;
     r.from = (const unsigned char*)(r.s + r.at) + 16 * t;
     return r;
   };
-  auto weight_of = [&](long long row) { return a.weights ? a.weights[row] : 1.0f; };
-  // a row of weight 0, or (an earlier call has left 0 there) without a teacher
+  // a row without a weight that counts
   auto pass_over = [&](long long row) {
     if constexpr (DO & DT_LOSS) {
       if (t == 0 && rank == 0 && a.row_loss) a.row_loss[row] = 0.f;
-      if (t == 0 && rank == 0 && a.stat) a.stat[row] = make_float2(0.f, 0.f);
     }
     if constexpr (DO & DT_GRAD) {
       const Row r = place(row);
       T* const grad = (T*)a.grad + row * V;
-      if (streams)
-        for (int j = r.lo + t; j < r.hi; j += STREAM) grad[j] = rw_to<T>(0.f);
+      for (int j = r.lo + t; j < r.hi; j += STREAM) grad[j] = rw_to<T>(0.f);
     }
   };
-  // the next row from `row` on that counts, its weight and (of an earlier call) its maximum and sum
-  struct Next { long long row; float w; float2 st; };
+  // the next row that counts, its teacher's sums and (of an earlier call) its maximum and sum
+  struct Next { long long row; float4 teacher; float2 st; };
   auto look = [&](long long row) {
-    Next n = {row, 0.f, make_float2(0.f, 1.f)};
+    Next n = {row, make_float4(0.f, 0.f, 0.f, 0.f), make_float2(0.f, 0.f)};
     if (row < a.rows) {
-      n.w = weight_of(row);
+      n.teacher = a.teachers[row];
       if constexpr (!(DO & DT_LOSS)) n.st = a.stat[row];
     }
     return n;
@@ -824,7 +884,7 @@ __global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(c
   Next peeked = look(blockIdx.x / share);   // asked for a row ahead
   auto find = [&] {
     Next n = peeked;
-    while (n.row < a.rows && (n.w == 0.f || n.st.y == 0.f)) {
+    while (n.row < a.rows && n.teacher.x == 0.f) {
       pass_over(n.row);
       n = look(n.row + groups);
     }
@@ -854,14 +914,17 @@ __global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(c
     next = find();
     coming = place(next.row < a.rows ? next.row : 0);
     if (next.row >= a.rows) coming.count = 0;
-    const float w = now.w;
+    const float w = now.teacher.x;
     float2 st = now.st;
-    DtEntry* const e = entries + buf * K;
     T* const grad = DO & DT_GRAD ? (T*)a.grad + row * V : nullptr;
     const float f = DO & DT_GRAD ? factor * w * (a.upstream && a.per_row ? a.upstream[row] : 1.0f) : 0.f;
+    // the teacher's entry whose column is this thread's
+    int2 entry = make_int2(-1, 0);
+    if constexpr (DO & DT_GRAD)
+      if (t < K) entry = a.columns[row * K + t];
     // an element before the row's first piece or behind its last
     const int head = rank == 0 ? r.at : 0, edge = t < head ? t : r.at + r.pieces * VN + t - head;
-    const bool has_edge = streams && (t < head || (rank == share - 1 && edge < V));
+    const bool has_edge = t < head || (rank == share - 1 && edge < V);
     const float edge_value = has_edge ? rw_float(r.s[edge]) : -CUDART_INF_F;
     static_assert(2 * (VN - 1) <= STREAM, "a thread per element outside of the pieces");
     // One pass over the row's pieces, each of which makes room for another: of this row, then of the next.  A piece was asked for `on_way` pieces before.
@@ -888,18 +951,21 @@ __global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(c
         rw_commit();
       }
       // a next row that is longer than this one
+      from = coming.from + most * STEP;
       for (int k = most; k < min(RING, coming.count); ++k, from += STEP) {
-        if (k == most) from = coming.from + k * STEP;
         copy(from);
         rw_commit();
       }
       on_way = min(RING, coming.count);
     };
-    // a piece of the gradient, from powers relative to m
+    // this thread's part of the gradient, from powers relative to m
     auto gradient = [&](float m, float total, auto&& over) {
       const float g = f * total;
       const uint64_t gg = rw_pair(g, g), mm = rw_pair(-m, -m);
       T* to = grad + r.at + t * VN;
+      float logit = 0.f;
+      const bool has_entry = entry.x >= r.lo && entry.x < r.hi;
+      if (has_entry) logit = rw_float(r.s[entry.x]);
       auto go = [&](auto aligned) {
         over([&](const RwPiece<T, VN>& v) {
           float x[VN];
@@ -920,11 +986,15 @@ __global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(c
       if (((uintptr_t)(grad + r.at) & 15) == 0) go(std::true_type());
       else go(std::false_type());
       if (has_edge) grad[edge] = rw_to<T>(g * dt_exp2(fmaf(edge_value, c, -m)));
+      __syncthreads();   // behind it, the columns of the teacher's entries are written again
+      if (has_entry) dt_column(grad, entry.x, __int_as_float(entry.y), logit, f, total, m, c);
+      for (int k = t + STREAM; k < K; k += STREAM) {
+        const int2 q = a.columns[row * K + k];
+        if (q.x >= r.lo && q.x < r.hi) dt_column(grad, q.x, __int_as_float(q.y), rw_float(r.s[q.x]), f, total, m, c);
+      }
     };
-    if (!streams) {
-      const bool any = dt_teacher(a, row, e, (int*)(entries + 2 * K));
-      if (lane == 0) s_any[buf] = any;
-    } else if constexpr (DO & DT_LOSS) {
+    if constexpr (!(DO & DT_LOSS)) gradient(st.x, st.y, sweep);
+    else {
       float m = LOWEST;   // scaled maximum
       uint64_t mm = rw_pair(-m, -m), sum = rw_pair(0.f, 0.f);   // sums of powers relative to it
       auto raise = [&](float to) {
@@ -953,9 +1023,11 @@ __global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(c
           if (k < on_way) copy(coming.from + k * STEP);
           rw_commit();
         }
-        for (int k = 0; k < r.count; ++k) {
-          rw_arrived(RING - 1 - k);
-          add(take());
+        for (int k = 0; k < r.count; k += 4) {
+          rw_arrived(RING - 1 - min(k + 3, RING - 1));
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (k + i < r.count) add(take());
         }
         out = first;
       }
@@ -963,49 +1035,43 @@ __global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(c
         if (edge_value * c > m) raise(edge_value * c);
         sum = rw_add2(sum, rw_pair(dt_exp2(fmaf(edge_value, c, -m)), 0.f));
       }
-      const float all = rw_warp_max(m), total = rw_warp_sum(rw_both(sum) * dt_exp2(m - all));
+      const float all = rw_warp_max(m);
+      float total = rw_warp_sum(rw_both(sum) * dt_exp2(m - all));
       if (lane < (int)share) {
         const uint32_t to = rw_at_rank(&s_part[buf][rank * PARTS + warp], lane);
         asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(all), "f"(total) : "memory");
       }
-    }
-    if constexpr (!(DO & DT_LOSS))
-      if (streams) gradient(st.x, st.y, sweep);
-    if ((DO & DT_LOSS) && share > 1) rw_cluster_sync();
-    else __syncthreads();
-    if constexpr (DO == DT_LOSS)
-      if (streams) { buf ^= 1; continue; }
-    if constexpr (DO & DT_LOSS) {
-      const int parts = (int)share * PARTS;
-      constexpr int EACH = DL_MOST_SHARE * PARTS / 32;   // of a lane
-      float2 x[EACH];
-      float m = LOWEST, total = 0.f;
+      if (share > 1) rw_cluster_sync();
+      else __syncthreads();
+      if (BOTH || warp == 0) {
+        const int parts = (int)share * PARTS;
+        constexpr int EACH = (DL_MOST_SHARE * PARTS + 31) / 32;   // of a lane
+        float2 x[EACH];
+        m = LOWEST;
+        total = 0.f;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        x[i] = lane + 32 * i < parts ? s_part[buf][lane + 32 * i] : make_float2(LOWEST, 0.f);
-        m = fmaxf(m, x[i].x);
-      }
-      m = rw_warp_max(m);
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) total += x[i].y * dt_exp2(x[i].x - m);
-      total = rw_warp_sum(total);
-      m = m == LOWEST ? 0.f : m;   // (then all are -inf, and total is 0)
-      st = make_float2(m, 1.0f / total);
-      const bool any = s_any[buf];
-      if (!streams) {
-        if (rank == 0) {
-          const float cross = any ? dt_cross(a, r.s, e, m) : 0.f;
-          if (lane == 0) {
-            const float loss = any ? w * a.temperature * a.temperature * DT_LN2 * (cross + log2f(total)) : 0.f;
-            if (a.row_loss) a.row_loss[row] = loss;
-            if (a.stat) a.stat[row] = any ? st : make_float2(0.f, 0.f);
-            loss_sum += loss;
-            weight_sum += any ? w : 0.f;
-          }
+        for (int i = 0; i < EACH; ++i) {
+          x[i] = lane + 32 * i < parts ? s_part[buf][lane + 32 * i] : make_float2(LOWEST, 0.f);
+          m = fmaxf(m, x[i].x);
         }
-      } else if constexpr (BOTH) {
+        m = rw_warp_max(m);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) total += x[i].y * dt_exp2(x[i].x - m);
+        total = rw_warp_sum(total);
+        m = m == LOWEST ? 0.f : m;   // (then all are -inf, and total is 0)
+        st = make_float2(m, 1.0f / total);
+        if (t == 0 && rank == 0) {
+          const float loss = w * a.temperature * a.temperature * DT_LN2 * fmaf(now.teacher.z, m, now.teacher.y + log2f(total));
+          if (a.row_loss) a.row_loss[row] = loss;
+          if (a.stat) a.stat[row] = st;
+          loss_sum += loss;
+          weight_sum += w;
+        }
+      }
+      buf ^= 1;
+      if constexpr (BOTH)
         // the second pass: each piece makes room for one of the next row
-        auto again = [&](auto&& work) {
+        gradient(st.x, st.y, [&](auto&& work) {
           const int from = on_way;
           on_way = min(from + r.count, coming.count);
           for (int k = 0; k < r.count; ++k) {
@@ -1013,23 +1079,12 @@ __global__ void __launch_bounds__(STREAM + 32, dl_ctas(STREAM)) k_distill_long(c
             if (from + k < on_way) copy(coming.from + (from + k) * STEP);
             rw_commit();
           }
-        };
-        if (any) gradient(st.x, st.y, again);
-        else {
-          again([](const RwPiece<T, VN>&) {});
-          for (int j = r.lo + t; j < r.hi; j += STREAM) grad[j] = rw_to<T>(0.f);
-        }
-        asm volatile("bar.sync 1, %0;" ::"n"(STREAM) : "memory");   // the streaming warps
-        if (any) dt_columns(a, r.s, grad, e, f, st.y, st.x, t, STREAM, r.lo, r.hi);
-      }
-    } else if (streams) {
-      dt_columns(a, r.s, grad, e, f, st.y, st.x, t, STREAM, r.lo, r.hi);
+        });
     }
-    buf ^= 1;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   if constexpr (DO & DT_LOSS)
-    if (t == STREAM && rank == 0) a.part[blockIdx.x / share] = make_double2(loss_sum, weight_sum);
+    if (t == 0 && rank == 0) a.part[blockIdx.x / share] = make_double2(loss_sum, weight_sum);
 }
 
 // The weights that count, before the gradient is scaled by their sum: a row's is zero if it has no teacher.
@@ -1076,46 +1131,73 @@ struct DtForm { int stream, share; bool fits; };   // fits: into the rings
 static DtForm dt_form(long long rows, int vocab, int type_bytes, bool both) {
   if (vocab <= DT_WARP_VOCAB) return {0, 1, true};
   const long long bytes = (long long)vocab * type_bytes;
-  const int stream = bytes <= 16384 ? 128 : bytes <= (both ? 32768 : 131072) ? 256 : 512;
-  const long long most = (long long)sm_count() * dl_ctas(stream);
+  const int stream = bytes <= (both ? 32768 : 131072) ? 128 : 256;
+  const long long most = (long long)sm_count() * dl_ctas(stream, both ? DT_LOSS | DT_GRAD : DT_LOSS);
   int share = 1;
   while (share < DL_MOST_SHARE && ((bytes >= share * 2 * 16384 && rows * share * 2 <= most) || (both && bytes > (long long)share * stream * 16 * DL_KEPT))) share *= 2;
   return {stream, share, bytes <= (long long)share * stream * 16 * dl_ring(DT_LOSS | DT_GRAD)};
 }
-#define DT_FITS_ANYWAY 196608   // classes of any type, DL_MOST_SHARE rings of 12 pieces of 512 threads
-static int dt_weight_ctas(long long rows) { return (int)(rows < 64 * NT ? (rows + NT - 1) / NT : 64); }
+static int dt_weight_ctas(long long rows) { return (int)(rows < 64 * NT ? (rows + NT - 1) / NT : 64); }   // at most as many as rows
+static size_t dt_teacher_smem(int top) { return (sizeof(DtEntry) * top + (size_t)4 * dt_slots(top)) * (DT_WARP_THREADS / 32); }
+// CTAs whose warps have a row each
+static int dt_warp_ctas(long long rows) {
+  const long long n = (rows + DT_WARP_THREADS / 32 - 1) / (DT_WARP_THREADS / 32), most = (long long)sm_count() * DT_MOST_CTAS;
+  return (int)(n < most ? n : most);
+}
 // Launches one pass; *groups: CTAs or clusters that begin with different rows, which is also the number of partial sums
 template <class T, int DO>
 static int dt_run(const DtArgs& a, const DtForm& form, int* groups, cudaStream_t s) {
-  const size_t slots = (size_t)4 * dt_slots(a.top), entries = sizeof(DtEntry) * a.top;
 #define DT_LONG(STREAM)                                                                                                              \
   {                                                                                                                                  \
     constexpr int RING = dl_ring(DO) * STREAM * 16;                                                                                  \
-    const size_t smem = RING + 2 * entries + slots;                                                                                  \
     static bool configured[PYLO_MAX_DEVICES] = {};                                                                                   \
-    if (int rc = allow_dynamic_smem(k_distill_long<T, DO, STREAM>, RING + (int)sizeof(DtEntry) * 2 * DT_MOST_K + 4 * dt_slots(DT_MOST_K), configured)) return rc; \
-    const long long most = form.share > 1 ? active_clusters<k_distill_long<T, DO, STREAM>>(STREAM + 32, form.share, smem)            \
-                                          : (long long)sm_count() * dl_ctas(STREAM);                                                 \
+    if (int rc = allow_dynamic_smem(k_distill_long<T, DO, STREAM>, RING, configured)) return rc;                                     \
+    const long long most = form.share > 1 ? active_clusters<k_distill_long<T, DO, STREAM>>(STREAM, form.share, RING)                 \
+                                          : (long long)sm_count() * dl_ctas(STREAM, DO);                                             \
     *groups = (int)(a.rows < most ? a.rows : most);                                                                                  \
-    launch_clusters(k_distill_long<T, DO, STREAM>, *groups * form.share, STREAM + 32, form.share, smem, s, a);                       \
+    launch_clusters(k_distill_long<T, DO, STREAM>, *groups * form.share, STREAM, form.share, RING, s, a);                            \
     return launch_status();                                                                                                          \
   }
   if (form.stream == 128) DT_LONG(128)
   if (form.stream == 256) DT_LONG(256)
-  if (form.stream == 512) DT_LONG(512)
 #undef DT_LONG
-  const size_t smem = (entries + slots) * (DT_WARP_THREADS / 32);
   static bool configured[PYLO_MAX_DEVICES] = {};
-  if (smem > 48 * 1024)
-    if (int rc = allow_dynamic_smem(k_distill_short<T, DO>, (int)(DT_WARP_THREADS / 32 * (sizeof(DtEntry) * DT_MOST_K + 4 * dt_slots(DT_MOST_K))), configured)) return rc;
-  const long long n = (a.rows + DT_WARP_THREADS / 32 - 1) / (DT_WARP_THREADS / 32), most = (long long)sm_count() * DT_MOST_CTAS;
-  *groups = (int)(n < most ? n : most);
-  launch(k_distill_short<T, DO>, *groups, DT_WARP_THREADS, smem, s, a);
+  if (int rc = allow_dynamic_smem(k_distill_short<T, DO>, (int)dt_teacher_smem(DT_MOST_K), configured)) return rc;
+  *groups = dt_warp_ctas(a.rows);
+  launch(k_distill_short<T, DO>, *groups, DT_WARP_THREADS, dt_teacher_smem(a.top), s, a);
   return launch_status();
 }
 template <int DO>
 static int dt_any_type(const DtArgs& a, int type, const DtForm& form, int* groups, cudaStream_t s) {
   return type == PYLO_FP32 ? dt_run<float, DO>(a, form, groups, s) : type == PYLO_BF16 ? dt_run<__nv_bfloat16, DO>(a, form, groups, s) : dt_run<__half, DO>(a, form, groups, s);
+}
+template <class T>
+static int dt_teachers(const DtArgs& a, double* sums, cudaStream_t s) {
+  static bool configured[PYLO_MAX_DEVICES] = {};
+  if (int rc = allow_dynamic_smem(k_distill_teachers<T>, (int)dt_teacher_smem(DT_MOST_K), configured)) return rc;
+  launch(k_distill_teachers<T>, dt_warp_ctas(a.rows), DT_WARP_THREADS, dt_teacher_smem(a.top), s, a, sums);
+  return launch_status();
+}
+// What lies in a call's workspace: the first is kept for a gradient alone
+struct DtWork {
+  float2* stat; float* inv; float4* teachers; int2* columns;
+  double2* part; double* sums;
+  int64_t bytes;
+};
+static DtWork dt_work(void* base, int64_t rows, int vocab, int top) {
+  char* p = (char*)base;
+  const bool is_long = vocab > DT_WARP_VOCAB;
+  const int64_t most = (int64_t)sm_count() * DT_MOST_CTAS, groups = rows < most ? rows : most;
+  auto take = [&](int64_t bytes) { char* q = p; p += (bytes + 15) / 16 * 16; return (void*)q; };
+  DtWork w = {};
+  w.inv = (float*)take(4);
+  w.stat = (float2*)take(8 * rows);
+  w.teachers = (float4*)take(is_long ? 16 * rows : 0);
+  w.columns = (int2*)take(is_long ? 8 * rows * top : 0);
+  w.part = (double2*)take(16 * groups);
+  w.sums = (double*)take(8 * groups);
+  w.bytes = p - (char*)base;
+  return w;
 }
 static bool dt_good(const pylo_distill* d) {
   return d && d->rows >= 0 && d->rows <= (1ll << 40) && d->vocab > 0 && d->vocab <= (1 << 30) && d->top > 0 && d->top <= DT_MOST_K && rw_type(d->type) &&
@@ -1125,7 +1207,7 @@ static bool dt_good(const pylo_distill* d) {
 static DtArgs dt_args(const pylo_distill* d) {
   DtArgs a = {};
   a.logits = d->logits; a.teacher = d->teacher; a.ids = d->ids; a.weights = d->weights;
-  a.row_loss = d->row_loss; a.stat = (float2*)d->stat; a.grad = d->grad; a.upstream = d->upstream; a.per_row = d->reduction == PYLO_REDUCE_NONE;
+  a.row_loss = d->row_loss; a.grad = d->grad; a.upstream = d->upstream; a.per_row = d->reduction == PYLO_REDUCE_NONE;
   a.rows = d->rows; a.stride = d->stride; a.vocab = d->vocab; a.top = d->top; a.teacher_type = d->teacher_type; a.wide_ids = d->ids_bytes == 8;
   a.c = (float)(DT_LOG2E / d->temperature); a.temperature = d->temperature; a.scale = 1.0f;
   return a;
@@ -1175,47 +1257,43 @@ int pylo_b200_layer_norm_backward(const pylo_norm* n, void* stream) {
   return launch_status();
 }
 
-// [partial sums of loss and weights][parts of the weights][a row's maximum and sum, where loss and gradient take two launches]
-static int64_t dt_part_bytes(int64_t rows) {
-  const int64_t most = (int64_t)sm_count() * DT_MOST_CTAS;
-  return 16 * (rows < most ? rows : most);
-}
-int64_t pylo_b200_distill_workspace(int64_t rows, int vocab) {
-  if (rows <= 0 || vocab <= 0) return 16;
-  return dt_part_bytes(rows) + 8 * (int64_t)dt_weight_ctas(rows) + (vocab > DT_FITS_ANYWAY ? 8 * rows : 0);
-}
+int64_t pylo_b200_distill_workspace(int64_t rows, int vocab, int top) { return rows < 0 || vocab <= 0 || top <= 0 ? 0 : dt_work(nullptr, rows, vocab, top).bytes; }
 
 int pylo_b200_distill(const pylo_distill* d, int what, void* stream) {
   CHECK_ARG(dt_good(d) && (what == PYLO_DISTILL_LOSS || what == PYLO_DISTILL_GRAD || what == (PYLO_DISTILL_LOSS | PYLO_DISTILL_GRAD)));
   cudaStream_t s = (cudaStream_t)stream;
   const bool loss = what & PYLO_DISTILL_LOSS, grad = what & PYLO_DISTILL_GRAD, mean = d->reduction == PYLO_REDUCE_MEAN;
-  CHECK_ARG(!loss || (d->work && (uintptr_t)d->work % 16 == 0 && d->work_bytes >= pylo_b200_distill_workspace(d->rows, d->vocab)));
+  CHECK_ARG(d->work && (uintptr_t)d->work % 16 == 0 && d->work_bytes >= pylo_b200_distill_workspace(d->rows, d->vocab, d->top));
   CHECK_ARG(!grad || d->rows == 0 || (d->grad && (uintptr_t)d->grad % rw_bytes(d->type) == 0));
-  CHECK_ARG(!grad || loss || d->rows == 0 || (d->stat && (!mean || d->inv)));
-  DtArgs a = dt_args(d);
+  const DtWork w = dt_work(d->work, d->rows, d->vocab, d->top);
   int groups = 0;
   if (d->rows) {
     const DtForm form = dt_form(d->rows, d->vocab, (int)rw_bytes(d->type), loss && grad);
-    a.part = (double2*)d->work;
+    DtArgs a = dt_args(d);
+    a.part = w.part; a.stat = w.stat; a.teachers = w.teachers; a.columns = w.columns;
     if (grad) a.scale = d->scale;
-    if (grad && mean && loss) {
-      double* const sums = (double*)((char*)d->work + dt_part_bytes(d->rows));
-      a.weight_sums = sums;
-      a.n_sums = dt_weight_ctas(d->rows);
-      launch(k_distill_weights, a.n_sums, NT, 0, s, a, sums);
-    } else if (grad && mean) a.inv = d->inv;
-    int rc;
+    if (loss && form.stream) {
+      const int rc = d->type == PYLO_FP32 ? dt_teachers<float>(a, w.sums, s) : d->type == PYLO_BF16 ? dt_teachers<__nv_bfloat16>(a, w.sums, s) : dt_teachers<__half>(a, w.sums, s);
+      if (rc) return rc;
+    }
+    if (grad && mean) {
+      if (!loss) a.inv = w.inv;
+      else {
+        a.weight_sums = w.sums;
+        a.n_sums = form.stream ? dt_warp_ctas(d->rows) : dt_weight_ctas(d->rows);
+        if (!form.stream) launch(k_distill_weights, a.n_sums, NT, 0, s, a, w.sums);
+      }
+    }
+    int rc, unused;
     if (loss && grad && form.fits) rc = dt_any_type<DT_LOSS | DT_GRAD>(a, d->type, form, &groups, s);
     else {
-      if (loss && grad && !a.stat) a.stat = (float2*)((char*)d->work + dt_part_bytes(d->rows) + 8 * (int64_t)dt_weight_ctas(d->rows));
       rc = loss ? dt_any_type<DT_LOSS>(a, d->type, form, &groups, s) : 0;
-      int unused;
       if (grad && !rc) rc = dt_any_type<DT_GRAD>(a, d->type, form, &unused, s);
     }
     if (rc) return rc;
   }
   if (loss && d->reduction != PYLO_REDUCE_NONE)
-    launch(k_distill_total, 1, NT, 0, s, (const double2*)d->work, groups, (int)mean, 1.0f, d->loss, d->inv);
+    launch(k_distill_total, 1, NT, 0, s, (const double2*)w.part, groups, (int)mean, 1.0f, d->loss, w.inv);
   return launch_status();
 }
 

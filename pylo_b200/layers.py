@@ -367,52 +367,50 @@ def _contiguous(t):
     return t if t.is_contiguous() else t.detach().contiguous()
 
 
-def _distill_struct(rows, teacher, ids, weights, temperature, reduction):
+def _distill_struct(rows, teacher, ids, weights, temperature, reduction, work):
     n, vocab = rows.shape
     return L.Distill(logits=rows.data_ptr(), teacher=teacher.data_ptr(), ids=ids.data_ptr(), weights=None if weights is None else weights.data_ptr(),
                      rows=n, stride=vocab if n == 1 else rows.stride(0), vocab=vocab, top=ids.shape[-1], type=TYPES[rows.dtype],
-                     teacher_type=TYPES[teacher.dtype], ids_bytes=ids.element_size(), reduction=reduction, temperature=temperature, scale=1.0)
+                     teacher_type=TYPES[teacher.dtype], ids_bytes=ids.element_size(), reduction=reduction, temperature=temperature, scale=1.0,
+                     work=work.data_ptr(), work_bytes=work.numel())
 
 
-def _distill_forward(rows, teacher, ids, weights, temperature, reduction, lead, keep):
-    """(loss, a buffer that begins with the rows' statistics and has the sum of the weights behind them)"""
-    n, vocab = rows.shape
-    device = rows.get_device()
-    d = _distill_struct(rows, teacher, ids, weights, temperature, reduction)
-    loss = torch.empty(lead if reduction == L.REDUCE_NONE else (), dtype=torch.float32, device=rows.device)
-    work_bytes = _size("pylo_b200_distill_workspace", device, n, vocab)
-    stat_bytes = (8 * n + 4 + 15) // 16 * 16 if keep else 0
-    buffer = torch.empty(stat_bytes + work_bytes, dtype=torch.uint8, device=rows.device)
-    at = buffer.data_ptr()
-    d.work, d.work_bytes = at + stat_bytes, work_bytes
+def _distill_work(rows, ids):
+    size = _size("pylo_b200_distill_workspace", rows.get_device(), *rows.shape, ids.shape[-1])
+    return torch.empty(size, dtype=torch.uint8, device=rows.device)
+
+
+def _distill_forward(rows, teacher, ids, weights, temperature, reduction, lead):
+    """(loss, the workspace, which a gradient is made from)"""
+    work = _distill_work(rows, ids)
+    d = _distill_struct(rows, teacher, ids, weights, temperature, reduction, work)
     if reduction == L.REDUCE_NONE:
+        loss = torch.empty(lead, dtype=torch.float32, device=rows.device)
         d.row_loss = loss.data_ptr()
     else:
+        loss = torch.empty((), dtype=torch.float32, device=rows.device)
         d.loss = loss.data_ptr()
-    if keep:
-        d.stat, d.inv = at, at + 8 * n
-    _call(L.lib.pylo_b200_distill, "distillation_loss", device, C.byref(d), L.DISTILL_LOSS)
-    return loss, buffer
+    _call(L.lib.pylo_b200_distill, "distillation_loss", rows.get_device(), C.byref(d), L.DISTILL_LOSS)
+    return loss, work
 
 
 class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, rows, teacher, ids, weights, temperature, reduction):
-        loss, buffer = _distill_forward(rows, teacher, ids, weights, temperature, reduction, logits.shape[:-1], True)
-        ctx.save_for_backward(rows, teacher, ids, weights, buffer)
+        loss, work = _distill_forward(rows, teacher, ids, weights, temperature, reduction, logits.shape[:-1])
+        ctx.save_for_backward(rows, teacher, ids, weights, work)
         ctx.temperature, ctx.reduction, ctx.shape = temperature, reduction, logits.shape
         return loss
 
     @staticmethod
     @_once
     def backward(ctx, upstream):
-        rows, teacher, ids, weights, buffer = ctx.saved_tensors
+        rows, teacher, ids, weights, work = ctx.saved_tensors
         grad = _like(rows)
         if upstream.dtype is not torch.float32 or not upstream.is_contiguous():
             upstream = upstream.to(torch.float32).contiguous()
-        d = _distill_struct(rows, teacher, ids, weights, ctx.temperature, ctx.reduction)
-        d.stat, d.grad, d.upstream = buffer.data_ptr(), grad.data_ptr(), upstream.data_ptr()
-        d.inv = d.stat + 8 * d.rows
+        d = _distill_struct(rows, teacher, ids, weights, ctx.temperature, ctx.reduction, work)
+        d.grad, d.upstream = grad.data_ptr(), upstream.data_ptr()
         _call(L.lib.pylo_b200_distill, "distillation_loss backward", rows.get_device(), C.byref(d), L.DISTILL_GRAD)
         return grad.view(ctx.shape), None, None, None, None, None, None
 
@@ -429,7 +427,7 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     rows, teacher, ids, w, code = _distill_arguments(logits, teacher_logits, teacher_ids, temperature, weights, reduction)
     if _graph(logits):
         return _Distillation.apply(logits, rows, teacher, ids, w, float(temperature), code)
-    return _distill_forward(rows, teacher, ids, w, float(temperature), code, logits.shape[:-1], False)[0]
+    return _distill_forward(rows, teacher, ids, w, float(temperature), code, logits.shape[:-1])[0]
 
 
 def distillation_loss_and_grad(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor, temperature: float = 1.0,
@@ -441,7 +439,8 @@ def distillation_loss_and_grad(logits: torch.Tensor, teacher_logits: torch.Tenso
     rows, teacher, ids, w, code = _distill_arguments(logits, teacher_logits, teacher_ids, temperature, weights, reduction)
     if code == L.REDUCE_NONE:
         raise ValueError("reduction has to be 'mean' or 'sum'")
-    d = _distill_struct(rows, teacher, ids, w, float(temperature), code)
+    work = _distill_work(rows, ids)
+    d = _distill_struct(rows, teacher, ids, w, float(temperature), code, work)
     if isinstance(scale, torch.Tensor):
         _check("scale", scale, logits.get_device(), (torch.float32,))
         if scale.numel() != 1:
@@ -449,13 +448,10 @@ def distillation_loss_and_grad(logits: torch.Tensor, teacher_logits: torch.Tenso
         d.upstream = scale.data_ptr()
     else:
         d.scale = float(scale)
-    device = rows.get_device()
     loss = torch.empty((), dtype=torch.float32, device=rows.device)
     grad = _like(rows)
-    d.work_bytes = _size("pylo_b200_distill_workspace", device, *rows.shape)
-    work = torch.empty(d.work_bytes, dtype=torch.uint8, device=rows.device)
-    d.loss, d.grad, d.work = loss.data_ptr(), grad.data_ptr(), work.data_ptr()
-    _call(L.lib.pylo_b200_distill, "distillation_loss_and_grad", device, C.byref(d), L.DISTILL_LOSS | L.DISTILL_GRAD)
+    d.loss, d.grad = loss.data_ptr(), grad.data_ptr()
+    _call(L.lib.pylo_b200_distill, "distillation_loss_and_grad", rows.get_device(), C.byref(d), L.DISTILL_LOSS | L.DISTILL_GRAD)
     return loss, grad.view(logits.shape)
 
 

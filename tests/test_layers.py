@@ -524,7 +524,7 @@ def test_library_refuses_before_it_launches():
     for bad in (dict(logits=None), dict(ids=None), dict(vocab=0), dict(top=0), dict(top=L.DISTILL_MOST_TOP + 1), dict(ids_bytes=2), dict(temperature=0.0), dict(stride=9),
                 dict(work=None), dict(work_bytes=8), dict(type=5), dict(teacher_type=-1), dict(logits=18), dict(work=24), dict(temperature=float("nan"))):
         assert L.lib.pylo_b200_distill(C.byref(L.Distill(**{**distill, **bad})), L.DISTILL_LOSS, None) < 0, bad
-    assert L.lib.pylo_b200_distill(C.byref(L.Distill(**distill)), L.DISTILL_GRAD, None) < 0      # no stat, no grad
+    assert L.lib.pylo_b200_distill(C.byref(L.Distill(**distill)), L.DISTILL_GRAD, None) < 0      # no grad
     assert L.lib.pylo_b200_distill(C.byref(L.Distill(**distill)), 4, None) < 0
     ffn = dict(x=256, w_gate=256, w_up=256, w_down=256, y=256, kept=256, rows=4, ld_x=8, ld_gate=8, ld_up=8, ld_down=16, width=8, hidden=16, out=8, type=L.BF16)
     for bad in (dict(x=None), dict(x=264), dict(ld_x=7), dict(ld_x=12), dict(ld_down=8), dict(kept=16), dict(kept=None), dict(type=L.FP32), dict(activation=4), dict(width=0),
