@@ -781,9 +781,13 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_teachers(const DtAr
   DtEntry* const e = (DtEntry*)dt_raw + group * a.top;
   int* const slots = (int*)((DtEntry*)dt_raw + GROUPS * a.top) + group * dt_slots(a.top);
   double weight_sum = 0.0;
-  for (long long row = (long long)blockIdx.x * GROUPS + group; row < a.rows; row += (long long)gridDim.x * GROUPS) {
+  const long long first = (long long)blockIdx.x * GROUPS + group, step = (long long)gridDim.x * GROUPS;
+  DtPeek peek = dt_peek(a, first, 0);
+  for (long long row = first; row < a.rows; row += step) {
     const float weight = a.weights ? a.weights[row] : 1.0f;
-    const bool any = weight != 0.f && dt_teacher(a, row, dt_peek(a, row, 0), e, slots);
+    const DtPeek mine = peek;
+    peek = dt_peek(a, row + step, 0);
+    const bool any = weight != 0.f && dt_teacher(a, row, mine, e, slots);
     if (any) {
       const float cross = dt_cross(a, (const T*)a.logits + row * a.stride, e, 0.f);
       float sum = 0.f;
@@ -908,6 +912,8 @@ __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(co
   if (now.row >= a.rows) r.count = 0;
   int on_way = min(RING, r.count);   // this row's pieces that have been asked for
   for (int i = 0; i < on_way; ++i) { copy(r.from + i * STEP); rw_commit(); }
+  auto entry_of = [&](long long row) { return (DO & DT_GRAD) && t < K && row < a.rows ? a.columns[row * K + t] : make_int2(-1, 0); };
+  int2 entry1 = entry_of(now.row);   // asked for a row ahead
   int buf = 0;
   for (; now.row < a.rows; now = next, r = coming) {
     const long long row = now.row;
@@ -918,14 +924,13 @@ __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(co
     float2 st = now.st;
     T* const grad = DO & DT_GRAD ? (T*)a.grad + row * V : nullptr;
     const float f = DO & DT_GRAD ? factor * w * (a.upstream && a.per_row ? a.upstream[row] : 1.0f) : 0.f;
-    // the teacher's entry whose column is this thread's
-    int2 entry = make_int2(-1, 0);
-    if constexpr (DO & DT_GRAD)
-      if (t < K) entry = a.columns[row * K + t];
+    const int2 entry = entry1;   // the teacher's entry whose column is this thread's
+    entry1 = entry_of(next.row);
     // an element before the row's first piece or behind its last
     const int head = rank == 0 ? r.at : 0, edge = t < head ? t : r.at + r.pieces * VN + t - head;
     const bool has_edge = t < head || (rank == share - 1 && edge < V);
-    const float edge_value = has_edge ? rw_float(r.s[edge]) : -CUDART_INF_F;
+    T outside = rw_to<T>(0.f);   // (as it comes: anything computed of it would have to wait for it here)
+    if (has_edge) outside = r.s[edge];
     static_assert(2 * (VN - 1) <= STREAM, "a thread per element outside of the pieces");
     // One pass over the row's pieces, each of which makes room for another: of this row, then of the next.  A piece was asked for `on_way` pieces before.
     auto sweep = [&](auto&& work) {
@@ -963,9 +968,9 @@ __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(co
       const float g = f * total;
       const uint64_t gg = rw_pair(g, g), mm = rw_pair(-m, -m);
       T* to = grad + r.at + t * VN;
-      float logit = 0.f;
+      T logit = rw_to<T>(0.f);
       const bool has_entry = entry.x >= r.lo && entry.x < r.hi;
-      if (has_entry) logit = rw_float(r.s[entry.x]);
+      if (has_entry) logit = r.s[entry.x];
       auto go = [&](auto aligned) {
         over([&](const RwPiece<T, VN>& v) {
           float x[VN];
@@ -985,9 +990,9 @@ __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(co
       };
       if (((uintptr_t)(grad + r.at) & 15) == 0) go(std::true_type());
       else go(std::false_type());
-      if (has_edge) grad[edge] = rw_to<T>(g * dt_exp2(fmaf(edge_value, c, -m)));
+      if (has_edge) grad[edge] = rw_to<T>(g * dt_exp2(fmaf(rw_float(outside), c, -m)));
       __syncthreads();   // behind it, the columns of the teacher's entries are written again
-      if (has_entry) dt_column(grad, entry.x, __int_as_float(entry.y), logit, f, total, m, c);
+      if (has_entry) dt_column(grad, entry.x, __int_as_float(entry.y), rw_float(logit), f, total, m, c);
       for (int k = t + STREAM; k < K; k += STREAM) {
         const int2 q = a.columns[row * K + k];
         if (q.x >= r.lo && q.x < r.hi) dt_column(grad, q.x, __int_as_float(q.y), rw_float(r.s[q.x]), f, total, m, c);
@@ -1032,8 +1037,9 @@ __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(co
         out = first;
       }
       if (has_edge) {
-        if (edge_value * c > m) raise(edge_value * c);
-        sum = rw_add2(sum, rw_pair(dt_exp2(fmaf(edge_value, c, -m)), 0.f));
+        const float v = rw_float(outside);
+        if (v * c > m) raise(v * c);
+        sum = rw_add2(sum, rw_pair(dt_exp2(fmaf(v, c, -m)), 0.f));
       }
       const float all = rw_warp_max(m);
       float total = rw_warp_sum(rw_both(sum) * dt_exp2(m - all));
@@ -1155,6 +1161,7 @@ static int dt_run(const DtArgs& a, const DtForm& form, int* groups, cudaStream_t
     const long long most = form.share > 1 ? active_clusters<k_distill_long<T, DO, STREAM>>(STREAM, form.share, RING)                 \
                                           : (long long)sm_count() * dl_ctas(STREAM, DO);                                             \
     *groups = (int)(a.rows < most ? a.rows : most);                                                                                  \
+    t_plain_next = true;   /* beside a kernel that needs less shared memory, not as many CTAs would fit an SM as do */               \
     launch_clusters(k_distill_long<T, DO, STREAM>, *groups * form.share, STREAM, form.share, RING, s, a);                            \
     return launch_status();                                                                                                          \
   }
