@@ -33,6 +33,9 @@ struct RwPiece {
   __device__ __forceinline__ void load(const T* p) {   // read once: not kept in the L1 cache
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
   }
+  __device__ __forceinline__ void from_shared(uint32_t p) {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(p) : "memory");
+  }
   __device__ __forceinline__ void store(T* p) const { __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3])); }
   __device__ __forceinline__ float at(int j) const {
     if constexpr (std::is_same_v<T, float>) return __uint_as_float(w[j]);
@@ -48,8 +51,6 @@ struct RwPiece {
       return *reinterpret_cast<const T*>(&h);
     }
   }
-  // What is computed from the elements behind this is not taken from what was computed before it, which would have to be kept
-  __device__ __forceinline__ void anew() { asm volatile("" : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3])); }
   __device__ __forceinline__ uint64_t two(int j) const {   // elements j, j + 1
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(at(j)), "f"(at(j + 1)));
@@ -75,7 +76,6 @@ struct RwPiece<T, 1> {
   T v;
   __device__ __forceinline__ void load(const T* p) { v = *p; }   // (__ldg of 16-bit types is assembly that the compiler may move out of a branch, to where p is not valid)
   __device__ __forceinline__ void store(T* p) const { *p = v; }
-  __device__ __forceinline__ void anew() {}
   __device__ __forceinline__ float at(int) const { return rw_float(v); }
   template <class F>
   __device__ __forceinline__ void make(F&& f) { v = rw_to<T>(f(0)); }
@@ -141,6 +141,19 @@ __device__ __forceinline__ float rw_warp_max(float v) {
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
+// all copies of this thread but the last n groups have arrived
+__device__ __forceinline__ void rw_arrived(int n) {
+  switch (n) {
+#define RW_CASE(N) case N: asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); break;
+    RW_CASE(1) RW_CASE(2) RW_CASE(3) RW_CASE(4) RW_CASE(5) RW_CASE(6) RW_CASE(7) RW_CASE(8) RW_CASE(9) RW_CASE(10) RW_CASE(11)
+    RW_CASE(12) RW_CASE(13) RW_CASE(14) RW_CASE(15) RW_CASE(16) RW_CASE(17) RW_CASE(18) RW_CASE(19) RW_CASE(20) RW_CASE(21) RW_CASE(22) RW_CASE(23)
+#undef RW_CASE
+    default: asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
+}
+__device__ __forceinline__ void rw_copy(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void rw_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
 // ------------------------------------------------------------------------------------------------
 // Layer norm.  m = mean x, r = 1 / sqrt(mean (x - m)^2 + eps), xh = (x - m) r:
 //   y = xh w + b;   dx = r (q - mean q - xh mean(q xh)) with q = dy w;   dw = sum over rows dy xh, db = sum over rows dy
@@ -154,10 +167,11 @@ __device__ __forceinline__ float rw_warp_max(float v) {
 #define LN_WARPS (LN_WARP_THREADS / 32)
 #define LN_MOST 16384         // elements of a row
 #define LN_MOST_SHARE 4
-// CTAs of so many threads on an SM, with E elements per thread: 64 to 128 registers forward, 100 to 168 backward
-__host__ __device__ constexpr int ln_ctas(int threads, int e, bool backward) {
-  return threads > 128 ? backward ? 1 : 512 / threads : e <= 8 ? backward ? 5 : 8 : backward ? 3 : 4;
+// CTAs of so many threads on an SM, with E elements per thread: 64 to 128 registers
+__host__ __device__ constexpr int ln_ctas(int threads, int e, bool backward, bool ring) {
+  return threads > 128 ? 512 / threads : e <= 8 ? backward ? 6 : 8 : backward && !ring ? 3 : 4;
 }
+#define LN_DEPTH 3   // rows of a thread's ring: one that is worked on, two on their way
 struct LnArgs {
   const void *x, *dy, *weight, *bias;
   void *y;               // or dx, or NULL
@@ -181,10 +195,6 @@ struct LnVector {
         if (first + i * gap < width) p[i * PER + k].load(v + first + i * gap + k * WN);
         else p[i * PER + k].make([](int) { return 0.f; });
       }
-  }
-  __device__ __forceinline__ void anew() {
-#pragma unroll
-    for (int i = 0; i < NV * PER; ++i) p[i].anew();
   }
   __device__ __forceinline__ uint64_t two(int k) const {   // elements 2k, 2k + 1 of the thread's
     if constexpr (VN == 1) return rw_pair(p[2 * k].at(0), p[2 * k + 1].at(0));
@@ -262,7 +272,7 @@ struct LnPlace {
 };
 
 template <class T, class W, int VN, int E, int MOST>
-__global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS, ln_ctas(MOST, E, false)) k_layer_norm(const LnArgs a) {
+__global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS, ln_ctas(MOST, E, false, false)) k_layer_norm(const LnArgs a) {
   constexpr bool BLOCK = MOST > 0;   // a row is a CTA's, of so many threads at most
   constexpr int NV = E / VN;
   __shared__ float2 s_buf[2][32];   // a part of the sums per lane
@@ -316,11 +326,12 @@ __global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS, ln_ctas(MOST, E
 }
 
 template <class T, class W, int VN, int E, int MOST>
-__global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS, ln_ctas(MOST, E, true)) k_layer_norm_backward(const LnArgs a) {
-  constexpr bool BLOCK = MOST > 0;
+__global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS, ln_ctas(MOST, E, true, VN > 1)) k_layer_norm_backward(const LnArgs a) {
+  constexpr bool BLOCK = MOST > 0, RING = VN > 1;   // rows by asynchronous copies through the thread's own part of shared memory, or through registers
   constexpr int NV = E / VN;
   __shared__ float2 s_buf[2][32];   // a part of the sums per lane
   __shared__ float s_cols[BLOCK ? 1 : 2 * 32 * E];
+  extern __shared__ __align__(16) unsigned char ln_raw[];
   const LnPlace<BLOCK, VN, NV> at;
   const int width = a.width;
   if (at.share > 1) rw_cluster_sync();   // the others are running
@@ -331,54 +342,102 @@ __global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS, ln_ctas(MOST, E
   uint64_t dw2[E / 2], db2[E / 2];
 #pragma unroll
   for (int k = 0; k < E / 2; ++k) dw2[k] = db2[k] = rw_pair(0.f, 0.f);
-  RwPiece<T, VN> nx[NV], nd[NV];
-  float next_mean = 0.f, next_rstd = 0.f;
-  auto fetch = [&](long long r) {   // what lies behind the row has a gradient of zero
-    if (r >= a.rows) return;
-    next_mean = a.mean[r];
-    next_rstd = a.rstd[r];
+  // What lies behind a row has a gradient of zero.
+  const uint32_t piece = blockDim.x * 16, ring = smem_addr(ln_raw) + 16 * threadIdx.x;
+  constexpr int KEPT = RING ? 1 : NV;
+  RwPiece<T, VN> nx[KEPT], nd[KEPT], vx[KEPT], vd[KEPT];
+  if constexpr (RING) {
+    for (int i = 0; i < LN_DEPTH * 2 * NV; ++i) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + i * piece), "r"(0) : "memory");
+  } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (at.first + i * at.gap < width) {
-        nx[i].load((const T*)a.x + r * a.x_stride + at.first + i * at.gap);
-        nd[i].load((const T*)a.dy + r * a.dy_stride + at.first + i * at.gap);
-      }
+    for (int i = 0; i < NV; ++i) { nx[i].make([](int) { return 0.f; }); nd[i].make([](int) { return 0.f; }); }
+  }
+  uint32_t in = 0, out = 0;   // the ring's places, as offsets
+  auto fetch = [&](long long r) {
+    if (r < a.rows) {
+      const T* const x = (const T*)a.x + r * a.x_stride + at.first;
+      const T* const dy = (const T*)a.dy + r * a.dy_stride + at.first;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (at.first + i * at.gap < width) {
+          if constexpr (RING) {
+            rw_copy(ring + in + 2 * i * piece, x + i * at.gap);
+            rw_copy(ring + in + (2 * i + 1) * piece, dy + i * at.gap);
+          } else {
+            nx[i].load(x + i * at.gap);
+            nd[i].load(dy + i * at.gap);
+          }
+        }
+    }
+    if constexpr (RING) {
+      rw_commit();
+      in = in == (LN_DEPTH - 1) * 2 * NV * piece ? 0 : in + 2 * NV * piece;
+    }
   };
+  // elements 2k, 2k + 1 of x and dy of the row that is worked on, asked for in order
+  RwPiece<T, RING ? VN : RW_VEC<T>> px, pd;
+  auto taken = [&](int k, uint64_t& x, uint64_t& d) {
+    if constexpr (RING) {
+      if (2 * k % VN == 0) {
+        px.from_shared(ring + out + 2 * (2 * k / VN) * piece);
+        pd.from_shared(ring + out + (2 * (2 * k / VN) + 1) * piece);
+      }
+      x = px.two(2 * k % VN);
+      d = pd.two(2 * k % VN);
+    } else {
+      x = ln_two<T, VN, KEPT>(vx, k);
+      d = ln_two<T, VN, KEPT>(vd, k);
+    }
+  };
+  float next_mean = 0.f, next_rstd = 0.f;
+  auto stats = [&](long long r) {
+    if (r < a.rows) { next_mean = a.mean[r]; next_rstd = a.rstd[r]; }
+  };
+  stats(at.row);
+  if constexpr (RING) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) { nx[i].make([](int) { return 0.f; }); nd[i].make([](int) { return 0.f; }); }
-  fetch(at.row);
+    for (int d = 0; d < LN_DEPTH - 1; ++d) fetch(at.row + d * at.step);
+  } else fetch(at.row);
   int flip = 0;
 #pragma unroll 1
   for (long long row = at.row; row < a.rows; row += at.step, flip ^= 1) {
-    RwPiece<T, VN> vx[NV], vd[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) { vx[i] = nx[i]; vd[i] = nd[i]; }
-    if constexpr (sizeof(W) == 2 && VN > 1) weight.anew();   // its elements in fp32 would take twice the registers
     // xh = x rstd - mean rstd, one rounding: what the mean's own rounding does to it is as large
     const uint64_t r2 = rw_pair(next_rstd, next_rstd), off = rw_pair(-next_mean * next_rstd, -next_mean * next_rstd);
     const float rstd = next_rstd;
-    fetch(row + at.step);
+    if constexpr (RING) {
+      fetch(row + (LN_DEPTH - 1) * at.step);
+      rw_arrived(LN_DEPTH - 1);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) { vx[i] = nx[i]; vd[i] = nd[i]; }
+      fetch(row + at.step);
+    }
+    stats(row + at.step);
     uint64_t t1 = rw_pair(0.f, 0.f), t2 = t1;
 #pragma unroll
     for (int k = 0; k < E / 2; ++k) {
-      const uint64_t d = ln_two<T, VN, NV>(vd, k), xh = rw_fma2(ln_two<T, VN, NV>(vx, k), r2, off), q = a.weight ? rw_mul2(d, weight.two(k)) : d;
+      uint64_t x, d;
+      taken(k, x, d);
+      const uint64_t xh = rw_fma2(x, r2, off), q = a.weight ? rw_mul2(d, weight.two(k)) : d;
       dw2[k] = rw_fma2(d, xh, dw2[k]);
       db2[k] = rw_add2(d, db2[k]);
       t1 = rw_add2(t1, q);
       t2 = rw_fma2(q, xh, t2);
     }
-    if (a.y == nullptr) continue;
-    const float2 sums = ln_sums<BLOCK>(rw_both(t1), rw_both(t2), s_buf[flip], at.rank, at.share);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) { vx[i].anew(); vd[i].anew(); }
-    if constexpr (sizeof(W) == 2 && VN > 1) weight.anew();
-    // rstd (q - s1 - xh s2)
-    const uint64_t s1 = rw_pair(-sums.x * inv * rstd, -sums.x * inv * rstd), s2 = rw_pair(-sums.y * inv, -sums.y * inv);
-    at.store((T*)a.y + row * width, width, [&](int k) {
-      const uint64_t d = ln_two<T, VN, NV>(vd, k), xh = rw_fma2(ln_two<T, VN, NV>(vx, k), r2, off), q = a.weight ? rw_mul2(d, weight.two(k)) : d;
-      return rw_fma2(rw_fma2(xh, s2, q), r2, s1);
-    });
+    if (a.y) {
+      const float2 sums = ln_sums<BLOCK>(rw_both(t1), rw_both(t2), s_buf[flip], at.rank, at.share);
+      // rstd (q - s1 - xh s2)
+      const uint64_t s1 = rw_pair(-sums.x * inv * rstd, -sums.x * inv * rstd), s2 = rw_pair(-sums.y * inv, -sums.y * inv);
+      at.store((T*)a.y + row * width, width, [&](int k) {
+        uint64_t x, d;
+        taken(k, x, d);
+        const uint64_t xh = rw_fma2(x, r2, off), q = a.weight ? rw_mul2(d, weight.two(k)) : d;
+        return rw_fma2(rw_fma2(xh, s2, q), r2, s1);
+      });
+    }
+    if constexpr (RING) out = out == (LN_DEPTH - 1) * 2 * NV * piece ? 0 : out + 2 * NV * piece;
   }
+  if constexpr (RING) asm volatile("cp.async.wait_all;" ::: "memory");
   float dw[E], db[E];
 #pragma unroll
   for (int k = 0; k < E / 2; ++k) {
@@ -440,7 +499,7 @@ __global__ void __launch_bounds__(32 * LN_COLUMN_GROUPS) k_layer_norm_columns(co
 // A call's form: elements of a thread, the most threads of a CTA that the kernel is made for (0: a warp per row), its threads, CTAs that share a row,
 // groups of CTAs that begin with different rows
 struct LnForm { int elems, most, threads, share, groups; };
-static LnForm ln_form(long long rows, int width, bool wide, bool backward) {   // wide: 16-bit elements by 16 bytes
+static LnForm ln_form(long long rows, int width, bool wide, bool backward, bool ring) {   // wide: 16-bit elements by 16 bytes
   const int many = wide ? 32 : 16, few = wide ? 8 : 4;
   LnForm f = {many, 0, LN_WARP_THREADS, 1, 0};
   long long n = (rows + LN_WARPS - 1) / LN_WARPS;
@@ -449,29 +508,36 @@ static LnForm ln_form(long long rows, int width, bool wide, bool backward) {   /
   else if (width > 32 * many) {
     n = rows;
     f.threads = (width + 32 * many - 1) / (32 * many) * 32;
-    const int most = backward ? 256 : 512;
-    while (f.threads > most) f.threads = (f.threads / 2 + 31) / 32 * 32, f.share *= 2;
+    while (f.threads > 512) f.threads = (f.threads / 2 + 31) / 32 * 32, f.share *= 2;
     f.most = f.threads <= 128 ? 128 : f.threads <= 256 ? 256 : 512;
   }
-  long long at_once = (long long)sm_count() * ln_ctas(f.most, f.elems, backward) / f.share;
+  long long at_once = (long long)sm_count() * ln_ctas(f.most, f.elems, backward, ring) / f.share;
   if (f.most && f.threads < 128) at_once = at_once * 128 / f.threads;
   f.groups = (int)(n < at_once ? n : at_once);
   return f;
 }
 template <class T, class W, int VN>
-static void ln_launch(const LnArgs& a, bool backward, cudaStream_t s) {
+static int ln_launch(const LnArgs& a, bool backward, cudaStream_t s) {
   constexpr bool WIDE = sizeof(T) == 2 && VN > 1;
   constexpr int MANY = WIDE ? 32 : 16, FEW = WIDE ? 8 : 4;
-  const LnForm f = ln_form(a.rows, a.width, WIDE, backward);
+  const LnForm f = ln_form(a.rows, a.width, WIDE, backward, VN > 1);
 #define LN_GO(E, MOST)                                                                                                                   \
-  backward ? launch_clusters(k_layer_norm_backward<T, W, VN, E, MOST>, f.groups * f.share, f.threads, MOST ? f.share : 0, 0, s, a)       \
-           : launch_clusters(k_layer_norm<T, W, VN, E, MOST>, f.groups * f.share, f.threads, MOST ? f.share : 0, 0, s, a)
-  if (f.most == 128) LN_GO(MANY, 128);
-  else if (f.most == 256) LN_GO(MANY, 256);
-  else if (f.most == 512) launch_clusters(k_layer_norm<T, W, VN, MANY, 512>, f.groups * f.share, f.threads, f.share, 0, s, a);
-  else if (f.elems == FEW) LN_GO(FEW, 0);
-  else if (WIDE && f.elems == 16) LN_GO(16, 0);
-  else LN_GO(MANY, 0);
+  if (!backward) launch_clusters(k_layer_norm<T, W, VN, E, MOST>, f.groups * f.share, f.threads, MOST ? f.share : 0, 0, s, a);           \
+  else {                                                                                                                                 \
+    const int smem = VN > 1 ? LN_DEPTH * 2 * (E / VN) * 16 * f.threads : 0;                                                              \
+    static bool configured[PYLO_MAX_DEVICES] = {};                                                                                       \
+    if (int rc = VN > 1 ? allow_dynamic_smem(k_layer_norm_backward<T, W, VN, E, MOST>, LN_DEPTH * 2 * (E / VN) * 16 * (MOST ? MOST : LN_WARP_THREADS), configured) : 0) return rc; \
+    if (VN > 1 && f.groups > sm_count()) t_plain_next = true;   /* as many CTAs as an SM is to hold need more than a predecessor leaves of it */ \
+    launch_clusters(k_layer_norm_backward<T, W, VN, E, MOST>, f.groups * f.share, f.threads, MOST ? f.share : 0, smem, s, a);            \
+  }                                                                                                                                      \
+  return 0;
+  if (f.most == 128) { LN_GO(MANY, 128) }
+  if (f.most == 256) { LN_GO(MANY, 256) }
+  if (f.most == 512) { LN_GO(MANY, 512) }
+  if (f.elems == FEW) { LN_GO(FEW, 0) }
+  if constexpr (WIDE)
+    if (f.elems == 16) { LN_GO(16, 0) }
+  LN_GO(MANY, 0)
 #undef LN_GO
 }
 // 16 bytes at a time where every row begins on their boundary
@@ -481,17 +547,17 @@ static bool ln_aligned(const pylo_norm* n, bool backward) {
   return p % 16 == 0 && (n->width | n->x_stride | (backward ? n->dy_stride : 0)) % vec == 0;
 }
 template <class T, class W>
-static void ln_run(const LnArgs& a, bool aligned, bool backward, cudaStream_t s) {
-  aligned ? ln_launch<T, W, RW_VEC<T>>(a, backward, s) : ln_launch<T, W, 1>(a, backward, s);
+static int ln_run(const LnArgs& a, bool aligned, bool backward, cudaStream_t s) {
+  return aligned ? ln_launch<T, W, RW_VEC<T>>(a, backward, s) : ln_launch<T, W, 1>(a, backward, s);
 }
 static int ln_any(const LnArgs& a, int type, int weight_type, bool aligned, bool backward, cudaStream_t s) {
-  if (type == PYLO_FP32 && weight_type == PYLO_FP32) ln_run<float, float>(a, aligned, backward, s);
-  else if (type == PYLO_BF16 && weight_type == PYLO_BF16) ln_run<__nv_bfloat16, __nv_bfloat16>(a, aligned, backward, s);
-  else if (type == PYLO_FP16 && weight_type == PYLO_FP16) ln_run<__half, __half>(a, aligned, backward, s);
-  else if (type == PYLO_BF16 && weight_type == PYLO_FP32) ln_run<__nv_bfloat16, float>(a, aligned, backward, s);
-  else if (type == PYLO_FP16 && weight_type == PYLO_FP32) ln_run<__half, float>(a, aligned, backward, s);
-  else return -1;
-  return launch_status();
+  int rc = -1;
+  if (type == PYLO_FP32 && weight_type == PYLO_FP32) rc = ln_run<float, float>(a, aligned, backward, s);
+  else if (type == PYLO_BF16 && weight_type == PYLO_BF16) rc = ln_run<__nv_bfloat16, __nv_bfloat16>(a, aligned, backward, s);
+  else if (type == PYLO_FP16 && weight_type == PYLO_FP16) rc = ln_run<__half, __half>(a, aligned, backward, s);
+  else if (type == PYLO_BF16 && weight_type == PYLO_FP32) rc = ln_run<__nv_bfloat16, float>(a, aligned, backward, s);
+  else if (type == PYLO_FP16 && weight_type == PYLO_FP32) rc = ln_run<__half, float>(a, aligned, backward, s);
+  return rc ? rc : launch_status();
 }
 static size_t rw_bytes(int type) { return type == PYLO_FP32 ? 4 : 2; }
 static bool rw_type(int type) { return type == PYLO_FP32 || type == PYLO_BF16 || type == PYLO_FP16; }
@@ -818,19 +884,6 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_teachers(const DtAr
 #define DL_KEPT 16   // pieces of a row that stay in the ring of 24
 __host__ __device__ constexpr int dl_ring(int what) { return what == (DT_LOSS | DT_GRAD) ? 24 : 16; }
 __host__ __device__ constexpr int dl_ctas(int stream, int what) { return 768 * 16 / dl_ring(what) / stream; }   // of an SM: 192 KB of rings
-// all copies of this thread but the last n groups have arrived
-__device__ __forceinline__ void rw_arrived(int n) {
-  switch (n) {
-#define RW_CASE(N) case N: asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); break;
-    RW_CASE(1) RW_CASE(2) RW_CASE(3) RW_CASE(4) RW_CASE(5) RW_CASE(6) RW_CASE(7) RW_CASE(8) RW_CASE(9) RW_CASE(10) RW_CASE(11)
-    RW_CASE(12) RW_CASE(13) RW_CASE(14) RW_CASE(15) RW_CASE(16) RW_CASE(17) RW_CASE(18) RW_CASE(19) RW_CASE(20) RW_CASE(21) RW_CASE(22) RW_CASE(23)
-#undef RW_CASE
-    default: asm volatile("cp.async.wait_group 0;" ::: "memory");
-  }
-}
-__device__ __forceinline__ void rw_copy(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
-__device__ __forceinline__ void rw_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-
 template <class T, int DO, int STREAM>
 __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(const DtArgs a) {
   extern __shared__ __align__(16) unsigned char dt_raw[];
@@ -903,7 +956,7 @@ __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(co
   };
   auto take = [&] {
     RwPiece<T, VN> v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]) : "r"(ring + out) : "memory");
+    v.from_shared(ring + out);
     out = out == (RING - 1) * STEP ? 0 : out + STEP;
     return v;
   };
@@ -1224,7 +1277,7 @@ extern "C" {
 
 int64_t pylo_b200_layer_norm_workspace(int64_t rows, int width) {
   if (rows <= 0 || width <= 0 || width > LN_MOST) return 0;
-  const int a = ln_form(rows, width, false, true).groups, b = ln_form(rows, width, true, true).groups;
+  const int a = ln_form(rows, width, false, true, true).groups, b = ln_form(rows, width, true, true, true).groups;   // (those without rings have fewer)
   return (int64_t)(a > b ? a : b) * 2 * width;
 }
 
@@ -1242,7 +1295,7 @@ int pylo_b200_layer_norm_backward(const pylo_norm* n, void* stream) {
   CHECK_ARG(n && n->rows >= 0 && n->width > 0 && n->width <= LN_MOST && rw_type(n->type));
   cudaStream_t s = (cudaStream_t)stream;
   const bool columns = n->dweight || n->dbias, aligned = ln_aligned(n, true);
-  const int groups = n->rows ? ln_form(n->rows, n->width, aligned && n->type != PYLO_FP32, true).groups : 0;
+  const int groups = n->rows ? ln_form(n->rows, n->width, aligned && n->type != PYLO_FP32, true, aligned).groups : 0;
   CHECK_ARG(!columns || groups == 0 || (n->work && n->work_floats >= (int64_t)groups * 2 * n->width));
   if (groups) {
     CHECK_ARG(n->x && n->dy && n->mean && n->rstd && n->x_stride >= 0 && n->dy_stride >= 0);
