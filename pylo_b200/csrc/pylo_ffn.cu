@@ -109,6 +109,21 @@ __device__ __forceinline__ void ff_mma(uint32_t d, uint64_t a, uint64_t b, uint3
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
+// A kernel that is launched while its predecessor runs must not take tensor memory that the latter has yet to ask for, nor let a successor take what it
+// has yet to ask for itself: each would wait for the other.  So, other than pdl_begin(): wait, allocate, and only then let the next kernel be set up.
+template <bool PAIR>
+__device__ __forceinline__ void ff_take_tmem(uint32_t* at, int columns, int warp) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(columns) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(columns) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+}
 // Descriptor of a 128-byte-swizzled operand of 64 x 64 boxes.  K-major: rows of 64 k, groups of eight rows 1024 bytes apart, boxes one behind
 // the other.  MN-major: rows are k and hold 64 mn, groups of eight k 1024 bytes apart, boxes of 64 mn FF_BOX apart.
 __device__ __forceinline__ uint64_t ff_desc(uint32_t saddr, int mn) {
@@ -164,11 +179,13 @@ struct ff_kept {
 };
 struct ff_product {
   CUtensorMap A[2], B[2];   // the two parts of the contraction; GATE: B is Wg, Wu
+  CUtensorMap Cm;           // of C, where mapped
   void* C;                  // PLAIN: [M][ldc]
   long long ldc;
   int M, N, K;              // of each part; GATE, BACK: N = hidden
   int parts;                // of the contraction: 1 or 2
   int a_mn, b_mn;           // the operand's rows are the contraction index
+  int mapped;               // C's rows begin on 16-byte boundaries: it is written by copies from shared memory
   int tiles_m, tiles_n, tile0;   // tile0: tiles of the products before this one
 };
 struct ff_args {
@@ -327,20 +344,12 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
     sm.abort = 0;
   }
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  if (warp == 1) {
-    if constexpr (PAIR) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)), "r"(512) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)), "r"(512) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-  }
+  ff_take_tmem<PAIR>(&sm.tmem, 512, warp);
   ff_fence_before();
   __syncthreads();
   cluster_sync();   // the other CTAs' barriers exist
   ff_fence_after();
-  pdl_begin();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
   const int step = (int)gridDim.x / ctas, first = (int)blockIdx.x / ctas;
   // the product a tile belongs to and its place there: bands of FF_BAND rows of tiles, column by column
@@ -502,7 +511,26 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
             uint32_t w[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[j] = ff_pack<BF>(v[2 * j], v[2 * j + 1]);
-            ff_store16(stage, w, (uint16_t*)p.C + (long long)m0 * p.ldc + n0, p.ldc, rows, cols);
+            if (!p.mapped) ff_store16(stage, w, (uint16_t*)p.C + (long long)m0 * p.ldc + n0, p.ldc, rows, cols);
+            else {
+              // 64 columns to a copy, rows of 128 bytes in its swizzle
+              if (!(q & 1)) {
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the copy before has read the stage
+                __syncwarp();
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint4*>(stage + lane * 128 + 16 * ((4 * (q & 1) + i) ^ (lane & 7))) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+              if ((q & 1) || cols <= 32) {   // (what lies behind the matrix is not written, whatever the stage holds there)
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+                               ::"l"(&p.Cm), "r"(smem_addr(stage)), "r"(n0 - 32 * (q & 1)), "r"(m0) : "memory");
+                  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
+              }
+            }
           } else if constexpr (EPI == FF_GATE) {
             float g[32], u[32], q_[32];
             tile_sums(block, g);
@@ -549,6 +577,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
         read();
       }
     }
+    if (EPI == FF_PLAIN && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   ff_fence_before();
   __syncthreads();
@@ -561,6 +590,212 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
     if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Few rows (32 at most): the weights' bytes are the cost, so as many of them as possible are on their way.  The weights are operand A, 128 rows of them to
+// a tile, the rows of x operand B, ROWS = 16 or 32 of them: a stage is 16 KB of weights and 2 or 4 KB of the rest (the tiles above hold 16 KB of each,
+// nearly all of the latter zeros), and two CTAs share an SM.  A tile's sums lie feature by feature in the lanes, row by row in the columns, so that a
+// warp's lanes write neighbours.  The CTAs of a cluster share a tile as above.  Gate: a tile has 64 rows of Wg and the same 64 of Wu; the warps
+// of the latter hand their sums to those of the former.
+// ------------------------------------------------------------------------------------------------
+#define FF_FEW 32
+#define FF_FEW_THREADS 192
+template <int ROWS>
+struct FfFewSmem {
+  static constexpr int STAGES = ROWS == 16 ? 6 : 5, B_BYTES = ROWS * 128, STAGE = 2 * FF_BOX + B_BYTES;
+  unsigned char st[STAGES][STAGE];
+  uint64_t full[STAGES], empty[STAGES], ready, sums;
+  uint32_t tmem;
+  volatile int abort;
+};
+__device__ __forceinline__ float ff_load24(const uint16_t* hi, const uint8_t* lo, long long i) {
+  return __uint_as_float((uint32_t)hi[i] << 16 | (uint32_t)lo[i] << 8);
+}
+__device__ __forceinline__ void ff_keep24(uint16_t* hi, uint8_t* lo, long long i, float v) {
+  const uint32_t b = ff_round24(v);
+  hi[i] = (uint16_t)(b >> 16);
+  lo[i] = (uint8_t)(b >> 8);
+}
+template <bool BF>
+__device__ __forceinline__ uint16_t ff_one(float v) { return (uint16_t)ff_pack<BF>(v, 0.f); }
+
+template <int EPI, bool BF, int ROWS>
+__global__ void __launch_bounds__(FF_FEW_THREADS, 2) k_ffn_few(const __grid_constant__ ff_args a) {
+  extern __shared__ unsigned char ff_dyn[];
+  using Smem = FfFewSmem<ROWS>;
+  constexpr int STAGES = Smem::STAGES, COLUMNS = 32, OUT_M = EPI == FF_GATE ? 64 : 128;
+  Smem& sm = *reinterpret_cast<Smem*>(ff_dyn + ((1024 - (smem_addr(ff_dyn) & 1023)) & 1023));   // at the same place in all CTAs of a cluster
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int rank = (int)ff_cluster_rank(), ctas = (int)ff_cluster_size();
+  const ff_product& p = a.p[0];
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) { ff_init(&sm.full[s], 1); ff_init(&sm.empty[s], 1); }
+    ff_init(&sm.ready, 1);
+    ff_init(&sm.sums, ctas > 1 ? (ctas - 1) * 4 : 1);
+    sm.abort = 0;
+  }
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  ff_take_tmem<false>(&sm.tmem, COLUMNS, warp);
+  ff_fence_before();
+  __syncthreads();
+  cluster_sync();   // the other CTAs' barriers exist
+  ff_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+  const int tile = (int)blockIdx.x / ctas, per_part = (p.K + FF_BK - 1) / FF_BK, n_kb = per_part * p.parts, per = (n_kb + ctas - 1) / ctas;
+  const int kb0 = min(rank * per, n_kb), kb1 = min(kb0 + per, n_kb);
+  if (warp == 0) {
+    // ---------------------------------------------------------------- copies
+    if (ff_elect()) {
+      asm volatile("fence.proxy.async;" ::: "memory");   // what earlier kernels stored is read through the async proxy
+      uint32_t n = 0;
+      bool dead = false;
+      for (int kb = kb0; kb < kb1; ++kb, ++n) {
+        const uint32_t s = n % STAGES, use = n / STAGES;
+        if (use > 0 && !ff_wait(&sm.empty[s], (use - 1) & 1, &sm.abort)) { dead = true; break; }
+        ff_expect(&sm.full[s], Smem::STAGE);   // boxes that reach beyond the matrix are filled with zeros and count in full
+        const uint32_t bar = smem_addr(&sm.full[s]);
+        const int part = kb >= per_part, k = (kb - part * per_part) * FF_BK;
+        uint32_t dst = smem_addr(sm.st[s]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u, dst += FF_BOX) {
+          const int mn = EPI == FF_GATE ? tile * 64 : tile * 128 + 64 * u, which = EPI == FF_GATE ? u : part;
+          ff_copy<false>(dst, &p.A[which], bar, p.a_mn ? mn : k, p.a_mn ? k : mn);
+        }
+        ff_copy<false>(dst, &p.B[part], bar, k, 0);
+      }
+      // the CTA must not end while a copy into its shared memory is in flight
+      if (dead || sm.abort)
+        for (uint32_t f = n > STAGES ? n - STAGES : 0; f < n; ++f)
+          for (int it = 0; it < FF_SPIN_LIMIT; ++it)
+            if (ff_try(&sm.full[f % STAGES], (f / STAGES) & 1)) break;
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- products
+    if (ff_elect()) {
+      uint32_t n = 0;
+      bool dead = false;
+      const uint32_t idesc = ff_idesc(128, ROWS, p.a_mn, 0, BF);
+      const uint64_t a_step = (p.a_mn ? 2048 : 32) >> 4;   // 16 terms further
+      for (int kb = kb0; kb < kb1; ++kb, ++n) {
+        const uint32_t s = n % STAGES;
+        if (!ff_wait(&sm.full[s], (n / STAGES) & 1, &sm.abort)) { dead = true; break; }
+        ff_fence_after();
+        const uint64_t da = ff_desc(smem_addr(sm.st[s]), p.a_mn), db = ff_desc(smem_addr(sm.st[s]) + 2 * FF_BOX, 0);
+#pragma unroll
+        for (int ks = 0; ks < FF_BK / 16; ++ks) ff_mma<false>(tmem, da + ks * a_step, db + ks * 2, idesc, kb > kb0 || ks > 0);
+        ff_commit<false>(&sm.empty[s]);
+      }
+      if (!dead) ff_commit<false>(&sm.ready);
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- a thread per feature
+    const int quarter = warp & 3, at = quarter * 32 + lane;   // of the tile's 128
+    bool good = ff_wait(&sm.ready, 0, &sm.abort);
+    ff_fence_after();
+    float v[ROWS];
+    if (good) {
+#pragma unroll
+      for (int j = 0; j < ROWS; j += 16) {
+        uint32_t r[16];
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+              "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(tmem + ((uint32_t)(quarter * 32) << 16) + j) : "memory");
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[j + i] = kb1 > kb0 ? __uint_as_float(r[i]) : 0.f;   // (no share of the contraction: nothing has been written there)
+      }
+    }
+    float* const box = reinterpret_cast<float*>(sm.st);   // the stages are free: all products are done
+    if (rank > 0) {
+      if (good) {
+#pragma unroll
+        for (int n = 0; n < ROWS; ++n) box[n * 128 + at] = v[n];
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(nf_at_rank(&sm.sums, 0)) : "memory");
+      }
+    } else {
+      if (good && ctas > 1) {
+        good = ff_wait(&sm.sums, 0, &sm.abort);
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        if (good)
+          for (int r = 1; r < ctas; ++r) {   // in rank order
+            const uint32_t src = nf_at_rank(box + at, r);
+#pragma unroll
+            for (int n = 0; n < ROWS; ++n) {
+              float o;
+              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(src + 512 * n) : "memory");
+              v[n] += o;
+            }
+          }
+      }
+      good = __all_sync(0xffffffffu, good);
+      const int f = tile * OUT_M + (EPI == FF_GATE ? at & 63 : at);   // the feature
+      if constexpr (EPI == FF_GATE) {
+        if (at >= 64) {
+#pragma unroll
+          for (int n = 0; n < ROWS; ++n) box[n * 64 + at - 64] = v[n];
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");   // the four warps of the epilogue
+        if (good && at < 64 && f < p.M) {
+#pragma unroll
+          for (int n0 = 0; n0 < ROWS; n0 += 8) {   // eight rows at a time
+            if (n0 >= p.N) break;
+#pragma unroll
+            for (int n = n0; n < n0 + 8; ++n)
+              if (n < p.N) {
+                const float u = box[n * 64 + at];
+                float q, slope;
+                ff_act(a.activation, v[n], q, slope);
+                const long long i = n * a.ld + f;
+                a.kept.h[i] = ff_one<BF>(q * u);
+                if (a.keep) {
+                  ff_keep24(a.kept.p_hi, a.kept.p_lo, i, u * slope);
+                  ff_keep24(a.kept.q_hi, a.kept.q_lo, i, q);
+                }
+              }
+          }
+        }
+      } else if (good && f < p.M) {
+#pragma unroll
+        for (int n0 = 0; n0 < ROWS; n0 += 8) {
+          if (n0 >= p.N) break;
+          if constexpr (EPI == FF_PLAIN) {
+#pragma unroll
+            for (int n = n0; n < n0 + 8; ++n)
+              if (n < p.N) ((uint16_t*)p.C)[n * p.ldc + f] = ff_one<BF>(v[n]);
+          } else {
+            float pf[8], qf[8];   // on their way together
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const long long i = (long long)min(n0 + j, p.N - 1) * a.ld + f;
+              pf[j] = ff_load24(a.kept.p_hi, a.kept.p_lo, i);
+              qf[j] = ff_load24(a.kept.q_hi, a.kept.q_lo, i);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (n0 + j < p.N) {
+                const long long i = (n0 + j) * a.ld + f;
+                a.dg[i] = ff_one<BF>(v[n0 + j] * pf[j]);
+                a.du[i] = ff_one<BF>(v[n0 + j] * qf[j]);
+              }
+          }
+        }
+      }
+    }
+  }
+  ff_fence_before();
+  __syncthreads();
+  cluster_sync();   // no CTA leaves while another may reach into its shared memory
+  if (tid == 0 && sm.abort) {
+    if (a.status) atomicOr(a.status, 16);
+    if (a.host_status) *reinterpret_cast<volatile int*>(a.host_status) = 16;
+  }
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLUMNS) : "memory");
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -577,12 +812,12 @@ static FfEncode ff_encode() {
   }();
   return fn;
 }
-// [rows][cols] of 16-bit elements, boxes of 64 x 64; what a box reaches beyond the matrix reads as zero
-static int ff_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int type) {
+// [rows][cols] of 16-bit elements, boxes of so many rows of 64; what a box reaches beyond the matrix reads as zero
+static int ff_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int type, int box_rows = 64) {
   FfEncode fn = ff_encode();
   if (!fn) return -5;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {64, 64}, unit[2] = {1, 1};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, unit[2] = {1, 1};
   return fn(map, type == PYLO_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, unit,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -5;
 }
@@ -663,10 +898,35 @@ static int ff_run(const ff_args& all, int type, cudaStream_t s) {
     }
   return 0;
 }
+// Few rows: a.p[0] as it is for many, C[rows][features]; the operands change places
+template <int EPI, bool BF, int ROWS>
+static int ff_go_few(ff_args& a, cudaStream_t s) {
+  constexpr int SMEM = (int)sizeof(FfFewSmem<ROWS>) + 1024;
+  const int tiles = (a.p[0].M + (EPI == FF_GATE ? 63 : 127)) / (EPI == FF_GATE ? 64 : 128), blocks = (a.p[0].K + FF_BK - 1) / FF_BK * a.p[0].parts;
+  static bool configured[PYLO_MAX_DEVICES] = {};
+  if (int rc = allow_dynamic_smem(k_ffn_few<EPI, BF, ROWS>, SMEM, configured)) return rc;
+  // the CTAs that share a tile: as many as run at once, each with two stages at least
+  int cluster = 1;
+  while (cluster < 8 && blocks >= cluster * 2 * 2 && tiles <= active_clusters<k_ffn_few<EPI, BF, ROWS>>(FF_FEW_THREADS, cluster * 2, SMEM)) cluster *= 2;
+  launch_clusters(k_ffn_few<EPI, BF, ROWS>, tiles * cluster, FF_FEW_THREADS, cluster, SMEM, s, a);
+  return launch_status();
+}
+template <int EPI>
+static int ff_run_few(ff_args& a, int rows, int type, cudaStream_t s) {
+  const bool bf = type == PYLO_BF16;
+  if (rows <= 16) return bf ? ff_go_few<EPI, true, 16>(a, s) : ff_go_few<EPI, false, 16>(a, s);
+  return bf ? ff_go_few<EPI, true, 32>(a, s) : ff_go_few<EPI, false, 32>(a, s);
+}
+static int ff_few_rows(int64_t rows) { return rows > FF_FEW ? 0 : rows <= 16 ? 16 : 32; }   // of a tile; 0: not few
 static bool ff_operand(const void* p, int64_t ld, int64_t cols) { return p && ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld >= cols; }
 static bool ff_good(const pylo_ffn* f) {
   return f && f->rows >= 0 && f->rows <= (1 << 30) && f->width > 0 && f->hidden > 0 && f->out > 0 && f->width <= (1 << 24) && f->hidden <= (1 << 24) &&
          f->out <= (1 << 24) && (f->type == PYLO_BF16 || f->type == PYLO_FP16) && f->activation >= PYLO_ACT_SILU && f->activation <= PYLO_ACT_RELU;
+}
+// C's map, where its rows allow for one: boxes of 32 rows of 64
+static int ff_map_c(ff_product& p, int type) {
+  p.mapped = ((uintptr_t)p.C & 15) == 0 && p.ldc % 8 == 0;
+  return p.mapped ? ff_map(&p.Cm, p.C, p.M, p.N, p.ldc, type, 32) : 0;
 }
 static ff_product ff_of(void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, int parts, int a_mn, int b_mn) {
   ff_product p = {};
@@ -692,15 +952,28 @@ int pylo_b200_gated_ffn(const pylo_ffn* f, void* stream) {
   const int64_t ld = ff_ld(f->hidden);
   ff_args a = {};
   a.kept = kept; a.ld = ld; a.n = 1; a.activation = f->activation; a.keep = f->keep; a.status = f->status; a.host_status = f->host_status;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (const int few = ff_few_rows(f->rows)) {
+    a.p[0] = ff_of(nullptr, 0, f->hidden, f->rows, f->width, 1, 0, 0);
+    if (int rc = ff_map(&a.p[0].A[0], f->w_gate, f->hidden, f->width, f->ld_gate, f->type)) return rc;
+    if (int rc = ff_map(&a.p[0].A[1], f->w_up, f->hidden, f->width, f->ld_up, f->type)) return rc;
+    if (int rc = ff_map(&a.p[0].B[0], f->x, f->rows, f->width, f->ld_x, f->type, few)) return rc;
+    if (int rc = ff_run_few<FF_GATE>(a, (int)f->rows, f->type, s)) return rc;
+    a.p[0] = ff_of(f->y, f->out, f->out, f->rows, f->hidden, 1, 0, 0);
+    if (int rc = ff_map(&a.p[0].A[0], f->w_down, f->out, f->hidden, f->ld_down, f->type)) return rc;
+    if (int rc = ff_map(&a.p[0].B[0], kept.h, f->rows, f->hidden, ld, f->type, few)) return rc;
+    return ff_run_few<FF_PLAIN>(a, (int)f->rows, f->type, s);
+  }
   a.p[0] = ff_of(nullptr, 0, f->rows, f->hidden, f->width, 1, 0, 0);
   if (int rc = ff_map(&a.p[0].A[0], f->x, f->rows, f->width, f->ld_x, f->type)) return rc;
   if (int rc = ff_map(&a.p[0].B[0], f->w_gate, f->hidden, f->width, f->ld_gate, f->type)) return rc;
   if (int rc = ff_map(&a.p[0].B[1], f->w_up, f->hidden, f->width, f->ld_up, f->type)) return rc;
-  if (int rc = ff_run<FF_GATE>(a, f->type, (cudaStream_t)stream)) return rc;
+  if (int rc = ff_run<FF_GATE>(a, f->type, s)) return rc;
   a.p[0] = ff_of(f->y, f->out, f->rows, f->out, f->hidden, 1, 0, 0);
   if (int rc = ff_map(&a.p[0].A[0], kept.h, f->rows, f->hidden, ld, f->type)) return rc;
   if (int rc = ff_map(&a.p[0].B[0], f->w_down, f->out, f->hidden, f->ld_down, f->type)) return rc;
-  return ff_run<FF_PLAIN>(a, f->type, (cudaStream_t)stream);
+  if (int rc = ff_map_c(a.p[0], f->type)) return rc;
+  return ff_run<FF_PLAIN>(a, f->type, s);
 }
 
 int pylo_b200_gated_ffn_backward(const pylo_ffn* f, void* stream) {
@@ -717,15 +990,32 @@ int pylo_b200_gated_ffn_backward(const pylo_ffn* f, void* stream) {
   a.kept = kept; a.ld = ld; a.activation = f->activation; a.status = f->status; a.host_status = f->host_status;
   a.dg = (uint16_t*)f->work;
   a.du = (uint16_t*)((char*)f->work + ff_plane(f->rows, f->hidden, 2));
+  cudaStream_t s = (cudaStream_t)stream;
+  const int few = ff_few_rows(f->rows);
   if (inner) {   // dh (m: rows, n: hidden, k: out), Wd's rows being the contraction index
     a.n = 1;
-    a.p[0] = ff_of(nullptr, 0, f->rows, f->hidden, f->out, 1, 0, 1);
-    if (int rc = ff_map(&a.p[0].A[0], f->dy, f->rows, f->out, f->ld_dy, f->type)) return rc;
-    if (int rc = ff_map(&a.p[0].B[0], f->w_down, f->out, f->hidden, f->ld_down, f->type)) return rc;
-    if (int rc = ff_run<FF_BACK>(a, f->type, (cudaStream_t)stream)) return rc;
+    if (few) {
+      a.p[0] = ff_of(nullptr, 0, f->hidden, f->rows, f->out, 1, 1, 0);
+      if (int rc = ff_map(&a.p[0].A[0], f->w_down, f->out, f->hidden, f->ld_down, f->type)) return rc;
+      if (int rc = ff_map(&a.p[0].B[0], f->dy, f->rows, f->out, f->ld_dy, f->type, few)) return rc;
+      if (int rc = ff_run_few<FF_BACK>(a, (int)f->rows, f->type, s)) return rc;
+    } else {
+      a.p[0] = ff_of(nullptr, 0, f->rows, f->hidden, f->out, 1, 0, 1);
+      if (int rc = ff_map(&a.p[0].A[0], f->dy, f->rows, f->out, f->ld_dy, f->type)) return rc;
+      if (int rc = ff_map(&a.p[0].B[0], f->w_down, f->out, f->hidden, f->ld_down, f->type)) return rc;
+      if (int rc = ff_run<FF_BACK>(a, f->type, s)) return rc;
+    }
+  }
+  if (f->dx && few) {
+    a.p[0] = ff_of(f->dx, f->width, f->width, f->rows, f->hidden, 2, 1, 0);
+    if (int rc = ff_map(&a.p[0].A[0], f->w_gate, f->hidden, f->width, f->ld_gate, f->type)) return rc;
+    if (int rc = ff_map(&a.p[0].A[1], f->w_up, f->hidden, f->width, f->ld_up, f->type)) return rc;
+    if (int rc = ff_map(&a.p[0].B[0], a.dg, f->rows, f->hidden, ld, f->type, few)) return rc;
+    if (int rc = ff_map(&a.p[0].B[1], a.du, f->rows, f->hidden, ld, f->type, few)) return rc;
+    if (int rc = ff_run_few<FF_PLAIN>(a, (int)f->rows, f->type, s)) return rc;
   }
   a.n = 0;
-  if (f->dx) {
+  if (f->dx && !few) {
     ff_product& p = a.p[a.n++] = ff_of(f->dx, f->width, f->rows, f->width, f->hidden, 2, 0, 1);
     if (int rc = ff_map(&p.A[0], a.dg, f->rows, f->hidden, ld, f->type)) return rc;
     if (int rc = ff_map(&p.A[1], a.du, f->rows, f->hidden, ld, f->type)) return rc;
@@ -743,7 +1033,9 @@ int pylo_b200_gated_ffn_backward(const pylo_ffn* f, void* stream) {
     if (int rc = ff_map(&p.A[0], f->dy, f->rows, f->out, f->ld_dy, f->type)) return rc;
     if (int rc = ff_map(&p.B[0], kept.h, f->rows, f->hidden, ld, f->type)) return rc;
   }
-  return a.n ? ff_run<FF_PLAIN>(a, f->type, (cudaStream_t)stream) : 0;
+  for (int k = 0; k < a.n; ++k)
+    if (int rc = ff_map_c(a.p[k], f->type)) return rc;
+  return a.n ? ff_run<FF_PLAIN>(a, f->type, s) : 0;
 }
 
 int pylo_b200_sizeof_layers(int what) {
