@@ -648,7 +648,15 @@ int64_t pylo_b200_gated_ffn_kept(int64_t rows, int hidden, int keep);
 int64_t pylo_b200_gated_ffn_workspace(int64_t rows, int hidden);
 int pylo_b200_gated_ffn(const pylo_ffn* f, void* stream);
 int pylo_b200_gated_ffn_backward(const pylo_ffn* f, void* stream);
-/* bytes of pylo_norm (0), pylo_distill (1), pylo_ffn (2) */
+/* Copies of up to 4 matrices of 16-bit elements, of any strides, with rows ld elements apart (ld % 8 = 0; dst on a 16-byte boundary): operands
+ * of the block that do not lie as it wants them.  What lies between a row's end and ld is zero. */
+typedef struct pylo_pad {
+  const void* src;
+  void* dst;
+  int64_t rows, cols, row_stride, col_stride, ld;
+} pylo_pad;
+int pylo_b200_pad_rows(const pylo_pad* items, int n, void* stream);
+/* bytes of pylo_norm (0), pylo_distill (1), pylo_ffn (2), pylo_pad (3) */
 int pylo_b200_sizeof_layers(int what);
 
 #ifdef __cplusplus

@@ -153,6 +153,11 @@ class Ffn(C.Structure):
         (name, C.c_int32) for name in ("width", "hidden", "out", "type", "activation", "keep")] + [("status", C.c_void_p), ("host_status", C.c_void_p)]
 
 
+class Pad(C.Structure):
+    """pylo_pad: a matrix that is copied so that its rows begin on 16-byte boundaries."""
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p)] + [(name, C.c_int64) for name in ("rows", "cols", "row_stride", "col_stride", "ld")]
+
+
 DISTILL_LOSS, DISTILL_GRAD = 1, 2
 REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
 ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU = 0, 1, 2, 3
@@ -222,6 +227,7 @@ def _load():
         "pylo_b200_gated_ffn_backward": [C.POINTER(Ffn), vp],
         "pylo_b200_gated_ffn_kept": [C.c_int64, i32, i32],
         "pylo_b200_gated_ffn_workspace": [C.c_int64, i32],
+        "pylo_b200_pad_rows": [C.POINTER(Pad), i32, vp],
     }
     for name, argtypes in sigs.items():
         fn = getattr(lib, name)  # AttributeError if a declared symbol is missing
@@ -232,7 +238,7 @@ def _load():
         raise ImportError("libpylo_b200.so was built from a different ABI version; rebuild it")
     if (lib.pylo_b200_sizeof_desc() != DESC_DTYPE.itemsize or lib.pylo_b200_sizeof_params() != C.sizeof(StepParams)
             or [lib.pylo_b200_sizeof_adamw(k) for k in range(3)] != [ADAMW_DTYPE.itemsize, C.sizeof(AdamwSet), C.sizeof(AdamwCall)]
-            or [lib.pylo_b200_sizeof_layers(k) for k in range(3)] != [C.sizeof(Norm), C.sizeof(Distill), C.sizeof(Ffn)]):
+            or [lib.pylo_b200_sizeof_layers(k) for k in range(4)] != [C.sizeof(Norm), C.sizeof(Distill), C.sizeof(Ffn), C.sizeof(Pad)]):
         raise ImportError("descriptor layout mismatch between the Python binding and libpylo_b200.so")
     return lib, sorted(sigs)
 

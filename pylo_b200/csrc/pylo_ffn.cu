@@ -236,7 +236,8 @@ __device__ __forceinline__ void ff_store16(unsigned char* s, const uint32_t (&w)
       }
     }
   } else if (lane < cols) {   // rows that begin anywhere: a row at a time
-    for (int r = 0; r < 32 && r < rows; ++r)
+#pragma unroll 8
+    for (int r = 0; r < min(32, rows); ++r)
       dst[r * ld + lane] = reinterpret_cast<const uint16_t*>(ff_at64(s, r, lane >> 3))[lane & 7];
   }
 }
@@ -799,6 +800,33 @@ __global__ void __launch_bounds__(FF_FEW_THREADS, 2) k_ffn_few(const __grid_cons
 }
 
 // ------------------------------------------------------------------------------------------------
+// Operands whose rows do not begin on 16-byte boundaries, copied so that they do: 16 bytes of the copy to a thread, all matrices in one launch
+// ------------------------------------------------------------------------------------------------
+#define FF_PADS 4
+struct ff_pads {
+  pylo_pad p[FF_PADS];
+  long long first[FF_PADS + 1];   // pieces of 8 elements of the matrices before
+  int n;
+};
+__global__ void __launch_bounds__(NT) k_ffn_pad(const ff_pads a) {
+  pdl_begin();
+  for (long long i = (long long)blockIdx.x * NT + threadIdx.x; i < a.first[a.n]; i += (long long)gridDim.x * NT) {
+    int k = 0;
+    while (k + 1 < a.n && i >= a.first[k + 1]) ++k;
+    const pylo_pad& p = a.p[k];
+    const long long at = i - a.first[k];
+    const uint32_t per = (uint32_t)(p.ld / 8);
+    const long long row = at < (1ll << 32) ? (uint32_t)at / per : at / per, c = (at - row * per) * 8;
+    const uint16_t* const src = (const uint16_t*)p.src + row * p.row_stride + c * p.col_stride;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < p.cols) w[j >> 1] |= (uint32_t)src[j * p.col_stride] << (16 * (j & 1));
+    *reinterpret_cast<uint4*>((uint16_t*)p.dst + row * p.ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
 // host
 // ------------------------------------------------------------------------------------------------
 typedef CUresult (*FfEncode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -838,11 +866,16 @@ static ff_kept ff_planes(void* base, int64_t rows, int hidden) {
   return {(uint16_t*)p, (uint16_t*)(p + two), (uint16_t*)(p + 2 * two), (uint8_t*)(p + 3 * two), (uint8_t*)(p + 3 * two + one)};
 }
 
-// Which form a product takes.  Pairs where their tiles fill the GPU more than half (74 run at once): rows x 1024 by 1024 x 4096, both projections,
-// 512 rows (64 tiles) 17 us and 22 in tiles of 128 x 128, 256 rows (32) 16 and 13.
-static bool ff_pairs(const ff_product& p, int epi) {
-  const int64_t n = (p.N + (epi == FF_GATE ? 127 : 255)) / (epi == FF_GATE ? 128 : 256);
-  return (int64_t)((p.M + 255) / 256) * n >= 48;
+// Which form a product takes.  Pairs where their tiles, with those of the products beside it whose contractions are equally long, fill the GPU more than half
+// (74 run at once): rows x 1024 by 1024 x 4096, both projections, 512 rows (64 tiles) 17 us and 22 in tiles of 128 x 128, 256 rows (32) 16 and 13.
+static int ff_length(const ff_product& p) { return p.K * p.parts; }
+static bool ff_pairs(const ff_args& all, const ff_product& q, int epi) {
+  int64_t tiles = 0;
+  for (int k = 0; k < all.n; ++k) {
+    const ff_product& p = all.p[k];
+    if (ff_length(p) == ff_length(q)) tiles += (int64_t)((p.M + 255) / 256) * ((p.N + (epi == FF_GATE ? 127 : 255)) / (epi == FF_GATE ? 128 : 256));
+  }
+  return tiles >= 48;
 }
 template <bool PAIR, int EPI, bool BF>
 static int ff_go(ff_args& a, cudaStream_t s) {
@@ -881,21 +914,26 @@ static int ff_go(ff_args& a, cudaStream_t s) {
   launch_clusters(k_ffn_product<PAIR, EPI, BF>, grid, FF_THREADS, cluster, SMEM, s, a);
   return launch_status();
 }
-// The products of a that take pairs in one launch, the others in one each
+// The products of a that take pairs in one launch, the others in one for those whose contractions are equally long
 template <int EPI>
 static int ff_run(const ff_args& all, int type, cudaStream_t s) {
   ff_args a = all;
   a.n = 0;
   for (int k = 0; k < all.n; ++k)
-    if (ff_pairs(all.p[k], EPI)) a.p[a.n++] = all.p[k];
+    if (ff_pairs(all, all.p[k], EPI)) a.p[a.n++] = all.p[k];
   if (a.n)
     if (int rc = type == PYLO_BF16 ? ff_go<true, EPI, true>(a, s) : ff_go<true, EPI, false>(a, s)) return rc;
-  for (int k = 0; k < all.n; ++k)
-    if (!ff_pairs(all.p[k], EPI)) {
-      a.n = 1;
-      a.p[0] = all.p[k];
-      if (int rc = type == PYLO_BF16 ? ff_go<false, EPI, true>(a, s) : ff_go<false, EPI, false>(a, s)) return rc;
-    }
+  bool done[FF_GROUP] = {};
+  for (int k = 0; k < all.n; ++k) {
+    if (done[k] || ff_pairs(all, all.p[k], EPI)) continue;
+    a.n = 0;
+    for (int j = k; j < all.n; ++j)
+      if (ff_length(all.p[j]) == ff_length(all.p[k])) {
+        a.p[a.n++] = all.p[j];
+        done[j] = true;
+      }
+    if (int rc = type == PYLO_BF16 ? ff_go<false, EPI, true>(a, s) : ff_go<false, EPI, false>(a, s)) return rc;
+  }
   return 0;
 }
 // Few rows: a.p[0] as it is for many, C[rows][features]; the operands change places
@@ -1039,7 +1077,23 @@ int pylo_b200_gated_ffn_backward(const pylo_ffn* f, void* stream) {
 }
 
 int pylo_b200_sizeof_layers(int what) {
-  return what == 0 ? (int)sizeof(pylo_norm) : what == 1 ? (int)sizeof(pylo_distill) : what == 2 ? (int)sizeof(pylo_ffn) : -1;
+  return what == 0 ? (int)sizeof(pylo_norm) : what == 1 ? (int)sizeof(pylo_distill) : what == 2 ? (int)sizeof(pylo_ffn) : what == 3 ? (int)sizeof(pylo_pad) : -1;
+}
+
+int pylo_b200_pad_rows(const pylo_pad* items, int n, void* stream) {
+  CHECK_ARG(items && n >= 0 && n <= FF_PADS);
+  ff_pads a = {};
+  a.n = n;
+  for (int k = 0; k < n; ++k) {
+    const pylo_pad& p = items[k];
+    CHECK_ARG(p.rows >= 0 && p.rows <= (1 << 30) && p.cols >= 0 && p.ld >= p.cols && p.ld <= (1 << 25) && p.ld % 8 == 0 && (p.rows == 0 || (p.src && p.dst)) &&
+              ((uintptr_t)p.dst & 15) == 0 && ((uintptr_t)p.src & 1) == 0);
+    a.p[k] = p;
+    a.first[k + 1] = a.first[k] + p.rows * (p.ld / 8);
+  }
+  const long long ctas = (a.first[n] + NT - 1) / NT, most = (long long)sm_count() * 16;
+  if (ctas) launch(k_ffn_pad, (int)(ctas < most ? ctas : most), NT, 0, (cudaStream_t)stream, a);
+  return launch_status();
 }
 
 }  // extern "C"

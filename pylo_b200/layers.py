@@ -224,64 +224,103 @@ def clear_status():
         _reported[1][0] = 0
 
 
-def _operand(t):
-    """Rows as the copies to the tensor cores need them, on 16-byte boundaries: (tensor, elements between rows)."""
+def _spacing(t):
+    """Elements between the rows of a matrix that lies as the copies to the tensor cores need it, on 16-byte boundaries; else 0."""
     rows, cols = t.shape
-    if t.stride(1) == 1 and t.data_ptr() % 16 == 0:
-        if rows == 1:
-            return t, -(-cols // 8) * 8
-        if t.stride(0) % 8 == 0 and t.stride(0) >= cols:
-            return t, t.stride(0)
-    out = torch.empty((rows, -(-cols // 8) * 8), dtype=t.dtype, device=t.device)
-    out[:, :cols] = t
-    return out[:, :cols], out.stride(0)
+    if t.data_ptr() % 16 == 0:
+        if cols % 8 == 0 and t.is_contiguous():
+            return cols
+        apart, beside = t.stride()
+        if beside == 1:
+            if rows == 1:
+                return -(-cols // 8) * 8
+            if apart % 8 == 0 and apart >= cols:
+                return apart
+    return 0
 
 
-def _ffn_struct(x, w_gate, w_up, w_down, activation):
-    """The call's struct with its operands, and what has to stay alive until it is made."""
-    n, width = x.shape
-    (x, ld_x), (w_gate, ld_gate), (w_up, ld_up), (w_down, ld_down) = map(_operand, (x, w_gate, w_up, w_down))
-    f = L.Ffn(x=x.data_ptr(), w_gate=w_gate.data_ptr(), w_up=w_up.data_ptr(), w_down=w_down.data_ptr(), rows=n, ld_x=ld_x, ld_gate=ld_gate, ld_up=ld_up,
-              ld_down=ld_down, width=width, hidden=w_gate.shape[0], out=w_down.shape[0], type=TYPES[x.dtype], activation=activation,
-              host_status=_status_word())
-    return f, (x, w_gate, w_up, w_down)
+class _Operands:
+    """Matrices as the block's products take them: those that do not lie as they should are copied, all in one launch."""
+
+    def __init__(self, tensors):
+        self.apart = apart = list(map(_spacing, tensors))   # elements between rows
+        self.room, self.at = None, None                     # the copies, and where in them (bytes) each matrix is, or -1
+        if 0 not in apart:
+            return
+        first = tensors[0]
+        odd = [k for k, n in enumerate(apart) if not n]
+        items, self.at, size = (L.Pad * len(odd))(), [-1] * len(tensors), 0
+        for k in odd:
+            rows, cols = tensors[k].shape
+            apart[k] = ld = -(-cols // 8) * 8
+            self.at[k] = size
+            size += 2 * ld * rows
+        self.room = torch.empty(size, dtype=torch.uint8, device=first.device)
+        base = self.room.data_ptr()
+        for item, k in zip(items, odd):
+            t = tensors[k]
+            item.src, item.dst = t.data_ptr(), base + self.at[k]
+            item.rows, item.cols = t.shape
+            item.row_stride, item.col_stride = t.stride()
+            item.ld = apart[k]
+        _call(L.lib.pylo_b200_pad_rows, "gated_ffn", first.get_device(), items, len(odd))
+
+    def pointers(self, tensors, room):
+        if room is None:
+            return [t.data_ptr() for t in tensors]
+        base = room.data_ptr()
+        return [t.data_ptr() if at < 0 else base + at for t, at in zip(tensors, self.at)]
 
 
-def _ffn_forward(rows, w_gate, w_up, w_down, activation, keep):
-    """(y, the rows as they are saved for the backward pass, what else is)"""
-    y = torch.empty((rows.shape[0], w_down.shape[0]), dtype=rows.dtype, device=rows.device)
+def _ffn_struct(tensors, operands, room, activation):
+    x, w_gate, w_up, w_down = operands.pointers(tensors, room)
+    ld_x, ld_gate, ld_up, ld_down = operands.apart
+    (rows, width), (out, hidden) = tensors[0].shape, tensors[3].shape
+    return L.Ffn(x=x, w_gate=w_gate, w_up=w_up, w_down=w_down, rows=rows, ld_x=ld_x, ld_gate=ld_gate, ld_up=ld_up, ld_down=ld_down, width=width,
+                 hidden=hidden, out=out, type=TYPES[tensors[0].dtype], activation=activation, host_status=_status_word())
+
+
+def _ffn_forward(tensors, activation, keep):
+    """(y, how the operands lie, what is kept for the backward pass)"""
+    rows = tensors[0]
+    y = torch.empty((rows.shape[0], tensors[3].shape[0]), dtype=rows.dtype, device=rows.device)
     if not rows.shape[0]:
-        return y, rows, None
-    f, alive = _ffn_struct(rows, w_gate, w_up, w_down, activation)
-    kept = torch.empty(L.lib.pylo_b200_gated_ffn_kept(f.rows, f.hidden, keep), dtype=torch.uint8, device=rows.device)
+        return y, None, None
+    device = rows.get_device()
+    operands = _Operands(tensors)
+    f = _ffn_struct(tensors, operands, operands.room, activation)
+    kept = torch.empty(_size("pylo_b200_gated_ffn_kept", device, f.rows, f.hidden, keep), dtype=torch.uint8, device=rows.device)
     f.y, f.kept, f.keep = y.data_ptr(), kept.data_ptr(), keep
-    _call(L.lib.pylo_b200_gated_ffn, "gated_ffn", rows.get_device(), C.byref(f))
-    return y, alive[0], kept
+    _call(L.lib.pylo_b200_gated_ffn, "gated_ffn", device, C.byref(f))
+    return y, operands, kept
 
 
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, w_gate, w_up, w_down, activation):
-        y, rows, kept = _ffn_forward(rows, w_gate, w_up, w_down, activation, 1)
-        ctx.save_for_backward(rows, w_gate, w_up, w_down, kept)
-        ctx.activation = activation
+        y, operands, kept = _ffn_forward((rows, w_gate, w_up, w_down), activation, 1)
+        ctx.save_for_backward(rows, w_gate, w_up, w_down, kept, operands and operands.room)
+        if operands:
+            operands.room = None   # (it is saved)
+        ctx.operands, ctx.activation = operands, activation
         return y
 
     @staticmethod
     @_once
     def backward(ctx, dy):
-        rows, w_gate, w_up, w_down, kept = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        like = dict(dtype=rows.dtype, device=rows.device)
-        make = torch.empty if kept is not None else torch.zeros
-        grads = [make(shape, **like) if wanted else None for wanted, shape in zip(need, (rows.shape, w_gate.shape, w_up.shape, w_down.shape))]
+        *tensors, kept, room = ctx.saved_tensors
+        rows = tensors[0]
+        make = _like if kept is not None else lambda t: torch.zeros(t.shape, dtype=t.dtype, device=t.device)
+        grads = [make(t) if wanted else None for wanted, t in zip(ctx.needs_input_grad, tensors)]
         if kept is not None:
-            dy, ld = _operand(_rows(dy))
-            f, alive = _ffn_struct(rows, w_gate, w_up, w_down, ctx.activation)
-            work = torch.empty(L.lib.pylo_b200_gated_ffn_workspace(f.rows, f.hidden), dtype=torch.uint8, device=rows.device)
-            f.dy, f.ld_dy, f.kept, f.work = dy.data_ptr(), ld, kept.data_ptr(), work.data_ptr()
+            device = rows.get_device()
+            dy = _rows(dy)
+            lies = _Operands((dy,))
+            f = _ffn_struct(tensors, ctx.operands, room, ctx.activation)
+            work = torch.empty(_size("pylo_b200_gated_ffn_workspace", device, f.rows, f.hidden), dtype=torch.uint8, device=rows.device)
+            (f.dy,), (f.ld_dy,), f.kept, f.work = lies.pointers((dy,), lies.room), lies.apart, kept.data_ptr(), work.data_ptr()
             f.dx, f.dw_gate, f.dw_up, f.dw_down = (None if g is None else g.data_ptr() for g in grads)
-            _call(L.lib.pylo_b200_gated_ffn_backward, "gated_ffn backward", rows.get_device(), C.byref(f))
+            _call(L.lib.pylo_b200_gated_ffn_backward, "gated_ffn backward", device, C.byref(f))
         return *grads, None
 
 
@@ -291,7 +330,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     ``x`` is ``[..., width]``, ``w_gate`` and ``w_up`` are ``[hidden, width]``, ``w_down`` is ``[out, hidden]``; all are bf16 or all fp16.
     ``activation``: ``"silu"``, ``"gelu"`` (with the error function), ``"gelu_tanh"`` or ``"relu"``.  Sums are fp32; the hidden values, and backward
     their gradients, are rounded to the type once, where they become operands of the next product.  Sizes and strides are free; matrices whose rows do
-    not begin on 16-byte boundaries are copied first.  For a backward pass 8 bytes are kept per hidden value."""
+    not begin on 16-byte boundaries are copied first (the copies are kept for the backward pass).  For a backward pass 8 bytes are kept per hidden value."""
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"activation is {activation!r}, supported are {', '.join(ACTIVATIONS)}")
@@ -305,7 +344,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if min(*w_gate.shape, *w_down.shape) == 0 or max(*w_gate.shape, *w_down.shape) > 1 << 24 or math.prod(x.shape[:-1]) > 1 << 30:
         raise ValueError("sizes from 1 to 2^24 and up to 2^30 rows are supported")
     rows = _rows(x)
-    y = _GatedFFN.apply(rows, w_gate, w_up, w_down, code) if _graph(x, w_gate, w_up, w_down) else _ffn_forward(rows, w_gate, w_up, w_down, code, 0)[0]
+    y = _GatedFFN.apply(rows, w_gate, w_up, w_down, code) if _graph(x, w_gate, w_up, w_down) else _ffn_forward((rows, w_gate, w_up, w_down), code, 0)[0]
     return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
 
 

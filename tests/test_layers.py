@@ -533,6 +533,10 @@ def test_library_refuses_before_it_launches():
     back = {**ffn, "dy": 256, "ld_dy": 8, "work": 256, "dx": 256}
     for bad in (dict(dy=None), dict(ld_dy=4), dict(work=None), dict(work=16), dict(rows=0), dict(w_up=None), dict(kept=None)):
         assert L.lib.pylo_b200_gated_ffn_backward(C.byref(L.Ffn(**{**back, **bad})), None) < 0, bad
+    pad = dict(src=16, dst=16, rows=4, cols=5, row_stride=5, col_stride=1, ld=8)
+    for bad in (dict(src=None), dict(dst=None), dict(dst=24), dict(src=17), dict(ld=4), dict(ld=12), dict(rows=-1)):
+        assert L.lib.pylo_b200_pad_rows((L.Pad * 1)(L.Pad(**{**pad, **bad})), 1, None) < 0, bad
+    assert L.lib.pylo_b200_pad_rows((L.Pad * 5)(), 5, None) < 0
     for call in (L.lib.pylo_b200_layer_norm, L.lib.pylo_b200_layer_norm_backward, L.lib.pylo_b200_gated_ffn, L.lib.pylo_b200_gated_ffn_backward):
         assert call(None, None) < 0
 
