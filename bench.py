@@ -3,6 +3,7 @@
 
     python bench.py [--gpus N] [--steps K] [--warmup W] [--impl b200|reference]
                     [--workload llama3_8b|gpt2_medium|vit_b16|celo2_4096|mlp_784] [--optimizer adafaclo|...]
+    python bench.py --workload student_llama|student_small     a whole training step around an optimizer's (see run_student)
 
 One "step" is one ``optimizer.step()`` over every parameter tensor of the
 workload (plus, with more than one GPU, the exchange of the updated
@@ -650,6 +651,72 @@ def run_b200(args):
         raise SystemExit("replica_check failed: the ranks' parameter buffers differ after the last step")
 
 
+def run_student(args):
+    """A training step of a student model on one GPU: layer norms, gated feed-forward blocks and the distillation loss forward and
+    backward (``pylo_b200.layers``; the classifier is torch's product), clipping by the global norm and AdamW with fp32 copies of the
+    bf16 parameters."""
+    from pylo_b200 import layers, optim
+    from pylo_b200 import workloads as W
+
+    if int(os.environ.get("WORLD_SIZE", "1")) > 1:
+        raise SystemExit("the student's step runs on one GPU")
+    dev = torch.device("cuda", 0)
+    torch.cuda.set_device(dev)
+    tokens, width, hidden, blocks, classes = W.STUDENTS[args.workload]
+    torch.manual_seed(0)
+    model = W.student(width, hidden, blocks, classes, dev)
+    params = list(model.parameters())
+    opt = optim.AdamW_CUDA(params, lr=1e-4, weight_decay=0.1, master_weights=True, clip_grad=True, clip_norm=1.0)
+    batch = W.student_batch(tokens, width, classes, device=dev)
+
+    def step(batch):
+        x, teacher, ids, weights = batch
+        loss = layers.distillation_loss(model(x), teacher, ids, temperature=2.0, weights=weights)
+        loss.backward()
+        opt.step()
+        opt.zero_grad(set_to_none=True)
+        return loss.detach()
+
+    def timed(one):
+        begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        torch.cuda.synchronize()
+        begin.record()
+        for _ in range(args.steps):
+            one()
+        end.record()
+        torch.cuda.synchronize()
+        return begin.elapsed_time(end) / args.steps
+
+    for _ in range(args.warmup):
+        step(batch)
+    clocks = ClockSampler(0)
+    clocks.start()
+    ms = timed(lambda: step(batch))
+    clocks = clocks.stop()
+    layers.check_status()
+    # end to end: the step's inputs from pinned host memory, its loss back
+    host = [t.cpu().pin_memory() for t in batch]
+    ms_e2e = timed(lambda: float(step([t.to(dev, non_blocking=True) for t in host])))
+    flops = tokens * (blocks * 18 * width * hidden + 6 * width * classes)
+    emit({"metric": "student_train_tokens_per_sec", "value": tokens / ms * 1e3, "unit": "tokens/s", "n_gpus": 1, "steps": args.steps, "warmup": args.warmup,
+          "ms_per_step": ms, "higher_is_better": True, "scaling": "weak", "vs_baseline": None, "dtype": "bf16", "data": "synthetic",
+          "config": {"model": args.workload, "global_batch": tokens, "width": width, "hidden": hidden, "blocks": blocks, "classes": classes, "top": 64,
+                     "parameters": sum(p.numel() for p in params), "parallelism": "none", "cache": "inputs larger than L2" if width >= 4096 else "warm"},
+          "model_tflops": flops / ms / 1e9,
+          "e2e": {"value": tokens / ms_e2e * 1e3, "unit": "tokens/s", "h2d_bytes_per_step": sum(t.numel() * t.element_size() for t in host), "d2h_bytes_per_step": 4},
+          "gpu_launches": student_launches(step, batch) * args.steps, "clocks": clocks})
+
+
+def student_launches(step, batch):
+    """This library's kernels in one step, counted by the profiler after the timed region."""
+    import torch.profiler as P
+
+    with P.profile(activities=[P.ProfilerActivity.CUDA]) as profile:
+        step(batch)
+        torch.cuda.synchronize()
+    return sum("k_" in e.name and e.device_type == torch.autograd.DeviceType.CUDA for e in profile.events() if e.name.startswith(("void k_", "k_")))
+
+
 def run_reference_cuda(dev):
     """The reference's OWN CUDA kernels (built from its sources into oracle/_ref/ by oracle/build_ref.py) timed on
     this GPU next to this library, on a bounded sample: the "kernel to beat"."""
@@ -681,8 +748,12 @@ def main():
     _REAL_STDOUT = os.dup(1)
     os.dup2(2, 1)
     args = parse()
-    if args.impl == "reference":
+    if args.impl == "reference" and args.workload.startswith("student"):
+        emit({"impl": "reference", "unavailable": "the reference has optimizers only, no layers or losses"})
+    elif args.impl == "reference":
         run_reference(args)
+    elif args.workload.startswith("student"):
+        run_student(args)
     else:
         run_b200(args)
 

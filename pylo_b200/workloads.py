@@ -64,6 +64,42 @@ WORKLOADS = {
 }
 
 
+# (tokens, width, hidden, blocks, classes): two of Llama-3-8B's gated blocks under its vocabulary, and a small one
+STUDENTS = {"student_llama": (8192, 4096, 14336, 2, 128256), "student_small": (512, 256, 704, 2, 5003)}
+
+
+def student(width: int, hidden: int, blocks: int, classes: int, device="cuda", dtype=torch.bfloat16) -> torch.nn.Module:
+    """A model that is distilled from a teacher's largest logits: pre-norm gated feed-forward blocks with residuals, a last norm and a
+    classifier, of this package's layers (which need the CUDA library: it is loaded here and not with this module)."""
+    from . import layers
+
+    class Student(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            make = dict(device=device, dtype=dtype)
+            self.norms = torch.nn.ModuleList(layers.LayerNorm(width, **make) for _ in range(blocks + 1))
+            self.blocks = torch.nn.ModuleList(layers.GatedFFN(width, hidden, **make) for _ in range(blocks))
+            self.head = torch.nn.Linear(width, classes, bias=False, **make)
+
+        def forward(self, x):
+            for norm, block in zip(self.norms, self.blocks):
+                x = x + block(norm(x))
+            return self.head(self.norms[-1](x))
+
+    return Student()
+
+
+def student_batch(tokens: int, width: int, classes: int, top: int = 64, device="cuda", dtype=torch.bfloat16, seed: int = 3):
+    """Seeded (inputs, teacher's logits, their classes, weights of the tokens) of a student's step: one token in eight is padding."""
+    gen = torch.Generator(device=device).manual_seed(seed)
+    x = torch.randn(tokens, width, generator=gen, device=device).to(dtype)
+    teacher = torch.randn(tokens, top, generator=gen, device=device).mul_(2.0).sort(dim=1, descending=True).values.to(dtype)
+    # classes without repetition: a step through all of them from a random one on
+    first = torch.randint(classes, (tokens, 1), generator=gen, device=device)
+    ids = (first + torch.arange(top, device=device) * max(1, classes // top)) % classes
+    return x, teacher, ids, (torch.rand(tokens, generator=gen, device=device) >= 0.125).float()
+
+
 def numel(shape: Shape) -> int:
     n = 1
     for d in shape:

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from pylo_b200 import _lib as L
-from pylo_b200 import layers
+from pylo_b200 import layers, workloads
 
 gpu = pytest.mark.gpu
 F32, BF16, FP16 = torch.float32, torch.bfloat16, torch.float16
@@ -602,22 +602,6 @@ def test_a_reported_wait_stops_the_next_call(monkeypatch):
 # ---------------------------------------------------------------------------------------------------------------------
 
 
-class Student(torch.nn.Module):
-    """Two pre-norm gated blocks with residuals, a norm and a classifier."""
-
-    def __init__(self, width, hidden, classes, dtype=BF16):
-        super().__init__()
-        make = dict(device="cuda", dtype=dtype)
-        self.norms = torch.nn.ModuleList(layers.LayerNorm(width, **make) for _ in range(3))
-        self.blocks = torch.nn.ModuleList(layers.GatedFFN(width, hidden, **make) for _ in range(2))
-        self.head = torch.nn.Linear(width, classes, bias=False, **make)
-
-    def forward(self, x):
-        for norm, block in zip(self.norms, self.blocks):
-            x = x + block(norm(x))
-        return self.head(self.norms[2](x))
-
-
 def student_step(student, x, teacher, ids, weights):
     loss = layers.distillation_loss(student(x), teacher, ids, 2.0, weights)
     loss.backward()
@@ -626,7 +610,7 @@ def student_step(student, x, teacher, ids, weights):
 
 def student_and_batch(seed=0, classes=1003):
     torch.manual_seed(seed)
-    student = Student(72, 136, classes)
+    student = workloads.student(72, 136, 2, classes)
     x = randn(5, 31, 72, seed=seed + 1, dtype=BF16)
     _, teacher, ids = distill_inputs(155, classes, 16, BF16, seed=seed + 2)
     return student, (x, teacher.view(5, 31, 16), ids.view(5, 31, 16), (torch.rand(5, 31, generator=gen(seed), device="cuda") < 0.9))
@@ -759,3 +743,14 @@ def test_a_saved_input_that_is_changed_is_noticed():
     z.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.sum().backward()
+
+
+@gpu
+def test_the_benchmark_runs_a_student(monkeypatch):
+    import bench
+
+    lines = []
+    monkeypatch.setattr(bench, "emit", lines.append)
+    bench.run_student(bench.parse(["--workload", "student_small", "--steps", "2", "--warmup", "3"]))
+    (line,) = lines
+    assert line["value"] > 0 and line["e2e"]["value"] > 0 and line["gpu_launches"] > 0 and line["gpu_launches"] % 2 == 0
