@@ -29,7 +29,6 @@
 #define FF_BM 128               // rows of a CTA's tile
 #define FF_BK 64                // terms per stage
 #define FF_BOX 8192             // bytes of a box: 64 x 64 elements
-#define FF_STAGES 6             // of 32 KB
 #define FF_EPI_WARPS 8
 #define FF_THREADS ((FF_EPI_WARPS + 2) * 32)
 #define FF_SPIN_LIMIT (1 << 22)
@@ -197,12 +196,14 @@ struct ff_args {
   int *status, *host_status;
 };
 
-template <bool PAIR>
+template <int EPI>
 struct FfSmem {
+  static constexpr int STAGES = EPI == FF_BACK ? 4 : 6, OUT = EPI == FF_BACK ? 2 * 6144 : 4096;
   // per stage: A (128 x 64), B (128 x 64; of a pair one half of the tile's 256)
-  unsigned char st[FF_STAGES][4 * FF_BOX];
-  unsigned char out[FF_EPI_WARPS][4096];   // per epilogue warp: 32 rows of 32 elements on their way
-  uint64_t full[FF_STAGES], empty[FF_STAGES], ready[2], free[2], sums;
+  unsigned char st[STAGES][4 * FF_BOX];
+  // per epilogue warp: results on their way; BACK: two blocks of 32 rows and columns of P and Q (each 2 KB and 1 KB), one that is worked on, one on its way
+  unsigned char out[FF_EPI_WARPS][OUT];
+  uint64_t full[STAGES], empty[STAGES], ready[2], free[2], sums;
   uint32_t tmem;
   volatile int abort;
 };
@@ -269,29 +270,25 @@ __device__ __forceinline__ void ff_store24(unsigned char* s, const float (&v)[32
   ff_store16(s, h, hi, ld, rows, cols);
   ff_store8(s, l, lo, ld, rows, cols);
 }
-struct ff_raw24 { uint4 hi[4], lo[2]; };
-__device__ __forceinline__ void ff_fetch24(ff_raw24& r, const uint16_t* hi, const uint8_t* lo, long long ld, int rows, int cols) {
+__device__ __forceinline__ void ff_ask(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+// 32 x 32 values of 24 bits on their way to shared memory (3 KB), row by row as they lie
+__device__ __forceinline__ void ff_ask24(unsigned char* s, const uint16_t* hi, const uint8_t* lo, long long ld, int rows, int cols) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = (lane >> 2) + 8 * i, c = 8 * (lane & 3);
-    r.hi[i] = row < rows && c < cols ? __ldg(reinterpret_cast<const uint4*>(hi + row * ld + c)) : make_uint4(0, 0, 0, 0);
+    if (row < rows && c < cols) ff_ask(smem_addr(ff_at64(s, row, lane & 3)), hi + row * ld + c);
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = (lane >> 1) + 16 * i, c = 16 * (lane & 1);
-    r.lo[i] = row < rows && c < cols ? __ldg(reinterpret_cast<const uint4*>(lo + row * ld + c)) : make_uint4(0, 0, 0, 0);
+    if (row < rows && c < cols) ff_ask(smem_addr(ff_at32(s + 2048, row, lane & 1)), lo + row * ld + c);
   }
 }
-__device__ __forceinline__ void ff_turn24(unsigned char* s, const ff_raw24& r, float (&v)[32]) {   // to a row per lane
+// Once they are there, a row to each lane (beyond the matrix: anything)
+__device__ __forceinline__ void ff_take24(unsigned char* s, float (&v)[32]) {
   const int lane = threadIdx.x & 31;
   uint32_t h[16], l[8];
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) *ff_at64(s, (lane >> 2) + 8 * i, lane & 3) = r.hi[i];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) *ff_at32(s + 2048, (lane >> 1) + 16 * i, lane & 1) = r.lo[i];
-  __syncwarp();
 #pragma unroll
   for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(h + 4 * q) = *ff_at64(s, lane, q);
 #pragma unroll
@@ -332,14 +329,15 @@ __device__ __forceinline__ void ff_act(int activation, float g, float& a, float&
 template <bool PAIR, int EPI, bool BF>
 __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_constant__ ff_args a) {
   extern __shared__ unsigned char ff_dyn[];
-  using Smem = FfSmem<PAIR>;
+  using Smem = FfSmem<EPI>;
+  constexpr int STAGES = Smem::STAGES;
   constexpr int BN = PAIR ? 256 : 128, TILE_M = PAIR ? 256 : 128, OUT_N = EPI == FF_GATE ? BN / 2 : BN;
   constexpr uint32_t STAGE = 4 * FF_BOX;
   Smem& sm = *reinterpret_cast<Smem*>(ff_dyn + ((1024 - (smem_addr(ff_dyn) & 1023)) & 1023));   // at the same place in all CTAs of a cluster
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int rank = (int)ff_cluster_rank(), ctas = (int)ff_cluster_size();
   if (tid == 0) {
-    for (int s = 0; s < FF_STAGES; ++s) { ff_init(&sm.full[s], 1); ff_init(&sm.empty[s], 1); }
+    for (int s = 0; s < STAGES; ++s) { ff_init(&sm.full[s], 1); ff_init(&sm.empty[s], 1); }
     for (int s = 0; s < 2; ++s) { ff_init(&sm.ready[s], 1); ff_init(&sm.free[s], (PAIR ? 2 : 1) * FF_EPI_WARPS); }
     ff_init(&sm.sums, ctas > 1 ? (ctas - 1) * FF_EPI_WARPS : 1);
     sm.abort = 0;
@@ -382,7 +380,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
         const ff_product& p = locate(tile, tm, tn);
         const int per_part = share(p, kb0, kb1);
         for (int kb = kb0; kb < kb1; ++kb, ++n) {
-          const uint32_t s = n % FF_STAGES, use = n / FF_STAGES;
+          const uint32_t s = n % STAGES, use = n / STAGES;
           if (use > 0 && !ff_wait(&sm.empty[s], (use - 1) & 1, &sm.abort)) { dead = true; break; }
           // boxes that reach beyond the matrix are filled with zeros and count in full; of a pair the first CTA's barrier takes the bytes of both
           if (!PAIR || rank == 0) ff_expect(&sm.full[s], (PAIR ? 2 : 1) * STAGE);
@@ -408,9 +406,9 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
       // the CTA must not end while a copy into its shared memory is in flight: normally the issuing lane has waited for every stage; after an
       // abort wait (bounded) for the stages filled last
       if ((!PAIR || rank == 0) && (dead || sm.abort))
-        for (uint32_t f = n > FF_STAGES ? n - FF_STAGES : 0; f < n; ++f)
+        for (uint32_t f = n > STAGES ? n - STAGES : 0; f < n; ++f)
           for (int it = 0; it < FF_SPIN_LIMIT; ++it)
-            if (ff_try(&sm.full[f % FF_STAGES], (f / FF_STAGES) & 1)) break;
+            if (ff_try(&sm.full[f % STAGES], (f / STAGES) & 1)) break;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -429,8 +427,8 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
           ff_fence_after();
         }
         for (int kb = kb0; kb < kb1; ++kb, ++n) {
-          const uint32_t s = n % FF_STAGES;
-          if (!ff_wait(&sm.full[s], (n / FF_STAGES) & 1, &sm.abort)) { dead = true; break; }
+          const uint32_t s = n % STAGES;
+          if (!ff_wait(&sm.full[s], (n / STAGES) & 1, &sm.abort)) { dead = true; break; }
           ff_fence_after();
           const uint64_t da = ff_desc(smem_addr(sm.st[s]), p.a_mn), db = ff_desc(smem_addr(sm.st[s]) + 2 * FF_BOX, p.b_mn);
 #pragma unroll
@@ -447,6 +445,26 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
     const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
     unsigned char* const stage = sm.out[e];
     uint32_t c = 0;
+    constexpr int BLOCKS = OUT_N / 64;   // of 32 columns for this warp
+    // BACK: the block of P and Q that is on its way
+    struct { int tile, q, buf; } ahead = {first, -1, 1};
+    auto ask = [&] {   // for the one behind it that has rows and columns
+      ++ahead.q;
+      ahead.buf ^= 1;
+      for (; ahead.tile < a.tiles; ahead.tile += step, ahead.q = 0) {
+        int tm, tn;
+        const ff_product& p = locate(ahead.tile, tm, tn);
+        const int m = tm * TILE_M + (PAIR ? rank * FF_BM : 0) + quarter * 32, n = tn * OUT_N + 32 * (half * BLOCKS + ahead.q);
+        if (ahead.q >= BLOCKS || m >= p.M || n >= p.N) continue;
+        const long long at = (long long)m * a.ld + n;
+        unsigned char* const to = stage + 6144 * ahead.buf;
+        ff_ask24(to, a.kept.p_hi + at, a.kept.p_lo + at, a.ld, p.M - m, p.N - n);
+        ff_ask24(to + 3072, a.kept.q_hi + at, a.kept.q_lo + at, a.ld, p.M - m, p.N - n);
+        break;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (EPI == FF_BACK && (PAIR || rank == 0)) ask();
     for (int tile = first; tile < a.tiles && !sm.abort; tile += step, ++c) {
       int tm, tn, kb0, kb1;
       const ff_product& p = locate(tile, tm, tn);
@@ -491,7 +509,6 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
           }
         }
       };
-      constexpr int BLOCKS = OUT_N / 64;   // of 32 columns for this warp
       int left = BLOCKS;                   // of them to be read; behind the last, the accumulator is free
       auto read = [&] {
         if (--left > 0) return;
@@ -555,21 +572,23 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
               ff_store24(stage, q_, a.kept.q_hi + at, a.kept.q_lo + at, a.ld, rows, cols);
             }
           } else {
-            ff_raw24 rp, rq;
-            ff_fetch24(rp, a.kept.p_hi + at, a.kept.p_lo + at, a.ld, rows, cols);
-            ff_fetch24(rq, a.kept.q_hi + at, a.kept.q_lo + at, a.ld, rows, cols);
+            unsigned char* const here = stage + 6144 * ahead.buf;
+            __syncwarp();   // the other buffer has been read by all lanes
+            ask();
             float v[32], f[32];
             tile_sums(block, v);
             read();
-            uint32_t w[16];
-            ff_turn24(stage, rp, f);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncwarp();   // every lane's copies are there
+            uint32_t w[2][16];
+            ff_take24(here, f);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = ff_pack<BF>(v[2 * j] * f[2 * j], v[2 * j + 1] * f[2 * j + 1]);
-            ff_store16(stage, w, a.dg + at, a.ld, rows, cols);
-            ff_turn24(stage, rq, f);
+            for (int j = 0; j < 16; ++j) w[0][j] = ff_pack<BF>(v[2 * j] * f[2 * j], v[2 * j + 1] * f[2 * j + 1]);
+            ff_take24(here + 3072, f);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = ff_pack<BF>(v[2 * j] * f[2 * j], v[2 * j + 1] * f[2 * j + 1]);
-            ff_store16(stage, w, a.du + at, a.ld, rows, cols);
+            for (int j = 0; j < 16; ++j) w[1][j] = ff_pack<BF>(v[2 * j] * f[2 * j], v[2 * j + 1] * f[2 * j + 1]);
+            ff_store16(here, w[0], a.dg + at, a.ld, rows, cols);   // (through where P and Q were)
+            ff_store16(here + 3072, w[1], a.du + at, a.ld, rows, cols);
           }
         }
       }
@@ -579,6 +598,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
       }
     }
     if (EPI == FF_PLAIN && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (EPI == FF_BACK) asm volatile("cp.async.wait_all;" ::: "memory");
   }
   ff_fence_before();
   __syncthreads();
@@ -895,7 +915,7 @@ static int ff_go(ff_args& a, cudaStream_t s) {
   a.tiles = (int)tiles;
   if (!tiles) return 0;
   static bool configured[PYLO_MAX_DEVICES] = {};
-  constexpr int SMEM = (int)sizeof(FfSmem<PAIR>) + 1024;
+  constexpr int SMEM = (int)sizeof(FfSmem<EPI>) + 1024;
   if (int rc = allow_dynamic_smem(k_ffn_product<PAIR, EPI, BF>, SMEM, configured)) return rc;
   int cluster = 2, grid;
   if constexpr (PAIR) {
