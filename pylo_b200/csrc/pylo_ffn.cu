@@ -189,7 +189,8 @@ struct ff_product {
 };
 struct ff_args {
   ff_product p[FF_GROUP];
-  ff_kept kept;             // GATE: written, BACK: read
+  CUtensorMap planes[5];    // GATE: h, the 16-bit planes of P and Q, the 8-bit ones
+  ff_kept kept;             // GATE: written (of few rows; else through the maps), BACK: read
   uint16_t *dg, *du;        // BACK
   long long ld;             // of kept, dg, du
   int n, tiles, activation, keep;
@@ -198,10 +199,10 @@ struct ff_args {
 
 template <int EPI>
 struct FfSmem {
-  static constexpr int STAGES = EPI == FF_BACK ? 4 : 6, OUT = EPI == FF_BACK ? 2 * 6144 : 4096;
+  static constexpr int STAGES = EPI == FF_BACK ? 4 : EPI == FF_GATE ? 5 : 6, OUT = EPI == FF_BACK ? 2 * 6144 : EPI == FF_GATE ? 8192 : 4096;
   // per stage: A (128 x 64), B (128 x 64; of a pair one half of the tile's 256)
   unsigned char st[STAGES][4 * FF_BOX];
-  // per epilogue warp: results on their way; BACK: two blocks of 32 rows and columns of P and Q (each 2 KB and 1 KB), one that is worked on, one on its way
+  // per epilogue warp: results on their way (GATE: h, and both planes of P and Q, of 32 rows and columns); BACK: two blocks of 32 rows and columns of P and Q (each 2 KB and 1 KB), one that is worked on, one on its way
   unsigned char out[FF_EPI_WARPS][OUT];
   uint64_t full[STAGES], empty[STAGES], ready[2], free[2], sums;
   uint32_t tmem;
@@ -213,12 +214,12 @@ struct FfSmem {
 __device__ __forceinline__ uint4* ff_at64(unsigned char* s, int row, int piece) { return reinterpret_cast<uint4*>(s + row * 64 + 16 * (piece ^ ((row >> 1) & 3))); }
 __device__ __forceinline__ uint4* ff_at32(unsigned char* s, int row, int piece) { return reinterpret_cast<uint4*>(s + row * 32 + 16 * (piece ^ ((row >> 2) & 1))); }
 
+__device__ __forceinline__ void ff_put64(unsigned char* s, const uint32_t (&w)[16]);
 // 32 x 32 elements of 16 bits from a row per lane to memory; rows and columns beyond the matrix are left out
 __device__ __forceinline__ void ff_store16(unsigned char* s, const uint32_t (&w)[16], uint16_t* dst, long long ld, int rows, int cols) {
   const int lane = threadIdx.x & 31;
   __syncwarp();
-#pragma unroll
-  for (int q = 0; q < 4; ++q) *ff_at64(s, lane, q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+  ff_put64(s, w);
   __syncwarp();
   if ((((uintptr_t)dst | (uintptr_t)(2 * ld)) & 15) == 0) {
 #pragma unroll
@@ -242,21 +243,14 @@ __device__ __forceinline__ void ff_store16(unsigned char* s, const uint32_t (&w)
       dst[r * ld + lane] = reinterpret_cast<const uint16_t*>(ff_at64(s, r, lane >> 3))[lane & 7];
   }
 }
-// the same for a plane of bytes, whose rows are aligned and have room for whole pieces
-__device__ __forceinline__ void ff_store8(unsigned char* s, const uint32_t (&w)[8], uint8_t* dst, long long ld, int rows, int cols) {
+// A lane's row of 32 elements into such a block: of 16 bits, or of 24 into one block of 16 and one of 8
+__device__ __forceinline__ void ff_put64(unsigned char* s, const uint32_t (&w)[16]) {
   const int lane = threadIdx.x & 31;
-  __syncwarp();
 #pragma unroll
-  for (int q = 0; q < 2; ++q) *ff_at32(s, lane, q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = (lane >> 1) + 16 * i, c = 16 * (lane & 1);
-    if (r < rows && c < cols) *reinterpret_cast<uint4*>(dst + r * ld + c) = *ff_at32(s, r, lane & 1);
-  }
+  for (int q = 0; q < 4; ++q) *ff_at64(s, lane, q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
 }
-// 32 columns in 24 bits, as two planes
-__device__ __forceinline__ void ff_store24(unsigned char* s, const float (&v)[32], uint16_t* hi, uint8_t* lo, long long ld, int rows, int cols) {
+__device__ __forceinline__ void ff_put24(unsigned char* high, unsigned char* low, const float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
   uint32_t h[16], l[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -267,8 +261,9 @@ __device__ __forceinline__ void ff_store24(unsigned char* s, const float (&v)[32
     h[2 * j + 1] = __byte_perm(b[2], b[3], 0x7632);
     l[j] = __byte_perm(__byte_perm(b[0], b[1], 0x0051), __byte_perm(b[2], b[3], 0x0051), 0x5410);
   }
-  ff_store16(s, h, hi, ld, rows, cols);
-  ff_store8(s, l, lo, ld, rows, cols);
+  ff_put64(high, h);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) *ff_at32(low, lane, q) = make_uint4(l[4 * q], l[4 * q + 1], l[4 * q + 2], l[4 * q + 3]);
 }
 __device__ __forceinline__ void ff_ask(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 // 32 x 32 values of 24 bits on their way to shared memory (3 KB), row by row as they lie
@@ -566,10 +561,21 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
               }
               w[j] = ff_pack<BF>(h[0], h[1]);
             }
-            ff_store16(stage, w, a.kept.h + at, a.ld, rows, cols);
+            // Out by copies from shared memory, rows of 64 or 32 bytes in their swizzles: what lies behind the matrix is not written
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the block before has left
+            __syncwarp();
+            ff_put64(stage, w);
             if (a.keep) {
-              ff_store24(stage, u, a.kept.p_hi + at, a.kept.p_lo + at, a.ld, rows, cols);
-              ff_store24(stage, q_, a.kept.q_hi + at, a.kept.q_lo + at, a.ld, rows, cols);
+              ff_put24(stage + 2048, stage + 6144, u);
+              ff_put24(stage + 4096, stage + 7168, q_);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              for (int i = 0; i < (a.keep ? 5 : 1); ++i)
+                asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+                             ::"l"(&a.planes[i]), "r"(smem_addr(stage + (i < 3 ? 2048 * i : 6144 + 1024 * (i - 3)))), "r"(n0), "r"(m0) : "memory");
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
           } else {
             unsigned char* const here = stage + 6144 * ahead.buf;
@@ -597,7 +603,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
         read();
       }
     }
-    if (EPI == FF_PLAIN && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (EPI != FF_BACK && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     if (EPI == FF_BACK) asm volatile("cp.async.wait_all;" ::: "memory");
   }
   ff_fence_before();
@@ -981,6 +987,20 @@ static bool ff_good(const pylo_ffn* f) {
   return f && f->rows >= 0 && f->rows <= (1 << 30) && f->width > 0 && f->hidden > 0 && f->out > 0 && f->width <= (1 << 24) && f->hidden <= (1 << 24) &&
          f->out <= (1 << 24) && (f->type == PYLO_BF16 || f->type == PYLO_FP16) && f->activation >= PYLO_ACT_SILU && f->activation <= PYLO_ACT_RELU;
 }
+// The maps of what the gate writes: planes [rows][hidden], boxes of 32 x 32 elements in the swizzle of their rows
+static int ff_map_planes(ff_args& a, int64_t rows, int64_t hidden) {
+  FfEncode fn = ff_encode();
+  if (!fn) return -5;
+  void* const at[5] = {a.kept.h, a.kept.p_hi, a.kept.q_hi, a.kept.p_lo, a.kept.q_lo};
+  for (int i = 0; i < (a.keep ? 5 : 1); ++i) {
+    const bool wide = i < 3;
+    const cuuint64_t dims[2] = {(cuuint64_t)hidden, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)a.ld * (wide ? 2 : 1)};
+    const cuuint32_t box[2] = {32, 32}, unit[2] = {1, 1};
+    if (fn(&a.planes[i], wide ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, at[i], dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           wide ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) return -5;
+  }
+  return 0;
+}
 // C's map, where its rows allow for one: boxes of 32 rows of 64
 static int ff_map_c(ff_product& p, int type) {
   p.mapped = ((uintptr_t)p.C & 15) == 0 && p.ldc % 8 == 0;
@@ -1026,6 +1046,7 @@ int pylo_b200_gated_ffn(const pylo_ffn* f, void* stream) {
   if (int rc = ff_map(&a.p[0].A[0], f->x, f->rows, f->width, f->ld_x, f->type)) return rc;
   if (int rc = ff_map(&a.p[0].B[0], f->w_gate, f->hidden, f->width, f->ld_gate, f->type)) return rc;
   if (int rc = ff_map(&a.p[0].B[1], f->w_up, f->hidden, f->width, f->ld_up, f->type)) return rc;
+  if (int rc = ff_map_planes(a, f->rows, f->hidden)) return rc;
   if (int rc = ff_run<FF_GATE>(a, f->type, s)) return rc;
   a.p[0] = ff_of(f->y, f->out, f->rows, f->out, f->hidden, 1, 0, 0);
   if (int rc = ff_map(&a.p[0].A[0], kept.h, f->rows, f->hidden, ld, f->type)) return rc;
