@@ -569,7 +569,8 @@ static bool rw_type(int type) { return type == PYLO_FP32 || type == PYLO_BF16 ||
 // An id outside of [0, V) is padding, whatever the teacher's logit beside it is; a row whose entries are all padding or -inf has no
 // teacher and the weight zero.  Rows of weight zero are not read, whatever they hold: their loss and gradient are zero.
 //
-// One pass over a row with a running maximum and sum per thread; powers of two of values that are scaled by log2(e) / T.  The
+// One pass over a row with a running maximum and sum per thread; powers of two of differences from the maximum, scaled by log2(e) / T (not of scaled logits
+// less the scaled maximum in one operation: of masks of -1e30 what that rounds off is a power of its own).  The
 // gradient reads the row again (in the call that makes both, out of the L2 cache: the rows that are being worked on fit it).  The K
 // columns with a teacher's entry are written a second time, behind a barrier, with what their entries add up to.
 // ------------------------------------------------------------------------------------------------
@@ -579,20 +580,21 @@ static bool rw_type(int type) { return type == PYLO_FP32 || type == PYLO_BF16 ||
 #define DT_MOST_CTAS 8         // of an SM, in whatever form
 #define DT_LOG2E 1.4426950408889634
 #define DT_LN2 0.6931471805599453f
+#define DT_LOWEST (-3.402823466e38f)   // a maximum of nothing
 enum { DT_LOSS = 1, DT_GRAD = 2 };
 
 struct DtArgs {
   const void *logits, *teacher, *ids;
   const float* weights;     // [rows] or NULL
   float* row_loss;          // [rows]: weight * loss, or NULL
-  float2* stat;             // [rows]: maximum (scaled), 1 / sum of powers; written with the loss, read for a gradient alone; or NULL
+  float2* stat;             // [rows]: maximum, 1 / sum of powers; written with the loss, read for a gradient alone; or NULL
   double2* part;            // [CTAs or clusters]: sums of weight * loss, of weights
   void* grad;               // [rows][vocab]
   const float* upstream;    // of the loss: a scalar, or (per_row) [rows]; NULL: 1
   const float* inv;         // scalar: 1 / sum of the weights; NULL: 1, or
   const double* weight_sums;// [n_sums]: its parts
   // of long rows, what their teachers come to (k_distill_teachers)
-  float4* teachers;         // [rows]: weight (0 where no entry counts), sum of p (log2 p - scaled logit), sum of p
+  float4* teachers;         // [rows]: weight (0 where no entry counts), sum of p (log2 p - scaled difference of logit and r), sum of p, r
   int2* columns;            // [rows][top]: a class that an entry gives (the first of several; else -1), the bits of its probability; or NULL
   long long rows, stride;
   int vocab, top, teacher_type, wide_ids, n_sums, per_row;
@@ -664,7 +666,8 @@ __device__ __forceinline__ bool dt_teacher(const DtArgs& a, long long row, DtPee
     for (int i = 0; i < 4; ++i) {
       const int k = first + 32 * i + lane, id = peek.id[i];
       if (k >= K) break;
-      const float z = id >= 0 ? peek.t[i] * a.c : -CUDART_INF_F;
+      float z = id >= 0 ? peek.t[i] * a.c : -CUDART_INF_F;
+      if (id >= 0 && fabsf(peek.t[i]) < CUDART_INF_F) z = fminf(fmaxf(z, DT_LOWEST), -DT_LOWEST);   // what is a number stays one
       e[k].id = id >= 0 ? id : DT_PADDING;
       e[k].lp = z;
       most = fmaxf(most, z);
@@ -704,7 +707,7 @@ __device__ __forceinline__ bool dt_teacher(const DtArgs& a, long long row, DtPee
   }
   return true;
 }
-// The loss of a row to base 2, without the student's sum: sum of p (log p - s), by a warp
+// The loss of a row to base 2, without the student's sum: sum of p (log p - s) with logits relative to m, by a warp
 template <class T>
 __device__ __forceinline__ float dt_cross(const DtArgs& a, const T* s, const DtEntry* e, float m) {
   float sum = 0.f;
@@ -719,14 +722,14 @@ __device__ __forceinline__ float dt_cross(const DtArgs& a, const T* s, const DtE
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (!(q[i].p == 0.f)) sum = fmaf(q[i].p, q[i].lp - fmaf(v[i], a.c, -m), sum);
+      if (!(q[i].p == 0.f)) sum = fmaf(q[i].p, fmaf(v[i] - m, -a.c, q[i].lp), sum);
   }
   return rw_warp_sum(sum);
 }
 // The column of a teacher's entry, once more
 template <class T>
 __device__ __forceinline__ void dt_column(T* grad, int id, float p, float logit, float f, float total, float m, float c) {
-  grad[id] = rw_to<T>(f * (total * dt_exp2(fmaf(logit, c, -m)) - p));
+  grad[id] = rw_to<T>(f * (total * dt_exp2((logit - m) * c) - p));
 }
 
 // Where a row's 16-byte pieces lie, and the element before or behind them that is thread t's
@@ -771,17 +774,17 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs 
     }
     const DtRow<T> r((const T*)a.logits + row * a.stride, V, t);
     const T* const body = r.s + r.head;
-    float m = -CUDART_INF_F, total = 0.f;   // scaled maximum; sum of powers relative to it
+    float m = DT_LOWEST, total = 0.f;   // maximum; sum of powers relative to it
     if constexpr (DO & DT_LOSS) {
       auto add = [&](const float (&v)[VN]) {
         float most = v[0];
 #pragma unroll
         for (int j = 1; j < VN; ++j) most = fmaxf(most, v[j]);
-        const float up = fmaxf(m, most * a.c), ref = up == -CUDART_INF_F ? 0.f : up;
+        const float up = fmaxf(m, most);
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < VN; ++j) sum += dt_exp2(fmaf(v[j], a.c, -ref));
-        total = fmaf(total, dt_exp2(m - ref), sum);
+        for (int j = 0; j < VN; ++j) sum += dt_exp2((v[j] - up) * a.c);
+        total = fmaf(total, dt_exp2((m - up) * a.c), sum);
         m = up;
       };
       float f[VN];
@@ -798,9 +801,9 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs 
         for (int j = 1; j < VN; ++j) f[j] = -CUDART_INF_F;
         add(f);
       }
-      const float all = rw_warp_max(m), ref = all == -CUDART_INF_F ? 0.f : all;
-      total = rw_warp_sum(total * dt_exp2(m - ref));
-      m = ref;
+      const float all = rw_warp_max(m);
+      total = rw_warp_sum(total * dt_exp2((m - all) * a.c));
+      m = all;
       const float cross = dt_cross(a, r.s, e, m);
       if (t == 0) {
         const float loss = weight * a.temperature * a.temperature * DT_LN2 * (cross + log2f(total));
@@ -817,7 +820,7 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs 
     }
     if constexpr (DO & DT_GRAD) {
       const float f = factor * weight * (a.upstream && a.per_row ? a.upstream[row] : 1.0f), g = f * total;
-      for (int i = t; i < V; i += 32) grad[i] = rw_to<T>(g * dt_exp2(fmaf(rw_float(r.s[i]), a.c, -m)));
+      for (int i = t; i < V; i += 32) grad[i] = rw_to<T>(g * dt_exp2((rw_float(r.s[i]) - m) * a.c));
       __syncwarp();   // behind it, the columns of the teacher's entries are written again
       for (int k = t; k < a.top; k += 32)
         if (e[k].id >= 0) dt_column(grad, e[k].id, e[k].column, rw_float(r.s[e[k].id]), f, total, m, a.c);
@@ -855,13 +858,17 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_teachers(const DtAr
     peek = dt_peek(a, row + step, 0);
     const bool any = weight != 0.f && dt_teacher(a, row, mine, e, slots);
     if (any) {
-      const float cross = dt_cross(a, (const T*)a.logits + row * a.stride, e, 0.f);
+      // relative to the first entry's logit, or another number that the logits are not far from
+      const T* const s = (const T*)a.logits + row * a.stride;
+      float near = e[0].p > 0.f ? rw_float(s[e[0].id < 0 ? ~e[0].id : e[0].id]) : 0.f;
+      if (!(fabsf(near) < 1e30f)) near = 0.f;
+      const float cross = dt_cross(a, s, e, near);
       float sum = 0.f;
       for (int k = lane; k < a.top; k += 32) sum += e[k].p;
       sum = rw_warp_sum(sum);
       if (a.columns)
         for (int k = lane; k < a.top; k += 32) a.columns[row * a.top + k] = make_int2(e[k].id < 0 ? -1 : e[k].id, __float_as_int(e[k].column));
-      if (lane == 0) a.teachers[row] = make_float4(weight, cross, sum, 0.f);
+      if (lane == 0) a.teachers[row] = make_float4(weight, cross, sum, near);
       weight_sum += weight;
     } else if (lane == 0) a.teachers[row] = make_float4(0.f, 0.f, 0.f, 0.f);
     __syncwarp();
@@ -890,7 +897,6 @@ __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(co
   __shared__ float2 s_part[2][DL_MOST_SHARE * STREAM / 32];
   constexpr int VN = RW_VEC<T>, PARTS = STREAM / 32, RING = dl_ring(DO), STEP = STREAM * 16;
   constexpr bool BOTH = DO == (DT_LOSS | DT_GRAD);
-  constexpr float LOWEST = -3.0e38f;   // in the place of a maximum of -inf
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, K = a.top, V = a.vocab;
   uint32_t rank, share;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -1029,7 +1035,7 @@ __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(co
           float x[VN];
 #pragma unroll
           for (int j = 0; j < VN; j += 2) {
-            rw_unpair(rw_fma2(v.two(j), cc, mm), x[j], x[j + 1]);
+            rw_unpair(rw_mul2(rw_add2(v.two(j), mm), cc), x[j], x[j + 1]);
             rw_unpair(rw_mul2(gg, rw_pair(dt_exp2(x[j]), dt_exp2(x[j + 1]))), x[j], x[j + 1]);
           }
           RwPiece<T, VN> o;
@@ -1043,7 +1049,7 @@ __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(co
       };
       if (((uintptr_t)(grad + r.at) & 15) == 0) go(std::true_type());
       else go(std::false_type());
-      if (has_edge) grad[edge] = rw_to<T>(g * dt_exp2(fmaf(rw_float(outside), c, -m)));
+      if (has_edge) grad[edge] = rw_to<T>(g * dt_exp2((rw_float(outside) - m) * c));
       __syncthreads();   // behind it, the columns of the teacher's entries are written again
       if (has_entry) dt_column(grad, entry.x, __int_as_float(entry.y), rw_float(logit), f, total, m, c);
       for (int k = t + STREAM; k < K; k += STREAM) {
@@ -1053,21 +1059,21 @@ __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(co
     };
     if constexpr (!(DO & DT_LOSS)) gradient(st.x, st.y, sweep);
     else {
-      float m = LOWEST;   // scaled maximum
+      float m = DT_LOWEST;   // maximum
       uint64_t mm = rw_pair(-m, -m), sum = rw_pair(0.f, 0.f);   // sums of powers relative to it
       auto raise = [&](float to) {
-        const float by = dt_exp2(m - to);
+        const float by = dt_exp2((m - to) * c);
         sum = rw_mul2(sum, rw_pair(by, by));
         m = to;
         mm = rw_pair(-m, -m);
       };
       auto add = [&](const RwPiece<T, VN>& v) {
-        const float most = rw_most(v) * c;
+        const float most = rw_most(v);
         if (most > m) raise(most);
 #pragma unroll
         for (int j = 0; j < VN; j += 2) {
           float x, y;
-          rw_unpair(rw_fma2(v.two(j), cc, mm), x, y);
+          rw_unpair(rw_mul2(rw_add2(v.two(j), mm), cc), x, y);
           sum = rw_add2(sum, rw_pair(dt_exp2(x), dt_exp2(y)));
         }
       };
@@ -1091,11 +1097,11 @@ __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(co
       }
       if (has_edge) {
         const float v = rw_float(outside);
-        if (v * c > m) raise(v * c);
-        sum = rw_add2(sum, rw_pair(dt_exp2(fmaf(v, c, -m)), 0.f));
+        if (v > m) raise(v);
+        sum = rw_add2(sum, rw_pair(dt_exp2((v - m) * c), 0.f));
       }
       const float all = rw_warp_max(m);
-      float total = rw_warp_sum(rw_both(sum) * dt_exp2(m - all));
+      float total = rw_warp_sum(rw_both(sum) * dt_exp2((m - all) * c));
       if (lane < (int)share) {
         const uint32_t to = rw_at_rank(&s_part[buf][rank * PARTS + warp], lane);
         asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(all), "f"(total) : "memory");
@@ -1106,21 +1112,20 @@ __global__ void __launch_bounds__(STREAM, dl_ctas(STREAM, DO)) k_distill_long(co
         const int parts = (int)share * PARTS;
         constexpr int EACH = (DL_MOST_SHARE * PARTS + 31) / 32;   // of a lane
         float2 x[EACH];
-        m = LOWEST;
+        m = DT_LOWEST;
         total = 0.f;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-          x[i] = lane + 32 * i < parts ? s_part[buf][lane + 32 * i] : make_float2(LOWEST, 0.f);
+          x[i] = lane + 32 * i < parts ? s_part[buf][lane + 32 * i] : make_float2(DT_LOWEST, 0.f);
           m = fmaxf(m, x[i].x);
         }
         m = rw_warp_max(m);
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) total += x[i].y * dt_exp2(x[i].x - m);
+        for (int i = 0; i < EACH; ++i) total += x[i].y * dt_exp2((x[i].x - m) * c);
         total = rw_warp_sum(total);
-        m = m == LOWEST ? 0.f : m;   // (then all are -inf, and total is 0)
         st = make_float2(m, 1.0f / total);
         if (t == 0 && rank == 0) {
-          const float loss = w * a.temperature * a.temperature * DT_LN2 * fmaf(now.teacher.z, m, now.teacher.y + log2f(total));
+          const float loss = w * a.temperature * a.temperature * DT_LN2 * fmaf(now.teacher.z, (m - now.teacher.w) * c, now.teacher.y + log2f(total));
           if (a.row_loss) a.row_loss[row] = loss;
           if (a.stat) a.stat[row] = st;
           loss_sum += loss;

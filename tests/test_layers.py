@@ -462,6 +462,35 @@ def test_distill_of_infinite_logits(vocab):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, FP16])
+@pytest.mark.parametrize("vocab", [60, 5001])
+def test_distill_beside_masks_of_the_lowest_value(vocab, dtype):
+    """Classes that are masked with the type's lowest number, among others, have no probability and no gradient."""
+    logits, teacher, ids = distill_inputs(7, vocab, 6, dtype, seed=5)
+    out = torch.rand(7, vocab, generator=gen(3), device="cuda") < 0.9
+    out.scatter_(1, ids, False)
+    for value, T in ((torch.finfo(dtype).min, 1.0), (torch.finfo(dtype).min, 4.0), (-1e4, 1.0), (-1e30 if dtype != FP16 else -3e4, 1.0), (-1e38 if dtype != FP16 else -6e4, 0.5)):
+        logits[out] = value
+        rows = layers.distillation_loss(logits, teacher, ids, T, reduction="none")
+        want, *_ = distill64(logits.double().masked_fill(out, -math.inf), teacher, ids, T)
+        # the magnitudes of the exponents: those of the logits that are left
+        slack = T * T * E * (16 * float(logits[~out].abs().max()) * 1.45 / T + 64 + vocab / 32 + 8 * want / T / T)
+        near(rows, want, slack, "rows")
+        _, g = layers.distillation_loss_and_grad(logits, teacher, ids, T)
+        assert bool(g.isfinite().all()) and not bool(g[out].any())
+    # nothing but such values: all classes are alike
+    logits[:] = torch.finfo(dtype).min
+    check_distill(logits, torch.zeros_like(teacher), ids, 2.0)
+    same = layers.distillation_loss(logits, torch.full_like(teacher, torch.finfo(dtype).min), ids, 1.0, reduction="none")
+    assert torch.equal(same, layers.distillation_loss(logits, torch.zeros_like(teacher), ids, 1.0, reduction="none"))
+    # far off centre: as exact as the logits
+    near_one = (torch.randn(7, vocab, generator=gen(4), device="cuda") + 1e3).to(dtype)
+    rows = layers.distillation_loss(near_one, teacher, ids, reduction="none")
+    want, *_ = distill64(near_one - 1e3 if dtype == F32 else near_one.double() - 1e3, teacher, ids, 1.0)
+    near(rows, want, E * (16 * 8 * 1.45 + 64 + vocab / 32 + 8 * want + 16 * float(teacher.abs().max())), "off centre")
+
+
+@gpu
 def test_distill_of_strided_logits_and_other_types_of_teacher():
     big = randn(12, 3, 1200, seed=1, dtype=BF16, scale=2.0)
     for logits in (big[:, 1, 8:1108], big[:, 1, 3:1104], big[:, 0, :30], big[:, 0, ::3]):
@@ -686,6 +715,97 @@ def test_on_another_stream():
             got = [student_step(student, *batch)] + [p.grad for p in student.parameters()]
         torch.cuda.current_stream().wait_stream(side)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+def test_two_streams_at_once():
+    """Calls that run beside one another have nothing in common."""
+    batches = [student_and_batch(seed=k) for k in (11, 12)]
+    want = []
+    for student, batch in batches:
+        want.append([student_step(student, *batch)] + [p.grad.clone() for p in student.parameters()])
+    streams = [torch.cuda.Stream() for _ in batches]
+    for _ in range(5):
+        got = []
+        for student, _ in batches:
+            for p in student.parameters():
+                p.grad = None
+        for stream, (student, batch) in zip(streams, batches):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                got.append([student_step(student, *batch)] + [p.grad for p in student.parameters()])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+
+
+@gpu
+def test_on_another_device_than_the_current_one():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU visible")
+    student, batch = student_and_batch(seed=5)
+    want = [student_step(student, *batch)] + [p.grad.clone() for p in student.parameters()]
+    for p in student.parameters():
+        p.grad = None
+    student, batch = student.to("cuda:1"), [t.to("cuda:1") for t in batch]
+    got = [student_step(student, *batch)] + [p.grad for p in student.parameters()]
+    assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(got, want))
+
+
+@gpu
+def test_norm_beyond_32_bits():
+    """More than 2^31 elements: the last rows are those of a small call; the columns' sums hold for gradients that are equal."""
+    rows, width = 2_100_003, 1024
+    x, dy = randn(1, width, seed=1, dtype=BF16).repeat(rows, 1), randn(1, width, seed=2, dtype=BF16).repeat(rows, 1)
+    x[-3:], dy[-3:] = randn(3, width, seed=3, dtype=BF16), randn(3, width, seed=4, dtype=BF16)
+    w, b = randn(width, seed=5).requires_grad_(), randn(width, seed=6).requires_grad_()
+    y = layers.layer_norm(x.requires_grad_(), w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    few = [t[-5:].detach().clone() for t in (x, dy)]
+    small = few[0].requires_grad_()
+    z = layers.layer_norm(small, w, b)
+    assert torch.equal(y[-5:], z) and torch.equal(dx[-5:], torch.autograd.grad(z, small, few[1])[0])
+    assert torch.equal(y[0], z[0]) and torch.equal(dx[0], dx[1000])
+    want = norm64(small.detach()[:1], w.detach(), b.detach(), few[1][:1], 1e-5)
+    # a column's sum of equal terms: rows / 592 / 4 in a line per warp, then those
+    for got, name in ((dw, "dweight"), (db, "dbias")):
+        value, slack = (v * (rows - 3) for v in want[name])
+        near(got, value, slack + 6e3 * E * value.abs() + 50, name)   # (three rows of other terms, of 5 at most each)
+
+
+@gpu
+def test_distill_beyond_32_bits():
+    rows, vocab = 43_000, 50_257
+    logits, teacher, ids = distill_inputs(5, vocab, 8, BF16)
+    many = torch.empty(rows, vocab, device="cuda", dtype=BF16)
+    many[:-5] = logits[:1]
+    many[-5:] = logits
+    t, i = (torch.cat([v[:1].expand(rows - 5, 8), v]) for v in (teacher, ids))
+    got = layers.distillation_loss(many.requires_grad_(), t, i, reduction="none")
+    (g,) = torch.autograd.grad(got, many, torch.ones_like(got))
+    small = logits.requires_grad_()
+    want = layers.distillation_loss(small, teacher, ids, reduction="none")
+    (h,) = torch.autograd.grad(want, small, torch.ones_like(want))
+    # (few rows are shared by several CTAs, whose sums are added up in another order)
+    assert torch.allclose(got[-5:], want, rtol=64 * E, atol=64 * E)
+    assert bool((got[:-5] == got[0]).all()) and torch.equal(g[0], g[-6])
+    near(g[-5:], h.double(), 2 * half_step(BF16) * h.double().abs() + 1e-9)
+
+
+@gpu
+def test_ffn_beyond_32_bits():
+    """More than 2^31 hidden values: the last rows are those of a small call."""
+    rows, width, hidden = 270_003, 64, 8008
+    x, wg, wu, wd, dy = ffn_inputs(300, width, hidden, 8, BF16, seed=3)
+    many, many_dy = torch.empty(rows, width, device="cuda", dtype=BF16), torch.empty(rows, 8, device="cuda", dtype=BF16)
+    for a, b in ((many, x), (many_dy, dy)):
+        a[:-300] = b[:1]
+        a[-300:] = b
+    many.requires_grad_()
+    (dx,) = torch.autograd.grad(layers.gated_ffn(many, wg, wu, wd), many, many_dy)
+    want = ffn64(x, wg, wu, wd, dy, "silu")
+    near(dx[-300:], *want["dx"], "dx")
+    assert torch.equal(dx[0], dx[-301])
+    layers.check_status()
 
 
 @gpu
