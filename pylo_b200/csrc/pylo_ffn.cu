@@ -310,7 +310,8 @@ __device__ __forceinline__ void ff_act(int activation, float g, float& a, float&
   } else if (activation == PYLO_ACT_GELU_TANH) {
     const float k = 0.7978845608028654f, t = tanhf(k * fmaf(0.044715f * g * g, g, g));
     a = 0.5f * g * (1.0f + t);
-    slope = 0.5f * (1.0f + t) + 0.5f * g * (1.0f - t * t) * k * fmaf(3.0f * 0.044715f * g, g, 1.0f);
+    const float b = fminf(fmaxf(g, -100.0f), 100.0f);   // beyond, 1 - t^2 is 0, and a square might be infinite
+    slope = 0.5f * (1.0f + t) + 0.5f * b * (1.0f - t * t) * k * fmaf(3.0f * 0.044715f * b, b, 1.0f);
   } else {
     a = g > 0.f ? g : g != g ? g : 0.f;
     slope = g > 0.f ? 1.0f : 0.f;

@@ -858,10 +858,10 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_teachers(const DtAr
     peek = dt_peek(a, row + step, 0);
     const bool any = weight != 0.f && dt_teacher(a, row, mine, e, slots);
     if (any) {
-      // relative to the first entry's logit, or another number that the logits are not far from
+      // relative to the first entry's logit, where it is a number: of all logits far off centre the differences count
       const T* const s = (const T*)a.logits + row * a.stride;
       float near = e[0].p > 0.f ? rw_float(s[e[0].id < 0 ? ~e[0].id : e[0].id]) : 0.f;
-      if (!(fabsf(near) < 1e30f)) near = 0.f;
+      if (!(fabsf(near) < CUDART_INF_F)) near = 0.f;
       const float cross = dt_cross(a, s, e, near);
       float sum = 0.f;
       for (int k = lane; k < a.top; k += 32) sum += e[k].p;

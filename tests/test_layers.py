@@ -266,6 +266,12 @@ def test_ffn_of_large_values():
         x, wg, wu, wd, dy = ffn_inputs(40, 64, 128, 64, BF16, seed=9)
         for name, got in check_ffn(x * 16, wg * 16, wu, wd, dy, act=act).items():
             assert bool(got.isfinite().all()), name
+        for v in (1e25, -1e25):   # whose squares are infinite
+            x1 = torch.full((2, 8), v, device="cuda", dtype=BF16).requires_grad_()
+            w = torch.eye(8, device="cuda", dtype=BF16)
+            y = layers.gated_ffn(x1, w, w * 0, w, activation=act)
+            (g,) = torch.autograd.grad(y, x1, torch.ones_like(y))
+            assert not bool(y.any()) and not bool(g.any()), act
 
 
 @gpu
@@ -480,9 +486,13 @@ def test_distill_beside_masks_of_the_lowest_value(vocab, dtype):
         assert bool(g.isfinite().all()) and not bool(g[out].any())
     # nothing but such values: all classes are alike
     logits[:] = torch.finfo(dtype).min
-    check_distill(logits, torch.zeros_like(teacher), ids, 2.0)
-    same = layers.distillation_loss(logits, torch.full_like(teacher, torch.finfo(dtype).min), ids, 1.0, reduction="none")
-    assert torch.equal(same, layers.distillation_loss(logits, torch.zeros_like(teacher), ids, 1.0, reduction="none"))
+    for T in (1.0, 2.0):
+        for t in (torch.zeros_like(teacher), torch.full_like(teacher, torch.finfo(dtype).min)):
+            loss, g = layers.distillation_loss_and_grad(logits, t, ids, T, reduction="sum")
+            want = T * T * math.log(vocab / 6) * 7   # uniform over the classes, and over the six entries
+            assert abs(float(loss) - want) < want * 64 * E
+            full = torch.full((7, vocab), T / vocab, device="cuda", dtype=torch.float64).scatter_add_(1, ids, torch.full((7, 6), -T / 6, device="cuda", dtype=torch.float64))
+            near(g, full, 64 * E * full.abs(), "uniform")
     # far off centre: as exact as the logits
     near_one = (torch.randn(7, vocab, generator=gen(4), device="cuda") + 1e3).to(dtype)
     rows = layers.distillation_loss(near_one, teacher, ids, reduction="none")
