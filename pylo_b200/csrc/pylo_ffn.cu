@@ -32,6 +32,7 @@
 #define FF_EPI_WARPS 8
 #define FF_THREADS ((FF_EPI_WARPS + 2) * 32)
 #define FF_SPIN_LIMIT (1 << 22)
+#define FF_SPINS 64             // more for each stage of a whole tile that is waited for: a stage takes less time than so many looks at a barrier
 #define FF_GROUP 4              // products of a launch
 #define FF_BAND 8               // rows of tiles that are taken together, so that what is in flight shares operands in the L2 cache
 enum { FF_PLAIN = 0, FF_GATE = 1, FF_BACK = 2 };
@@ -65,9 +66,9 @@ __device__ __forceinline__ bool ff_try(uint64_t* bar, uint32_t parity) {
                : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
   return ok;
 }
-// false if the wait ran out, here or in another warp of the CTA
-__device__ __forceinline__ bool ff_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  for (int it = 0; it < FF_SPIN_LIMIT; ++it) {
+// false if the wait ran out, here or in another warp of the CTA; stages: how many are worked on meanwhile (2^24 at most)
+__device__ __forceinline__ bool ff_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int stages = 0) {
+  for (int it = 0; it < FF_SPIN_LIMIT + FF_SPINS * stages; ++it) {
     if (ff_try(bar, parity)) return true;
     if ((it & 63) == 63 && *abort) return false;
   }
@@ -466,7 +467,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
       const ff_product& p = locate(tile, tm, tn);
       share(p, kb0, kb1);
       const int m0 = tm * TILE_M + (PAIR ? rank * FF_BM : 0) + quarter * 32, rows = p.M - m0;
-      if (!ff_wait(&sm.ready[c & 1], (c >> 1) & 1, &sm.abort)) break;
+      if (!ff_wait(&sm.ready[c & 1], (c >> 1) & 1, &sm.abort, kb1 - kb0)) break;
       ff_fence_after();
       const uint32_t acc = t_lane + (c & 1) * 256;
       bool leave = false;
@@ -486,7 +487,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
           if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(nf_at_rank(&sm.sums, 0)) : "memory");
           leave = true;
         } else if (ctas > 1) {
-          if (!ff_wait(&sm.sums, 0, &sm.abort)) break;
+          if (!ff_wait(&sm.sums, 0, &sm.abort, kb1 - kb0)) break;
           asm volatile("fence.acq_rel.cluster;" ::: "memory");
         }
       }
@@ -722,7 +723,7 @@ __global__ void __launch_bounds__(FF_FEW_THREADS, 2) k_ffn_few(const __grid_cons
   } else {
     // ---------------------------------------------------------------- a thread per feature
     const int quarter = warp & 3, at = quarter * 32 + lane;   // of the tile's 128
-    bool good = ff_wait(&sm.ready, 0, &sm.abort);
+    bool good = ff_wait(&sm.ready, 0, &sm.abort, kb1 - kb0);
     ff_fence_after();
     float v[ROWS];
     if (good) {
@@ -748,7 +749,7 @@ __global__ void __launch_bounds__(FF_FEW_THREADS, 2) k_ffn_few(const __grid_cons
       }
     } else {
       if (good && ctas > 1) {
-        good = ff_wait(&sm.sums, 0, &sm.abort);
+        good = ff_wait(&sm.sums, 0, &sm.abort, kb1 - kb0);
         asm volatile("fence.acq_rel.cluster;" ::: "memory");
         if (good)
           for (int r = 1; r < ctas; ++r) {   // in rank order

@@ -159,14 +159,13 @@ __device__ __forceinline__ void rw_commit() { asm volatile("cp.async.commit_grou
 //   y = xh w + b;   dx = r (q - mean q - xh mean(q xh)) with q = dy w;   dw = sum over rows dy xh, db = sum over rows dy
 //
 // A row is read once and stays in registers, 16 or 32 elements of each thread, so that the variance is that of the differences from the mean (a
-// sum of squares less the mean's would lose what rows far off centre have).  A row is a warp's, a CTA's, or a cluster's of two or four
+// sum of squares less the mean's would lose what rows far off centre have).  A row is a warp's, a CTA's, or that of a cluster of two
 // CTAs; the next one is on its way while one is worked on.  The weights stay in registers from row to row, the sums of their
 // gradients too; those leave as one partial sum per CTA, and a second kernel adds them up in a fixed order.
 // ------------------------------------------------------------------------------------------------
 #define LN_WARP_THREADS 128   // of a CTA whose warps have a row each
 #define LN_WARPS (LN_WARP_THREADS / 32)
 #define LN_MOST 16384         // elements of a row
-#define LN_MOST_SHARE 4
 // CTAs of so many threads on an SM, with E elements per thread: 64 to 128 registers
 __host__ __device__ constexpr int ln_ctas(int threads, int e, bool backward, bool ring) {
   return threads > 128 ? 512 / threads : e <= 8 ? backward ? 6 : 8 : backward && !ring ? 3 : 4;
@@ -1188,7 +1187,6 @@ __global__ void __launch_bounds__(NT) k_distill_total(const double2* __restrict_
   }
 }
 
-// Rows' groups of a call, one CTA or a cluster each, which is also the number of its partial sums
 // A call's form.  Threads that stream through a long row: few for short ones, so that more rows' latencies lie side by side.  share: CTAs that share a
 // row, until all have work, or (loss and gradient) until DL_KEPT pieces of a thread are its part of the row.
 struct DtForm { int stream, share; bool fits; };   // fits: into the rings

@@ -819,6 +819,22 @@ def test_ffn_beyond_32_bits():
 
 
 @gpu
+def test_ffn_of_a_contraction_of_many_stages():
+    """The weights' gradients of 2^28 rows, of which the last 300 are not zero: no wait for a whole tile runs out, and every row counts."""
+    rows, width, hidden = (1 << 28) + 5, 8, 8
+    x, wg, wu, wd, dy = ffn_inputs(300, width, hidden, 8, BF16, seed=4)
+    many, many_dy = torch.zeros(rows, width, device="cuda", dtype=BF16), torch.zeros(rows, 8, device="cuda", dtype=BF16)
+    many_dy[:] = dy[:1]
+    many[-300:], many_dy[-300:] = x, dy
+    weights = [w.clone().requires_grad_() for w in (wg, wu, wd)]
+    grads = torch.autograd.grad(layers.gated_ffn(many, *weights), weights, many_dy)
+    layers.check_status()
+    want = ffn64(x, wg, wu, wd, dy, "silu")
+    for name, g in zip(("dw_gate", "dw_up", "dw_down"), grads):
+        near(g, *want[name], name)
+
+
+@gpu
 def test_captured_into_graphs():
     """Forward and backward of a student in a graph; two graphs that are replayed in turn, with new inputs."""
     graphs = []
