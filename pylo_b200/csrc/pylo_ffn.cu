@@ -14,11 +14,11 @@
 // need them.
 //
 // What is kept for the backward pass: h in 16 bits, which the forward pass needs in memory anyway, P and Q with 24 (16 significant bits, an fp32
-// value's upper three bytes, rounded; in two planes, so that rows stay aligned): 8 bytes per element of h, what g, u, act(g) and h take in 16 bits.
+// value's upper three bytes, rounded): 8 bytes per element of h, what g, u, act(g) and h take in 16 bits.
 // With P and Q in 16 bits, dg and du would be rounded twice on their way into dx, dWg and dWu: an error of 1.7 instead of 1.4 times that of the
 // result's own rounding.
 //
-// A CTA has ten warps: one lane issues the copies (TMA, 128-byte swizzle), one the products, eight warps run the epilogue.  Every wait is bounded;
+// A CTA has ten or eighteen warps: one lane issues the copies (TMA, 128-byte swizzle), one the products, the others run the epilogue.  Every wait is bounded;
 // one that runs out ends the CTA's work in order and sets a bit of the caller's status word.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -29,13 +29,16 @@
 #define FF_BM 128               // rows of a CTA's tile
 #define FF_BK 64                // terms per stage
 #define FF_BOX 8192             // bytes of a box: 64 x 64 elements
-#define FF_EPI_WARPS 8
-#define FF_THREADS ((FF_EPI_WARPS + 2) * 32)
 #define FF_SPIN_LIMIT (1 << 22)
 #define FF_SPINS 64             // more for each stage of a whole tile that is waited for: a stage takes less time than so many looks at a barrier
 #define FF_GROUP 4              // products of a launch
 #define FF_BAND 8               // rows of tiles that are taken together, so that what is in flight shares operands in the L2 cache
 enum { FF_PLAIN = 0, FF_GATE = 1, FF_BACK = 2 };
+// Warps of the epilogue, and columns that each takes at a time.  8192 rows x 1024 x 4096: gate 101 us with 8 warps and 105 with 16 (one more wait for the
+// tile's sums per warp); back, whose warps wait for P and Q, 110 and 94.
+__host__ __device__ constexpr int ff_epi_warps(int epi) { return epi == FF_BACK ? 16 : 8; }
+__host__ __device__ constexpr int ff_columns(int epi) { return epi == FF_PLAIN ? 32 : 16; }
+__host__ __device__ constexpr int ff_threads(int epi) { return (ff_epi_warps(epi) + 2) * 32; }
 
 // ------------------------------------------------------------------------------------------------
 // tensor cores and barriers
@@ -136,7 +139,7 @@ __device__ __forceinline__ uint32_t ff_idesc(uint32_t m, uint32_t n, int a_mn, i
 __device__ __forceinline__ void ff_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void ff_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // 32 columns of a warp's 32 rows, a row per lane
-__device__ __forceinline__ void ff_ld32(uint32_t taddr, float (&f)[32]) {
+__device__ __forceinline__ void ff_ld(uint32_t taddr, float (&f)[32]) {
   uint32_t r[32];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -148,6 +151,17 @@ __device__ __forceinline__ void ff_ld32(uint32_t taddr, float (&f)[32]) {
       : "r"(taddr) : "memory");
 #pragma unroll
   for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(r[j]);
+}
+// 16 of them
+__device__ __forceinline__ void ff_ld(uint32_t taddr, float (&f)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+#pragma unroll
+  for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(r[j]);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -172,11 +186,20 @@ __device__ __forceinline__ uint32_t ff_round24(float v) {
 // ------------------------------------------------------------------------------------------------
 // the product kernel
 // ------------------------------------------------------------------------------------------------
-// What is kept of a tile of h: planes [rows][ld]
+// What is kept: h [rows][ld], and of P and Q the upper 16 bits and the 8 below, in the order in which the epilogues' lanes have them: blocks of 32 rows and 16
+// columns (3 KB), row by row of blocks, of which each lane writes and reads its row in pieces of 16 bytes, side by side with its neighbours' (P's upper bits
+// 2, Q's 2, P's lower ones, Q's).  Few rows: planes [rows][2 ld], 16 columns of P, the same 16 of Q, the next 16 of P.
+#define FF_KEPT_PIECES 6
 struct ff_kept {
-  uint16_t *h, *p_hi, *q_hi;
-  uint8_t *p_lo, *q_lo;
+  uint16_t* h;
+  uint4* blocks;
+  uint16_t* hi;
+  uint8_t* lo;
 };
+__device__ __forceinline__ long long ff_place(long long row, long long ld, int col) { return row * 2 * ld + (col >> 4) * 32 + (col & 15); }   // of P; Q is 16 behind
+__device__ __forceinline__ uint4* ff_block(const ff_kept& kept, int row, long long ld, int col) {   // this lane's first piece
+  return kept.blocks + ((row >> 5) * (ld >> 4) + (col >> 4)) * (32 * FF_KEPT_PIECES) + (threadIdx.x & 31);
+}
 struct ff_product {
   CUtensorMap A[2], B[2];   // the two parts of the contraction; GATE: B is Wg, Wu
   CUtensorMap Cm;           // of C, where mapped
@@ -190,9 +213,9 @@ struct ff_product {
 };
 struct ff_args {
   ff_product p[FF_GROUP];
-  CUtensorMap planes[5];    // GATE: h, the 16-bit planes of P and Q, the 8-bit ones
+  CUtensorMap planes[2];    // what the epilogue writes by copies from shared memory, 32 rows of 16 columns at a time: GATE: h; BACK: dg, du
   ff_kept kept;             // GATE: written (of few rows; else through the maps), BACK: read
-  uint16_t *dg, *du;        // BACK
+  uint16_t *dg, *du;        // BACK, written as kept is
   long long ld;             // of kept, dg, du
   int n, tiles, activation, keep;
   int *status, *host_status;
@@ -200,11 +223,11 @@ struct ff_args {
 
 template <int EPI>
 struct FfSmem {
-  static constexpr int STAGES = EPI == FF_BACK ? 4 : EPI == FF_GATE ? 5 : 6, OUT = EPI == FF_BACK ? 2 * 6144 : EPI == FF_GATE ? 8192 : 4096;
+  static constexpr int STAGES = 6, WARPS = ff_epi_warps(EPI), OUT = EPI == FF_PLAIN ? 4096 : EPI == FF_BACK ? 2048 : 1024;
   // per stage: A (128 x 64), B (128 x 64; of a pair one half of the tile's 256)
   unsigned char st[STAGES][4 * FF_BOX];
-  // per epilogue warp: results on their way (GATE: h, and both planes of P and Q, of 32 rows and columns); BACK: two blocks of 32 rows and columns of P and Q (each 2 KB and 1 KB), one that is worked on, one on its way
-  unsigned char out[FF_EPI_WARPS][OUT];
+  // per epilogue warp: results on their way
+  unsigned char out[WARPS][OUT];
   uint64_t full[STAGES], empty[STAGES], ready[2], free[2], sums;
   uint32_t tmem;
   volatile int abort;
@@ -244,17 +267,23 @@ __device__ __forceinline__ void ff_store16(unsigned char* s, const uint32_t (&w)
       dst[r * ld + lane] = reinterpret_cast<const uint16_t*>(ff_at64(s, r, lane >> 3))[lane & 7];
   }
 }
-// A lane's row of 32 elements into such a block: of 16 bits, or of 24 into one block of 16 and one of 8
+// A lane's row of 32 elements of 16 bits into such a block
 __device__ __forceinline__ void ff_put64(unsigned char* s, const uint32_t (&w)[16]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int q = 0; q < 4; ++q) *ff_at64(s, lane, q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
 }
-__device__ __forceinline__ void ff_put24(unsigned char* high, unsigned char* low, const float (&v)[32]) {
+// of 16
+__device__ __forceinline__ void ff_put32(unsigned char* s, const uint32_t (&w)[8]) {
   const int lane = threadIdx.x & 31;
-  uint32_t h[16], l[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int q = 0; q < 2; ++q) *ff_at32(s, lane, q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+}
+// 16 values of P (which = 0) or Q to their pieces of a block, and back
+__device__ __forceinline__ void ff_put24(uint4* to, int which, const float (&v)[16]) {
+  uint32_t h[8], l[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
     uint32_t b[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) b[i] = ff_round24(v[4 * j + i]);
@@ -262,40 +291,24 @@ __device__ __forceinline__ void ff_put24(unsigned char* high, unsigned char* low
     h[2 * j + 1] = __byte_perm(b[2], b[3], 0x7632);
     l[j] = __byte_perm(__byte_perm(b[0], b[1], 0x0051), __byte_perm(b[2], b[3], 0x0051), 0x5410);
   }
-  ff_put64(high, h);
 #pragma unroll
-  for (int q = 0; q < 2; ++q) *ff_at32(low, lane, q) = make_uint4(l[4 * q], l[4 * q + 1], l[4 * q + 2], l[4 * q + 3]);
+  for (int q = 0; q < 2; ++q) __stcs(to + 32 * (2 * which + q), make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]));
+  __stcs(to + 32 * (4 + which), make_uint4(l[0], l[1], l[2], l[3]));
 }
-__device__ __forceinline__ void ff_ask(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
-// 32 x 32 values of 24 bits on their way to shared memory (3 KB), row by row as they lie
-__device__ __forceinline__ void ff_ask24(unsigned char* s, const uint16_t* hi, const uint8_t* lo, long long ld, int rows, int cols) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void ff_take24(const uint4 (&from)[FF_KEPT_PIECES], int which, float (&v)[16]) {
+  const uint4 h0 = from[2 * which], h1 = from[2 * which + 1], l0 = from[4 + which];
+  const uint32_t h[8] = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w}, l[4] = {l0.x, l0.y, l0.z, l0.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = (lane >> 2) + 8 * i, c = 8 * (lane & 3);
-    if (row < rows && c < cols) ff_ask(smem_addr(ff_at64(s, row, lane & 3)), hi + row * ld + c);
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = (lane >> 1) + 16 * i, c = 16 * (lane & 1);
-    if (row < rows && c < cols) ff_ask(smem_addr(ff_at32(s + 2048, row, lane & 1)), lo + row * ld + c);
-  }
-}
-// Once they are there, a row to each lane (beyond the matrix: anything)
-__device__ __forceinline__ void ff_take24(unsigned char* s, float (&v)[32]) {
-  const int lane = threadIdx.x & 31;
-  uint32_t h[16], l[8];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(h + 4 * q) = *ff_at64(s, lane, q);
-#pragma unroll
-  for (int q = 0; q < 2; ++q) *reinterpret_cast<uint4*>(l + 4 * q) = *ff_at32(s + 2048, lane, q);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {   // an fp32 value's upper half, and the byte below
+  for (int j = 0; j < 4; ++j) {   // an fp32 value's upper half, and the byte below
     v[4 * j] = __uint_as_float((h[2 * j] << 16) | ((l[j] << 8) & 0xff00u));
     v[4 * j + 1] = __uint_as_float((h[2 * j] & 0xffff0000u) | (l[j] & 0xff00u));
     v[4 * j + 2] = __uint_as_float((h[2 * j + 1] << 16) | ((l[j] >> 8) & 0xff00u));
     v[4 * j + 3] = __uint_as_float((h[2 * j + 1] & 0xffff0000u) | ((l[j] >> 16) & 0xff00u));
   }
+}
+// One of the epilogue's blocks to memory; what of it lies behind the matrix is not written
+__device__ __forceinline__ void ff_send(const CUtensorMap* map, const unsigned char* from, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_addr(from)), "r"(x), "r"(y) : "memory");
 }
 
 // act(g) and its slope
@@ -324,10 +337,10 @@ __device__ __forceinline__ void ff_act(int activation, float g, float& a, float&
 // Otherwise the CTAs of a cluster (1, 2, 4 or 8) share one tile of 128 x 128, each with its part of the contraction; the first adds their sums up
 // through distributed shared memory, in rank order.
 template <bool PAIR, int EPI, bool BF>
-__global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_constant__ ff_args a) {
+__global__ void __launch_bounds__(ff_threads(EPI), 1) k_ffn_product(const __grid_constant__ ff_args a) {
   extern __shared__ unsigned char ff_dyn[];
   using Smem = FfSmem<EPI>;
-  constexpr int STAGES = Smem::STAGES;
+  constexpr int STAGES = Smem::STAGES, WARPS = Smem::WARPS, COLS = ff_columns(EPI);
   constexpr int BN = PAIR ? 256 : 128, TILE_M = PAIR ? 256 : 128, OUT_N = EPI == FF_GATE ? BN / 2 : BN;
   constexpr uint32_t STAGE = 4 * FF_BOX;
   Smem& sm = *reinterpret_cast<Smem*>(ff_dyn + ((1024 - (smem_addr(ff_dyn) & 1023)) & 1023));   // at the same place in all CTAs of a cluster
@@ -335,8 +348,8 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
   const int rank = (int)ff_cluster_rank(), ctas = (int)ff_cluster_size();
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) { ff_init(&sm.full[s], 1); ff_init(&sm.empty[s], 1); }
-    for (int s = 0; s < 2; ++s) { ff_init(&sm.ready[s], 1); ff_init(&sm.free[s], (PAIR ? 2 : 1) * FF_EPI_WARPS); }
-    ff_init(&sm.sums, ctas > 1 ? (ctas - 1) * FF_EPI_WARPS : 1);
+    for (int s = 0; s < 2; ++s) { ff_init(&sm.ready[s], 1); ff_init(&sm.free[s], (PAIR ? 2 : 1) * WARPS); }
+    ff_init(&sm.sums, ctas > 1 ? (ctas - 1) * WARPS : 1);
     sm.abort = 0;
   }
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -437,29 +450,27 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
     }
     __syncwarp();
   } else {
-    // ---------------------------------------------------------------- epilogue: a warp's 32 rows, half of the tile's columns, 32 at a time
-    const int quarter = warp & 3, half = (warp - 2) >> 2, e = warp - 2;
+    // ---------------------------------------------------------------- epilogue: a warp's 32 rows, a half or a quarter of the tile's columns, COLS at a time
+    constexpr int PARTS = WARPS / 4, BLOCKS = OUT_N / COLS / PARTS;   // BLOCKS of COLS columns for this warp
+    const int quarter = warp & 3, part = (warp - 2) >> 2, e = warp - 2;
     const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
     unsigned char* const stage = sm.out[e];
     uint32_t c = 0;
-    constexpr int BLOCKS = OUT_N / 64;   // of 32 columns for this warp
     // BACK: the block of P and Q that is on its way
-    struct { int tile, q, buf; } ahead = {first, -1, 1};
+    struct { int tile, q; } ahead = {first, -1};
+    uint4 coming[EPI == FF_BACK ? FF_KEPT_PIECES : 1] = {};
     auto ask = [&] {   // for the one behind it that has rows and columns
       ++ahead.q;
-      ahead.buf ^= 1;
       for (; ahead.tile < a.tiles; ahead.tile += step, ahead.q = 0) {
         int tm, tn;
         const ff_product& p = locate(ahead.tile, tm, tn);
-        const int m = tm * TILE_M + (PAIR ? rank * FF_BM : 0) + quarter * 32, n = tn * OUT_N + 32 * (half * BLOCKS + ahead.q);
+        const int m = tm * TILE_M + (PAIR ? rank * FF_BM : 0) + quarter * 32, n = tn * OUT_N + COLS * (part * BLOCKS + ahead.q);
         if (ahead.q >= BLOCKS || m >= p.M || n >= p.N) continue;
-        const long long at = (long long)m * a.ld + n;
-        unsigned char* const to = stage + 6144 * ahead.buf;
-        ff_ask24(to, a.kept.p_hi + at, a.kept.p_lo + at, a.ld, p.M - m, p.N - n);
-        ff_ask24(to + 3072, a.kept.q_hi + at, a.kept.q_lo + at, a.ld, p.M - m, p.N - n);
+        const uint4* const from = ff_block(a.kept, m, a.ld, n);
+#pragma unroll
+        for (int i = 0; i < (EPI == FF_BACK ? FF_KEPT_PIECES : 1); ++i) coming[i] = __ldcs(from + 32 * i);
         break;
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
     };
     if (EPI == FF_BACK && (PAIR || rank == 0)) ask();
     for (int tile = first; tile < a.tiles && !sm.abort; tile += step, ++c) {
@@ -474,14 +485,15 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
       if constexpr (!PAIR) {
         // this CTA's sums, where another one has the tile: the stages are free, all products being done
         if (rank > 0) {
-          for (int q = 0; q < 2; ++q) {   // GATE: 32 columns of either half, else 64 columns of one
-            const int block = EPI == FF_GATE ? half + 2 * q : 2 * half + q;
-            float v[32];
-            ff_ld32(acc + 32 * block, v);
+          constexpr int MINE = BN / COLS / PARTS;
+          for (int q = 0; q < MINE; ++q) {
+            const int block = part * MINE + q;
+            float v[COLS];
+            ff_ld(acc + COLS * block, v);
             const bool none = kb0 == kb1;   // no share: nothing has been written there
-            float4* const box = reinterpret_cast<float4*>(sm.st) + (block * 4 + quarter) * 256 + lane;
+            float4* const box = reinterpret_cast<float4*>(sm.st) + (block * 4 + quarter) * 8 * COLS + lane;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) box[32 * j] = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            for (int j = 0; j < COLS / 4; ++j) box[32 * j] = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           }
           __syncwarp();
           if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(nf_at_rank(&sm.sums, 0)) : "memory");
@@ -491,14 +503,14 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
           asm volatile("fence.acq_rel.cluster;" ::: "memory");
         }
       }
-      // 32 columns of the tile's sums
-      auto tile_sums = [&](int block, float (&v)[32]) {
-        ff_ld32(acc + 32 * block, v);
+      // COLS columns of the tile's sums
+      auto tile_sums = [&](int block, float (&v)[COLS]) {
+        ff_ld(acc + COLS * block, v);
         if constexpr (!PAIR) {
           for (int r = 1; r < ctas; ++r) {
-            const uint32_t src = nf_at_rank(reinterpret_cast<float4*>(sm.st) + (block * 4 + quarter) * 256 + lane, r);
+            const uint32_t src = nf_at_rank(reinterpret_cast<float4*>(sm.st) + (block * 4 + quarter) * 8 * COLS + lane, r);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < COLS / 4; ++j) {
               float4 o;
               asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w) : "r"(src + 512 * j) : "memory");
               v[4 * j] += o.x; v[4 * j + 1] += o.y; v[4 * j + 2] += o.z; v[4 * j + 3] += o.w;
@@ -516,8 +528,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
       if (!leave && rows > 0) {
 #pragma unroll 1
         for (int q = 0; q < BLOCKS; ++q) {
-          const int block = half * BLOCKS + q, n0 = tn * OUT_N + 32 * block, cols = p.N - n0;
-          const long long at = (long long)m0 * a.ld + n0;
+          const int block = part * BLOCKS + q, n0 = tn * OUT_N + COLS * block, cols = p.N - n0;
           if (cols <= 0) break;
           if constexpr (EPI == FF_PLAIN) {
             float v[32];
@@ -540,20 +551,19 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
-                  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
-                               ::"l"(&p.Cm), "r"(smem_addr(stage)), "r"(n0 - 32 * (q & 1)), "r"(m0) : "memory");
+                  ff_send(&p.Cm, stage, n0 - 32 * (q & 1), m0);
                   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
               }
             }
           } else if constexpr (EPI == FF_GATE) {
-            float g[32], u[32], q_[32];
+            float g[COLS], u[COLS], q_[COLS];
             tile_sums(block, g);
-            tile_sums(block + OUT_N / 32, u);
+            tile_sums(block + OUT_N / COLS, u);
             read();
-            uint32_t w[16];
+            uint32_t w[COLS / 2];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
+            for (int j = 0; j < COLS / 2; ++j) {
               float slope[2], h[2];
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
@@ -563,40 +573,44 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
               }
               w[j] = ff_pack<BF>(h[0], h[1]);
             }
-            // Out by copies from shared memory, rows of 64 or 32 bytes in their swizzles: what lies behind the matrix is not written
+            // h: out by copies from shared memory, rows of 32 bytes in their swizzle
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the block before has left
             __syncwarp();
-            ff_put64(stage, w);
-            if (a.keep) {
-              ff_put24(stage + 2048, stage + 6144, u);
-              ff_put24(stage + 4096, stage + 7168, q_);
-            }
+            ff_put32(stage, w);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-              for (int i = 0; i < (a.keep ? 5 : 1); ++i)
-                asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
-                             ::"l"(&a.planes[i]), "r"(smem_addr(stage + (i < 3 ? 2048 * i : 6144 + 1024 * (i - 3)))), "r"(n0), "r"(m0) : "memory");
+              ff_send(&a.planes[0], stage, n0, m0);
               asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
+            if (a.keep) {
+              uint4* const to = ff_block(a.kept, m0, a.ld, n0);
+              ff_put24(to, 0, u);
+              ff_put24(to, 1, q_);
+            }
           } else {
-            unsigned char* const here = stage + 6144 * ahead.buf;
-            __syncwarp();   // the other buffer has been read by all lanes
-            ask();
-            float v[32], f[32];
+            float v[COLS], f[COLS];
             tile_sums(block, v);
             read();
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            __syncwarp();   // every lane's copies are there
-            uint32_t w[2][16];
-            ff_take24(here, f);
+            uint32_t w[2][COLS / 2];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[0][j] = ff_pack<BF>(v[2 * j] * f[2 * j], v[2 * j + 1] * f[2 * j + 1]);
-            ff_take24(here + 3072, f);
+            for (int k = 0; k < 2; ++k) {
+              ff_take24(coming, k, f);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[1][j] = ff_pack<BF>(v[2 * j] * f[2 * j], v[2 * j + 1] * f[2 * j + 1]);
-            ff_store16(here, w[0], a.dg + at, a.ld, rows, cols);   // (through where P and Q were)
-            ff_store16(here + 3072, w[1], a.du + at, a.ld, rows, cols);
+              for (int j = 0; j < COLS / 2; ++j) w[k][j] = ff_pack<BF>(v[2 * j] * f[2 * j], v[2 * j + 1] * f[2 * j + 1]);
+            }
+            ask();
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the block before has left
+            __syncwarp();
+            ff_put32(stage, w[0]);
+            ff_put32(stage + 1024, w[1]);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              ff_send(&a.planes[0], stage, n0, m0);
+              ff_send(&a.planes[1], stage + 1024, n0, m0);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
           }
         }
       }
@@ -605,8 +619,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) k_ffn_product(const __grid_cons
         read();
       }
     }
-    if (EPI != FF_BACK && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-    if (EPI == FF_BACK) asm volatile("cp.async.wait_all;" ::: "memory");
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   ff_fence_before();
   __syncthreads();
@@ -780,11 +793,11 @@ __global__ void __launch_bounds__(FF_FEW_THREADS, 2) k_ffn_few(const __grid_cons
                 const float u = box[n * 64 + at];
                 float q, slope;
                 ff_act(a.activation, v[n], q, slope);
-                const long long i = n * a.ld + f;
-                a.kept.h[i] = ff_one<BF>(q * u);
+                a.kept.h[n * a.ld + f] = ff_one<BF>(q * u);
                 if (a.keep) {
-                  ff_keep24(a.kept.p_hi, a.kept.p_lo, i, u * slope);
-                  ff_keep24(a.kept.q_hi, a.kept.q_lo, i, q);
+                  const long long i = ff_place(n, a.ld, f);
+                  ff_keep24(a.kept.hi, a.kept.lo, i, u * slope);
+                  ff_keep24(a.kept.hi, a.kept.lo, i + 16, q);
                 }
               }
           }
@@ -801,9 +814,9 @@ __global__ void __launch_bounds__(FF_FEW_THREADS, 2) k_ffn_few(const __grid_cons
             float pf[8], qf[8];   // on their way together
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const long long i = (long long)min(n0 + j, p.N - 1) * a.ld + f;
-              pf[j] = ff_load24(a.kept.p_hi, a.kept.p_lo, i);
-              qf[j] = ff_load24(a.kept.q_hi, a.kept.q_lo, i);
+              const long long i = ff_place(min(n0 + j, p.N - 1), a.ld, f);
+              pf[j] = ff_load24(a.kept.hi, a.kept.lo, i);
+              qf[j] = ff_load24(a.kept.hi, a.kept.lo, i + 16);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -888,10 +901,10 @@ static int ff_begin() {
 }
 static int64_t ff_ld(int hidden) { return ((int64_t)hidden + 15) / 16 * 16; }   // of h and what is made like it
 static int64_t ff_plane(int64_t rows, int hidden, int bytes) { return (rows * ff_ld(hidden) * bytes + 255) / 256 * 256; }
+static int64_t ff_kept_bytes(int64_t rows, int hidden) { return ff_plane((rows + 31) / 32 * 32, hidden, 6) + 256; }   // of P and Q, in either form
 static ff_kept ff_planes(void* base, int64_t rows, int hidden) {
-  char* p = (char*)base;
-  const int64_t two = ff_plane(rows, hidden, 2), one = ff_plane(rows, hidden, 1);
-  return {(uint16_t*)p, (uint16_t*)(p + two), (uint16_t*)(p + 2 * two), (uint8_t*)(p + 3 * two), (uint8_t*)(p + 3 * two + one)};
+  char* const p = (char*)base + ff_plane(rows, hidden, 2);
+  return {(uint16_t*)base, (uint4*)p, (uint16_t*)p, (uint8_t*)(p + ff_plane(rows, hidden, 4))};
 }
 
 // Which form a product takes.  Pairs where their tiles, with those of the products beside it whose contractions are equally long, fill the GPU more than half
@@ -933,13 +946,13 @@ static int ff_go(ff_args& a, cudaStream_t s) {
     // how many CTAs share a tile, by the time that is to be expected: 0.15 us a stage, and what a tile costs besides
     float best = 0.f;
     for (int c = 1; c <= 8; c *= 2) {
-      const int64_t at_once = active_clusters<k_ffn_product<PAIR, EPI, BF>>(FF_THREADS, c, SMEM), waves = (tiles + at_once - 1) / at_once;
+      const int64_t at_once = active_clusters<k_ffn_product<PAIR, EPI, BF>>(ff_threads(EPI), c, SMEM), waves = (tiles + at_once - 1) / at_once;
       const float t = (float)waves * (0.15f * (float)((longest + c - 1) / c) + (c > 1 ? 4.0f + 0.3f * (float)c : 3.0f));
       if (c == 1 || t < best) { best = t; cluster = c; }
     }
     grid = (int)tiles * cluster;
   }
-  launch_clusters(k_ffn_product<PAIR, EPI, BF>, grid, FF_THREADS, cluster, SMEM, s, a);
+  launch_clusters(k_ffn_product<PAIR, EPI, BF>, grid, ff_threads(EPI), cluster, SMEM, s, a);
   return launch_status();
 }
 // The products of a that take pairs in one launch, the others in one for those whose contractions are equally long
@@ -989,18 +1002,15 @@ static bool ff_good(const pylo_ffn* f) {
   return f && f->rows >= 0 && f->rows <= (1 << 30) && f->width > 0 && f->hidden > 0 && f->out > 0 && f->width <= (1 << 24) && f->hidden <= (1 << 24) &&
          f->out <= (1 << 24) && (f->type == PYLO_BF16 || f->type == PYLO_FP16) && f->activation >= PYLO_ACT_SILU && f->activation <= PYLO_ACT_RELU;
 }
-// The maps of what the gate writes: planes [rows][hidden], boxes of 32 x 32 elements in the swizzle of their rows
-static int ff_map_planes(ff_args& a, int64_t rows, int64_t hidden) {
+// Maps of [rows][hidden] that an epilogue writes: boxes of 32 rows and 16 columns
+static int ff_map_planes(ff_args& a, int64_t rows, int64_t hidden, void* first, void* second) {
   FfEncode fn = ff_encode();
   if (!fn) return -5;
-  void* const at[5] = {a.kept.h, a.kept.p_hi, a.kept.q_hi, a.kept.p_lo, a.kept.q_lo};
-  for (int i = 0; i < (a.keep ? 5 : 1); ++i) {
-    const bool wide = i < 3;
-    const cuuint64_t dims[2] = {(cuuint64_t)hidden, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)a.ld * (wide ? 2 : 1)};
-    const cuuint32_t box[2] = {32, 32}, unit[2] = {1, 1};
-    if (fn(&a.planes[i], wide ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, at[i], dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           wide ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) return -5;
-  }
+  const cuuint64_t dims[2] = {(cuuint64_t)hidden, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)a.ld * 2};
+  const cuuint32_t box[2] = {16, 32}, unit[2] = {1, 1};
+  for (int i = 0; i < (second ? 2 : 1); ++i)
+    if (fn(&a.planes[i], CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, i ? second : first, dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B,
+           CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) return -5;
   return 0;
 }
 // C's map, where its rows allow for one: boxes of 32 rows of 64
@@ -1018,7 +1028,7 @@ extern "C" {
 
 int64_t pylo_b200_gated_ffn_kept(int64_t rows, int hidden, int keep) {
   if (rows <= 0 || hidden <= 0) return 0;
-  return ff_plane(rows, hidden, 2) * (keep ? 3 : 1) + ff_plane(rows, hidden, 1) * (keep ? 2 : 0);
+  return ff_plane(rows, hidden, 2) + (keep ? ff_kept_bytes(rows, hidden) : 0);
 }
 int64_t pylo_b200_gated_ffn_workspace(int64_t rows, int hidden) { return rows <= 0 || hidden <= 0 ? 0 : 2 * ff_plane(rows, hidden, 2); }
 
@@ -1048,7 +1058,7 @@ int pylo_b200_gated_ffn(const pylo_ffn* f, void* stream) {
   if (int rc = ff_map(&a.p[0].A[0], f->x, f->rows, f->width, f->ld_x, f->type)) return rc;
   if (int rc = ff_map(&a.p[0].B[0], f->w_gate, f->hidden, f->width, f->ld_gate, f->type)) return rc;
   if (int rc = ff_map(&a.p[0].B[1], f->w_up, f->hidden, f->width, f->ld_up, f->type)) return rc;
-  if (int rc = ff_map_planes(a, f->rows, f->hidden)) return rc;
+  if (int rc = ff_map_planes(a, f->rows, f->hidden, kept.h, nullptr)) return rc;
   if (int rc = ff_run<FF_GATE>(a, f->type, s)) return rc;
   a.p[0] = ff_of(f->y, f->out, f->rows, f->out, f->hidden, 1, 0, 0);
   if (int rc = ff_map(&a.p[0].A[0], kept.h, f->rows, f->hidden, ld, f->type)) return rc;
@@ -1084,6 +1094,7 @@ int pylo_b200_gated_ffn_backward(const pylo_ffn* f, void* stream) {
       a.p[0] = ff_of(nullptr, 0, f->rows, f->hidden, f->out, 1, 0, 1);
       if (int rc = ff_map(&a.p[0].A[0], f->dy, f->rows, f->out, f->ld_dy, f->type)) return rc;
       if (int rc = ff_map(&a.p[0].B[0], f->w_down, f->out, f->hidden, f->ld_down, f->type)) return rc;
+      if (int rc = ff_map_planes(a, f->rows, f->hidden, a.dg, a.du)) return rc;
       if (int rc = ff_run<FF_BACK>(a, f->type, s)) return rc;
     }
   }
