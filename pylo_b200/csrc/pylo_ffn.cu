@@ -22,6 +22,7 @@
 // one that runs out ends the CTA's work in order and sets a bit of the caller's status word.
 #include <cuda.h>
 #include <cuda_bf16.h>
+#include <math_constants.h>
 
 #include "pylo_common.cuh"
 #include "pylo_launch.cuh"
@@ -640,8 +641,13 @@ __global__ void __launch_bounds__(ff_threads(EPI), 1) k_ffn_product(const __grid
 // nearly all of the latter zeros), and two CTAs share an SM.  A tile's sums lie feature by feature in the lanes, row by row in the columns, so that a
 // warp's lanes write neighbours.  The CTAs of a cluster share a tile as above.  Gate: a tile has 64 rows of Wg and the same 64 of Wu; the warps
 // of the latter hand their sums to those of the former.
+//
+// Up to FF_FINE rows, h, dg and du are 16 bits and 16 more of what their rounding left, FF_FINE rows below: of so few values the roundings' average may be far
+// from what it is expected to be, and as more rows of operand B, beside the same weights, they cost next to nothing.  The result adds both rows' sums up; the
+// weights' gradients take them as two parts of their contractions.
 // ------------------------------------------------------------------------------------------------
 #define FF_FEW 32
+#define FF_FINE 16
 #define FF_FEW_THREADS 192
 template <int ROWS>
 struct FfFewSmem {
@@ -661,6 +667,18 @@ __device__ __forceinline__ void ff_keep24(uint16_t* hi, uint8_t* lo, long long i
 }
 template <bool BF>
 __device__ __forceinline__ uint16_t ff_one(float v) { return (uint16_t)ff_pack<BF>(v, 0.f); }
+// A value that becomes an operand: rounded, and FF_FINE rows below what that left of it
+template <bool BF>
+__device__ __forceinline__ void ff_two(uint16_t* to, long long ld, bool fine, float v) {
+  const uint16_t high = ff_one<BF>(v);
+  *to = high;
+  if (fine) {
+    float f;
+    if constexpr (BF) f = __uint_as_float((uint32_t)high << 16);
+    else f = __half2float(__ushort_as_half(high));
+    to[FF_FINE * ld] = fabsf(f) < CUDART_INF_F ? ff_one<BF>(v - f) : 0;
+  }
+}
 
 template <int EPI, bool BF, int ROWS>
 __global__ void __launch_bounds__(FF_FEW_THREADS, 2) k_ffn_few(const __grid_constant__ ff_args a) {
@@ -793,7 +811,7 @@ __global__ void __launch_bounds__(FF_FEW_THREADS, 2) k_ffn_few(const __grid_cons
                 const float u = box[n * 64 + at];
                 float q, slope;
                 ff_act(a.activation, v[n], q, slope);
-                a.kept.h[n * a.ld + f] = ff_one<BF>(q * u);
+                ff_two<BF>(a.kept.h + n * a.ld + f, a.ld, ROWS == FF_FINE, q * u);
                 if (a.keep) {
                   const long long i = ff_place(n, a.ld, f);
                   ff_keep24(a.kept.hi, a.kept.lo, i, u * slope);
@@ -803,6 +821,10 @@ __global__ void __launch_bounds__(FF_FEW_THREADS, 2) k_ffn_few(const __grid_cons
           }
         }
       } else if (good && f < p.M) {
+        if (EPI == FF_PLAIN && p.N <= FF_FINE) {
+#pragma unroll
+          for (int n = 0; n < ROWS - FF_FINE; ++n) v[n] += v[n + FF_FINE];
+        }
 #pragma unroll
         for (int n0 = 0; n0 < ROWS; n0 += 8) {
           if (n0 >= p.N) break;
@@ -822,8 +844,8 @@ __global__ void __launch_bounds__(FF_FEW_THREADS, 2) k_ffn_few(const __grid_cons
             for (int j = 0; j < 8; ++j)
               if (n0 + j < p.N) {
                 const long long i = (n0 + j) * a.ld + f;
-                a.dg[i] = ff_one<BF>(v[n0 + j] * pf[j]);
-                a.du[i] = ff_one<BF>(v[n0 + j] * qf[j]);
+                ff_two<BF>(a.dg + i, a.ld, ROWS == FF_FINE, v[n0 + j] * pf[j]);
+                ff_two<BF>(a.du + i, a.ld, ROWS == FF_FINE, v[n0 + j] * qf[j]);
               }
           }
         }
@@ -901,9 +923,10 @@ static int ff_begin() {
 }
 static int64_t ff_ld(int hidden) { return ((int64_t)hidden + 15) / 16 * 16; }   // of h and what is made like it
 static int64_t ff_plane(int64_t rows, int hidden, int bytes) { return (rows * ff_ld(hidden) * bytes + 255) / 256 * 256; }
+static int64_t ff_rows(int64_t rows) { return rows <= FF_FINE ? 2 * FF_FINE : rows; }   // of h, dg, du
 static int64_t ff_kept_bytes(int64_t rows, int hidden) { return ff_plane((rows + 31) / 32 * 32, hidden, 6) + 256; }   // of P and Q, in either form
 static ff_kept ff_planes(void* base, int64_t rows, int hidden) {
-  char* const p = (char*)base + ff_plane(rows, hidden, 2);
+  char* const p = (char*)base + ff_plane(ff_rows(rows), hidden, 2);
   return {(uint16_t*)base, (uint4*)p, (uint16_t*)p, (uint8_t*)(p + ff_plane(rows, hidden, 4))};
 }
 
@@ -993,10 +1016,11 @@ static int ff_go_few(ff_args& a, cudaStream_t s) {
 template <int EPI>
 static int ff_run_few(ff_args& a, int rows, int type, cudaStream_t s) {
   const bool bf = type == PYLO_BF16;
-  if (rows <= 16) return bf ? ff_go_few<EPI, true, 16>(a, s) : ff_go_few<EPI, false, 16>(a, s);
+  if constexpr (EPI != FF_PLAIN)
+    if (rows <= FF_FINE) return bf ? ff_go_few<EPI, true, 16>(a, s) : ff_go_few<EPI, false, 16>(a, s);
   return bf ? ff_go_few<EPI, true, 32>(a, s) : ff_go_few<EPI, false, 32>(a, s);
 }
-static int ff_few_rows(int64_t rows) { return rows > FF_FEW ? 0 : rows <= 16 ? 16 : 32; }   // of a tile; 0: not few
+static int ff_few_rows(int64_t rows) { return rows > FF_FEW ? 0 : rows <= FF_FINE ? FF_FINE : FF_FEW; }   // of a tile; 0: not few
 static bool ff_operand(const void* p, int64_t ld, int64_t cols) { return p && ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld >= cols; }
 static bool ff_good(const pylo_ffn* f) {
   return f && f->rows >= 0 && f->rows <= (1 << 30) && f->width > 0 && f->hidden > 0 && f->out > 0 && f->width <= (1 << 24) && f->hidden <= (1 << 24) &&
@@ -1028,9 +1052,9 @@ extern "C" {
 
 int64_t pylo_b200_gated_ffn_kept(int64_t rows, int hidden, int keep) {
   if (rows <= 0 || hidden <= 0) return 0;
-  return ff_plane(rows, hidden, 2) + (keep ? ff_kept_bytes(rows, hidden) : 0);
+  return ff_plane(ff_rows(rows), hidden, 2) + (keep ? ff_kept_bytes(rows, hidden) : 0);
 }
-int64_t pylo_b200_gated_ffn_workspace(int64_t rows, int hidden) { return rows <= 0 || hidden <= 0 ? 0 : 2 * ff_plane(rows, hidden, 2); }
+int64_t pylo_b200_gated_ffn_workspace(int64_t rows, int hidden) { return rows <= 0 || hidden <= 0 ? 0 : 2 * ff_plane(ff_rows(rows), hidden, 2); }
 
 int pylo_b200_gated_ffn(const pylo_ffn* f, void* stream) {
   CHECK_ARG(ff_good(f));
@@ -1044,6 +1068,7 @@ int pylo_b200_gated_ffn(const pylo_ffn* f, void* stream) {
   a.kept = kept; a.ld = ld; a.n = 1; a.activation = f->activation; a.keep = f->keep; a.status = f->status; a.host_status = f->host_status;
   cudaStream_t s = (cudaStream_t)stream;
   if (const int few = ff_few_rows(f->rows)) {
+    const bool fine = few == FF_FINE;
     a.p[0] = ff_of(nullptr, 0, f->hidden, f->rows, f->width, 1, 0, 0);
     if (int rc = ff_map(&a.p[0].A[0], f->w_gate, f->hidden, f->width, f->ld_gate, f->type)) return rc;
     if (int rc = ff_map(&a.p[0].A[1], f->w_up, f->hidden, f->width, f->ld_up, f->type)) return rc;
@@ -1051,7 +1076,7 @@ int pylo_b200_gated_ffn(const pylo_ffn* f, void* stream) {
     if (int rc = ff_run_few<FF_GATE>(a, (int)f->rows, f->type, s)) return rc;
     a.p[0] = ff_of(f->y, f->out, f->out, f->rows, f->hidden, 1, 0, 0);
     if (int rc = ff_map(&a.p[0].A[0], f->w_down, f->out, f->hidden, f->ld_down, f->type)) return rc;
-    if (int rc = ff_map(&a.p[0].B[0], kept.h, f->rows, f->hidden, ld, f->type, few)) return rc;
+    if (int rc = ff_map(&a.p[0].B[0], kept.h, fine ? FF_FINE + f->rows : f->rows, f->hidden, ld, f->type, FF_FEW)) return rc;
     return ff_run_few<FF_PLAIN>(a, (int)f->rows, f->type, s);
   }
   a.p[0] = ff_of(nullptr, 0, f->rows, f->hidden, f->width, 1, 0, 0);
@@ -1080,9 +1105,10 @@ int pylo_b200_gated_ffn_backward(const pylo_ffn* f, void* stream) {
   ff_args a = {};
   a.kept = kept; a.ld = ld; a.activation = f->activation; a.status = f->status; a.host_status = f->host_status;
   a.dg = (uint16_t*)f->work;
-  a.du = (uint16_t*)((char*)f->work + ff_plane(f->rows, f->hidden, 2));
+  a.du = (uint16_t*)((char*)f->work + ff_plane(ff_rows(f->rows), f->hidden, 2));
   cudaStream_t s = (cudaStream_t)stream;
   const int few = ff_few_rows(f->rows);
+  const bool fine = few == FF_FINE;
   if (inner) {   // dh (m: rows, n: hidden, k: out), Wd's rows being the contraction index
     a.n = 1;
     if (few) {
@@ -1102,8 +1128,8 @@ int pylo_b200_gated_ffn_backward(const pylo_ffn* f, void* stream) {
     a.p[0] = ff_of(f->dx, f->width, f->width, f->rows, f->hidden, 2, 1, 0);
     if (int rc = ff_map(&a.p[0].A[0], f->w_gate, f->hidden, f->width, f->ld_gate, f->type)) return rc;
     if (int rc = ff_map(&a.p[0].A[1], f->w_up, f->hidden, f->width, f->ld_up, f->type)) return rc;
-    if (int rc = ff_map(&a.p[0].B[0], a.dg, f->rows, f->hidden, ld, f->type, few)) return rc;
-    if (int rc = ff_map(&a.p[0].B[1], a.du, f->rows, f->hidden, ld, f->type, few)) return rc;
+    for (int k = 0; k < 2; ++k)
+      if (int rc = ff_map(&a.p[0].B[k], k ? a.du : a.dg, fine ? FF_FINE + f->rows : f->rows, f->hidden, ld, f->type, FF_FEW)) return rc;
     if (int rc = ff_run_few<FF_PLAIN>(a, (int)f->rows, f->type, s)) return rc;
   }
   a.n = 0;
@@ -1116,14 +1142,18 @@ int pylo_b200_gated_ffn_backward(const pylo_ffn* f, void* stream) {
   }
   for (int k = 0; k < 2; ++k)
     if (void* const out = k ? f->dw_up : f->dw_gate) {
-      ff_product& p = a.p[a.n++] = ff_of(out, f->width, f->hidden, f->width, f->rows, 1, 1, 1);
-      if (int rc = ff_map(&p.A[0], k ? a.du : a.dg, f->rows, f->hidden, ld, f->type)) return rc;
-      if (int rc = ff_map(&p.B[0], f->x, f->rows, f->width, f->ld_x, f->type)) return rc;
+      ff_product& p = a.p[a.n++] = ff_of(out, f->width, f->hidden, f->width, f->rows, 1 + fine, 1, 1);
+      for (int i = 0; i <= (int)fine; ++i) {
+        if (int rc = ff_map(&p.A[i], (k ? a.du : a.dg) + i * FF_FINE * ld, f->rows, f->hidden, ld, f->type)) return rc;
+        if (int rc = ff_map(&p.B[i], f->x, f->rows, f->width, f->ld_x, f->type)) return rc;
+      }
     }
   if (f->dw_down) {
-    ff_product& p = a.p[a.n++] = ff_of(f->dw_down, f->hidden, f->out, f->hidden, f->rows, 1, 1, 1);
-    if (int rc = ff_map(&p.A[0], f->dy, f->rows, f->out, f->ld_dy, f->type)) return rc;
-    if (int rc = ff_map(&p.B[0], kept.h, f->rows, f->hidden, ld, f->type)) return rc;
+    ff_product& p = a.p[a.n++] = ff_of(f->dw_down, f->hidden, f->out, f->hidden, f->rows, 1 + fine, 1, 1);
+    for (int i = 0; i <= (int)fine; ++i) {
+      if (int rc = ff_map(&p.A[i], f->dy, f->rows, f->out, f->ld_dy, f->type)) return rc;
+      if (int rc = ff_map(&p.B[i], kept.h + i * FF_FINE * ld, f->rows, f->hidden, ld, f->type)) return rc;
+    }
   }
   for (int k = 0; k < a.n; ++k)
     if (int rc = ff_map_c(a.p[k], f->type)) return rc;

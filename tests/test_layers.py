@@ -182,9 +182,10 @@ def act64(name, g):
     return g.clamp(min=0), (g > 0).double()
 
 
-def ffn64(x, wg, wu, wd, dy, act):
-    """{name: (value, slack)}: slack without the last rounding."""
-    u_ = half_step(x.dtype)
+def ffn64(x, wg, wu, wd, dy, act, operands=None):
+    """{name: (value, slack)}: slack without the last rounding.  operands: how far h, dg and du are off, relative to their size: half a step of the type,
+    or what is given."""
+    u_ = half_step(x.dtype) if operands is None else operands
     tiny = least(x.dtype)
     x, wg, wu, wd = (t.double() for t in (x, wg, wu, wd))
     rows, width = x.shape
@@ -250,6 +251,28 @@ def check_ffn(x, wg, wu, wd, dy, act="silu"):
     (300, 264, 136, 8), (520, 520, 1032, 520)])
 def test_ffn(rows, width, hidden, out, dtype):
     check_ffn(*ffn_inputs(rows, width, hidden, out, dtype))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,width,hidden,out", [(1, 64, 64, 64), (2, 3, 5, 7), (1, 40, 64, 1200), (5, 1001, 333, 77), (16, 136, 200, 72), (16, 512, 2000, 512)])
+def test_ffn_of_few_rows_rounds_only_results(rows, width, hidden, out, dtype):
+    """Up to 16 rows, h, dg and du are two numbers of the type each: what the second leaves is half a step of half a step."""
+    x, wg, wu, wd, dy = ffn_inputs(rows, width, hidden, out, dtype, seed=11)
+    want = ffn64(x, wg, wu, wd, dy, "silu", operands=half_step(dtype) ** 2)
+    leaves = [t.detach().requires_grad_() for t in (x, wg, wu, wd)]
+    y = layers.gated_ffn(*leaves)
+    for name, got in {"y": y.detach(), **dict(zip(("dx", "dw_gate", "dw_up", "dw_down"), torch.autograd.grad(y, leaves, dy)))}.items():
+        near(got, *want[name], name)
+    layers.check_status()
+
+
+@gpu
+def test_ffn_of_few_rows_beyond_the_type():
+    """A hidden value that rounds to infinity leaves nothing behind that a second number could hold."""
+    one = torch.ones(1, 1, device="cuda", dtype=FP16)
+    with torch.no_grad():
+        assert layers.gated_ffn(300 * one, one, one, one, "relu").item() == math.inf
 
 
 @gpu
