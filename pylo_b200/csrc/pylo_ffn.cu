@@ -337,6 +337,8 @@ __device__ __forceinline__ void ff_act(int activation, float g, float& a, float&
 // read both halves); persistent, with two accumulators, so that one tile's epilogue runs beside the next one's products.
 // Otherwise the CTAs of a cluster (1, 2, 4 or 8) share one tile of 128 x 128, each with its part of the contraction; the first adds their sums up
 // through distributed shared memory, in rank order.
+//
+// 8192 rows x 4096 x 14336 bf16 on a B200: gate 1213 us (1.59 PFLOP/s), y 631, back 759 (1.27), dx and the weights' gradients 3005 (1.60), at the power limit.
 template <bool PAIR, int EPI, bool BF>
 __global__ void __launch_bounds__(ff_threads(EPI), 1) k_ffn_product(const __grid_constant__ ff_args a) {
   extern __shared__ unsigned char ff_dyn[];
