@@ -687,7 +687,7 @@ __device__ __forceinline__ bool dt_teacher(const DtArgs& a, long long row, DtPee
   for (int k = lane; k < K; k += 32) sum += dt_exp2(e[k].lp - most);
   const float log_sum = log2f(rw_warp_sum(sum));
   for (int k = lane; k < K; k += 32) {
-    const float lp = e[k].lp - most - log_sum, p = dt_exp2(lp);
+    const float lp = e[k].lp - most - log_sum, p = e[k].id == DT_PADDING ? 0.f : dt_exp2(lp);   // (beside a teacher's NaN or infinity lp is NaN)
     e[k].lp = lp;
     e[k].p = p;
     e[k].column = p;
@@ -715,15 +715,18 @@ __device__ __forceinline__ float dt_cross(const DtArgs& a, const T* s, const DtE
   for (int first = threadIdx.x & 31; first < a.top; first += 128) {
     DtEntry q[4];
     float v[4];
+    bool counts[4];   // padding has no class to read, whatever its p
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      q[i].p = v[i] = 0.f;
+      q[i] = {DT_PADDING, 0.f, 0.f, 0.f};
+      v[i] = 0.f;
       if (first + 32 * i < a.top) q[i] = e[first + 32 * i];
-      if (!(q[i].p == 0.f)) v[i] = rw_float(s[q[i].id < 0 ? ~q[i].id : q[i].id]);   // all four on their way together
+      counts[i] = q[i].id != DT_PADDING && !(q[i].p == 0.f);
+      if (counts[i]) v[i] = rw_float(s[q[i].id < 0 ? ~q[i].id : q[i].id]);   // all four on their way together
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (!(q[i].p == 0.f)) sum = fmaf(q[i].p, fmaf(v[i] - m, -a.c, q[i].lp), sum);
+      if (counts[i]) sum = fmaf(q[i].p, fmaf(v[i] - m, -a.c, q[i].lp), sum);
   }
   return rw_warp_sum(sum);
 }
@@ -861,7 +864,7 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_teachers(const DtAr
     if (any) {
       // relative to the first entry's logit, where it is a number: of all logits far off centre the differences count
       const T* const s = (const T*)a.logits + row * a.stride;
-      float near = e[0].p > 0.f ? rw_float(s[e[0].id < 0 ? ~e[0].id : e[0].id]) : 0.f;
+      float near = e[0].id != DT_PADDING && e[0].p > 0.f ? rw_float(s[e[0].id < 0 ? ~e[0].id : e[0].id]) : 0.f;
       if (!(fabsf(near) < CUDART_INF_F)) near = 0.f;
       const float cross = dt_cross(a, s, e, near);
       float sum = 0.f;
