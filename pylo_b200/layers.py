@@ -122,6 +122,7 @@ class _LayerNorm(torch.autograd.Function):
     @_once
     def backward(ctx, dy):
         rows, weight, stat = ctx.saved_tensors
+        rows, stat = _rows(rows), _rows(stat)   # (hooks may have laid them out anew)
         n, width = rows.shape
         device = rows.get_device()
         dy = _rows(dy)
@@ -130,7 +131,7 @@ class _LayerNorm(torch.autograd.Function):
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty_like(weight) if need_b else None
         kind, mean = TYPES[rows.dtype], stat.data_ptr()
-        w = L.Norm(x=rows.data_ptr(), dy=dy.data_ptr(), weight=None if weight is None else weight.data_ptr(), mean=mean, rstd=mean + 4 * n,
+        w = L.Norm(x=rows.data_ptr(), dy=dy.data_ptr(), weight=None if weight is None else weight.data_ptr(), mean=mean, rstd=mean + 4 * stat.stride(0),
                    dx=dx.data_ptr() if need_x else None, dweight=dw.data_ptr() if need_w else None, dbias=db.data_ptr() if need_b else None, rows=n,
                    x_stride=rows.stride(0), dy_stride=dy.stride(0), width=width, type=kind, weight_type=kind if weight is None else TYPES[weight.dtype])
         if need_w or need_b:
@@ -265,16 +266,25 @@ class _Operands:
             item.ld = apart[k]
         _call(L.lib.pylo_b200_pad_rows, "gated_ffn", first.get_device(), items, len(odd))
 
-    def pointers(self, tensors, room):
-        if room is None:
+    def pointers(self, tensors):
+        if self.room is None:
             return [t.data_ptr() for t in tensors]
-        base = room.data_ptr()
+        base = self.room.data_ptr()
         return [t.data_ptr() if at < 0 else base + at for t, at in zip(tensors, self.at)]
 
+    def again(self, tensors, room):
+        """(operands, what holds them) of a backward pass: the forward pass's copies, ``room``, and the other matrices as autograd hands them back.  Its
+        hooks may have laid those out anew (a slice that was offloaded comes back without its gaps), so how they lie is looked up again."""
+        copied = [False] * len(tensors) if room is None else [at >= 0 for at in self.at]
+        rest = [t for t, c in zip(tensors, copied) if not c]
+        lies = _Operands(rest) if rest else None
+        found = iter(zip(lies.pointers(rest), lies.apart) if rest else ())
+        return [(room.data_ptr() + at, apart) if c else next(found) for c, at, apart in zip(copied, self.at or copied, self.apart)], lies
 
-def _ffn_struct(tensors, operands, room, activation):
-    x, w_gate, w_up, w_down = operands.pointers(tensors, room)
-    ld_x, ld_gate, ld_up, ld_down = operands.apart
+
+def _ffn_struct(tensors, operands, activation):
+    """operands: the tensors' addresses, and elements between their rows"""
+    (x, ld_x), (w_gate, ld_gate), (w_up, ld_up), (w_down, ld_down) = operands
     (rows, width), (out, hidden) = tensors[0].shape, tensors[3].shape
     return L.Ffn(x=x, w_gate=w_gate, w_up=w_up, w_down=w_down, rows=rows, ld_x=ld_x, ld_gate=ld_gate, ld_up=ld_up, ld_down=ld_down, width=width,
                  hidden=hidden, out=out, type=TYPES[tensors[0].dtype], activation=activation, host_status=_status_word())
@@ -288,7 +298,7 @@ def _ffn_forward(tensors, activation, keep):
         return y, None, None
     device = rows.get_device()
     operands = _Operands(tensors)
-    f = _ffn_struct(tensors, operands, operands.room, activation)
+    f = _ffn_struct(tensors, zip(operands.pointers(tensors), operands.apart), activation)
     kept = torch.empty(_size("pylo_b200_gated_ffn_kept", device, f.rows, f.hidden, keep), dtype=torch.uint8, device=rows.device)
     f.y, f.kept, f.keep = y.data_ptr(), kept.data_ptr(), keep
     _call(L.lib.pylo_b200_gated_ffn, "gated_ffn", device, C.byref(f))
@@ -316,9 +326,10 @@ class _GatedFFN(torch.autograd.Function):
             device = rows.get_device()
             dy = _rows(dy)
             lies = _Operands((dy,))
-            f = _ffn_struct(tensors, ctx.operands, room, ctx.activation)
+            operands, held = ctx.operands.again(tensors, room)
+            f = _ffn_struct(tensors, operands, ctx.activation)
             work = torch.empty(_size("pylo_b200_gated_ffn_workspace", device, f.rows, f.hidden), dtype=torch.uint8, device=rows.device)
-            (f.dy,), (f.ld_dy,), f.kept, f.work = lies.pointers((dy,), lies.room), lies.apart, kept.data_ptr(), work.data_ptr()
+            (f.dy,), (f.ld_dy,), f.kept, f.work = lies.pointers((dy,)), lies.apart, kept.data_ptr(), work.data_ptr()
             f.dx, f.dw_gate, f.dw_up, f.dw_down = (None if g is None else g.data_ptr() for g in grads)
             _call(L.lib.pylo_b200_gated_ffn_backward, "gated_ffn backward", device, C.byref(f))
         return *grads, None
@@ -445,6 +456,8 @@ class _Distillation(torch.autograd.Function):
     @_once
     def backward(ctx, upstream):
         rows, teacher, ids, weights, work = ctx.saved_tensors
+        # (hooks may have laid them out anew)
+        rows, teacher, ids, weights = _rows(rows), _contiguous(teacher), _contiguous(ids), None if weights is None else _contiguous(weights)
         grad = _like(rows)
         if upstream.dtype is not torch.float32 or not upstream.is_contiguous():
             upstream = upstream.to(torch.float32).contiguous()

@@ -1,13 +1,14 @@
 """Layer norm, the gated feed-forward block and distillation where calls leave the ordinary: values that are no numbers, tensors that come back
 from autograd's hooks, forward-mode derivatives, first calls of several threads."""
 
+import contextlib
 import math
 
 import pytest
 import torch
 
 from pylo_b200 import layers
-from test_layers import BF16, F32, FP16, E, distill64, distill_inputs, near
+from test_layers import BF16, F32, FP16, E, distill64, distill_inputs, ffn_inputs, near, norm64, randn
 
 gpu = pytest.mark.gpu
 
@@ -47,3 +48,101 @@ def test_distill_of_teachers_that_are_no_numbers(vocab, top, dtype):
             both = layers.distillation_loss_and_grad(logits, teacher, ids, 2.0, reduction=reduction)
             assert bool(both[0].isnan()) and torch.equal(both[1].isnan(), there & off[:, None])
             near(both[1][~off], want[2][~off] * by, (want[4][~off] + 8 * E * want[2][~off].abs()) * by, "of both")
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# hooks on what autograd saves
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def elsewhere(t, gap=3):
+    """The same matrix, rows `gap` elements further apart, beginning off a 16-byte boundary; vectors as they are."""
+    if t.dim() != 2 or t.dtype == torch.uint8:
+        return t.clone()
+    wide = torch.full((t.shape[0], t.shape[1] + gap), 7.0, device=t.device, dtype=t.dtype)
+    wide[:, 1:1 + t.shape[1]] = t
+    return wide[:, 1:1 + t.shape[1]]
+
+
+HOOKS = {
+    "offloaded": lambda: torch.autograd.graph.save_on_cpu(),
+    "offloaded, pinned": lambda: torch.autograd.graph.save_on_cpu(pin_memory=True),
+    "packed": lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t.contiguous().clone(), lambda t: t),
+    "unpacked elsewhere": lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t, elsewhere),
+    "by columns": lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 and t.is_floating_point() else t),
+}
+
+
+def operators_of_strided_tensors():
+    """(name, function of leaves, leaves): slices with gaps between their rows, on and off 16-byte boundaries."""
+    big, wide = randn(70, 3, 144, seed=1, dtype=BF16), randn(96, 400, seed=8, dtype=BF16, scale=0.1)
+    _, _, wu, wd, dy = ffn_inputs(70, 128, 96, 128, BF16, seed=3)
+    tall = randn(128, 104, seed=9, dtype=BF16, scale=0.1)
+    for name, x, gate, down in (("on", big[:, 1, :128], wide[:, 16:144], tall[:, 8:]), ("off", big[:, 1, 3:131], wide[:, 5:133], wd), ("mixed", big[:, 1, 8:136], wide[:, 5:133], tall[:, 8:]),
+                                ("one row", big[:1, 1, :128], wide[:, 16:144], tall[:, :96])):
+        yield "block " + name, lambda *t: layers.gated_ffn(*t), (x, gate, wu, down)
+    yield "norm on", lambda *t: layers.layer_norm(*t), (big[:, 1, :128], randn(128, seed=2, dtype=BF16), randn(128, seed=4, dtype=BF16))
+    yield "norm off", lambda *t: layers.layer_norm(*t), (big[:, 1, 3:131], randn(128, seed=2))
+    logits = randn(12, 3, 1200, seed=1, dtype=BF16, scale=2.0)
+    for cut in (logits[:, 1, 8:1108], logits[:, 1, 3:1104], logits[:, 0, :30]):
+        _, teacher, ids = distill_inputs(12, cut.shape[1], 9, BF16, seed=2)
+        yield f"distillation {cut.shape[1]}", lambda t, teacher=teacher, ids=ids: layers.distillation_loss(t, teacher, ids, 2.0), (cut,)
+
+
+def upstream(out):
+    return torch.linspace(-1, 1, out.numel(), device="cuda").view(out.shape).to(out.dtype)
+
+
+def pass_through(function, leaves, hooks):
+    """(result, gradients) with the leaves as they lie"""
+    leaves = [t.detach().requires_grad_() for t in leaves]
+    with hooks():
+        out = function(*leaves)
+    return out.detach(), torch.autograd.grad(out, leaves, upstream(out))
+
+
+@gpu
+@pytest.mark.parametrize("how", HOOKS)
+def test_hooks_that_lay_saved_tensors_out_anew(how):
+    """A slice that was offloaded or packed comes back with other distances between its rows, or off its boundaries: the gradients are the same bits, but for
+    layer norm, which adds a row up in an order that goes by whether 16 bytes at a time can be read: there they keep to the formulas' bounds."""
+    for name, function, leaves in operators_of_strided_tensors():
+        want, want_grads = pass_through(function, leaves, contextlib.nullcontext)
+        got, grads = pass_through(function, leaves, HOOKS[how])
+        assert torch.equal(got, want), (name, how)
+        if name.startswith("norm"):
+            exact = norm64(leaves[0], leaves[1], leaves[2] if len(leaves) > 2 else None, upstream(got), 1e-5)
+            for g, which in zip(grads, ("dx", "dweight", "dbias")):
+                near(g, *exact[which], (name, how, which))
+        else:
+            assert all(torch.equal(a, b) for a, b in zip(grads, want_grads)), (name, how)
+    layers.check_status()
+
+
+@gpu
+def test_recomputed_by_checkpoints():
+    from torch.utils.checkpoint import checkpoint
+
+    for name, function, leaves in operators_of_strided_tensors():
+        want, want_grads = pass_through(function, leaves, contextlib.nullcontext)
+        for reentrant in (False, True):
+            got, grads = [t.detach().requires_grad_() for t in leaves], None
+            out = checkpoint(function, *got, use_reentrant=reentrant)
+            out.backward(upstream(out))
+            assert torch.equal(out, want) and all(torch.equal(t.grad, b) for t, b in zip(got, want_grads)), (name, reentrant)
+
+
+def test_operands_of_a_backward_pass_lie_as_they_are():
+    """Host side: addresses and distances of what autograd hands back, not those of the forward pass (matrices that lie right are not copied, so no GPU is
+    asked)."""
+    big = torch.zeros(70, 3, 144, dtype=BF16)
+    forward = [big[:, 1, :128], torch.zeros(96, 128, dtype=BF16), torch.zeros(96, 400, dtype=BF16)[:, 16:144], torch.zeros(128, 96, dtype=BF16)]
+    operands = layers._Operands(forward)
+    assert operands.apart == [432, 128, 400, 96] and operands.room is None
+    back = [t.contiguous() for t in forward]
+    lies, _ = operands.again(back, None)
+    assert lies == [(t.data_ptr(), t.shape[1]) for t in back]
+    # those that were copied stay where the copies are
+    operands.at, operands.apart, room = [-1, 0, -1, 4096], [432, 128, 400, 104], torch.zeros(1 << 16, dtype=torch.uint8)
+    lies, _ = operands.again(back, room)
+    assert lies == [(back[0].data_ptr(), 128), (room.data_ptr(), 128), (back[2].data_ptr(), 128), (room.data_ptr() + 4096, 104)]
