@@ -1,10 +1,11 @@
 """What a model's training step needs beside the optimizer, where the gradients come from: layer norm, the gated feed-forward block and the
 loss of a distillation from a teacher's largest logits, each with its gradients.
 
-Functions that autograd differentiates once, and modules that hold their parameters.  They take CUDA tensors of fp32, bf16 or fp16 (the
-feed-forward block: bf16 or fp16), run on the current stream of the tensors' device, wait for nothing, and leave their arguments as they are.
-A call can be captured into a CUDA graph, forward and backward, ``gated_ffn`` after one that is not; as with any other operator, no result of an
-earlier pass over the same parameters may be alive when a backward pass is captured (autograd would make the capture wait for that pass's stream).
+Functions that autograd differentiates once, backward (a forward-mode derivative is refused), and modules that hold their parameters.  They take
+CUDA tensors of fp32, bf16 or fp16 (the feed-forward block: bf16 or fp16), run on the current stream of the tensors' device, wait for nothing, and
+leave their arguments as they are.  A call can be captured into a CUDA graph, forward and backward, ``gated_ffn`` after one that is not; as with any
+other operator, no result of an earlier pass over the same parameters may be alive when a backward pass is captured (autograd would make the capture
+wait for that pass's stream).
 """
 
 from __future__ import annotations
@@ -13,6 +14,7 @@ import ctypes as C
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -82,6 +84,14 @@ def _graph(*tensors):
     return False
 
 
+def _refuse_tangents(*tensors):
+    """What a kernel makes of a tensor's values has no tangent: without this, a forward-mode derivative would be lost."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, _Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("forward-mode derivatives are not supported, only backward ones")
+
+
 def _once(backward):
     """``once_differentiable``, whose contexts a plain backward pass does without."""
     guarded = once_differentiable(backward)
@@ -149,6 +159,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 
     ``weight`` and ``bias`` are vectors of ``x``'s type or fp32, and their gradients are of that type; a bias needs a weight beside it.  Means,
     variances and the sums of the gradients are fp32, each result is rounded once.  Rows of up to 16384 elements, of any stride."""
+    _refuse_tangents(x, weight, bias)
     _check("x", x)
     dim, device, dtype = x.dim(), x.get_device(), x.dtype
     width = x.shape[-1] if dim else 0
@@ -345,6 +356,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"activation is {activation!r}, supported are {', '.join(ACTIVATIONS)}")
+    _refuse_tangents(x, w_gate, w_up, w_down)
     _check("x", x, types=(torch.bfloat16, torch.float16))
     for name, t in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
         _check(name, t, x.get_device(), (x.dtype,))
@@ -384,6 +396,7 @@ class GatedFFN(torch.nn.Module):
 
 def _distill_arguments(logits, teacher_logits, teacher_ids, temperature, weights, reduction):
     """Checked arguments: (logits' rows, teacher, ids, weights, code of the reduction)."""
+    _refuse_tangents(logits, teacher_logits, weights)
     _check("logits", logits)
     device = logits.get_device()
     _check("teacher_logits", teacher_logits, device)
@@ -494,6 +507,7 @@ def distillation_loss_and_grad(logits: torch.Tensor, teacher_logits: torch.Tenso
     work = _distill_work(rows, ids)
     d = _distill_struct(rows, teacher, ids, w, float(temperature), code, work)
     if isinstance(scale, torch.Tensor):
+        _refuse_tangents(scale)
         _check("scale", scale, logits.get_device(), (torch.float32,))
         if scale.numel() != 1:
             raise ValueError("scale has to have one element")

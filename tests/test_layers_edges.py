@@ -6,6 +6,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward
 
 from pylo_b200 import layers
 from test_layers import BF16, F32, FP16, E, distill64, distill_inputs, ffn_inputs, near, norm64, randn
@@ -146,3 +147,42 @@ def test_operands_of_a_backward_pass_lie_as_they_are():
     operands.at, operands.apart, room = [-1, 0, -1, 4096], [432, 128, 400, 104], torch.zeros(1 << 16, dtype=torch.uint8)
     lies, _ = operands.again(back, room)
     assert lies == [(back[0].data_ptr(), 128), (room.data_ptr(), 128), (back[2].data_ptr(), 128), (room.data_ptr() + 4096, 104)]
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# forward-mode derivatives
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def calls_of_each_argument(device):
+    """(name, function of one tensor, that tensor) for every argument that numbers go into"""
+    make = lambda *shape: torch.ones(*shape, device=device)
+    x, w, b, h = make(3, 8), make(8), make(8), make(4, 8).bfloat16()
+    ids = torch.zeros(3, 2, device=device, dtype=torch.int64)
+    yield "x of a norm", lambda t: layers.layer_norm(t, w, b), x
+    yield "weight", lambda t: layers.layer_norm(x, t, b), w
+    yield "bias", lambda t: layers.layer_norm(x, w, t), b
+    for k, name in enumerate(("x", "w_gate", "w_up", "w_down")):
+        args = [make(3, 8).bfloat16(), h, h, h.t().contiguous()]
+        yield name, lambda t, k=k, args=args: layers.gated_ffn(*args[:k], t, *args[k + 1:]), args[k]
+    for function in (layers.distillation_loss, layers.distillation_loss_and_grad):
+        yield "logits", lambda t, f=function: f(t, make(3, 2), ids), x
+        yield "teacher", lambda t, f=function: f(x, t, ids), make(3, 2)
+        yield "weights", lambda t, f=function: f(x, make(3, 2), ids, weights=t), make(3)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_forward_mode_derivatives_are_refused(device):
+    """A dual tensor needs no gradient and holds its tangent beside its values, which is all that a kernel sees."""
+    for name, function, t in calls_of_each_argument(device):
+        with forward.dual_level():
+            dual = forward.make_dual(t, torch.ones_like(t))
+            for context in (contextlib.nullcontext, torch.no_grad):
+                with context(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    function(dual)
+            if device == "cuda":
+                function(t)   # beside a level that it takes no part in
+        if device == "cuda":
+            function(t)
+    if device == "cuda":
+        layers.check_status()
