@@ -708,10 +708,17 @@ __device__ __forceinline__ bool dt_teacher(const DtArgs& a, long long row, DtPee
   }
   return true;
 }
-// The loss of a row to base 2, without the student's sum: sum of p (log p - s) with logits relative to m, by a warp
+// The loss of a row to base 2, without the student's sum: sum of p (log p - s) with logits relative to the largest of them, by a warp.  Relative to that,
+// as to the row's maximum (which long rows do not know yet), the terms in s have one sign, so that no large ones cancel: not of logits far off centre, nor
+// where the student masks a class that the teacher gives next to nothing.
+struct DtCross { float cross, sum, near; };   // sum: of p; near: the largest logit of an entry that counts
 template <class T>
-__device__ __forceinline__ float dt_cross(const DtArgs& a, const T* s, const DtEntry* e, float m) {
-  float sum = 0.f;
+__device__ __forceinline__ DtCross dt_cross(const DtArgs& a, const T* s, const DtEntry* e) {
+  DtCross r = {0.f, 0.f, DT_LOWEST};
+  auto raise = [&](float to) {
+    if (to > r.near && r.sum != 0.f) r.cross = fmaf(r.sum * (to - r.near), a.c, r.cross);
+    r.near = to;
+  };
   for (int first = threadIdx.x & 31; first < a.top; first += 128) {
     DtEntry q[4];
     float v[4];
@@ -726,9 +733,16 @@ __device__ __forceinline__ float dt_cross(const DtArgs& a, const T* s, const DtE
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (counts[i]) sum = fmaf(q[i].p, fmaf(v[i] - m, -a.c, q[i].lp), sum);
+      if (counts[i]) {
+        raise(fmaxf(r.near, v[i]));
+        r.cross = fmaf(q[i].p, fmaf(v[i] - r.near, -a.c, q[i].lp), r.cross);
+        r.sum += q[i].p;
+      }
   }
-  return rw_warp_sum(sum);
+  raise(rw_warp_max(r.near));
+  r.cross = rw_warp_sum(r.cross);
+  r.sum = rw_warp_sum(r.sum);
+  return r;
 }
 // The column of a teacher's entry, once more
 template <class T>
@@ -808,9 +822,9 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_short(const DtArgs 
       const float all = rw_warp_max(m);
       total = rw_warp_sum(total * dt_exp2((m - all) * a.c));
       m = all;
-      const float cross = dt_cross(a, r.s, e, m);
+      const DtCross of = dt_cross(a, r.s, e);
       if (t == 0) {
-        const float loss = weight * a.temperature * a.temperature * DT_LN2 * (cross + log2f(total));
+        const float loss = weight * a.temperature * a.temperature * DT_LN2 * fmaf(of.sum, (m - of.near) * a.c, of.cross + log2f(total));
         if (a.row_loss) a.row_loss[row] = loss;
         if (a.stat) a.stat[row] = make_float2(m, 1.0f / total);
         loss_sum += loss;
@@ -862,17 +876,10 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_teachers(const DtAr
     peek = dt_peek(a, row + step, 0);
     const bool any = weight != 0.f && dt_teacher(a, row, mine, e, slots);
     if (any) {
-      // relative to the first entry's logit, where it is a number: of all logits far off centre the differences count
-      const T* const s = (const T*)a.logits + row * a.stride;
-      float near = e[0].id != DT_PADDING && e[0].p > 0.f ? rw_float(s[e[0].id < 0 ? ~e[0].id : e[0].id]) : 0.f;
-      if (!(fabsf(near) < CUDART_INF_F)) near = 0.f;
-      const float cross = dt_cross(a, s, e, near);
-      float sum = 0.f;
-      for (int k = lane; k < a.top; k += 32) sum += e[k].p;
-      sum = rw_warp_sum(sum);
+      const DtCross of = dt_cross(a, (const T*)a.logits + row * a.stride, e);
       if (a.columns)
         for (int k = lane; k < a.top; k += 32) a.columns[row * a.top + k] = make_int2(e[k].id < 0 ? -1 : e[k].id, __float_as_int(e[k].column));
-      if (lane == 0) a.teachers[row] = make_float4(weight, cross, sum, near);
+      if (lane == 0) a.teachers[row] = make_float4(weight, of.cross, of.sum, of.near);
       weight_sum += weight;
     } else if (lane == 0) a.teachers[row] = make_float4(0.f, 0.f, 0.f, 0.f);
     __syncwarp();

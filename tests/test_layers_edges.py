@@ -186,3 +186,57 @@ def test_forward_mode_derivatives_are_refused(device):
             function(t)
     if device == "cuda":
         layers.check_status()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# distillation far off centre
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def check_losses(logits, teacher, ids, T, logits_span, teacher_span):
+    """Rows' losses and their sum against 64 bits.  Each p_k is off by two roundings of its exponent, at most 1.45 times the span over T, and by those of the
+    sums; each term p_k (log p_k - log q_k) by as much of its size, and the sizes add up to the loss and twice what -sum p log p can be (log K < 7)."""
+    want, *_ = distill64(logits.double() - logits.double().median(), teacher.double() - teacher.double().amax(1, keepdim=True), ids, T)
+    slack = E * (16 * 1.45 * (logits_span + teacher_span) / T + 64 + logits.shape[1] / 32) * (want + 14 * T * T)
+    rows = layers.distillation_loss(logits, teacher, ids, T, reduction="none")
+    near(rows, want, slack, "rows")
+    loss, _ = layers.distillation_loss_and_grad(logits, teacher, ids, T, reduction="sum")
+    near(loss, want.sum(), slack.sum() + 16 * E * want.sum(), "sum")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, FP16])
+@pytest.mark.parametrize("vocab", [60, 5001])
+@pytest.mark.parametrize("centre", [1e3, -1e4])
+def test_distill_of_logits_far_off_centre_whatever_the_first_entry_is(centre, vocab, dtype):
+    """As exact as the logits where the first entry is padding, or has no probability."""
+    logits, teacher, ids = distill_inputs(9, vocab, 6, F32, seed=31)
+    logits, ids = (logits + centre).to(dtype), ids.clone()
+    span = float((logits.double() - logits.double().median()).abs().max())
+    teacher = teacher - teacher.amax(1, keepdim=True)
+    tspan = float(teacher.abs().max())
+    check_losses(logits, teacher, ids, 1.0, span, tspan)
+    left_out = teacher.clone()
+    left_out[:, 0] = -math.inf
+    check_losses(logits, left_out, ids, 2.0, span, tspan)
+    ids[:, 0] = -1
+    check_losses(logits, teacher, ids, 1.0, span, tspan)
+    ids[:, 4] = vocab
+    check_losses(logits, teacher.flip(1), ids, 0.5, span, tspan)
+
+
+@gpu
+@pytest.mark.parametrize("vocab,top", [(60, 6), (5001, 6), (5001, 300)])
+@pytest.mark.parametrize("mask", [-1e4, -1e9, -1e30])
+def test_distill_of_a_first_entry_that_the_student_masks(mask, vocab, top):
+    """A class that the student leaves out by a large negative number and the teacher gives next to nothing, first among the entries or last: its term
+    is a small probability times a large number, and the other terms do not drown in it."""
+    logits, teacher, ids = distill_inputs(7, vocab, min(top, vocab), F32, seed=33)
+    top = ids.shape[1]
+    teacher = teacher - teacher.amax(1, keepdim=True)
+    span = float(logits.abs().max())
+    for at in (0, top // 2, top - 1):
+        x, t = logits.clone(), teacher.clone()
+        t[:, at] = -4.0 - math.log(-mask)      # its term is about e^-4
+        x.scatter_(1, ids[:, at:at + 1], mask)
+        check_losses(x, t, ids, 1.0, span, float(t.abs().max()))
