@@ -667,12 +667,11 @@ __device__ __forceinline__ bool dt_teacher(const DtArgs& a, long long row, DtPee
     for (int i = 0; i < 4; ++i) {
       const int k = first + 32 * i + lane, id = peek.id[i];
       if (k >= K) break;
-      float z = id >= 0 ? peek.t[i] * a.c : -CUDART_INF_F;
-      if (id >= 0 && fabsf(peek.t[i]) < CUDART_INF_F) z = fminf(fmaxf(z, DT_LOWEST), -DT_LOWEST);   // what is a number stays one
+      const float logit = id >= 0 ? peek.t[i] : -CUDART_INF_F;
       e[k].id = id >= 0 ? id : DT_PADDING;
-      e[k].lp = z;
-      most = fmaxf(most, z);
-      any |= !(z == -CUDART_INF_F);
+      e[k].lp = logit;
+      most = fmaxf(most, logit);
+      any |= !(logit == -CUDART_INF_F);
       if (id >= 0)
         for (unsigned at = (unsigned)id * 2654435761u;; ++at) {   // ends: half of the slots stay free
           const int found = atomicCAS(&slots[(at ^ at >> 16) & (n - 1)], -1, id);
@@ -684,10 +683,10 @@ __device__ __forceinline__ bool dt_teacher(const DtArgs& a, long long row, DtPee
   if (!__any_sync(0xffffffffu, any)) return false;
   twice = __any_sync(0xffffffffu, twice);
   most = rw_warp_max(most);
-  for (int k = lane; k < K; k += 32) sum += dt_exp2(e[k].lp - most);
+  for (int k = lane; k < K; k += 32) sum += dt_exp2((e[k].lp - most) * a.c);   // (the difference first, as of the student's)
   const float log_sum = log2f(rw_warp_sum(sum));
   for (int k = lane; k < K; k += 32) {
-    const float lp = e[k].lp - most - log_sum, p = e[k].id == DT_PADDING ? 0.f : dt_exp2(lp);   // (beside a teacher's NaN or infinity lp is NaN)
+    const float lp = fmaf(e[k].lp - most, a.c, -log_sum), p = e[k].id == DT_PADDING ? 0.f : dt_exp2(lp);   // (beside a teacher's NaN or infinity lp is NaN)
     e[k].lp = lp;
     e[k].p = p;
     e[k].column = p;

@@ -240,3 +240,39 @@ def test_distill_of_a_first_entry_that_the_student_masks(mask, vocab, top):
         t[:, at] = -4.0 - math.log(-mask)      # its term is about e^-4
         x.scatter_(1, ids[:, at:at + 1], mask)
         check_losses(x, t, ids, 1.0, span, float(t.abs().max()))
+
+
+@gpu
+@pytest.mark.parametrize("teacher_type", [F32, BF16, FP16])
+@pytest.mark.parametrize("vocab,top", [(60, 6), (1000, 200), (5001, 6), (5001, 300)])
+@pytest.mark.parametrize("centre", [1e3, -3e4])
+def test_distill_of_a_teacher_far_off_centre(centre, vocab, top, teacher_type):
+    """The teacher's probabilities are those of its logits' differences: a centre that all of them have in common takes none of their bits."""
+    logits, teacher, ids = distill_inputs(9, vocab, min(top, vocab), F32, seed=35)
+    span = float(logits.abs().max())
+    teacher = (teacher + centre).to(teacher_type)
+    d = teacher.double()
+    for T in (1.0, 0.75):
+        tspan = float((d.amax(1) - d.amin(1)).max())
+        check_losses(logits, teacher, ids, T, span, tspan)
+        # the gradient's columns of the entries are probabilities themselves
+        _, g = layers.distillation_loss_and_grad(logits, teacher, ids, T, reduction="sum")
+        _, _, want, _, slack = distill64(logits, d - d.amax(1, keepdim=True), ids, T)
+        near(g, want, slack + 8 * E * want.abs(), "gradient")
+
+
+@gpu
+@pytest.mark.parametrize("vocab", [60, 5001])
+def test_distill_of_a_teacher_of_extreme_numbers(vocab):
+    """Logits whose differences, or multiples, are beyond fp32: the largest alone counts; equal ones share, however large they are."""
+    logits, teacher, ids = distill_inputs(4, vocab, 6, F32, seed=37)
+    teacher[0] = torch.tensor([3e38, 1.0, 0.0, -1.0, -3e38, -math.inf], device="cuda")
+    teacher[1] = 3.4e38
+    teacher[2] = torch.finfo(F32).min
+    teacher[3] = torch.tensor([2.5, 2.5, 2.0, -1e30, 2.5, -1e30], device="cuda")
+    alike = torch.full_like(teacher, -math.inf)
+    alike[0, 0], alike[1], alike[2] = 0.0, 0.0, 0.0
+    for T in (2.0 ** -60, 1.0):
+        alike[3] = torch.where(teacher[3] == 2.5, 0.0, -math.inf if T < 1 else torch.where(teacher[3] == 2.0, -0.5, -math.inf))
+        want, _, _, slack, _ = distill64(logits, alike, ids, T)
+        near(layers.distillation_loss(logits, teacher, ids, T, reduction="none"), want, slack, "rows")
