@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 
 import torch
 from torch.autograd import forward_ad
@@ -206,7 +207,12 @@ class LayerNorm(torch.nn.Module):
 # the gated feed-forward block
 # ---------------------------------------------------------------------------------------------------------------------
 
-_reported = None   # a word in pinned memory that a kernel sets when one of its waits ran out
+_reported = None   # a word in pinned memory that a kernel sets when one of its waits ran out: kernels hold its address, so it is made once for good
+_reported_lock = threading.Lock()
+
+
+def _pinned_word():
+    return torch.zeros(1, dtype=torch.int32).pin_memory()
 
 
 def _status_word():
@@ -214,8 +220,10 @@ def _status_word():
     if _reported is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("gated_ffn has to run once before it is captured into a CUDA graph")
-        word = torch.zeros(1, dtype=torch.int32).pin_memory()
-        _reported = (word, word.numpy(), word.data_ptr())
+        with _reported_lock:
+            if _reported is None:
+                word = _pinned_word()
+                _reported = (word, word.numpy(), word.data_ptr())
     if _reported[1][0]:
         raise L.PyloLibError("gated_ffn: a wait in a kernel of an earlier call ran out, its results are incomplete (clear_status() to go on)")
     return _reported[2]

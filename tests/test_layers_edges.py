@@ -1,8 +1,11 @@
 """Layer norm, the gated feed-forward block and distillation where calls leave the ordinary: values that are no numbers, tensors that come back
 from autograd's hooks, forward-mode derivatives, first calls of several threads."""
 
+import concurrent.futures
 import contextlib
 import math
+import threading
+import time
 
 import pytest
 import torch
@@ -276,3 +279,31 @@ def test_distill_of_a_teacher_of_extreme_numbers(vocab):
         alike[3] = torch.where(teacher[3] == 2.5, 0.0, -math.inf if T < 1 else torch.where(teacher[3] == 2.0, -0.5, -math.inf))
         want, _, _, slack, _ = distill64(logits, alike, ids, T)
         near(layers.distillation_loss(logits, teacher, ids, T, reduction="none"), want, slack, "rows")
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# first calls of several threads
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def test_first_calls_of_several_threads_share_a_word(monkeypatch):
+    """The word that the block's kernels report in is made once: a second one would leave the first to the allocator with a kernel's pointer to it alive."""
+    made = []
+
+    def make():
+        time.sleep(0.05)
+        made.append(torch.zeros(1, dtype=torch.int32))
+        return made[-1]
+
+    monkeypatch.setattr(layers, "_reported", None)
+    monkeypatch.setattr(layers, "_pinned_word", make)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    begin = threading.Barrier(8)
+
+    def call():
+        begin.wait()
+        return layers._status_word()
+
+    with concurrent.futures.ThreadPoolExecutor(8) as pool:
+        words = [f.result() for f in [pool.submit(call) for _ in range(8)]]
+    assert len(made) == 1 and set(words) == {made[0].data_ptr()}
