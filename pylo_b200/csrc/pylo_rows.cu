@@ -402,8 +402,8 @@ __global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS, ln_ctas(MOST, E
   int flip = 0;
 #pragma unroll 1
   for (long long row = at.row; row < a.rows; row += at.step, flip ^= 1) {
-    // xh = x rstd - mean rstd, one rounding: what the mean's own rounding does to it is as large
-    const uint64_t r2 = rw_pair(next_rstd, next_rstd), off = rw_pair(-next_mean * next_rstd, -next_mean * next_rstd);
+    // xh = (x - mean) rstd, as the forward pass has it: x rstd - mean rstd in one operation would add a rounding of mean rstd, which may be beyond fp32
+    const uint64_t r2 = rw_pair(next_rstd, next_rstd), off = rw_pair(-next_mean, -next_mean);
     const float rstd = next_rstd;
     if constexpr (RING) {
       fetch(row + (LN_DEPTH - 1) * at.step);
@@ -419,21 +419,22 @@ __global__ void __launch_bounds__(MOST ? MOST : LN_WARP_THREADS, ln_ctas(MOST, E
     for (int k = 0; k < E / 2; ++k) {
       uint64_t x, d;
       taken(k, x, d);
-      const uint64_t xh = rw_fma2(x, r2, off), q = a.weight ? rw_mul2(d, weight.two(k)) : d;
+      const uint64_t from = rw_add2(x, off), xh = rw_mul2(from, r2), q = a.weight ? rw_mul2(d, weight.two(k)) : d;
       dw2[k] = rw_fma2(d, xh, dw2[k]);
       db2[k] = rw_add2(d, db2[k]);
       t1 = rw_add2(t1, q);
-      t2 = rw_fma2(q, xh, t2);
+      t2 = rw_fma2(q, from, t2);   // (not of xh: what lies behind the row is 0 times a difference, and xh may be infinite there)
     }
     if (a.y) {
       const float2 sums = ln_sums<BLOCK>(rw_both(t1), rw_both(t2), s_buf[flip], at.rank, at.share);
-      // rstd (q - s1 - xh s2)
-      const uint64_t s1 = rw_pair(-sums.x * inv * rstd, -sums.x * inv * rstd), s2 = rw_pair(-sums.y * inv, -sums.y * inv);
+      // rstd (q - s1 - (x - mean) s2); of a row whose variance is beyond fp32 xh is 0, whatever the differences add up to
+      const float by = rstd != 0.f ? -sums.y * rstd * inv * rstd : 0.f;
+      const uint64_t s1 = rw_pair(-sums.x * inv * rstd, -sums.x * inv * rstd), s2 = rw_pair(by, by);
       at.store((T*)a.y + row * width, width, [&](int k) {
         uint64_t x, d;
         taken(k, x, d);
-        const uint64_t xh = rw_fma2(x, r2, off), q = a.weight ? rw_mul2(d, weight.two(k)) : d;
-        return rw_fma2(rw_fma2(xh, s2, q), r2, s1);
+        const uint64_t q = a.weight ? rw_mul2(d, weight.two(k)) : d;
+        return rw_fma2(rw_fma2(rw_add2(x, off), s2, q), r2, s1);
       });
     }
     if constexpr (RING) out = out == (LN_DEPTH - 1) * 2 * NV * piece ? 0 : out + 2 * NV * piece;

@@ -307,3 +307,32 @@ def test_first_calls_of_several_threads_share_a_word(monkeypatch):
     with concurrent.futures.ThreadPoolExecutor(8) as pool:
         words = [f.result() for f in [pool.submit(call) for _ in range(8)]]
     assert len(made) == 1 and set(words) == {made[0].data_ptr()}
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# layer norm of large numbers
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("width", [30, 64, 100, 1000, 1024, 5000])
+def test_norm_of_rows_far_off_centre(width, dtype):
+    """Means so large that they, over a deviation, are beyond fp32: the differences from them are not, and the gradients are the formula's.  A row of one value
+    has differences of 0 (equal powers of two add up exactly), so its gradient is r (q - mean q)."""
+    x = torch.full((5, width), 1.0, device="cuda")
+    x[0], x[1], x[2], x[3, ::2] = 2.0 ** 114, -(2.0 ** 113), 2.0 ** 105, 2.0
+    x = x.to(dtype).requires_grad_()
+    dy = randn(5, width, seed=41, dtype=dtype)
+    w = (1 + 0.2 * randn(width, seed=42, dtype=dtype)).requires_grad_()
+    y = layers.layer_norm(x, w, eps=1e-12)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    on = torch.tensor([True, True, True, False, True], device="cuda")
+    q = dy.double() * w.detach().double()
+    r = 1e-12 ** -0.5
+    mean = q.mean(1, keepdim=True)
+    assert not bool(y[on].any())
+    near(dx[on], (r * (q - mean))[on], (128 * E * r * (q.abs() + q.abs().mean(1, keepdim=True)))[on], "dx")
+    want = norm64(x.detach()[3:4], w.detach(), None, dy[3:4], 1e-12)   # the other rows add nothing to it
+    near(dx[3:4], *want["dx"], "dx of the row of two values")
+    near(dw, want["dweight"][0], want["dweight"][1] + 8 * E * want["dweight"][0].abs(), "dweight")
