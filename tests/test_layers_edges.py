@@ -12,7 +12,7 @@ import torch
 import torch.autograd.forward_ad as forward
 
 from pylo_b200 import layers
-from test_layers import BF16, F32, FP16, E, distill64, distill_inputs, ffn_inputs, near, norm64, randn
+from test_layers import BF16, F32, FP16, E, check_ffn, distill64, distill_inputs, ffn_inputs, near, norm64, randn
 
 gpu = pytest.mark.gpu
 
@@ -336,3 +336,47 @@ def test_norm_of_rows_far_off_centre(width, dtype):
     want = norm64(x.detach()[3:4], w.detach(), None, dy[3:4], 1e-12)   # the other rows add nothing to it
     near(dx[3:4], *want["dx"], "dx of the row of two values")
     near(dw, want["dweight"][0], want["dweight"][1] + 8 * E * want["dweight"][0].abs(), "dweight")
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# forms of the block that large sizes take
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("act", sorted(layers.ACTIVATIONS))
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_ffn_on_pairs(dtype, act):
+    """Tiles of two SMs in every launch, both types and all activations."""
+    x, *rest = ffn_inputs(1300, 328, 2600, 1608, dtype, seed=51)
+    check_ffn(x * 2, *rest, act=act)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_ffn_on_pairs_with_results_off_their_boundaries(dtype):
+    """Odd widths: no row of a result but the first begins on a 16-byte boundary, and tiles end inside of rows and columns."""
+    check_ffn(*ffn_inputs(2100, 1601, 2603, 1603, dtype, seed=52))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 5, 16, 17, 32, 33, 300, 1300])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_ffn_keeps_rows_apart(rows, dtype):
+    """A row that is no number spoils itself alone, in the result and in its own gradient; so does a gradient's."""
+    x, wg, wu, wd, dy = ffn_inputs(rows, 1001 if rows < 300 else 1000, 1300, 1608, dtype, seed=53)
+
+    def both(x, dy):
+        leaf = x.clone().requires_grad_()
+        y = layers.gated_ffn(leaf, wg, wu, wd)
+        return y.detach(), torch.autograd.grad(y, leaf, dy)[0]
+
+    y, dx = both(x, dy)
+    bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    bad[rows // 2] = True
+    x2, dy2 = x.clone(), dy.clone()
+    x2[bad, 3], dy2[bad, 7] = math.nan, math.inf
+    y2, dx2 = both(x2, dy2)
+    assert bool(y2[bad].isnan().all()) and torch.equal(y2[~bad], y[~bad]) and torch.equal(dx2[~bad], dx[~bad])
+    assert not bool(dx2[bad].isfinite().any())
+    layers.check_status()
