@@ -925,8 +925,8 @@ static int ff_begin() {
 }
 static int64_t ff_ld(int hidden) { return ((int64_t)hidden + 15) / 16 * 16; }   // of h and what is made like it
 static int64_t ff_plane(int64_t rows, int hidden, int bytes) { return (rows * ff_ld(hidden) * bytes + 255) / 256 * 256; }
-static int64_t ff_rows(int64_t rows) { return rows <= FF_FINE ? 2 * FF_FINE : rows; }   // of h, dg, du
-static int64_t ff_kept_bytes(int64_t rows, int hidden) { return ff_plane((rows + 31) / 32 * 32, hidden, 6) + 256; }   // of P and Q, in either form
+static int64_t ff_rows(int64_t rows) { return rows <= FF_FINE ? FF_FINE + rows : rows; }   // of h, dg, du
+static int64_t ff_kept_bytes(int64_t rows, int hidden) { return ff_plane(rows <= FF_FEW ? rows : (rows + 31) / 32 * 32, hidden, 6) + 256; }   // of P and Q: planes or blocks
 static ff_kept ff_planes(void* base, int64_t rows, int hidden) {
   char* const p = (char*)base + ff_plane(ff_rows(rows), hidden, 2);
   return {(uint16_t*)base, (uint4*)p, (uint16_t*)p, (uint8_t*)(p + ff_plane(rows, hidden, 4))};

@@ -359,8 +359,10 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 
     ``x`` is ``[..., width]``, ``w_gate`` and ``w_up`` are ``[hidden, width]``, ``w_down`` is ``[out, hidden]``; all are bf16 or all fp16.
     ``activation``: ``"silu"``, ``"gelu"`` (with the error function), ``"gelu_tanh"`` or ``"relu"``.  Sums are fp32; the hidden values, and backward
-    their gradients, are rounded to the type once, where they become operands of the next product (up to 16 rows: to two numbers of the type each).  Sizes and strides are free; matrices whose rows do
-    not begin on 16-byte boundaries are copied first (the copies are kept for the backward pass).  For a backward pass 8 bytes are kept per hidden value."""
+    their gradients, are rounded to the type once, where they become operands of the next product (up to 16 rows: to two numbers of the type each).  In
+    fp16 one beyond 65504 is infinite.  Sizes and strides are free; matrices whose rows do not begin on 16-byte boundaries are copied first (the copies
+    are kept for the backward pass).  For a backward pass 8 bytes are kept per hidden value: the value, and the activation and its slope times the other
+    projection in 24 bits each (more than 32 rows are counted in 32s; up to 16 rows take 32 bytes more per column)."""
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"activation is {activation!r}, supported are {', '.join(ACTIVATIONS)}")

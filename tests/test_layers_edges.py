@@ -11,6 +11,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward
 
+from pylo_b200 import _lib as L
 from pylo_b200 import layers
 from test_layers import BF16, F32, FP16, E, check_ffn, distill64, distill_inputs, ffn_inputs, near, norm64, randn
 
@@ -380,3 +381,15 @@ def test_ffn_keeps_rows_apart(rows, dtype):
     assert bool(y2[bad].isnan().all()) and torch.equal(y2[~bad], y[~bad]) and torch.equal(dx2[~bad], dx[~bad])
     assert not bool(dx2[bad].isfinite().any())
     layers.check_status()
+
+
+@pytest.mark.parametrize("hidden", [1, 16, 1000, 14336])
+def test_what_is_kept_for_a_backward_pass_is_what_the_documentation_says(hidden):
+    """8 bytes per hidden value, rows counted in 32s beyond 32, 32 bytes per column up to 16 rows; columns are counted in 16s, planes on boundaries of 256."""
+    columns = -(-hidden // 16) * 16
+    for rows in (1, 2, 15, 16, 17, 31, 32, 33, 64, 1000, 270_003):
+        h = columns * 2 * (rows + 16 if rows <= 16 else rows)
+        both = columns * 6 * (rows if rows <= 32 else -(-rows // 32) * 32)
+        assert 0 <= L.lib.pylo_b200_gated_ffn_kept(rows, hidden, 0) - h < 256
+        assert 0 <= L.lib.pylo_b200_gated_ffn_kept(rows, hidden, 1) - h - both < 3 * 256
+        assert 0 <= L.lib.pylo_b200_gated_ffn_workspace(rows, hidden) - 2 * h < 512
