@@ -627,7 +627,7 @@ int64_t pylo_b200_distill_workspace(int64_t rows, int vocab, int top);
 
 /* The gated feed-forward block: h = act(x w_gate^T) * (x w_up^T), y = h w_down^T, with its gradients.  PYLO_BF16 or PYLO_FP16 throughout,
  * products on the tensor cores with fp32 sums.  Matrices are row-major with rows ld elements apart; operands (x, dy and the weights) begin
- * on 16-byte boundaries and have ld % 8 = 0, results may lie anywhere. */
+ * on 16-byte boundaries and have ld % 8 = 0, results may lie wherever their elements can. */
 #define PYLO_ACT_SILU 0
 #define PYLO_ACT_GELU 1      /* with the error function */
 #define PYLO_ACT_GELU_TANH 2

@@ -1026,7 +1026,9 @@ static int ff_few_rows(int64_t rows) { return rows > FF_FEW ? 0 : rows <= FF_FIN
 static bool ff_operand(const void* p, int64_t ld, int64_t cols) { return p && ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld >= cols; }
 static bool ff_good(const pylo_ffn* f) {
   return f && f->rows >= 0 && f->rows <= (1 << 30) && f->width > 0 && f->hidden > 0 && f->out > 0 && f->width <= (1 << 24) && f->hidden <= (1 << 24) &&
-         f->out <= (1 << 24) && (f->type == PYLO_BF16 || f->type == PYLO_FP16) && f->activation >= PYLO_ACT_SILU && f->activation <= PYLO_ACT_RELU;
+         f->out <= (1 << 24) && (f->type == PYLO_BF16 || f->type == PYLO_FP16) && f->activation >= PYLO_ACT_SILU && f->activation <= PYLO_ACT_RELU &&
+         (((uintptr_t)f->y | (uintptr_t)f->dx | (uintptr_t)f->dw_gate | (uintptr_t)f->dw_up | (uintptr_t)f->dw_down) & 1) == 0 &&
+         (((uintptr_t)f->status | (uintptr_t)f->host_status) & 3) == 0;
 }
 // Maps of [rows][hidden] that an epilogue writes: boxes of 32 rows and 16 columns
 static int ff_map_planes(ff_args& a, int64_t rows, int64_t hidden, void* first, void* second) {

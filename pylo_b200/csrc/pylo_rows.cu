@@ -562,6 +562,9 @@ static int ln_any(const LnArgs& a, int type, int weight_type, bool aligned, bool
   return rc ? rc : launch_status();
 }
 static size_t rw_bytes(int type) { return type == PYLO_FP32 ? 4 : 2; }
+// no element lies at another address: pointers that may be NULL
+template <class... P>
+static bool rw_on(size_t bytes, P... p) { return (((uintptr_t)p | ...) & (bytes - 1)) == 0; }
 static bool rw_type(int type) { return type == PYLO_FP32 || type == PYLO_BF16 || type == PYLO_FP16; }
 
 // ------------------------------------------------------------------------------------------------
@@ -1279,7 +1282,8 @@ static DtWork dt_work(void* base, int64_t rows, int vocab, int top) {
 static bool dt_good(const pylo_distill* d) {
   return d && d->rows >= 0 && d->rows <= (1ll << 40) && d->vocab > 0 && d->vocab <= (1 << 30) && d->top > 0 && d->top <= DT_MOST_K && rw_type(d->type) &&
          rw_type(d->teacher_type) && (d->ids_bytes == 4 || d->ids_bytes == 8) && d->temperature > 0.f && (d->rows == 0 || (d->logits && d->teacher && d->ids)) &&
-         d->stride >= d->vocab && (uintptr_t)d->logits % rw_bytes(d->type) == 0;
+         d->stride >= d->vocab && d->reduction >= PYLO_REDUCE_NONE && d->reduction <= PYLO_REDUCE_MEAN && rw_on(rw_bytes(d->type), d->logits, d->grad) &&
+         rw_on(rw_bytes(d->teacher_type), d->teacher) && rw_on(d->ids_bytes, d->ids) && rw_on(4, d->weights, d->loss, d->row_loss, d->upstream);
 }
 static DtArgs dt_args(const pylo_distill* d) {
   DtArgs a = {};
@@ -1288,6 +1292,11 @@ static DtArgs dt_args(const pylo_distill* d) {
   a.rows = d->rows; a.stride = d->stride; a.vocab = d->vocab; a.top = d->top; a.teacher_type = d->teacher_type; a.wide_ids = d->ids_bytes == 8;
   a.c = (float)(DT_LOG2E / d->temperature); a.temperature = d->temperature; a.scale = 1.0f;
   return a;
+}
+
+static bool ln_good(const pylo_norm* n) {
+  return n && n->rows >= 0 && n->width > 0 && n->width <= LN_MOST && rw_type(n->type) && rw_type(n->weight_type) && rw_on(rw_bytes(n->type), n->x, n->y, n->dy, n->dx) &&
+         rw_on(rw_bytes(n->weight_type), n->weight, n->bias, n->dweight, n->dbias) && rw_on(4, n->mean, n->rstd, n->work);
 }
 
 extern "C" {
@@ -1299,7 +1308,7 @@ int64_t pylo_b200_layer_norm_workspace(int64_t rows, int width) {
 }
 
 int pylo_b200_layer_norm(const pylo_norm* n, void* stream) {
-  CHECK_ARG(n && n->rows >= 0 && n->width > 0 && n->width <= LN_MOST && rw_type(n->type) && n->eps >= 0.f);
+  CHECK_ARG(ln_good(n) && n->eps >= 0.f);
   if (n->rows == 0) return 0;
   CHECK_ARG(n->x && n->y && (n->mean == nullptr) == (n->rstd == nullptr) && (n->weight || !n->bias) && n->x_stride >= 0);
   LnArgs a = {};
@@ -1309,7 +1318,7 @@ int pylo_b200_layer_norm(const pylo_norm* n, void* stream) {
 }
 
 int pylo_b200_layer_norm_backward(const pylo_norm* n, void* stream) {
-  CHECK_ARG(n && n->rows >= 0 && n->width > 0 && n->width <= LN_MOST && rw_type(n->type));
+  CHECK_ARG(ln_good(n));
   cudaStream_t s = (cudaStream_t)stream;
   const bool columns = n->dweight || n->dbias, aligned = ln_aligned(n, true);
   const int groups = n->rows ? ln_form(n->rows, n->width, aligned && n->type != PYLO_FP32, true, aligned).groups : 0;
@@ -1341,7 +1350,7 @@ int pylo_b200_distill(const pylo_distill* d, int what, void* stream) {
   cudaStream_t s = (cudaStream_t)stream;
   const bool loss = what & PYLO_DISTILL_LOSS, grad = what & PYLO_DISTILL_GRAD, mean = d->reduction == PYLO_REDUCE_MEAN;
   CHECK_ARG(d->work && (uintptr_t)d->work % 16 == 0 && d->work_bytes >= pylo_b200_distill_workspace(d->rows, d->vocab, d->top));
-  CHECK_ARG(!grad || d->rows == 0 || (d->grad && (uintptr_t)d->grad % rw_bytes(d->type) == 0));
+  CHECK_ARG(!grad || d->rows == 0 || d->grad);
   const DtWork w = dt_work(d->work, d->rows, d->vocab, d->top);
   int groups = 0;
   if (d->rows) {

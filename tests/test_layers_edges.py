@@ -2,6 +2,7 @@
 from autograd's hooks, forward-mode derivatives, first calls of several threads."""
 
 import concurrent.futures
+import ctypes as C
 import contextlib
 import math
 import threading
@@ -393,3 +394,35 @@ def test_what_is_kept_for_a_backward_pass_is_what_the_documentation_says(hidden)
         assert 0 <= L.lib.pylo_b200_gated_ffn_kept(rows, hidden, 0) - h < 256
         assert 0 <= L.lib.pylo_b200_gated_ffn_kept(rows, hidden, 1) - h - both < 3 * 256
         assert 0 <= L.lib.pylo_b200_gated_ffn_workspace(rows, hidden) - 2 * h < 512
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# refusals at the C entries
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def test_pointers_off_their_elements_are_refused():
+    """An address that no element of its type can have gets a negative code on the host, before anything is launched; so does a reduction that there is not."""
+    norm = dict(x=16, weight=16, bias=16, y=16, mean=16, rstd=16, rows=4, width=8, x_stride=8, type=L.FP32, weight_type=L.FP32, eps=1e-5)
+    for kind, odd in ((dict(), 18), (dict(type=L.BF16, weight_type=L.BF16), 17), (dict(type=L.FP16, weight_type=L.FP16), 17)):
+        for name in ("x", "weight", "bias", "y"):
+            assert L.lib.pylo_b200_layer_norm(C.byref(L.Norm(**{**norm, **kind, name: odd})), None) == -1, (kind, name)
+    for name in ("mean", "rstd"):
+        assert L.lib.pylo_b200_layer_norm(C.byref(L.Norm(**{**norm, name: 18})), None) == -1, name
+    assert L.lib.pylo_b200_layer_norm(C.byref(L.Norm(**{**norm, "type": L.BF16, "weight": 18})), None) == -1   # fp32 beside bf16
+    back = dict(x=16, dy=16, dx=16, weight=16, dweight=16, dbias=16, mean=16, rstd=16, work=16, work_floats=1 << 20, rows=4, width=8, x_stride=8, dy_stride=8,
+                type=L.FP32, weight_type=L.FP32)
+    for name in ("x", "dy", "dx", "weight", "dweight", "dbias", "mean", "rstd", "work"):
+        assert L.lib.pylo_b200_layer_norm_backward(C.byref(L.Norm(**{**back, name: 18})), None) == -1, name
+    distill = dict(logits=16, teacher=16, ids=16, weights=16, loss=16, row_loss=16, grad=16, upstream=16, work=16, work_bytes=1 << 20, rows=4, stride=10, vocab=10,
+                   top=3, type=L.FP32, teacher_type=L.FP32, ids_bytes=8, reduction=L.REDUCE_MEAN, temperature=1.0, scale=1.0)
+    both = L.DISTILL_LOSS | L.DISTILL_GRAD
+    for bad in (*({name: 18} for name in ("teacher", "weights", "loss", "row_loss", "grad", "upstream")), dict(ids=20), dict(ids=18, ids_bytes=4), dict(teacher=17, teacher_type=L.BF16),
+                dict(reduction=3), dict(reduction=-1)):
+        assert L.lib.pylo_b200_distill(C.byref(L.Distill(**{**distill, **bad})), both, None) == -1, bad
+    ffn = dict(x=256, w_gate=256, w_up=256, w_down=256, y=256, kept=256, rows=4, ld_x=8, ld_gate=8, ld_up=8, ld_down=16, width=8, hidden=16, out=8, type=L.BF16)
+    for bad in (dict(y=257), dict(status=18), dict(host_status=18)):
+        assert L.lib.pylo_b200_gated_ffn(C.byref(L.Ffn(**{**ffn, **bad})), None) == -1, bad
+    back = {**ffn, "dy": 256, "ld_dy": 8, "work": 256, "dx": 256}
+    for bad in (dict(dx=257), dict(dw_gate=257), dict(dw_up=257), dict(dw_down=257), dict(status=18)):
+        assert L.lib.pylo_b200_gated_ffn_backward(C.byref(L.Ffn(**{**back, **bad})), None) == -1, bad
