@@ -443,7 +443,7 @@ def _contiguous(t):
 def _distill_struct(rows, teacher, ids, weights, temperature, reduction, work):
     n, vocab = rows.shape
     return L.Distill(logits=rows.data_ptr(), teacher=teacher.data_ptr(), ids=ids.data_ptr(), weights=None if weights is None else weights.data_ptr(),
-                     rows=n, stride=vocab if n == 1 else rows.stride(0), vocab=vocab, top=ids.shape[-1], type=TYPES[rows.dtype],
+                     rows=n, stride=vocab if n <= 1 else rows.stride(0), vocab=vocab, top=ids.shape[-1], type=TYPES[rows.dtype],
                      teacher_type=TYPES[teacher.dtype], ids_bytes=ids.element_size(), reduction=reduction, temperature=temperature, scale=1.0,
                      work=work.data_ptr(), work_bytes=work.numel())
 

@@ -426,3 +426,67 @@ def test_pointers_off_their_elements_are_refused():
     back = {**ffn, "dy": 256, "ld_dy": 8, "work": 256, "dx": 256}
     for bad in (dict(dx=257), dict(dw_gate=257), dict(dw_up=257), dict(dw_down=257), dict(status=18)):
         assert L.lib.pylo_b200_gated_ffn_backward(C.byref(L.Ffn(**{**back, **bad})), None) == -1, bad
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# shapes and strides at their ends
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+@gpu
+def test_no_rows_of_any_stride():
+    """No rows, however far they would be apart: results and gradients are empty, the weights' are zero."""
+    w = torch.ones(9, device="cuda", requires_grad=True)
+    for x in (torch.empty(1, 9, device="cuda").expand(0, 9), torch.empty(9, 4, device="cuda").t()[:0], torch.empty(0, 3, 9, device="cuda"), torch.empty(4, 0, 9, device="cuda")):
+        leaf = x.detach().requires_grad_()
+        y = layers.layer_norm(leaf, w)
+        (dx, dw) = torch.autograd.grad(y, (leaf, w), torch.ones_like(y))
+        assert y.shape == x.shape == dx.shape and not bool(dw.any())
+        teacher = torch.empty(*x.shape[:-1], 2, device="cuda")
+        for reduction in ("mean", "sum", "none"):
+            leaf = x.detach().requires_grad_()
+            loss = layers.distillation_loss(leaf, teacher, teacher.long(), reduction=reduction)
+            (g,) = torch.autograd.grad(loss, leaf, torch.ones_like(loss))
+            assert loss.shape == (x.shape[:-1] if reduction == "none" else ()) and g.shape == x.shape and not bool(loss.any())
+        loss, g = layers.distillation_loss_and_grad(x, teacher, teacher.long())
+        assert float(loss) == 0 and g.shape == x.shape
+        h = torch.ones(5, 9, device="cuda", dtype=BF16, requires_grad=True)
+        leaf = x.detach().bfloat16().requires_grad_()
+        y = layers.gated_ffn(leaf, h, h, h.t())
+        (dx, dh) = torch.autograd.grad(y, (leaf, h), torch.ones_like(y))
+        assert y.shape == x.shape == dx.shape and not bool(dh.any())
+
+
+@gpu
+def test_one_tensor_in_several_places():
+    """A leaf's gradient is the sum over the places that it has."""
+    w = randn(24, seed=71).requires_grad_()
+    dy = randn(5, 24, seed=72)
+    x = randn(5, 24, seed=73)
+    (both,) = torch.autograd.grad(layers.layer_norm(x, w, w), w, dy)
+    a, b = (w.detach().clone().requires_grad_() for _ in range(2))
+    assert torch.equal(both, sum(torch.autograd.grad(layers.layer_norm(x, a, b), (a, b), dy)))
+    m = randn(16, 16, seed=74, dtype=BF16).requires_grad_()
+    (both,) = torch.autograd.grad(layers.gated_ffn(m, m, m, m), m, randn(16, 16, seed=75, dtype=BF16))
+    parts = [m.detach().clone().requires_grad_() for _ in range(4)]
+    grads = torch.autograd.grad(layers.gated_ffn(*parts), parts, randn(16, 16, seed=75, dtype=BF16))
+    # three sums of two, each rounded, in whatever order autograd adds them up
+    assert bool(((both.double() - sum(g.double() for g in grads)).abs() <= 4 * 2.0 ** -8 * sum(g.double().abs() for g in grads)).all())
+
+
+@gpu
+def test_upstream_gradients_of_any_stride():
+    x, wg, wu, wd, dy = ffn_inputs(40, 72, 136, 80, BF16, seed=81)
+    leaves = [t.requires_grad_() for t in (x, wg, wu, wd)]
+    y = layers.gated_ffn(*leaves)
+    z = layers.layer_norm(x.detach().requires_grad_())
+    for cut in (lambda t: t.t().contiguous().t(), lambda t: t[:1].expand_as(t), lambda t: t[:, :1].expand_as(t), lambda t: torch.cat([t, t], 1)[:, t.shape[1]:], lambda t: t.as_strided(t.shape, (8, 1))):
+        want = torch.autograd.grad(y, leaves, cut(dy).contiguous(), retain_graph=True)
+        got = torch.autograd.grad(y, leaves, cut(dy), retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    logits, teacher, ids = distill_inputs(12, 50, 4, F32, seed=82)
+    leaf = logits.requires_grad_()
+    rows = layers.distillation_loss(leaf, teacher, ids, reduction="none")
+    up = randn(12, 3, seed=83)
+    for cut in (up[:, 1], up[:1, 0].expand(12), up.double()[:, 2].float()):
+        assert torch.equal(*(torch.autograd.grad(rows, leaf, u, retain_graph=True)[0] for u in (cut, cut.contiguous())))
