@@ -542,11 +542,11 @@ static int ln_launch(const LnArgs& a, bool backward, cudaStream_t s) {
   LN_GO(MANY, 0)
 #undef LN_GO
 }
-// 16 bytes at a time where every row begins on their boundary
+// 16 bytes at a time where every row begins on their boundary (how far the next one would be from a single row says nothing)
 static bool ln_aligned(const pylo_norm* n, bool backward) {
   const int vec = n->type == PYLO_FP32 ? 4 : 8;
   uintptr_t p = (uintptr_t)n->x | (uintptr_t)n->weight | (backward ? (uintptr_t)n->dy | (uintptr_t)n->dx : (uintptr_t)n->y | (uintptr_t)n->bias);
-  return p % 16 == 0 && (n->width | n->x_stride | (backward ? n->dy_stride : 0)) % vec == 0;
+  return p % 16 == 0 && (n->width | (n->rows > 1 ? n->x_stride | (backward ? n->dy_stride : 0) : 0)) % vec == 0;
 }
 template <class T, class W>
 static int ln_run(const LnArgs& a, bool aligned, bool backward, cudaStream_t s) {

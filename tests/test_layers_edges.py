@@ -458,6 +458,35 @@ def test_no_rows_of_any_stride():
 
 
 @gpu
+def test_one_column_one_row_and_vectors():
+    for x in (randn(7, 1, seed=61), randn(1, 7, seed=61).t(), randn(7, 5, seed=61)[:, 2:3], randn(1, 1, seed=62).expand(7, 1)):
+        leaf, w, b = x.detach().requires_grad_(), randn(1, seed=63).requires_grad_(), randn(1, seed=64).requires_grad_()
+        y = layers.layer_norm(leaf, w, b)
+        dx, dw, db = torch.autograd.grad(y, (leaf, w, b), torch.ones_like(y))
+        assert torch.equal(y, b.expand(7, 1)) and not bool(dw.any()) and float(db) == 7
+        near(dx, *norm64(x, w.detach(), b.detach(), torch.ones_like(x), 1e-5)["dx"], "dx")   # r q - r q, each rounded
+        ids = torch.zeros(7, 1, device="cuda", dtype=torch.int64)
+        loss, g = layers.distillation_loss_and_grad(x, torch.zeros(7, 1, device="cuda"), ids)
+        assert float(loss) == 0 and not bool(g.any())
+        check_ffn(x.to(BF16), *[randn(*s, seed=65 + k, dtype=BF16) for k, s in enumerate(((3, 1), (3, 1), (1, 3), (7, 1)))])
+    # one row, whose distance to the next means nothing
+    wide = randn(1, 40, seed=66)
+    row = wide.as_strided((1, 40), (3, 1))
+    assert torch.equal(layers.layer_norm(row), layers.layer_norm(wide))
+    teacher, ids = torch.zeros(1, 2, device="cuda"), torch.tensor([[3, 8]], device="cuda")
+    assert torch.equal(layers.distillation_loss(row, teacher, ids), layers.distillation_loss(wide, teacher, ids))
+    w = randn(6, 40, seed=67, dtype=BF16)
+    assert torch.equal(layers.gated_ffn(row.bfloat16().as_strided((1, 40), (3, 1)), w, w, w.t()), layers.gated_ffn(wide.bfloat16(), w, w, w.t()))
+    # vectors
+    assert torch.equal(layers.layer_norm(wide[0]), layers.layer_norm(wide)[0])
+    assert torch.equal(layers.gated_ffn(wide[0].bfloat16(), w, w, w.t()), layers.gated_ffn(wide.bfloat16(), w, w, w.t())[0])
+    leaf = wide[0].detach().requires_grad_()
+    loss = layers.distillation_loss(leaf, teacher[0], ids[0], reduction="none")
+    (g,) = torch.autograd.grad(loss, leaf)
+    assert loss.shape == () and torch.equal(loss.detach(), layers.distillation_loss(wide, teacher, ids)) and g.shape == (40,)
+
+
+@gpu
 def test_one_tensor_in_several_places():
     """A leaf's gradient is the sum over the places that it has."""
     w = randn(24, seed=71).requires_grad_()
