@@ -86,11 +86,10 @@ def _graph(*tensors):
 
 
 def _refuse_tangents(*tensors):
-    """What a kernel makes of a tensor's values has no tangent: without this, a forward-mode derivative would be lost."""
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if isinstance(t, _Tensor) and forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError("forward-mode derivatives are not supported, only backward ones")
+    """Inside of a forward-mode level: what a kernel makes of a tensor's values has no tangent, so that a derivative would be lost."""
+    for t in tensors:
+        if isinstance(t, _Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("forward-mode derivatives are not supported, only backward ones")
 
 
 def _once(backward):
@@ -111,7 +110,7 @@ def _once(backward):
 def _norm_forward(x, weight, bias, eps, keep):
     n, width = x.shape
     y = _like(x)
-    stat = torch.empty((2, n), dtype=torch.float32, device=x.device) if keep else None
+    stat = torch.empty(2 * n, dtype=torch.float32, device=x.device) if keep else None   # means, 1 / deviations
     if n:
         mean = stat.data_ptr() if keep else None
         kind = TYPES[x.dtype]
@@ -133,7 +132,8 @@ class _LayerNorm(torch.autograd.Function):
     @_once
     def backward(ctx, dy):
         rows, weight, stat = ctx.saved_tensors
-        rows, stat = _rows(rows), _rows(stat)   # (hooks may have laid them out anew)
+        if rows.stride(1) != 1 or not stat.is_contiguous():   # hooks have laid them out anew
+            rows, stat = _rows(rows), stat.contiguous()
         n, width = rows.shape
         device = rows.get_device()
         dy = _rows(dy)
@@ -142,7 +142,7 @@ class _LayerNorm(torch.autograd.Function):
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty_like(weight) if need_b else None
         kind, mean = TYPES[rows.dtype], stat.data_ptr()
-        w = L.Norm(x=rows.data_ptr(), dy=dy.data_ptr(), weight=None if weight is None else weight.data_ptr(), mean=mean, rstd=mean + 4 * stat.stride(0),
+        w = L.Norm(x=rows.data_ptr(), dy=dy.data_ptr(), weight=None if weight is None else weight.data_ptr(), mean=mean, rstd=mean + 4 * n,
                    dx=dx.data_ptr() if need_x else None, dweight=dw.data_ptr() if need_w else None, dbias=db.data_ptr() if need_b else None, rows=n,
                    x_stride=rows.stride(0), dy_stride=dy.stride(0), width=width, type=kind, weight_type=kind if weight is None else TYPES[weight.dtype])
         if need_w or need_b:
@@ -160,7 +160,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 
     ``weight`` and ``bias`` are vectors of ``x``'s type or fp32, and their gradients are of that type; a bias needs a weight beside it.  Means,
     variances and the sums of the gradients are fp32, each result is rounded once.  Rows of up to 16384 elements, of any stride."""
-    _refuse_tangents(x, weight, bias)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, weight, bias)
     _check("x", x)
     dim, device, dtype = x.dim(), x.get_device(), x.dtype
     width = x.shape[-1] if dim else 0
@@ -292,13 +293,21 @@ class _Operands:
         return [t.data_ptr() if at < 0 else base + at for t, at in zip(tensors, self.at)]
 
     def again(self, tensors, room):
-        """(operands, what holds them) of a backward pass: the forward pass's copies, ``room``, and the other matrices as autograd hands them back.  Its
-        hooks may have laid those out anew (a slice that was offloaded comes back without its gaps), so how they lie is looked up again."""
-        copied = [False] * len(tensors) if room is None else [at >= 0 for at in self.at]
-        rest = [t for t, c in zip(tensors, copied) if not c]
-        lies = _Operands(rest) if rest else None
-        found = iter(zip(lies.pointers(rest), lies.apart) if rest else ())
-        return [(room.data_ptr() + at, apart) if c else next(found) for c, at, apart in zip(copied, self.at or copied, self.apart)], lies
+        """((address, elements between rows) of each operand, what holds them) of a backward pass: the forward pass's copies, ``room``, and the other matrices
+        as autograd hands them back.  Its hooks may have laid those out anew (a slice that was offloaded comes back without its gaps), so how they lie is
+        looked up again."""
+        if room is None:
+            lies = _Operands(tensors)
+            return zip(lies.pointers(tensors), lies.apart), lies
+        base, operands, held = room.data_ptr(), [], []
+        for t, at, apart in zip(tensors, self.at, self.apart):
+            if at >= 0:
+                operands.append((base + at, apart))
+                continue
+            lies = _Operands((t,))
+            held.append(lies)
+            operands.append((*lies.pointers((t,)), *lies.apart))
+        return operands, held
 
 
 def _ffn_struct(tensors, operands, activation):
@@ -366,7 +375,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"activation is {activation!r}, supported are {', '.join(ACTIVATIONS)}")
-    _refuse_tangents(x, w_gate, w_up, w_down)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, w_gate, w_up, w_down)
     _check("x", x, types=(torch.bfloat16, torch.float16))
     for name, t in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
         _check(name, t, x.get_device(), (x.dtype,))
@@ -406,7 +416,8 @@ class GatedFFN(torch.nn.Module):
 
 def _distill_arguments(logits, teacher_logits, teacher_ids, temperature, weights, reduction):
     """Checked arguments: (logits' rows, teacher, ids, weights, code of the reduction)."""
-    _refuse_tangents(logits, teacher_logits, weights)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(logits, teacher_logits, weights)
     _check("logits", logits)
     device = logits.get_device()
     _check("teacher_logits", teacher_logits, device)
@@ -479,8 +490,9 @@ class _Distillation(torch.autograd.Function):
     @_once
     def backward(ctx, upstream):
         rows, teacher, ids, weights, work = ctx.saved_tensors
-        # (hooks may have laid them out anew)
-        rows, teacher, ids, weights = _rows(rows), _contiguous(teacher), _contiguous(ids), None if weights is None else _contiguous(weights)
+        if rows.stride(1) != 1 or not (teacher.is_contiguous() and ids.is_contiguous() and (weights is None or weights.is_contiguous())):
+            # hooks have laid them out anew
+            rows, teacher, ids, weights = _rows(rows), teacher.contiguous(), ids.contiguous(), None if weights is None else weights.contiguous()
         grad = _like(rows)
         if upstream.dtype is not torch.float32 or not upstream.is_contiguous():
             upstream = upstream.to(torch.float32).contiguous()
@@ -517,7 +529,8 @@ def distillation_loss_and_grad(logits: torch.Tensor, teacher_logits: torch.Tenso
     work = _distill_work(rows, ids)
     d = _distill_struct(rows, teacher, ids, w, float(temperature), code, work)
     if isinstance(scale, torch.Tensor):
-        _refuse_tangents(scale)
+        if forward_ad._current_level >= 0:
+            _refuse_tangents(scale)
         _check("scale", scale, logits.get_device(), (torch.float32,))
         if scale.numel() != 1:
             raise ValueError("scale has to have one element")
