@@ -298,7 +298,7 @@ class _Operands:
         looked up again."""
         if room is None:
             lies = _Operands(tensors)
-            return zip(lies.pointers(tensors), lies.apart), lies
+            return list(zip(lies.pointers(tensors), lies.apart)), lies
         base, operands, held = room.data_ptr(), [], []
         for t, at, apart in zip(tensors, self.at, self.apart):
             if at >= 0:
