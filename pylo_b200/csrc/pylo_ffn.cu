@@ -214,9 +214,9 @@ struct ff_product {
 };
 struct ff_args {
   ff_product p[FF_GROUP];
-  CUtensorMap planes[2];    // what the epilogue writes by copies from shared memory, 32 rows of 16 columns at a time: GATE: h; BACK: dg, du
-  ff_kept kept;             // GATE: written (of few rows; else through the maps), BACK: read
-  uint16_t *dg, *du;        // BACK, written as kept is
+  CUtensorMap planes[2];    // what the epilogue writes by copies from shared memory, 32 rows of 16 columns at a time: GATE: h; BACK: dg, du (of many rows)
+  ff_kept kept;             // GATE: P and Q written, of few rows h too; BACK: read
+  uint16_t *dg, *du;        // BACK of few rows: written
   long long ld;             // of kept, dg, du
   int n, tiles, activation, keep;
   int *status, *host_status;
@@ -234,35 +234,20 @@ struct FfSmem {
   volatile int abort;
 };
 
-// A warp's block of 32 rows x 64 bytes (32 x 16 bit) or 32 x 32 bytes (32 x 8 bit) between rows per lane and rows of four (two) lanes: 16-byte
+// A warp's block of 32 rows x 64 bytes (32 x 16 bit) or 32 x 32 bytes (16 x 16 bit) between rows per lane and rows of four (two) lanes: 16-byte
 // pieces, spread over the banks.
 __device__ __forceinline__ uint4* ff_at64(unsigned char* s, int row, int piece) { return reinterpret_cast<uint4*>(s + row * 64 + 16 * (piece ^ ((row >> 1) & 3))); }
 __device__ __forceinline__ uint4* ff_at32(unsigned char* s, int row, int piece) { return reinterpret_cast<uint4*>(s + row * 32 + 16 * (piece ^ ((row >> 2) & 1))); }
 
 __device__ __forceinline__ void ff_put64(unsigned char* s, const uint32_t (&w)[16]);
-// 32 x 32 elements of 16 bits from a row per lane to memory; rows and columns beyond the matrix are left out
+// 32 x 32 elements of 16 bits from a row per lane to memory where rows begin anywhere (else they leave by copies), a row at a time; rows and columns beyond
+// the matrix are left out
 __device__ __forceinline__ void ff_store16(unsigned char* s, const uint32_t (&w)[16], uint16_t* dst, long long ld, int rows, int cols) {
   const int lane = threadIdx.x & 31;
   __syncwarp();
   ff_put64(s, w);
   __syncwarp();
-  if ((((uintptr_t)dst | (uintptr_t)(2 * ld)) & 15) == 0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = (lane >> 2) + 8 * i, c = 8 * (lane & 3);
-      if (r < rows && c < cols) {
-        const uint4 v = *ff_at64(s, r, lane & 3);
-        uint16_t* const to = dst + r * ld + c;
-        if (c + 8 <= cols) *reinterpret_cast<uint4*>(to) = v;
-        else {
-          const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (c + j < cols) to[j] = (uint16_t)(e[j >> 1] >> (16 * (j & 1)));
-        }
-      }
-    }
-  } else if (lane < cols) {   // rows that begin anywhere: a row at a time
+  if (lane < cols) {
 #pragma unroll 8
     for (int r = 0; r < min(32, rows); ++r)
       dst[r * ld + lane] = reinterpret_cast<const uint16_t*>(ff_at64(s, r, lane >> 3))[lane & 7];
@@ -338,7 +323,8 @@ __device__ __forceinline__ void ff_act(int activation, float g, float& a, float&
 // Otherwise the CTAs of a cluster (1, 2, 4 or 8) share one tile of 128 x 128, each with its part of the contraction; the first adds their sums up
 // through distributed shared memory, in rank order.
 //
-// 8192 rows x 4096 x 14336 bf16 on a B200: gate 1213 us (1.59 PFLOP/s), y 631, back 759 (1.27), dx and the weights' gradients 3005 (1.60), at the power limit.
+// 8192 rows x 4096 x 14336 bf16 on a B200, passes in loops of their own: forward 2051 us (1.41 PFLOP/s), backward 4356 (1.33); one behind the other 6.6 to 7.0 ms, all at the
+// power limit.  8192 x 1024 x 4096: 173, 335 and 547 to 581.
 template <bool PAIR, int EPI, bool BF>
 __global__ void __launch_bounds__(ff_threads(EPI), 1) k_ffn_product(const __grid_constant__ ff_args a) {
   extern __shared__ unsigned char ff_dyn[];

@@ -163,12 +163,14 @@ __device__ __forceinline__ void rw_commit() { asm volatile("cp.async.commit_grou
 // CTAs; the next one is on its way while one is worked on.  The weights stay in registers from row to row, the sums of their
 // gradients too; those leave as one partial sum per CTA, and a second kernel adds them up in a fixed order.
 //
-// 32768 x 4096 bf16 on a B200: forward 104 us (5.2 TB/s), backward 165 (4.9 TB/s), whose bound is as much the issue slots as the memory.
+// 32768 x 4096 on a B200: bf16 forward 101 us (5.3 TB/s), backward with the columns' sums 175 (4.6 TB/s), whose bound is as much the issue slots as the memory; fp16 93 and
+// 183, fp32 177 (6.1 TB/s) and 286.  A row's elements one at a time, 12289 x 1001 fp16: 22 and 32.
 // ------------------------------------------------------------------------------------------------
 #define LN_WARP_THREADS 128   // of a CTA whose warps have a row each
 #define LN_WARPS (LN_WARP_THREADS / 32)
 #define LN_MOST 16384         // elements of a row
-// CTAs of so many threads on an SM, with E elements per thread: 64 to 128 registers
+// CTAs of so many threads on an SM, with E elements per thread: 64 to 168 registers.  At 128, 32 elements of a warp's row spill (forward 24 to 40 bytes of stack, backward 72, fp16
+// weights 176), 16 of a larger CTA's that come one at a time up to 56.
 __host__ __device__ constexpr int ln_ctas(int threads, int e, bool backward, bool ring) {
   return threads > 128 ? 512 / threads : e <= 8 ? backward ? 6 : 8 : backward && !ring ? 3 : 4;
 }
@@ -575,9 +577,10 @@ static bool rw_type(int type) { return type == PYLO_FP32 || type == PYLO_BF16 ||
 // teacher and the weight zero.  Rows of weight zero are not read, whatever they hold: their loss and gradient are zero.
 //
 // One pass over a row with a running maximum and sum per thread; powers of two of differences from the maximum, scaled by log2(e) / T (not of scaled logits
-// less the scaled maximum in one operation: of masks of -1e30 what that rounds off is a power of its own).  The
-// gradient reads the row again (in the call that makes both, out of the L2 cache: the rows that are being worked on fit it).  The K
-// columns with a teacher's entry are written a second time, behind a barrier, with what their entries add up to.
+// less the scaled maximum in one operation: of masks of -1e30, or far off centre, what that rounds off is a power of its own), of the teacher's logits as of the
+// student's.  The gradient reads the row again (in the call that makes both, out of the SMs' shared memory, where a long row stays between the passes, or
+// a short one through the caches).  The K columns with a teacher's entry are written a second time, behind a barrier, with what their entries add up to.
+// Exponentials are ex2.approx: 2 ulp each, beside exponents that are rounded to 2^-24 of their size anyway.
 // ------------------------------------------------------------------------------------------------
 #define DT_MOST_K 1024
 #define DT_WARP_VOCAB 1024     // classes up to which a row is a warp's
@@ -902,7 +905,8 @@ __global__ void __launch_bounds__(DT_WARP_THREADS) k_distill_teachers(const DtAr
 //
 // A cluster shares a row where there are too few rows for all CTAs, and where a row would not fit the ring.
 //
-// 8192 x 50257 bf16 on a B200: loss 163 us (5.1 TB/s; issue slots 70 %, exponentials 68 %), gradient alone 303 (5.4 TB/s).
+// 8192 x 50257 bf16 on a B200: this kernel's loss 163 us (5.1 TB/s; issue slots 70 %, exponentials 68 %), gradient alone 303 (5.4 TB/s).  Calls, teachers and totals among
+// them: fp16 171 and 312; 4096 x 50257 fp32 149 and 291, both in one 389 (4.2 TB/s).
 #define DL_MOST_SHARE 8
 #define DL_KEPT 16   // pieces of a row that stay in the ring of 24
 __host__ __device__ constexpr int dl_ring(int what) { return what == (DT_LOSS | DT_GRAD) ? 24 : 16; }
@@ -1188,7 +1192,7 @@ __global__ void __launch_bounds__(NT) k_distill_weights(const DtArgs a, double* 
   }
 }
 // The CTAs' sums: loss[0] their sum, or (mean) over that of the weights; inv[0] one over that
-__global__ void __launch_bounds__(NT) k_distill_total(const double2* __restrict__ part, int n, int mean, float scale, float* loss, float* inv) {
+__global__ void __launch_bounds__(NT) k_distill_total(const double2* __restrict__ part, int n, int mean, float* loss, float* inv) {
   pdl_begin();
   __shared__ double s_d[2][NWARP];
   double l = 0.0, w = 0.0;
@@ -1199,7 +1203,7 @@ __global__ void __launch_bounds__(NT) k_distill_total(const double2* __restrict_
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < NWARP; ++i) { l += s_d[0][i]; w += s_d[1][i]; }
-    if (loss) loss[0] = (float)(mean ? (w != 0.0 ? l / w : 0.0) * scale : l * scale);
+    if (loss) loss[0] = (float)(!mean ? l : w != 0.0 ? l / w : 0.0);
     if (inv) inv[0] = w != 0.0 ? (float)(1.0 / w) : 0.f;
   }
 }
@@ -1379,7 +1383,7 @@ int pylo_b200_distill(const pylo_distill* d, int what, void* stream) {
     if (rc) return rc;
   }
   if (loss && d->reduction != PYLO_REDUCE_NONE)
-    launch(k_distill_total, 1, NT, 0, s, (const double2*)w.part, groups, (int)mean, 1.0f, d->loss, w.inv);
+    launch(k_distill_total, 1, NT, 0, s, (const double2*)w.part, groups, (int)mean, d->loss, w.inv);
   return launch_status();
 }
 
