@@ -519,3 +519,53 @@ def test_upstream_gradients_of_any_stride():
     up = randn(12, 3, seed=83)
     for cut in (up[:, 1], up[:1, 0].expand(12), up.double()[:, 2].float()):
         assert torch.equal(*(torch.autograd.grad(rows, leaf, u, retain_graph=True)[0] for u in (cut, cut.contiguous())))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# what must not pass in silence
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+@gpu
+def test_saved_arguments_that_are_changed_are_noticed():
+    """Every argument that a backward pass reads again: changed in place between the passes, it raises."""
+    x, wg, wu, wd, dy = ffn_inputs(40, 72, 136, 80, BF16, seed=91)
+    logits, teacher, ids = distill_inputs(12, 50, 4, F32, seed=92)
+    weights = torch.ones(12, device="cuda")
+    calls = {
+        "norm": (lambda x, w, b: layers.layer_norm(x, w, b), [randn(5, 24, seed=93), randn(24, seed=94), randn(24, seed=95)], (0, 1)),
+        "block": (lambda *t: layers.gated_ffn(*t), [x, wg, wu, wd], (0, 1, 2, 3)),
+        "block, copied": (lambda *t: layers.gated_ffn(*t), [t[..., 1:] if k == 0 else t for k, t in enumerate((randn(40, 73, seed=96, dtype=BF16), wg, wu, wd))], (0, 1, 2, 3)),
+        "distillation": (lambda t, a, i, w: layers.distillation_loss(t, a, i, weights=w), [logits, teacher, ids, weights], (0, 1, 2, 3)),
+    }
+    for name, (function, args, saved) in calls.items():
+        for k in saved:
+            mine = [t.detach().clone() if not name.endswith("copied") else t.detach() for t in args]
+            mine = [t.requires_grad_() if t.is_floating_point() and (not name.startswith("dist") or j == 0) else t for j, t in enumerate(mine)]
+            views = [t * 1 if t.requires_grad else t for t in mine]   # no leaves, which must not be changed in place
+            out = function(*views)
+            with torch.no_grad():
+                views[k].add_(1)
+            with pytest.raises(RuntimeError, match="modified by an inplace"):
+                out.sum().backward()
+
+
+@gpu
+def test_transforms_that_the_calls_do_not_know_are_refused():
+    """torch.func's transforms and batched gradients raise instead of computing something else."""
+    x, w = randn(4, 6, 24, seed=97), randn(24, seed=98)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: layers.layer_norm(t, w))(x)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: layers.layer_norm(t, w).sum())(x[0])
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda t: layers.layer_norm(t, w), (x[0],), (x[1],))
+    leaf = x[0].clone().requires_grad_()
+    y = layers.layer_norm(leaf, w)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, leaf, x[:2], is_grads_batched=True)
+    h = randn(24, 24, seed=99, dtype=BF16)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: layers.gated_ffn(t, h, h, h))(x.bfloat16())
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: layers.distillation_loss(t, t[:, :2], torch.zeros(6, 2, device="cuda", dtype=torch.int64)))(x)
